@@ -229,6 +229,42 @@ int r3d_gfx950_stream_probe(const void* src, int64_t bytes, int waves_per_wg, in
 int r3d_gfx950_mfma_valu_probe(int nv, int lag3, int iters, void* work, int64_t* cycles,
                                RadStream s);
 
+/* The second row table, with no counterpart in the reference: rows of ops and encodings past the
+ * set that radiance's other plugins declare (int8: gemm_nt_q at i8a8 and its producers), in the
+ * same structures, resolved and launched the same way.  A loader compares the schemas of
+ * rad_kernel_schema_at with other plugins', so these are listed apart; an engine that knows the ops
+ * reads them here.  R3D_NO_I8 and R3D_NO_I8_DEC hide rows at registration.  gemm_nt_q's schema is
+ * rad_kernel_schema_at's. */
+int r3d_gfx950_ext_schema_count(void);
+const RadOpSchema* r3d_gfx950_ext_schema_at(int i);
+int r3d_gfx950_ext_kernel_count(void);
+const RadKernelInfo* r3d_gfx950_ext_kernel_at(int i);
+
+/* gemm_nt_q at i8a8: Y[m, n] = bf16((f32(sum_k A[m, k] B[n, k]) * a_scale[m]) * b_scale[n]), the
+ * sum exact in i32.  Operands (a int8 [M, K], a_scale f32 [M] or [M, 1], b int8 [N, K], b_scale
+ * f32 [N] or [N, 1], y bf16 [M, N]); params N, K, dtype "i8a8", group K if given; M =
+ * numel(y) / N.  K <= 131071.  The _decode entry takes M <= 16.  RAD_OK, RAD_E_UNSUPPORTED /
+ * RAD_E_SHAPE / RAD_E_STRIDE for refused operands, RAD_E_DEVICE for a failed launch.
+ * Asynchronous on `s`. */
+int r3d_rad_gemm_nt_q_i8(const RadArgs* a, RadStream s);
+int r3d_rad_gemm_nt_q_i8_decode(const RadArgs* a, RadStream s);
+
+/* Producers of i8a8 activations: int8 codes q [M, n] and one f32 scale a row, [M] or [M, 1], of
+ *   quant_act_i8       (x bf16/f32 [M, n], q, scale)
+ *   gated_quant_i8     (gate_up bf16/f32 [M, 2n], q, scale, out?): act(gate) * up in f32, act
+ *                      "silu" (default) or "sigmoid"
+ *   rmsnorm_quant_i8   (x bf16, residual? bf16, w bf16/f32 [n], q, scale, out?, residual_out?):
+ *                      r = bf16(residual + x) to residual_out (given together; residual_out may be
+ *                      the memory of residual or of x), then (r / rms) * (w + wadd) in f32
+ * scale = max(amax / 127, 2^-126), 1 for a row of zeros; q to nearest even.  A row with a NaN or
+ * an infinity has that as its scale and codes 0.  Params n, dtype (x's), eps, wadd, act; M =
+ * numel(x) / n.  out (bf16/f32 [M, n]) carries the values that the codes are of.  RAD_OK,
+ * RAD_E_INVAL for a missing operand, RAD_E_DTYPE / RAD_E_SHAPE / RAD_E_STRIDE / RAD_E_UNSUPPORTED
+ * (act) for refused ones, RAD_E_DEVICE.  Asynchronous on `s`. */
+int r3d_rad_quant_act_i8(const RadArgs* a, RadStream s);
+int r3d_rad_gated_quant_i8(const RadArgs* a, RadStream s);
+int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
+
 /* Build identity with no counterpart in the reference: the SHA-256 (hex) of the compile
  * flags and of the sources this library was compiled from -- the flags as one line, then
  * every file under libr3d_amd/csrc and include, in name order, each as "<relative

@@ -23,7 +23,9 @@ __all__ = [
     "check_build_id", "mxfp4a16_stage", "LogitsOperands", "logits_gemm", "head_bytes",
     "join_head", "split_head", "forget_head", "head_header", "RadEncoding", "RadEncPlane",
     "RadLayout", "RadPlanesHeader", "RadPlanesEntry", "head_encoding", "layout_head",
-    "relayout_head", "unrelayout_head",
+    "relayout_head", "unrelayout_head", "ext_rows", "ext_schemas", "QuantActI8Operands",
+    "GatedQuantI8Operands", "RmsNormQuantI8Operands", "quant_act_i8", "gated_quant_i8",
+    "rmsnorm_quant_i8",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -157,6 +159,12 @@ def lib():
         L.rad_kernel_count.restype = ctypes.c_int
         L.rad_kernel_at.restype = ctypes.POINTER(RadKernelInfo)
         L.rad_kernel_at.argtypes = [ctypes.c_int]
+        L.r3d_gfx950_ext_schema_count.restype = ctypes.c_int
+        L.r3d_gfx950_ext_schema_at.restype = ctypes.POINTER(RadOpSchema)
+        L.r3d_gfx950_ext_schema_at.argtypes = [ctypes.c_int]
+        L.r3d_gfx950_ext_kernel_count.restype = ctypes.c_int
+        L.r3d_gfx950_ext_kernel_at.restype = ctypes.POINTER(RadKernelInfo)
+        L.r3d_gfx950_ext_kernel_at.argtypes = [ctypes.c_int]
         for name in ("r3d_rad_gemm_nt_q", "r3d_rad_gemm_nt_q_mxfp4_decode",
                      "r3d_rad_gemm_nt_q_fp8", "r3d_rad_gemm_nt_q_fp8_decode"):
             fn = getattr(L, name)
@@ -233,10 +241,19 @@ def mxfp4a16_stage(ops, stage, stream=0):
 
 def rows():
     """The registered rows as dicts (after the registration-time kill switches)."""
-    L = lib()
+    return _rows(lib().rad_kernel_count(), lib().rad_kernel_at)
+
+
+def ext_rows():
+    """The rows of the second table (ops and encodings past the reference plugin's set), as
+    rows() gives them; resolve and the launches below look in both tables."""
+    return _rows(lib().r3d_gfx950_ext_kernel_count(), lib().r3d_gfx950_ext_kernel_at)
+
+
+def _rows(count, at):
     out = []
-    for i in range(L.rad_kernel_count()):
-        k = L.rad_kernel_at(i).contents
+    for i in range(count):
+        k = at(i).contents
         cons = [(_s(k.constraints[c].key), k.constraints[c].op, k.constraints[c].ival,
                  _s(k.constraints[c].sval)) for c in range(k.n_constraints)]
         tun = [_s(k.tunables[t].name) for t in range(k.n_tunables)]
@@ -248,10 +265,18 @@ def rows():
 
 
 def schemas():
-    L = lib()
+    return _schemas(lib().rad_kernel_schema_count(), lib().rad_kernel_schema_at)
+
+
+def ext_schemas():
+    """The op schemas of the second table."""
+    return _schemas(lib().r3d_gfx950_ext_schema_count(), lib().r3d_gfx950_ext_schema_at)
+
+
+def _schemas(count, at):
     out = []
-    for i in range(L.rad_kernel_schema_count()):
-        s = L.rad_kernel_schema_at(i).contents
+    for i in range(count):
+        s = at(i).contents
         out.append({
             "op": _s(s.op),
             "params": [(_s(s.params[j].key), s.params[j].kind, s.params[j].req)
@@ -285,7 +310,7 @@ def _holds(c, query):
 def resolve(op, query):
     """Highest-priority registered row of `op` whose constraints all hold, or None."""
     best = None
-    for r in rows():
+    for r in rows() + ext_rows():
         if r["op"] != op:
             continue
         if all(_holds(c, query) for c in r["constraints"]):
@@ -305,14 +330,17 @@ class GemmOperands:
     b_scale uint8 [N, K/32] E8M0 (mxfp4) or bf16/int16 [N or N/128, K/128] (fp8a8)
     y      bf16/int16 [M, N]
     scratch optional device tensor handed over as RadArgs::scratch (mxfp4a16)
+
+    i8a8: a int8 [M, K], a_scale float32 [M] or [M, 1], b int8 [N, K], b_scale float32 [N] or
+    [N, 1]; group is K.
     """
 
     def __init__(self, a, a_scale, b, b_scale, y, *, dtype, N, K, group=None, M=None,
                  a_sum=None, b_ref=None, extra_params=None, y_shape=None, tunables=None,
                  scratch=None):
-        mx = dtype in ("mxfp4a8", "mxfp4a16")
+        mx, i8 = dtype in ("mxfp4a8", "mxfp4a16"), dtype == "i8a8"
         self.dtype = dtype
-        group = group if group is not None else (32 if mx else 128)
+        group = group if group is not None else (32 if mx else K if i8 else 128)
         t = (RadTensor * 7)()
 
         def fill(i, x, dt, shape=None, stride=None):
@@ -332,17 +360,20 @@ class GemmOperands:
         # the launch reads raw pointers: hold the tensors so none is freed (and its memory
         # reused) while this object can still launch
         self._tensors = [a, a_scale, b, b_scale, y, a_sum, b_ref]
-        fused = a is not None and a_scale is None and a.element_size() == 2
-        fill(0, a, "BF16" if dtype == "mxfp4a16" or fused else "F8E4M3")
-        fill(1, a_scale, "F32")
+        fused = a is not None and a_scale is None and a.element_size() == 2 and not i8
+        fill(0, a, _type(a, "I8") if i8 else "BF16" if dtype == "mxfp4a16" or fused else "F8E4M3")
+        fill(1, a_scale, _type(a_scale, "F32") if i8 else "F32")
         if mx:
             # FP4 counts nibbles: [N, K] with strides {K, 1}
             fill(2, b, "FP4E2M1", [b.shape[0], b.shape[1] * 2], [b.stride(0) * 2, 1])
             fill(3, b_scale, "E8M0")
+        elif i8:
+            fill(2, b, _type(b, "I8"))
+            fill(3, b_scale, _type(b_scale, "F32"))
         else:
             fill(2, b, "F8E4M3")
             fill(3, b_scale, "BF16")
-        fill(4, y, "BF16", y_shape)
+        fill(4, y, _type(y, "BF16") if i8 else "BF16", y_shape)
         fill(5, a_sum, "F32")
         fill(6, b_ref, "BF16")
         self._t = t
@@ -504,6 +535,21 @@ def _elt(x, default="BF16"):
     return "F32" if str(x.dtype).endswith("float32") else default
 
 
+_TORCH_DT = {"float32": "F32", "bfloat16": "BF16", "int16": "BF16", "float16": "F16", "int8": "I8",
+             "uint8": "U8", "int32": "I32", "int64": "I64", "float8_e4m3fn": "F8E4M3"}
+
+
+def _type(x, default):
+    """The element type name that a tensor's own torch type stands for (int16 carries bf16 bits);
+    a row refuses one that is not its operand's.  `default` for an absent operand."""
+    if x is None:
+        return default
+    name = str(x.dtype).rsplit(".", 1)[-1]
+    if name not in _TORCH_DT:
+        raise TypeError("no element type stands for %s" % x.dtype)
+    return _TORCH_DT[name]
+
+
 class GatedQuantOperands(_Args):
     """One gated_quant_fp8 call (src/r3d_band.hip:492-541).
 
@@ -569,6 +615,47 @@ class GatedGemmOperands(_Args):
                          ([("M", M)] if M is not None else []))
         if scratch is not None:
             self.set_scratch(scratch)
+
+
+class QuantActI8Operands(_Args):
+    """One quant_act_i8 call: x float32 or bf16/int16 [M, n], q int8 [M, n] codes out, scale
+    float32 [M] or [M, 1] out."""
+
+    def __init__(self, x, q, scale, *, n, M=None):
+        ops = [(x, "BF16"), (q, "I8"), (scale, "F32")]
+        super().__init__([(t, _type(t, dt), None, None) for t, dt in ops],
+                         [("n", n), ("dtype", "f32" if _type(x, "") == "F32" else "bf16")] +
+                         ([("M", M)] if M is not None else []))
+
+
+class GatedQuantI8Operands(_Args):
+    """One gated_quant_i8 call: gate_up float32 or bf16/int16 [M, 2n] (gate columns, then up), q
+    int8 [M, n] and scale float32 [M] or [M, 1] out, out optional float32 or bf16/int16 [M, n]
+    (the values the codes are of), act "silu" (default when absent) or "sigmoid"."""
+
+    def __init__(self, gate_up, q, scale, out=None, *, n, act=None, M=None):
+        ops = [(gate_up, "BF16"), (q, "I8"), (scale, "F32"), (out, "BF16")]
+        super().__init__([(t, _type(t, dt), None, None) for t, dt in ops],
+                         [("n", n), ("dtype", "f32" if _type(gate_up, "") == "F32" else "bf16")] +
+                         ([("act", act)] if act is not None else []) +
+                         ([("M", M)] if M is not None else []))
+
+
+class RmsNormQuantI8Operands(_Args):
+    """One rmsnorm_quant_i8 call: x bf16/int16 [M, n], residual optional bf16/int16 [M, n] and
+    with it residual_out (bf16(residual + x); may be residual, the default, or x), w float32 or
+    bf16/int16 [n], q int8 [M, n] and scale float32 [M] or [M, 1] out, out optional float32 or
+    bf16/int16 [M, n] (the normed values)."""
+
+    def __init__(self, x, residual, w, q, scale, out=None, *, n, residual_out=None, eps=1e-6,
+                 wadd=None, M=None):
+        ro = residual if residual_out is None else residual_out
+        ops = [(x, "BF16"), (residual, "BF16"), (w, "BF16"), (q, "I8"), (scale, "F32"),
+               (out, "BF16"), (ro, "BF16")]
+        super().__init__([(t, _type(t, dt), None, None) for t, dt in ops],
+                         [("n", n), ("eps", float(eps)), ("dtype", "bf16")] +
+                         ([("wadd", float(wadd))] if wadd is not None else []) +
+                         ([("M", M)] if M is not None else []))
 
 
 class LogitsOperands(_Args):
@@ -750,9 +837,35 @@ def quant_act_fp8(x, q, scale, *, n, group=128, stream=None):
     return launch_row("quant_act_fp8_act", ops, stream)
 
 
+def _launch_on(row_name, ops, stream):
+    import torch
+    if stream is None:
+        stream = torch.cuda.current_stream().cuda_stream
+    return launch_row(row_name, ops, stream)
+
+
+def quant_act_i8(x, q, scale, *, n, stream=None):
+    """Launch the quant_act_i8 row on `stream` (default the current torch stream); its status."""
+    return _launch_on("quant_act_i8", QuantActI8Operands(x, q, scale, n=n), stream)
+
+
+def gated_quant_i8(gate_up, q, scale, out=None, *, n, act=None, stream=None):
+    """Launch the gated_quant_i8 row on `stream` (default the current torch stream); its status."""
+    return _launch_on("gated_quant_i8", GatedQuantI8Operands(gate_up, q, scale, out, n=n, act=act), stream)
+
+
+def rmsnorm_quant_i8(x, residual, w, q, scale, out=None, *, n, residual_out=None, eps=1e-6,
+                     wadd=None, stream=None):
+    """Launch the rmsnorm_quant_i8 row on `stream` (default the current torch stream); its
+    status."""
+    ops = RmsNormQuantI8Operands(x, residual, w, q, scale, out, n=n, residual_out=residual_out,
+                                 eps=eps, wadd=wadd)
+    return _launch_on("rmsnorm_quant_i8", ops, stream)
+
+
 def row_launcher(row_name):
     """The named row's launch pointer as a callable f(ops, stream) -> status."""
-    for r in rows():
+    for r in rows() + ext_rows():
         if r["name"] == row_name:
             fn = LaunchFn(r["launch"])
 
@@ -764,7 +877,7 @@ def row_launcher(row_name):
 
 def row_scratch_bytes(row_name, ops):
     """The named row's scratch hook on `ops` (bytes; 0 when the row has no hook)."""
-    for r in rows():
+    for r in rows() + ext_rows():
         if r["name"] == row_name:
             if not r.get("scratch"):
                 return 0
@@ -792,7 +905,8 @@ def gemm_nt_q(a, a_scale, b, b_scale, y, *, dtype, N, K, group=None, stream=None
     M = y.numel() // N
     if row is None:
         r = resolve("gemm_nt_q", {"dtype": dtype, "M": M, "N": N, "K": K,
-                                  "group": group if group is not None else (32 if dtype == "mxfp4a8" else 128)})
+                                  "group": group if group is not None else
+                                  {"mxfp4a8": 32, "i8a8": K}.get(dtype, 128)})
         if r is None:
             return RAD_E_UNSUPPORTED, None
         row = r["name"]

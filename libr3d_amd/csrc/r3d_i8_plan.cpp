@@ -1,0 +1,210 @@
+/* r3d_i8_plan.cpp -- host plans of the int8 rows (see r3d_i8.h). */
+#include "r3d_i8.h"
+
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+
+#include "rad_plugin.h"
+#include "r3d_plan.h"
+
+namespace r3d {
+
+static const int64_t kDimMax = 0x7FFFFFFLL;
+
+static bool pitch_ok(int64_t p) { return p >= 0 && p <= (int64_t(1) << 40); }
+
+/* One f32 a row: rank 1 [rows], or rank 2 [rows, 1]; the stride may be 0 (one scale for all). */
+static int scale_column(const RadTensor* t, int64_t rows, int64_t* stride) {
+    if (t->dtype != RAD_F32) return RAD_E_UNSUPPORTED;
+    if ((t->rank != 1 && t->rank != 2) || (t->rank == 2 && t->shape[1] != 1)) return RAD_E_SHAPE;
+    if (t->shape[0] < rows) return RAD_E_SHAPE;
+    *stride = t->stride[0];
+    return pitch_ok(*stride) ? RAD_OK : RAD_E_STRIDE;
+}
+
+/* The pitch of a [rows, cols] operand whose rows lie anywhere: rank 2 with its own row stride,
+ * or higher ranks whose outer axes are dense; rank 1 is one row. */
+static int rows_of(const RadTensor* t, int64_t rows, int64_t cols, int64_t* pitch) {
+    const long long n = rad_tensor_numel(t);
+    if (n < 0 || rows > INT64_MAX / cols || n < rows * cols) return RAD_E_SHAPE;
+    if (t->rank == 1) {
+        if (rows != 1 || n != cols) return RAD_E_SHAPE;
+        if (t->stride[0] != 1) return RAD_E_STRIDE;
+        *pitch = cols;
+        return RAD_OK;
+    }
+    if (t->rank < 2 || t->shape[t->rank - 1] != cols) return RAD_E_SHAPE;
+    if (t->stride[t->rank - 1] != 1) return RAD_E_STRIDE;
+    for (int i = 0; i + 2 < (int)t->rank; ++i) {
+        int64_t span = 0;
+        if (__builtin_mul_overflow(t->shape[i + 1], t->stride[i + 1], &span) || t->stride[i] != span)
+            return RAD_E_STRIDE;
+    }
+    *pitch = t->stride[t->rank - 2];
+    return pitch_ok(*pitch) ? RAD_OK : RAD_E_STRIDE;
+}
+
+int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
+    const RadTensor* A  = rad_arg_in(a, 0);
+    const RadTensor* AS = rad_arg_in(a, 1);
+    const RadTensor* B  = rad_arg_in(a, 2);
+    const RadTensor* BS = rad_arg_in(a, 3);
+    const RadTensor* Y  = rad_arg_in(a, 4);
+    if (!A || !AS || !B || !BS || !Y) return RAD_E_UNSUPPORTED;
+    if (rad_arg_in(a, 5) || rad_arg_in(a, 6)) return RAD_E_UNSUPPORTED;   /* symmetric codes only */
+    const char* dtype = rad_args_gets(a, "dtype");
+    if (!dtype || strcmp(dtype, "i8a8") != 0) return RAD_E_UNSUPPORTED;
+    long long v = 0;
+    if (rad_args_geti(a, "pb1", &v) && v > 0) return RAD_E_UNSUPPORTED;
+    if (rad_args_geti(a, "pb2", &v) && v > 0) return RAD_E_UNSUPPORTED;
+    if (A->dtype != RAD_I8 || B->dtype != RAD_I8 || Y->dtype != RAD_BF16) return RAD_E_UNSUPPORTED;
+    long long N = 0, K = 0;
+    if (!rad_args_geti(a, "N", &N) || !rad_args_geti(a, "K", &K)) return RAD_E_SHAPE;
+    if (N <= 0 || K <= 0 || N > kDimMax) return RAD_E_SHAPE;
+    if (K > kI8MaxK) return RAD_E_UNSUPPORTED;                  /* the sum could leave i32 */
+    const long long yn = rad_tensor_numel(Y);
+    if (yn <= 0 || yn % N) return RAD_E_SHAPE;
+    const int64_t M = yn / N;
+    if (M > kDimMax) return RAD_E_SHAPE;
+    if (m_max > 0 && M > m_max) return RAD_E_UNSUPPORTED;       /* the band's own bound */
+    /* one scale a row of K: a group that says otherwise contradicts the scales */
+    if (rad_args_geti(a, "group", &v) && v > 0 && v != K) return RAD_E_SHAPE;
+    int rc = scale_column(AS, M, &P->sa_stride);
+    if (!rc) rc = scale_column(BS, N, &P->sb_stride);
+    if (!rc) rc = rows_of(A, M, K, &P->a_pitch);
+    if (!rc) rc = rows_of(B, N, K, &P->b_pitch);
+    if (!rc) rc = rows_of(Y, M, N, &P->y_pitch);
+    if (rc) return rc;
+    if (P->y_pitch < N && M > 1) return RAD_E_STRIDE;           /* rows of Y overlap */
+    if (((uintptr_t)AS->data | (uintptr_t)BS->data) & 3 || (uintptr_t)Y->data & 1)
+        return RAD_E_STRIDE;
+    /* every kernel's least: 16 rows under 32-bit offsets */
+    if ((M > 1 && P->a_pitch > (1 << 26)) || (N > 1 && P->b_pitch > (1 << 26)))
+        return RAD_E_UNSUPPORTED;
+    P->A = (const uint8_t*)A->data;
+    P->SA = (const float*)AS->data;
+    P->B = (const uint8_t*)B->data;
+    P->SB = (const float*)BS->data;
+    P->Y = (uint16_t*)Y->data;
+    P->M = M;
+    P->N = N;
+    P->K = K;
+    /* the fast kernels move 16 bytes a lane and walk 256 rows with 32-bit offsets */
+    P->ua = (K & 15) || (((uintptr_t)P->A | (uintptr_t)P->B) & 15) ||
+            ((P->a_pitch | P->b_pitch) & 15) || P->a_pitch > (1 << 22) || P->b_pitch > (1 << 22);
+    return RAD_OK;
+}
+
+int plan_i8_band(const RadArgs* a, int op, I8BandPlan* P) {
+    /* operands: x, q, scale (quant); gate_up, q, scale, out? (gated);
+     * x, residual?, w, q, scale, out?, residual_out? (rmsnorm) */
+    const bool norm = op == I8_NORM;
+    const int iq = norm ? 3 : 1;
+    const RadTensor* x  = rad_arg_in(a, 0);
+    const RadTensor* rs = norm ? rad_arg_in(a, 1) : nullptr;
+    const RadTensor* w  = norm ? rad_arg_in(a, 2) : nullptr;
+    const RadTensor* q  = rad_arg_in(a, iq);
+    const RadTensor* sc = rad_arg_in(a, iq + 1);
+    const RadTensor* ob = op == I8_QUANT ? nullptr : rad_arg_in(a, iq + 2);
+    const RadTensor* ro = norm ? rad_arg_in(a, 6) : nullptr;
+    if (!x || !q || !sc || (norm && !w) || (rs == nullptr) != (ro == nullptr)) return RAD_E_INVAL;
+    if (x->dtype != RAD_BF16 && (norm || x->dtype != RAD_F32)) return RAD_E_DTYPE;
+    if (q->dtype != RAD_I8 || sc->dtype != RAD_F32) return RAD_E_DTYPE;
+    if (ob && ob->dtype != RAD_F32 && ob->dtype != RAD_BF16) return RAD_E_DTYPE;
+    if (norm && w->dtype != RAD_F32 && w->dtype != RAD_BF16) return RAD_E_DTYPE;
+    if (rs && (rs->dtype != RAD_BF16 || ro->dtype != RAD_BF16)) return RAD_E_DTYPE;
+    const char* dt = rad_args_gets(a, "dtype");            /* names x's type, if given */
+    if (dt && strcmp(dt, x->dtype == RAD_BF16 ? "bf16" : "f32") != 0) return RAD_E_DTYPE;
+    const int64_t per = op == I8_GATED ? 2 : 1;
+    long long v = 0;
+    if (!rad_args_geti(a, "n", &v) || v <= 0 || v > kDimMax) return RAD_E_SHAPE;
+    const int64_t n = v;
+    const long long xn = rad_tensor_numel(x);
+    if (xn <= 0 || xn % (per * n)) return RAD_E_SHAPE;
+    const int64_t rows = xn / (per * n);
+    if (rows > 0x7FFFFFFF) return RAD_E_SHAPE;
+    const char* act = rad_args_gets(a, "act");
+    if (op == I8_GATED && act && strcmp(act, "silu") != 0 && strcmp(act, "sigmoid") != 0)
+        return RAD_E_UNSUPPORTED;
+    P->silu = !act || strcmp(act, "silu") == 0;
+    int rc = rows_of(x, rows, per * n, &P->x_pitch);
+    if (!rc) rc = rows_of(q, rows, n, &P->q_pitch);
+    if (!rc) {
+        rc = scale_column(sc, rows, &P->s_stride);
+        if (rc == RAD_E_UNSUPPORTED) rc = RAD_E_DTYPE;
+    }
+    if (!rc && ob) rc = rows_of(ob, rows, n, &P->ob_pitch);
+    if (!rc && rs) rc = rows_of(rs, rows, n, &P->r_pitch);
+    if (!rc && ro) rc = rows_of(ro, rows, n, &P->ro_pitch);
+    if (rc) return rc;
+    if (norm && (rad_tensor_numel(w) != n || w->rank != 1)) return RAD_E_SHAPE;
+    if (norm && w->stride[0] != 1) return RAD_E_STRIDE;
+    /* outputs whose rows overlap would race */
+    if (rows > 1 && (P->q_pitch < n || P->s_stride < 1 || (ob && P->ob_pitch < n) ||
+                     (ro && P->ro_pitch < n)))
+        return RAD_E_STRIDE;
+    /* elements lie on their own alignment; nothing more is asked of any operand */
+    auto off = [](const RadTensor* t) {
+        return t && ((uintptr_t)t->data & (t->dtype == RAD_F32 ? 3 : t->dtype == RAD_BF16 ? 1 : 0));
+    };
+    if (off(x) || off(rs) || off(w) || off(sc) || off(ob) || off(ro)) return RAD_E_STRIDE;
+    P->x = (const uint8_t*)x->data;
+    P->res = rs ? (const uint8_t*)rs->data : nullptr;
+    P->res_out = ro ? (uint8_t*)ro->data : nullptr;
+    P->w = w ? (const uint8_t*)w->data : nullptr;
+    P->q = (uint8_t*)q->data;
+    P->scale = (float*)sc->data;
+    P->ob = ob ? (uint8_t*)ob->data : nullptr;
+    P->x_bf16 = x->dtype == RAD_BF16;
+    P->w_bf16 = w && w->dtype == RAD_BF16;
+    P->ob_bf16 = ob && ob->dtype == RAD_BF16;
+    P->rows = rows;
+    P->n = n;
+    P->eps = rad_args_getf_or(a, "eps", 1e-6);
+    P->wadd = (float)rad_args_getf_or(a, "wadd", 0.0);
+    if (!(P->eps >= 0.0)) return RAD_E_INVAL;
+    return RAD_OK;
+}
+
+I8BandGeom i8_band_geom(int64_t rows, int64_t n) {
+    const int64_t nc = (n + 7) / 8;
+    const bool few = rows <= 512;
+    for (int c = 1; c <= 4; ++c)
+        for (int lanes = 64; lanes <= 1024; lanes *= 2) {
+            if ((int64_t)lanes * c < nc) continue;
+            /* few rows: one chunk a lane while 1024 lanes hold the row; many rows: 256 lanes
+             * (several rows a compute unit) while three chunks a lane hold it */
+            if (!few && lanes > 256 && c < 3) break;
+            return I8BandGeom{lanes, c};
+        }
+    return I8BandGeom{1024, 0};
+}
+
+int describe_i8(const char* row, const RadArgs* a, char* buf, int len) {
+    const bool gemm = !strcmp(row, "gemm_nt_q_i8a8"), dec = !strcmp(row, "gemm_nt_q_i8a8_decode");
+    if (gemm || dec) {
+        I8Plan P{};
+        const int rc = plan_i8(a, dec ? 16 : 0, &P);
+        if (rc) { snprintf(buf, (size_t)len, "refused rc=%d (plan)", rc); return rc; }
+        snprintf(buf, (size_t)len, "arm=%s enc=i8a8 M=%lld N=%lld K=%lld", "any", (long long)P.M,
+                 (long long)P.N, (long long)P.K);
+        return RAD_OK;
+    }
+    const int op = !strcmp(row, "quant_act_i8") ? I8_QUANT : !strcmp(row, "gated_quant_i8") ? I8_GATED
+                 : !strcmp(row, "rmsnorm_quant_i8") ? I8_NORM : -1;
+    if (op < 0) return -1;
+    I8BandPlan P{};
+    const int rc = plan_i8_band(a, op, &P);
+    if (rc) { snprintf(buf, (size_t)len, "refused rc=%d (plan)", rc); return rc; }
+    const I8BandGeom g = i8_band_geom(P.rows, P.n);
+    snprintf(buf, (size_t)len, "arm=band op=%s x=%s rows=%lld n=%lld lanes=%d chunks=%d residual=%d "
+             "ob=%s", row, P.x_bf16 ? "bf16" : "f32", (long long)P.rows, (long long)P.n, g.lanes,
+             g.chunks, P.res != nullptr, P.ob ? (P.ob_bf16 ? "bf16" : "f32") : "none");
+    return RAD_OK;
+}
+
+bool env_no_i8()     { static const bool v = getenv("R3D_NO_I8") != nullptr;     return v; }
+bool env_no_i8_dec() { static const bool v = getenv("R3D_NO_I8_DEC") != nullptr; return v; }
+
+}  // namespace r3d
