@@ -32,6 +32,34 @@ struct I8Plan {
 /* The operands and params of a gemm_nt_q call at i8a8; m_max: the row's bound on M (0: none). */
 int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P);
 
+/* Which kernel a call takes, and its launch. */
+enum { I8_ANY = 0, I8_GEMV = 1, I8_TILE = 2 };
+enum { I8_T_256x256, I8_T_128x256, I8_T_128x128, I8_T_128x64, I8_T_64x64, I8_T_64x32, I8_TILES };
+
+struct I8Geom {
+    int arm;
+    int tile;                /* I8_TILE: one of the above (weight rows x tokens) */
+    int bn, bm;
+    int64_t tiles;
+    int kc;                  /* K chunks: waves of a workgroup (GEMV), or workgroups with an i32
+                                plane each in scratch (tiles, kc > 1) */
+    int per;                 /* 128-wide K steps a chunk */
+    int waves;               /* GEMV: waves a workgroup */
+    int64_t blocks;          /* workgroups */
+};
+
+/* GEMV: the tokens in LDS, rows this many bytes apart */
+constexpr int64_t i8_gemv_row(int64_t K) { return ((K + 127) & ~(int64_t)127) + 16; }
+/* and at most this much of it.  Up to it the GEMV takes 0.65 to 0.98 of the tiles' time (M 1..8, 430
+ * shapes, by M and 8 KB of tokens); with 56 KB and more, two workgroups a compute unit, 1.05 to 1.4 */
+constexpr int64_t kI8GemvLds = 48 * 1024;
+
+/* The launch that suits a shape on ncu compute units, with at most `scratch` bytes for planes. */
+void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g);
+
+/* The planes that a call's best launch wants: kc M N 4 bytes, 0 for none (the row's scratch hook). */
+int64_t i8_scratch_bytes(const RadArgs* a, int ncu);
+
 /* Codes out of a band producer, one scale a row. */
 struct I8BandPlan {
     const uint8_t* x;        /* the activation, or gate_up [rows, 2n] */

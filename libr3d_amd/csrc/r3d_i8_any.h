@@ -16,6 +16,11 @@
 
 namespace r3d {
 
+/* A value that is the same on every lane, as such: the quotient of two of them is computed on the
+ * vector unit, and a buffer resource made from one of its lanes' values would be loaded in a loop
+ * over the lanes. */
+__device__ __forceinline__ int i8_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 /* (f32(sum) * a_scale) * b_scale, the epilogue of every i8a8 kernel */
 __device__ __forceinline__ float i8_out(int sum, float sa, float sb) {
     return __fmul_rn(__fmul_rn((float)sum, sa), sb);

@@ -96,6 +96,102 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
     return RAD_OK;
 }
 
+/* What a launch of a tile takes, in ns: least squares over 2426 shapes (M 5..2048, N 512..21504, K
+ * 512..21504) and 4 to 40 launches of each, rows starting on 128-byte lines or not; the pick is 2.8 %
+ * slower than the best of 17 tiles on average (geometric), 10 % at the ninth decile.
+ *     a + max(ceil(units / ncu) * q * steps a unit, weights / rate) + the planes and their sum
+ * rate: 5.2 TB/s, or what the units in flight stream, `one` bytes a us each where every weight byte
+ * comes from memory (one tile of tokens), `more` where tiles of tokens share them in L2.  K off 128
+ * starts rows inside lines, and a step of 128 bytes then takes two lines: q * mis / 100. */
+struct I8Cost {
+    int bn, bm, resident;    /* workgroups a compute unit holds (LDS) */
+    int a, q, mis, one, more;
+};
+static const I8Cost kI8Cost[I8_TILES] = {
+    {256, 256, 1, 8107, 1065, 119, 30500, 48300},
+    {128, 256, 1, 4835,  888, 120, 48300, 30600},
+    {128, 128, 1, 4312,  474, 126, 46300, 18800},
+    {128,  64, 1, 3351,  398, 123, 59300, 49200},
+    { 64,  64, 2, 3147,  246, 120, 27400, 30500},
+    { 64,  32, 2, 2896,  202, 111, 42700, 28700},
+};
+
+static int64_t i8_tile_ns(const I8Cost& c, int64_t M, int64_t N, int64_t K, int64_t per, int64_t kc,
+                          int ncu) {
+    const int64_t gm = (M + c.bm - 1) / c.bm, units = (N + c.bn - 1) / c.bn * gm * kc;
+    const int64_t work = (units + ncu - 1) / ncu * c.q * per * (K % 128 ? c.mis : 100) / 100;
+    const int64_t busy = units < c.resident * ncu ? units : c.resident * ncu;
+    int64_t rate = busy * (gm == 1 ? c.one : c.more);               /* bytes a us */
+    if (rate > 5200000) rate = 5200000;
+    const int64_t stream = N * K * 1000 / rate;
+    return c.a + (work > stream ? work : stream) + (kc > 1 ? 2390 + kc * M * N * 18 / 10000 : 0);
+}
+
+constexpr int64_t kI8MaxPlanes = (int64_t)1 << 28;                 /* bytes of planes, at most */
+
+void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
+    *g = I8Geom{};
+    if (P.ua) return;
+    if (ncu <= 0) ncu = 256;
+    const int64_t steps = (P.K + 127) / 128;
+    if (P.M <= 8 && P.M * i8_gemv_row(P.K) <= kI8GemvLds) {
+        /* 8 weight rows a wave; K over waves until about 1600 of them stream (the K chunks of a row
+         * block are waves of one workgroup), two lines a wave at least */
+        const int64_t rows = (P.N + 7) / 8;
+        int kc = 1;
+        while (kc < 8 && rows * kc < 1600 && steps / (2 * kc) >= 2) kc *= 2;
+        g->arm = I8_GEMV;
+        g->bn = 8;
+        g->bm = 8;
+        g->tiles = rows;
+        g->kc = kc;
+        g->per = (int)((steps + kc - 1) / kc);
+        g->waves = kc > 4 ? kc : 4;
+        g->blocks = (rows + g->waves / kc - 1) / (g->waves / kc);
+        return;
+    }
+    int64_t best = 0;
+    for (int t = 0; t < I8_TILES; ++t) {
+        const I8Cost& c = kI8Cost[t];
+        const int64_t tiles = (P.N + c.bn - 1) / c.bn * ((P.M + c.bm - 1) / c.bm);
+        for (int64_t kc : {1, 2, 3, 4, 5, 6, 8, 12, 16, 24}) {
+            if (kc > 1 && steps / kc < 3) break;
+            const int64_t per = (steps + kc - 1) / kc;
+            if ((steps + per - 1) / per != kc || tiles * kc > 0x7FFFFFFF) continue;
+            if (kc > 1 && (tiles * kc > 4 * ncu || kc * P.M * P.N * 4 > scratch)) break;
+            const int64_t ns = i8_tile_ns(c, P.M, P.N, P.K, per, kc, ncu);
+            if (best && ns >= best) continue;
+            best = ns;
+            g->arm = I8_TILE;
+            g->tile = t;
+            g->bn = c.bn;
+            g->bm = c.bm;
+            g->tiles = tiles;
+            g->kc = (int)kc;
+            g->per = (int)per;
+            g->blocks = tiles * kc;
+        }
+    }
+}
+
+int64_t i8_scratch_bytes(const RadArgs* a, int ncu) {
+    I8Plan P{};
+    long long N = 0, K = 0, M = 0;
+    if (!rad_args_geti(a, "N", &N) || !rad_args_geti(a, "K", &K) || N <= 0 || K <= 0 || N > kDimMax ||
+        K > kI8MaxK)
+        return 0;
+    const RadTensor* Y = rad_arg_in(a, 4);
+    if (Y) M = rad_tensor_numel(Y) / N;
+    else if (!rad_args_geti(a, "M", &M)) M = 128;
+    if (M <= 0 || M > kDimMax || (K & 15)) return 0;
+    P.M = M;
+    P.N = N;
+    P.K = K;
+    I8Geom g;
+    i8_geom(P, ncu, kI8MaxPlanes, &g);
+    return g.arm == I8_TILE && g.kc > 1 ? (int64_t)g.kc * M * N * 4 : 0;
+}
+
 int plan_i8_band(const RadArgs* a, int op, I8BandPlan* P) {
     /* operands: x, q, scale (quant); gate_up, q, scale, out? (gated);
      * x, residual?, w, q, scale, out?, residual_out? (rmsnorm) */
@@ -187,8 +283,14 @@ int describe_i8(const char* row, const RadArgs* a, char* buf, int len) {
         I8Plan P{};
         const int rc = plan_i8(a, dec ? 16 : 0, &P);
         if (rc) { snprintf(buf, (size_t)len, "refused rc=%d (plan)", rc); return rc; }
-        snprintf(buf, (size_t)len, "arm=%s enc=i8a8 M=%lld N=%lld K=%lld", "any", (long long)P.M,
-                 (long long)P.N, (long long)P.K);
+        I8Geom g;
+        const bool sc = a->scratch && ((uintptr_t)a->scratch & 15) == 0;
+        i8_geom(P, 256, sc ? a->scratch_bytes : 0, &g);
+        static const char* kArm[] = {"any", "gemv", "tile"};
+        snprintf(buf, (size_t)len, "arm=%s enc=i8a8 M=%lld N=%lld K=%lld bn=%d bm=%d tiles=%lld kc=%d "
+                 "per=%d waves=%d blocks=%lld", kArm[g.arm], (long long)P.M, (long long)P.N,
+                 (long long)P.K, g.bn, g.bm, (long long)g.tiles, g.kc, g.per, g.waves,
+                 (long long)g.blocks);
         return RAD_OK;
     }
     const int op = !strcmp(row, "quant_act_i8") ? I8_QUANT : !strcmp(row, "gated_quant_i8") ? I8_GATED

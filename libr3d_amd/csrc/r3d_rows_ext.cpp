@@ -21,6 +21,7 @@
 extern "C" {
 int r3d_rad_gemm_nt_q_i8(const RadArgs* a, RadStream s);
 int r3d_rad_gemm_nt_q_i8_decode(const RadArgs* a, RadStream s);
+int64_t r3d_rad_gemm_nt_q_i8_scratch(const RadArgs* a);
 int r3d_rad_quant_act_i8(const RadArgs* a, RadStream s);
 int r3d_rad_gated_quant_i8(const RadArgs* a, RadStream s);
 int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
@@ -98,20 +99,22 @@ enum { kPrioTile = 1000, kPrioDecode = 1100 };
 
 const RadKernelInfo kRows[] = {
     {"gemm_nt_q_i8a8", "gemm_nt_q", "gemm",
-     "int8 GEMM on gfx950 matrix cores (v_mfma_i32_16x16x64_i8), summed exactly in i32, one scale "
-     "a token and one an output channel applied once",
+     "int8 GEMM on gfx950 matrix cores: LDS tiles of 64 x 32 to 256 x 256 (a GEMV up to M = 8), summed "
+     "exactly in i32, one scale a token and one an output channel applied once; K split over "
+     "workgroups into i32 planes in launch scratch where tiles leave compute units idle",
      "K up to 131071 (the sum stays in i32); operands at any alignment and pitch (K, bases and "
-     "pitches off 16 bytes: dword loads); M derives from numel(y)/N",
+     "pitches off 16 bytes: dword loads); M derives from numel(y)/N; scratch optional",
      "int8 a with f32 a_scale [M] or [M, 1], int8 b with f32 b_scale [N] or [N, 1], bf16 y; a_sum "
      "and b_ref refused",
      RAD_DOMAIN_DEVICE, kPrioTile, cI8, 1, nullptr, 0, nullptr, nullptr, nullptr,
-     r3d_rad_gemm_nt_q_i8, nullptr, nullptr, nullptr, nullptr, nullptr},
+     r3d_rad_gemm_nt_q_i8, r3d_rad_gemm_nt_q_i8_scratch, nullptr, nullptr, nullptr, nullptr},
     {"gemm_nt_q_i8a8_decode", "gemm_nt_q", "gemm",
-     "int8 decode-band GEMV on gfx950 matrix cores",
+     "int8 decode-band product on gfx950 matrix cores: up to M = 8 a wave 8 weight rows, whole lines "
+     "from memory to registers, the tokens in LDS; above, or with long tokens, LDS tiles",
      "M <= 16; else as gemm_nt_q_i8a8",
      "as gemm_nt_q_i8a8",
      RAD_DOMAIN_DEVICE, kPrioDecode, cI8Decode, 2, nullptr, 0, nullptr, nullptr, nullptr,
-     r3d_rad_gemm_nt_q_i8_decode, nullptr, nullptr, nullptr, nullptr, nullptr},
+     r3d_rad_gemm_nt_q_i8_decode, r3d_rad_gemm_nt_q_i8_scratch, nullptr, nullptr, nullptr, nullptr},
     {"quant_act_i8", "quant_act_i8", "band",
      "int8 quantisation with one scale a row: a workgroup a row, the row in registers",
      "any n, alignment and pitch; rows past 32768 elements are walked twice",
