@@ -230,10 +230,10 @@ int r3d_gfx950_mfma_valu_probe(int nv, int lag3, int iters, void* work, int64_t*
                                RadStream s);
 
 /* The second row table, with no counterpart in the reference: rows of ops and encodings past the
- * set that radiance's other plugins declare (int8: gemm_nt_q at i8a8 and its producers), in the
- * same structures, resolved and launched the same way.  A loader compares the schemas of
+ * set that radiance's other plugins declare (int8: gemm_nt_q at i8a8 and its producers; a
+ * sampler), in the same structures, resolved and launched the same way.  A loader compares the schemas of
  * rad_kernel_schema_at with other plugins', so these are listed apart; an engine that knows the ops
- * reads them here.  R3D_NO_I8 and R3D_NO_I8_DEC hide rows at registration.  gemm_nt_q's schema is
+ * reads them here.  R3D_NO_I8, R3D_NO_I8_DEC and R3D_NO_SAMPLE hide rows at registration.  gemm_nt_q's schema is
  * rad_kernel_schema_at's. */
 int r3d_gfx950_ext_schema_count(void);
 const RadOpSchema* r3d_gfx950_ext_schema_at(int i);
@@ -269,6 +269,20 @@ int64_t r3d_rad_gemm_nt_q_i8_scratch(const RadArgs* a);
 int r3d_rad_quant_act_i8(const RadArgs* a, RadStream s);
 int r3d_rad_gated_quant_i8(const RadArgs* a, RadStream s);
 int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
+
+/* sample_logits: one token a row.  Operands (logits f32/bf16 [M, n_vocab], u f32, temperature? f32,
+ * top_k? i32, top_p? f32, min_p? f32, token i32 out, prob? f32 out), the latter seven [M] or [M, 1],
+ * inputs with a stride of 0 for one value for all rows; params n_vocab, dtype (the logits'); M =
+ * numel(logits) / n_vocab.  In order: softmax at the temperature (<= 0: the lowest index of the
+ * maximum), top_k (<= 0: off; ties to the lowest index), top_p of those (>= 1: off; at least one
+ * token), min_p of those (times the largest probability; <= 0: off), then the first kept token in
+ * index order whose running mass passes u times the kept mass.  NaN and -inf logits are not there;
+ * a row of them gives token -1, prob 0.  n_vocab <= 4194304, M <= 65535.  Launch scratch of the size
+ * the hook gives, 16-byte aligned, is required (else RAD_E_UNSUPPORTED); calls that share it are
+ * ordered on one stream.  RAD_E_INVAL / RAD_E_DTYPE / RAD_E_SHAPE / RAD_E_STRIDE for refused operands,
+ * RAD_E_DEVICE for a failed launch.  Asynchronous on `s`; results do not depend on the run. */
+int r3d_rad_sample_logits(const RadArgs* a, RadStream s);
+int64_t r3d_rad_sample_logits_scratch(const RadArgs* a);
 
 /* Build identity with no counterpart in the reference: the SHA-256 (hex) of the compile
  * flags and of the sources this library was compiled from -- the flags as one line, then

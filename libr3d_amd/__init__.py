@@ -25,7 +25,7 @@ __all__ = [
     "RadLayout", "RadPlanesHeader", "RadPlanesEntry", "head_encoding", "layout_head",
     "relayout_head", "unrelayout_head", "ext_rows", "ext_schemas", "QuantActI8Operands",
     "GatedQuantI8Operands", "RmsNormQuantI8Operands", "quant_act_i8", "gated_quant_i8",
-    "rmsnorm_quant_i8",
+    "rmsnorm_quant_i8", "SampleOperands", "sample_logits",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -675,6 +675,28 @@ class LogitsOperands(_Args):
                           ("n_vocab", n_vocab), ("n_embd", n_embd), ("dtype", dtype)])
 
 
+class SampleOperands(_Args):
+    """One sample_logits call.
+
+    logits      float32 or bf16/int16 [M, n_vocab]
+    u           float32 [M] or [M, 1], uniform in [0, 1)
+    token       int32 [M] or [M, 1] out (-1: the row has no token)
+    prob        optional float32 [M] or [M, 1] out: the token's share of the kept mass
+    temperature, top_p, min_p   optional float32 [M] or [M, 1]; top_k optional int32 (a stride of 0
+                gives every row the same); absent, top_k <= 0, top_p >= 1 and min_p <= 0: no cut;
+                temperature <= 0: the lowest index of the maximum
+    The launch needs scratch of row_scratch_bytes("sample_logits", ops) bytes (set_scratch).
+    """
+
+    def __init__(self, logits, u, token, prob=None, *, n_vocab, temperature=None, top_k=None,
+                 top_p=None, min_p=None, M=None):
+        ops = [(logits, "F32"), (u, "F32"), (temperature, "F32"), (top_k, "I32"), (top_p, "F32"),
+               (min_p, "F32"), (token, "I32"), (prob, "F32")]
+        super().__init__([(t, _type(t, dt), None, None) for t, dt in ops],
+                         [("n_vocab", n_vocab), ("dtype", "bf16" if _type(logits, "") == "BF16" else "f32")] +
+                         ([("M", M)] if M is not None else []))
+
+
 _SCALE_DT = {"bf16": "BF16", "f16": "F16", "f32": "F32"}
 
 
@@ -861,6 +883,22 @@ def rmsnorm_quant_i8(x, residual, w, q, scale, out=None, *, n, residual_out=None
     ops = RmsNormQuantI8Operands(x, residual, w, q, scale, out, n=n, residual_out=residual_out,
                                  eps=eps, wadd=wadd)
     return _launch_on("rmsnorm_quant_i8", ops, stream)
+
+
+def sample_logits(logits, u, token, prob=None, *, n_vocab, temperature=None, top_k=None, top_p=None,
+                  min_p=None, stream=None):
+    """Launch the sample_logits row on `stream` (a raw hipStream_t int, default the current torch
+    stream), with launch scratch of the size its hook asks for; its status."""
+    import torch
+    ops = SampleOperands(logits, u, token, prob, n_vocab=n_vocab, temperature=temperature, top_k=top_k,
+                         top_p=top_p, min_p=min_p)
+    need = row_scratch_bytes("sample_logits", ops)
+    if need > 0:
+        # from the launch stream's pool, as gemm_nt_q's: freed on return
+        own = None if stream is None else torch.cuda.ExternalStream(stream, device=logits.device)
+        with torch.cuda.stream(own):
+            ops.set_scratch(torch.empty(need, dtype=torch.uint8, device=logits.device), need)
+    return _launch_on("sample_logits", ops, stream)
 
 
 def row_launcher(row_name):

@@ -8,6 +8,7 @@
 #include "rad_planes.h"
 #include "rad_plugin.h"
 #include "r3d_i8.h"
+#include "r3d_sample.h"
 #include "r3d_gemv_layout.h"
 #include "r3d_prefill_layout.h"
 
@@ -1455,6 +1456,7 @@ int64_t decode_splitk(const RadArgs* a) {
 int describe(const char* row, const RadArgs* a, char* buf, int len) {
     if (!row || !buf || len <= 0) return RAD_E_INVAL;
     if (const int rc = describe_i8(row, a, buf, len); rc >= 0) return rc;
+    if (const int rc = describe_sample(row, a, buf, len); rc >= 0) return rc;
     if (strstr(row, "quant_act_fp8") != nullptr) {
         QuantPlan Q{};
         const int rc = plan_quant_act_fp8(a, &Q);

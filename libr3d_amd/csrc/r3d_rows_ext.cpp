@@ -9,14 +9,16 @@
  *   quant_act_i8             prio 1000  n GE 1, dtype IN f32 bf16           activation producer
  *   gated_quant_i8           prio 1000  n GE 1, dtype IN f32 bf16           gated producer
  *   rmsnorm_quant_i8         prio 1000  n GE 1, dtype IN bf16               norm producer
+ *   sample_logits            prio 1000  n_vocab GE 1, dtype IN f32 bf16     sampler
  *
- * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row (presence-tested, read once;
- * hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row, R3D_NO_SAMPLE the
+ * sampler (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
 #include "rad_abi.h"
 #include "r3d_i8.h"
+#include "r3d_sample.h"
 
 extern "C" {
 int r3d_rad_gemm_nt_q_i8(const RadArgs* a, RadStream s);
@@ -25,6 +27,8 @@ int64_t r3d_rad_gemm_nt_q_i8_scratch(const RadArgs* a);
 int r3d_rad_quant_act_i8(const RadArgs* a, RadStream s);
 int r3d_rad_gated_quant_i8(const RadArgs* a, RadStream s);
 int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
+int r3d_rad_sample_logits(const RadArgs* a, RadStream s);
+int64_t r3d_rad_sample_logits_scratch(const RadArgs* a);
 }
 
 namespace {
@@ -68,6 +72,22 @@ const RadOperandSpec kNormOperands[] = {
     {"residual_out", RAD_OPD_OUT, 1},
 };
 
+const RadParamSpec kSampleParams[] = {
+    {"M", RAD_P_INT, RAD_REQUIRED, 0},
+    {"n_vocab", RAD_P_INT, RAD_REQUIRED, 0},
+    {"dtype", RAD_P_STR, RAD_REQUIRED, 0},
+};
+const RadOperandSpec kSampleOperands[] = {
+    {"logits", RAD_OPD_IN, 0},
+    {"u", RAD_OPD_IN, 0},
+    {"temperature", RAD_OPD_IN, 1},
+    {"top_k", RAD_OPD_IN, 1},
+    {"top_p", RAD_OPD_IN, 1},
+    {"min_p", RAD_OPD_IN, 1},
+    {"token", RAD_OPD_OUT, 0},
+    {"prob", RAD_OPD_OUT, 1},
+};
+
 const RadOpSchema kSchemas[] = {
     {"quant_act_i8", kQuantParams, 3, kQuantOperands, 3,
      "symmetric int8 quantisation of an activation with one f32 scale a row, amax/127."},
@@ -77,6 +97,10 @@ const RadOpSchema kSchemas[] = {
     {"rmsnorm_quant_i8", kNormParams, 5, kNormOperands, 7,
      "RMS norm, optionally of bf16(residual + x) written to residual_out (which may be residual "
      "or x itself), then quant_act_i8's quantiser over the f32 normed values; out carries them."},
+    {"sample_logits", kSampleParams, 3, kSampleOperands, 8,
+     "one token a row of logits from a uniform number u in [0, 1): softmax at the row's temperature, "
+     "top-k, top-p of those, min-p of those, then the first kept token in index order whose running "
+     "mass passes u times the kept mass; prob is its share of that mass."},
 };
 
 const RadConstraint cI8[] = {
@@ -88,6 +112,10 @@ const RadConstraint cI8Decode[] = {
 };
 const RadConstraint cBand[] = {
     {"n", RAD_C_GE, 1, nullptr},
+    {"dtype", RAD_C_IN, 0, "f32 bf16"},
+};
+const RadConstraint cSample[] = {
+    {"n_vocab", RAD_C_GE, 1, nullptr},
     {"dtype", RAD_C_IN, 0, "f32 bf16"},
 };
 const RadConstraint cNorm[] = {
@@ -133,9 +161,19 @@ const RadKernelInfo kRows[] = {
      "bf16 x, residual and residual_out, f32/bf16 w, int8 q, f32 scale, optional bf16/f32 out",
      RAD_DOMAIN_DEVICE, kPrioTile, cNorm, 2, nullptr, 0, nullptr, nullptr, nullptr,
      r3d_rad_rmsnorm_quant_i8, nullptr, nullptr, nullptr, nullptr, nullptr},
+    {"sample_logits", "sample_logits", "vocab",
+     "temperature, top-k, top-p and min-p sampling from given uniform numbers: masses in 64-bit "
+     "integers from an f64 exp, cuts through a histogram of the row and a sort of its border bins",
+     "n_vocab up to 4194304, at most 65535 rows, any alignment and pitch; launch scratch of the size "
+     "the hook asks for (16-byte aligned) required; settings per row, a stride of 0 for all rows; "
+     "temperature <= 0: the lowest index of the maximum; a row with no token: -1",
+     "f32/bf16 logits, f32 u, temperature, top_p, min_p, i32 top_k, i32 token, optional f32 prob",
+     RAD_DOMAIN_DEVICE, kPrioTile, cSample, 2, nullptr, 0, nullptr, nullptr, nullptr,
+     r3d_rad_sample_logits, r3d_rad_sample_logits_scratch, nullptr, nullptr, nullptr, nullptr},
 };
 
 bool row_hidden(const RadKernelInfo& k) {
+    if (!strcmp(k.name, "sample_logits")) return r3d::env_no_sample();
     if (!strcmp(k.name, "gemm_nt_q_i8a8_decode")) return r3d::env_no_i8() || r3d::env_no_i8_dec();
     return r3d::env_no_i8();
 }
