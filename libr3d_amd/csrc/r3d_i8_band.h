@@ -17,7 +17,9 @@
  *
  * One workgroup a row, the row in registers (C chunks of 8 elements a lane) from the load to the
  * codes: every operand is read once and every result written once, which is all the traffic there
- * is; the kernels are bound by it.  Operands move in 16-byte accesses at element alignment
+ * is; the kernels are bound by it (us, and all bytes a second: norm with its residual 2048 x 5376
+ * 21.8, 3.5 TB/s, 4096 x 5376 36.3, 4.2; gated 2048 x 21504 40, 5.5; quant 2048 x 4096 6.4, 3.9; a
+ * large copy reaches 5.1).  Operands move in 16-byte accesses at element alignment
  * (gfx950's global memory takes them anywhere), so no pitch or base needs a kernel of its own; the
  * last n % 8 elements go one by one.  A row past the registers (C = 0) is walked twice. */
 #ifndef R3D_I8_BAND_H
@@ -42,37 +44,36 @@ struct I8BandArgs {
     int silu, ob_bf16;
 };
 
-__device__ __forceinline__ float i8_bf(uint32_t b) { return __uint_as_float(b << 16); }
-
-/* Eight elements from element i of a row of n on; zeros past its end. */
+/* Eight elements of a row as they lie in memory. */
 template <bool BF16>
-__device__ __forceinline__ void i8_ld8(const uint8_t* row, int64_t i, int64_t n, float* v) {
+struct I8Raw {
+    r3d_i32x4 v[BF16 ? 1 : 2];
+    __device__ __forceinline__ float at(int j) const {
+        if (BF16) return __uint_as_float(j & 1 ? (uint32_t)v[0][j >> 1] & 0xFFFF0000u : (uint32_t)v[0][j >> 1] << 16);
+        return __int_as_float(v[BF16 ? 0 : j >> 2][j & 3]);
+    }
+};
+
+/* The eight from element i of a row of n on; zeros past its end. */
+template <bool BF16>
+__device__ __forceinline__ I8Raw<BF16> i8_ld8(const uint8_t* row, int64_t i, int64_t n) {
+    I8Raw<BF16> r;
     if (i + 8 <= n) {
-        if (BF16) {
-            const r3d_i32x4_u2 d = *reinterpret_cast<const r3d_i32x4_u2*>(row + 2 * i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[2 * j] = __uint_as_float((uint32_t)d[j] << 16);
-                v[2 * j + 1] = __uint_as_float((uint32_t)d[j] & 0xFFFF0000u);
-            }
-        } else {
-            const r3d_f32x4_u4 lo = *reinterpret_cast<const r3d_f32x4_u4*>(row + 4 * i);
-            const r3d_f32x4_u4 hi = *reinterpret_cast<const r3d_f32x4_u4*>(row + 4 * i + 16);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = lo[j];
-                v[4 + j] = hi[j];
-            }
-        }
+        r.v[0] = *reinterpret_cast<const r3d_i32x4_u2*>(row + (BF16 ? 2 : 4) * i);
+        if (!BF16) r.v[BF16 ? 0 : 1] = *reinterpret_cast<const r3d_i32x4_u2*>(row + 4 * i + 16);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = 0.0f;
-            if (i + j < n)
-                v[j] = BF16 ? i8_bf(reinterpret_cast<const uint16_t*>(row)[i + j])
-                            : reinterpret_cast<const float*>(row)[i + j];
-        }
+        for (int k = 0; k < (BF16 ? 1 : 2); ++k) r.v[k] = r3d_i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < n) {
+                if (BF16)
+                    r.v[0][j >> 1] |= (int)((uint32_t)reinterpret_cast<const uint16_t*>(row)[i + j] << (16 * (j & 1)));
+                else
+                    r.v[BF16 ? 0 : j >> 2][j & 3] = reinterpret_cast<const int*>(row)[i + j];
+            }
     }
+    return r;
 }
 
 /* Eight f32 as bf16 (or as they are) to element i of a row of n on. */
@@ -110,26 +111,31 @@ __device__ __forceinline__ float i8_sigmoid(float g) {
     return g != g ? g : r;
 }
 
-/* The eight values h of chunk i (before the norm's scale: r). */
-template <int OP, bool XBF16>
-__device__ __forceinline__ void i8_values(const I8BandArgs& P, const uint8_t* xr, const uint8_t* rr,
-                                          uint8_t* ro, int64_t i, float* h) {
-    i8_ld8<XBF16>(xr, i, P.n, h);
-    if (OP == I8_GATED) {
-        float up[8];
-        i8_ld8<XBF16>(xr + (XBF16 ? 2 : 4) * P.n, i, P.n, up);
+/* bf16(residual + x), also to element i of the row at ro on. */
+__device__ __forceinline__ I8Raw<true> i8_add8(const I8Raw<true>& x, const I8Raw<true>& a, uint8_t* ro, int64_t i,
+                                               int64_t n) {
+    I8Raw<true> r;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float s = i8_sigmoid(h[j]);
-            h[j] = (P.silu ? h[j] * s : s) * up[j];
-        }
+    for (int j = 0; j < 4; ++j)
+        r.v[0][j] = (int)r3d_pack_bf16x2(__fadd_rn(a.at(2 * j), x.at(2 * j)), __fadd_rn(a.at(2 * j + 1), x.at(2 * j + 1)));
+    if (i + 8 <= n) {
+        *reinterpret_cast<r3d_i32x4_u2*>(ro + 2 * i) = r.v[0];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i + j < n)
+                reinterpret_cast<uint16_t*>(ro)[i + j] = (uint16_t)((uint32_t)r.v[0][j >> 1] >> (16 * (j & 1)));
     }
-    if (OP == I8_NORM && rr) {
-        float a[8];
-        i8_ld8<true>(rr, i, P.n, a);
+    return r;
+}
+
+/* act(gate) * up */
+template <bool BF16>
+__device__ __forceinline__ void i8_gated8(const I8Raw<BF16>& g, const I8Raw<BF16>& u, int silu, float* h) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) h[j] = r3d_bf16_to_f32(r3d_bf16_rne(__fadd_rn(a[j], h[j])));
-        i8_st8(ro, i, P.n, h, 1);
+    for (int j = 0; j < 8; ++j) {
+        const float gv = g.at(j), s = i8_sigmoid(gv);
+        h[j] = (silu ? gv * s : s) * u.at(j);
     }
 }
 
@@ -170,9 +176,10 @@ __device__ __forceinline__ uint32_t i8_amax8(const float* h, uint32_t m) {
 }
 
 /* h = (r * rs) * (w + wadd) over a chunk. */
-__device__ __forceinline__ void i8_norm8(const float* w, float wadd, float rs, float* h) {
+template <bool WBF16>
+__device__ __forceinline__ void i8_norm8(const I8Raw<true>& r, const I8Raw<WBF16>& w, float wadd, float rs, float* h) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) h[j] = __fmul_rn(__fmul_rn(h[j], rs), __fadd_rn(w[j], wadd));
+    for (int j = 0; j < 8; ++j) h[j] = __fmul_rn(__fmul_rn(r.at(j), rs), __fadd_rn(w.at(j), wadd));
 }
 
 /* A row's scale from its largest magnitude's bits, and whether that is a number. */
@@ -183,17 +190,21 @@ __device__ __forceinline__ float i8_scale(uint32_t m, bool* fin) {
 }
 
 /* The codes of chunk i, four to a dword; 0 on a row whose scale is no number.  |h * inv| is 127 up
- * to a few roundings, so rint gives at most 127. */
+ * to a few roundings; added to 1.5 * 2^23 it is rounded to a whole number, to nearest even, whose two's
+ * complement is the low byte of the sum. */
 __device__ __forceinline__ void i8_codes8(uint8_t* qr, int64_t i, int64_t n, float inv, bool fin,
                                           const float* h) {
+#pragma clang fp contract(off)                   /* the product is rounded before the sum */
     uint32_t c[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-        int d[4];
+        uint32_t d[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] = fin ? (int)__builtin_rintf(__fmul_rn(h[4 * k + j], inv)) : 0;
-        c[k] = (uint32_t)(d[0] & 255) | (uint32_t)(d[1] & 255) << 8 | (uint32_t)(d[2] & 255) << 16 |
-               (uint32_t)d[3] << 24;
+        for (int j = 0; j < 4; ++j)
+            d[j] = __float_as_uint(h[4 * k + j] * inv + 12582912.0f);
+        const uint32_t lo = __builtin_amdgcn_perm(d[1], d[0], 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(d[3], d[2], 0x04000c0cu);
+        c[k] = fin ? lo | hi : 0u;
     }
     if (i + 8 <= n) {
         typedef uint32_t u32x2_u1 __attribute__((ext_vector_type(2), aligned(1)));
@@ -219,31 +230,47 @@ __global__ __launch_bounds__(1024) void i8_band_kernel(I8BandArgs P) {
     float rs = 1.0f;
     uint32_t m = 0;
     if constexpr (C > 0) {
+        /* every load of the row before the first use of one; a lane past the row's end has zeros */
         float h[C][8];
+        I8Raw<XBF16> x[C], y[C];                 /* y: up, or the residual */
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            const int64_t i = i0 + c * step;
-            if (i < n) {
-                i8_values<OP, XBF16>(P, xr, rr, ro, i, h[c]);
-            } else {
+        for (int c = 0; c < C; ++c) x[c] = i8_ld8<XBF16>(xr, i0 + c * step, n);
+        if (OP == I8_GATED || (OP == I8_NORM && rr)) {
+            const uint8_t* yr = OP == I8_GATED ? xr + (XBF16 ? 2 : 4) * n : rr;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[c][j] = 0.0f;
-            }
+            for (int c = 0; c < C; ++c) y[c] = i8_ld8<XBF16>(yr, i0 + c * step, n);
         }
-        if (OP == I8_NORM) {
-            float w[C][8];                       /* on its way while the sum is taken */
+        if constexpr (OP == I8_NORM) {
+            I8Raw<WBF16> w[C];
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (i0 + c * step < n) i8_ld8<WBF16>(P.w, i0 + c * step, n, w[c]);
+            for (int c = 0; c < C; ++c) w[c] = i8_ld8<WBF16>(P.w, i0 + c * step, n);
             double ss = 0.0;
 #pragma unroll
-            for (int c = 0; c < C; ++c)
+            for (int c = 0; c < C; ++c) {
+                if (rr) x[c] = i8_add8(x[c], y[c], ro, i0 + c * step, n);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)h[c][j], (double)h[c][j], ss);
+                for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)x[c].at(j), (double)x[c].at(j), ss);
+            }
             rs = (float)(1.0 / sqrt(i8_block_sum(ss, s_sum) / (double)n + P.eps));
 #pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (i0 + c * step < n) i8_norm8(w[c], P.wadd, rs, h[c]);
+            for (int c = 0; c < C; ++c) {
+                i8_norm8<WBF16>(x[c], w[c], P.wadd, rs, h[c]);
+                if (i0 + c * step + 8 > n) {     /* a zero past the end is no value (0 * inf) */
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (i0 + c * step + j >= n) h[c][j] = 0.0f;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                if (OP == I8_GATED) {
+                    i8_gated8<XBF16>(x[c], y[c], P.silu, h[c]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[c][j] = x[c].at(j);
+                }
+            }
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) m = i8_amax8(h[c], m);
@@ -261,24 +288,31 @@ __global__ __launch_bounds__(1024) void i8_band_kernel(I8BandArgs P) {
         }
     } else {
         float h[8];
-        if (OP == I8_NORM) {
+        if constexpr (OP == I8_NORM) {
             double ss = 0.0;
             for (int64_t i = i0; i < n; i += step) {
-                i8_values<OP, XBF16>(P, xr, rr, ro, i, h);
+                I8Raw<true> x = i8_ld8<true>(xr, i, n);
+                if (rr) x = i8_add8(x, i8_ld8<true>(rr, i, n), ro, i, n);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)h[j], (double)h[j], ss);
+                for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)x.at(j), (double)x.at(j), ss);
             }
             rs = (float)(1.0 / sqrt(i8_block_sum(ss, s_sum) / (double)n + P.eps));
         }
         /* the norm's later walks read r where the first one wrote it: the same lane's own chunks */
         auto value = [&](int64_t i) {
-            if (OP == I8_NORM) {
-                i8_ld8<true>(rr ? ro : xr, i, n, h);
-                float w[8];
-                i8_ld8<WBF16>(P.w, i, n, w);
-                i8_norm8(w, P.wadd, rs, h);
+            if constexpr (OP == I8_NORM) {
+                i8_norm8<WBF16>(i8_ld8<true>(rr ? ro : xr, i, n), i8_ld8<WBF16>(P.w, i, n), P.wadd, rs, h);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (i + j >= n) h[j] = 0.0f;
             } else {
-                i8_values<OP, XBF16>(P, xr, nullptr, nullptr, i, h);
+                const I8Raw<XBF16> x = i8_ld8<XBF16>(xr, i, n);
+                if (OP == I8_GATED) {
+                    i8_gated8<XBF16>(x, i8_ld8<XBF16>(xr + (XBF16 ? 2 : 4) * n, i, n), P.silu, h);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[j] = x.at(j);
+                }
             }
         };
         for (int64_t i = i0; i < n; i += step) {

@@ -265,16 +265,23 @@ int plan_i8_band(const RadArgs* a, int op, I8BandPlan* P) {
 
 I8BandGeom i8_band_geom(int64_t rows, int64_t n) {
     const int64_t nc = (n + 7) / 8;
-    const bool few = rows <= 512;
-    for (int c = 1; c <= 4; ++c)
-        for (int lanes = 64; lanes <= 1024; lanes *= 2) {
-            if ((int64_t)lanes * c < nc) continue;
-            /* few rows: one chunk a lane while 1024 lanes hold the row; many rows: 256 lanes
-             * (several rows a compute unit) while three chunks a lane hold it */
-            if (!few && lanes > 256 && c < 3) break;
-            return I8BandGeom{lanes, c};
-        }
-    return I8BandGeom{1024, 0};
+    if (nc > 4096) return I8BandGeom{1024, 0};
+    auto lanes = [&](int c) { return (int)(((nc + c - 1) / c + 63) / 64 * 64); };
+    /* us at the chunks a lane named, rows of n (norm; gated g):
+     *     1 x 5376     1: 4.3   2: 5.2   3: 5.4        1 x 8192     1: 4.9   2: 4.5   3: 5.7
+     *     1 x 21504 g  3: 6.5   4: 6.6                 1 x 12000 g  2: 4.4   3: 4.7   4: 5.4
+     *  2048 x 5376     1: 27.1  2: 24.2  3: 21.8    2048 x 8192     1: 30.8  2: 27.7  3: 31.1
+     *  4096 x 2304     1: 23.7  2: 21.2  3: 19.7    4096 x 2000 g   1: 12.0  2: 12.5  3: 15.9
+     * Few rows, or short ones: as few chunks as some 768 lanes allow.  Many long rows: two to four,
+     * the fewest idle lanes, three where they tie. */
+    if (nc <= 256 || rows * nc < 400000) {
+        const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : nc <= 3072 ? 3 : 4;
+        return I8BandGeom{lanes(c), c};
+    }
+    int best = 0;
+    for (int c : {3, 2, 4})
+        if (lanes(c) <= 1024 && (!best || lanes(c) * c < lanes(best) * best)) best = c;
+    return I8BandGeom{lanes(best), best};
 }
 
 int describe_i8(const char* row, const RadArgs* a, char* buf, int len) {
