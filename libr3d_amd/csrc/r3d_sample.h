@@ -10,19 +10,32 @@ namespace r3d {
 constexpr int kSampleSeg = 4096;         /* tokens a segment: the unit of the index-order search */
 constexpr int kSampleMaxSegs = 1024;
 constexpr int64_t kSampleMaxVocab = (int64_t)kSampleSeg * kSampleMaxSegs;
+constexpr int kSampleChunk = 64;         /* tokens a chunk: the unit that is skipped by its largest logit */
+constexpr int kSampleSegChunks = kSampleSeg / kSampleChunk;
 constexpr int kSampleBins = 2048;
-constexpr int kSampleList = 8192;        /* tokens of the border bins that are listed */
+constexpr int kSampleList = 8192;        /* tokens that are listed and sorted, at most */
+constexpr int kSampleListK = 2048;       /* the largest top-k that is looked for by chunks */
 
-/* The launch scratch, one of these a row, then seg_max, seg_min and seg_mass of its segments. */
+/* Where the cuts fall among the bins. */
+struct SampleCut {
+    int kb, pb_lo, pb_hi;        /* bins: top-k's, top-p's first and last; kSampleBins: that cut is off */
+    int count_k;                 /* tokens above bin kb */
+    unsigned long long mass_k, mass_p;             /* mass above bins kb and pb_lo */
+    unsigned long long mass_kb, total;             /* mass of bin kb, of all bins */
+};
+
+/* The launch scratch: one of these a row; of every segment its mass, of every quarter of one its sum,
+ * largest and least logit, and
+ * of every chunk its largest. */
 struct SampleRow {
     unsigned long long mass[kSampleBins];
     unsigned long long list[kSampleList];         /* ~key in the high half, index in the low */
-    unsigned long long mass_k, mass_p;            /* mass above the border bins of top-k and top-p */
+    SampleCut cut;
     unsigned int count[kSampleBins];
     unsigned int n_list;
-    int kb, pb_lo, pb_hi;                         /* border bins; kSampleBins: that cut is off */
-    int count_k;                                  /* tokens above bin kb */
-    int pad[3];
+    int binned, n_binned;                         /* not of this row: the i-th row that has a use for bins (in
+                                                     element i), and how many there are (in the first) */
+    int pad;
 };
 
 struct SamplePlan {

@@ -14,16 +14,27 @@
  * 2^-s sqrt(V) / mass, 2^-35 at V = 262144, where f32 sums would move it by 2^-20 and pick a
  * neighbour now and then.
  *
- * Three passes over the logits and one over a segment, four launches:
- *   1 largest and least logit of every segment (4096 tokens); the row's scratch is cleared
- *   2 rows with top-k or top-p: count and mass in 2048 bins, of equal width in x over the row's range
- *     (at most 32 T: below that w is 0); bins are in the order of x, so a cut falls into one bin
- *   3 the border bins are found from the 2048 sums; the tokens above them are added up a segment at a
- *     time, the tokens in them are listed
- *   4 a workgroup a row: the listed tokens are sorted, the cuts placed, the segment that holds
- *     u * mass found, and the token in it.  Past 8192 tokens in the border bins (many equal
- *     logits) the cuts are placed by radix selection over the row instead.
- * The row is read from L2 and the last-level cache after pass 1 where it fits. */
+ * A row is sorted nowhere; its cuts are looked for where they can be.  Four launches, for all rows:
+ *   1 the largest and least logit of every quarter of a segment (4096 tokens), and the largest of every
+ *     chunk (64 tokens).  Of a row without a cut also the quarters' sums of w, in f64: that row needs
+ *     no other pass but the last.  Greedy rows need the largest logits only
+ *   2 of rows whose cut may lie anywhere (top-p without a small top-k, or a top-k of more than a chunk in
+ *     four): count and mass in 2048 bins, of equal width in x over the row's range (at most 32 T: below
+ *     that w is 0); bins are in the order of x, so a cut falls into one bin
+ *   3 of these rows the border bins are found from the 2048 sums; the tokens above them are added up a
+ *     segment at a time, the tokens in them are listed.  Chunks below the borders are not read
+ *   4 a workgroup a row: the listed tokens are sorted, the cuts placed, the segment that holds u * mass
+ *     found, and the token in it.  Rows with a small top-k, or with min-p alone, are listed here: k chunks
+ *     whose largest logits are the k largest such hold the k first tokens above the least of those, so
+ *     only chunks above that are read.  Past 8192 listed tokens (many equal logits) the cuts are
+ *     placed by radix selection over the row instead.
+ * Passes 2 and 3 are not launched without a top-k or top-p operand.
+ *
+ * Bound by the one read of the row in pass 1 and by the four launches' chains of dependent loads.
+ * Measured on MI355X at V = 262144, f32: one row 21.6 us; 128 rows, each with settings of its own, 106 us
+ * (of which pass 1's read of 134 MB 31 to 37 us, 3.6 to 4.4 TB/s; passes 2 and 3 for the 22 rows that have a
+ * use for them 20 and 24, f64 exps; pass 4 32, of them 8 to list 1000 chunks).  With bins for every row, no chunks
+ * and a sort that waited at a barrier for every step the same took 27.7 and 143 us. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -42,9 +53,12 @@ typedef unsigned long long u64;
 struct SampleArgs {
     SamplePlan P;
     SampleRow* rows;
-    float* seg_max;              /* [M][segs] */
-    float* seg_min;
-    u64* seg_mass;
+    u64* seg_mass;               /* [M][segs] */
+    double* q_sum;               /* [M][4 segs], of every quarter of a segment: rows without a cut, the sum of
+                                    exp((x - its largest) / T); */
+    float* q_max;                /* its largest */
+    float* q_min;                /* and least logit */
+    float* chunk_max;            /* [M][64 segs] */
     int segs, per, shift;        /* per: segments a workgroup; shift: s of the masses */
 };
 
@@ -52,19 +66,25 @@ struct SampleArgs {
 struct SampleSet {
     float top;                   /* the largest logit; -inf: the row is empty */
     float bin;                   /* bins a unit of x */
+    float T;
     double inv_t, p, min_p;
     int k;
     bool greedy, use_k, use_p;
+    bool listed;                 /* cut by a small top-k, or by min-p alone: the row's last pass lists
+                                    what can be kept by way of the chunks' maxima */
+    bool plain;                  /* no cut at all */
+    bool binned;                 /* the others that are not greedy: passes 2 and 3 */
 };
 
-__device__ __forceinline__ SampleSet sample_set(const SampleArgs& a, int64_t row, float top, float low) {
+__device__ __forceinline__ SampleSet sample_set(const SampleArgs& a, int64_t row) {
     const SamplePlan& P = a.P;
     SampleSet s;
     const float T = P.temperature ? P.temperature[row * P.t_stride] : 1.0f;
     const int k = P.top_k ? P.top_k[row * P.k_stride] : 0;
     const float p = P.top_p ? P.top_p[row * P.p_stride] : 1.0f;
     const float m = P.min_p ? P.min_p[row * P.m_stride] : 0.0f;
-    s.top = top;
+    s.top = s.bin = 0.0f;
+    s.T = T;
     s.greedy = !(T > 0.0f);
     s.inv_t = 1.0 / (double)T;
     s.k = k;
@@ -72,7 +92,10 @@ __device__ __forceinline__ SampleSet sample_set(const SampleArgs& a, int64_t row
     s.p = (double)p;
     s.use_p = p < 1.0f;
     s.min_p = m > 0.0f ? (m < 1.0f ? (double)m : 1.0) : 0.0;
-    s.bin = (float)(kSampleBins - 1) / __builtin_fminf(top - low, 32.0f * T);
+    s.plain = !s.use_k && !s.use_p && s.min_p == 0.0;
+    s.listed = s.use_k ? P.V <= kSampleList || (k <= kSampleListK && k <= (P.V / kSampleChunk) / 4)
+                       : !s.use_p && s.min_p > 0.0;
+    s.binned = !s.greedy && !s.plain && !s.listed;
     return s;
 }
 
@@ -150,20 +173,16 @@ __device__ __forceinline__ void sample_ld4(const uint8_t* x, int64_t i, int64_t 
 }
 
 constexpr int kSampleT = 256;                      /* lanes of passes 1 to 3 */
-constexpr int kSampleU = kSampleSeg / kSampleT / 4; /* loads a lane and segment */
+constexpr int kSampleU = kSampleSeg / 4 / 64 / 4;    /* loads a lane and quarter of a segment */
 
-/* Segments [g per, min(segs, (g + 1) per)) of row blockIdx.y: f(segment, index, four logits). */
-template <bool BF16, typename F>
-__device__ __forceinline__ void sample_walk(const SampleArgs& a, F f) {
-    const uint8_t* x = sample_row(a.P, blockIdx.y);
-    const int s1 = ((int)blockIdx.x + 1) * a.per < a.segs ? ((int)blockIdx.x + 1) * a.per : a.segs;
-    for (int s = blockIdx.x * a.per; s < s1; ++s) {
-        float v[kSampleU][4];
+/* A lane's loads are in flight together and worked on one after the other from the same registers:
+ * unrolled, 16 exps side by side need twice the registers and four times the code. */
+template <int U>
+__device__ __forceinline__ void sample_next(float (*v)[4]) {
 #pragma unroll
-        for (int j = 0; j < kSampleU; ++j)
-            sample_ld4<BF16>(x, (int64_t)s * kSampleSeg + 4 * (threadIdx.x + kSampleT * j), a.P.V, v[j]);
-        f(s, (int64_t)s * kSampleSeg + 4 * threadIdx.x, v);
-    }
+    for (int j = 0; j + 1 < U; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][i] = v[j + 1][i];
 }
 
 template <int T>
@@ -212,80 +231,161 @@ __device__ __forceinline__ u64 sample_block_scan(u64 v, u64* s, u64* total) {
     return before + in - v;
 }
 
-/* The row's largest and least logit from its segments'. */
+/* The row's largest and least logit from its quarters', into the set. */
 template <int T>
-__device__ __forceinline__ void sample_range(const SampleArgs& a, int64_t row, float* s, float* top, float* low) {
+__device__ __forceinline__ void sample_range(const SampleArgs& a, int64_t row, float* s, SampleSet* set) {
     float hi = -__builtin_inff(), lo = __builtin_inff();
-    for (int i = threadIdx.x; i < a.segs; i += T) {
-        hi = __builtin_fmaxf(hi, a.seg_max[row * a.segs + i]);
-        lo = __builtin_fminf(lo, a.seg_min[row * a.segs + i]);
+    for (int i = threadIdx.x; i < 4 * a.segs; i += T) {
+        hi = __builtin_fmaxf(hi, a.q_max[row * 4 * a.segs + i]);
+        lo = __builtin_fminf(lo, a.q_min[row * 4 * a.segs + i]);
     }
-    *top = sample_block_max<T>(hi, s);
-    *low = -sample_block_max<T>(-lo, s);
+    hi = sample_block_max<T>(hi, s);
+    lo = -sample_block_max<T>(-lo, s);
+    set->top = hi;
+    set->bin = (float)(kSampleBins - 1) / __builtin_fminf(hi - lo, 32.0f * set->T);
 }
 
+/* Pass 1: a wave a quarter of a segment at a time, no barrier.  Bound by the read. */
 template <bool BF16>
 __global__ __launch_bounds__(kSampleT) void sample_range_kernel(SampleArgs a) {
-    __shared__ float s[kSampleT / 64];
     const int64_t row = blockIdx.y;
-    SampleRow& R = a.rows[row];
-    for (int i = blockIdx.x * kSampleT + threadIdx.x; i < kSampleBins; i += gridDim.x * kSampleT) {
-        R.mass[i] = 0;
-        R.count[i] = 0;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) R.n_list = 0;
-    sample_walk<BF16>(a, [&](int seg, int64_t, float (*v)[4]) {
-        float hi = -__builtin_inff(), lo = __builtin_inff();
+    if (row == 0 && blockIdx.x == 0) {
+        __shared__ unsigned int on[kSampleT / 64];
+        int n = 0;
+        for (int64_t r0 = 0; r0 < a.P.M; r0 += kSampleT) {
+            const u64 mask = __ballot(r0 + threadIdx.x < a.P.M && sample_set(a, r0 + threadIdx.x).binned);
+            if ((threadIdx.x & 63) == 0) on[threadIdx.x >> 6] = (unsigned int)__builtin_popcountll(mask);
+            __syncthreads();
+            int at = n + __builtin_popcountll(mask & (((u64)1 << (threadIdx.x & 63)) - 1));
 #pragma unroll
-        for (int j = 0; j < kSampleU; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (sample_in(v[j][i])) {
-                    hi = __builtin_fmaxf(hi, v[j][i]);
-                    lo = __builtin_fminf(lo, v[j][i]);
-                }
-        hi = sample_block_max<kSampleT>(hi, s);
-        lo = -sample_block_max<kSampleT>(-lo, s);
-        if (threadIdx.x == 0) {
-            a.seg_max[row * a.segs + seg] = hi;
-            a.seg_min[row * a.segs + seg] = lo;
+            for (int i = 0; i < kSampleT / 64; ++i) {
+                if (i < (int)threadIdx.x >> 6) at += (int)on[i];
+                n += (int)on[i];
+            }
+            if (mask >> (threadIdx.x & 63) & 1) a.rows[at].binned = (int)(r0 + threadIdx.x);
+            __syncthreads();
         }
-    });
+        if (threadIdx.x == 0) a.rows[0].n_binned = n;
+    }
+    const SampleSet set = sample_set(a, row);
+    if (set.binned) {
+        SampleRow& R = a.rows[row];
+        for (int i = blockIdx.x * kSampleT + threadIdx.x; i < kSampleBins; i += gridDim.x * kSampleT) {
+            R.mass[i] = 0;
+            R.count[i] = 0;
+        }
+        if (blockIdx.x == 0 && threadIdx.x == 0) R.n_list = 0;
+    }
+    const uint8_t* x = sample_row(a.P, row);
+    const int lane = threadIdx.x & 63;
+    const int s1 = ((int)blockIdx.x + 1) * a.per < a.segs ? ((int)blockIdx.x + 1) * a.per : a.segs;
+    for (int seg = blockIdx.x * a.per; seg < s1; ++seg) {
+        const int64_t q = (int64_t)seg * 4 + (threadIdx.x >> 6);
+        float v[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sample_ld4<BF16>(x, q * (kSampleSeg / 4) + 4 * (lane + 64 * j), a.P.V, v[j]);
+        float hi = -__builtin_inff(), lo = __builtin_inff();
+        float* const cm = a.chunk_max + row * a.segs * kSampleSegChunks + q * (kSampleSegChunks / 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float m = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                m = __builtin_fmaxf(m, v[j][i]);                      /* a NaN is passed over */
+                lo = __builtin_fminf(lo, sample_in(v[j][i]) ? v[j][i] : lo);
+            }
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, off, 64));
+            if ((lane & 15) == 0) cm[lane / 16 + 4 * j] = m;
+            hi = __builtin_fmaxf(hi, m);
+        }
+#pragma unroll
+        for (int off = 32; off >= 16; off >>= 1) hi = __builtin_fmaxf(hi, __shfl_xor(hi, off, 64));
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) lo = __builtin_fminf(lo, __shfl_xor(lo, off, 64));
+        if (lane == 0) {
+            a.q_max[row * 4 * a.segs + q] = hi;
+            a.q_min[row * 4 * a.segs + q] = lo;
+        }
+        if (set.plain && !set.greedy) {
+            SampleSet here = set;
+            here.top = hi;
+            double sum = 0.0;
+#pragma unroll 1
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (sample_in(v[0][i])) sum += sample_w(here, v[0][i]);
+                sample_next<kSampleU>(v);
+            }
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+            if (lane == 0) a.q_sum[row * 4 * a.segs + q] = sum;
+        }
+    }
+}
+
+/* Passes 2 and 3, a wave a quarter of a segment at a time.  The binned rows are dealt out to
+ * all workgroups, a row to as many as there are for it.  (A grid over every row's parts took 16 us of a
+ * 26 us launch to start the workgroups of the 106 other rows of 128 and see them end.) */
+constexpr int kBinT = 1024, kBinWaves = kBinT / 64, kBinGrid = 256, kBinLeast = kBinWaves / 4;
+constexpr unsigned int kBinList = 2048;
+struct SampleShare {
+    int items, parts, per;       /* shares in all, a row, and segments a share */
+};
+__device__ __forceinline__ SampleShare sample_share_out(const SampleArgs& a) {
+    const int rows = a.rows[0].n_binned;
+    int parts = rows ? (int)gridDim.x / rows : 1;
+    if (parts < 1) parts = 1;
+    int per = (a.segs + parts - 1) / parts;
+    if (per < kBinLeast) per = kBinLeast;          /* a quarter a wave at least */
+    parts = (a.segs + per - 1) / per;
+    return {rows * parts, parts, per};
 }
 
 template <bool BF16>
-__global__ __launch_bounds__(kSampleT) void sample_hist_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kBinT) void sample_hist_kernel(SampleArgs a) {
     __shared__ u64 mass[kSampleBins];
     __shared__ unsigned int count[kSampleBins];
-    __shared__ float s[kSampleT / 64];
-    const int64_t row = blockIdx.y;
-    float top, low;
-    sample_range<kSampleT>(a, row, s, &top, &low);
-    const SampleSet set = sample_set(a, row, top, low);
-    if (set.greedy || !sample_in(top) || !(set.use_k || set.use_p)) return;      /* the whole workgroup */
-    for (int i = threadIdx.x; i < kSampleBins; i += kSampleT) {
+    __shared__ float s[kBinT / 64];
+    const SampleShare share = sample_share_out(a);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x >= share.items) return;
+    const int64_t row = a.rows[blockIdx.x / share.parts].binned;
+    const int s0 = (int)blockIdx.x % share.parts * share.per;
+    const int s1 = s0 + share.per < a.segs ? s0 + share.per : a.segs;
+    SampleSet set = sample_set(a, row);
+    sample_range<kBinT>(a, row, s, &set);
+    if (!sample_in(set.top)) return;
+    for (int i = threadIdx.x; i < kSampleBins; i += kBinT) {
         mass[i] = 0;
         count[i] = 0;
     }
     __syncthreads();
-    sample_walk<BF16>(a, [&](int, int64_t, float (*v)[4]) {
+    const uint8_t* x = sample_row(a.P, row);
+    for (int q = 4 * s0 + wave; q < 4 * s1; q += kBinWaves) {
+        float v[kSampleU][4];
 #pragma unroll
         for (int j = 0; j < kSampleU; ++j)
+            sample_ld4<BF16>(x, (int64_t)q * (kSampleSeg / 4) + 4 * (lane + 64 * j), a.P.V, v[j]);
+#pragma unroll 1
+        for (int j = 0; j < kSampleU; ++j) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (sample_in(v[j][i])) {
-                    const int b = sample_bin(set, v[j][i]);
-                    atomicAdd(&count[b], 1u);
-                    if (set.use_p) atomicAdd(&mass[b], sample_mass(sample_w(set, v[j][i]), a.shift));
+                if (sample_in(v[0][i])) {
+                    const int b = sample_bin(set, v[0][i]);
+                    if (set.use_k) atomicAdd(&count[b], 1u);
+                    if (set.use_p) atomicAdd(&mass[b], sample_mass(sample_w(set, v[0][i]), a.shift));
                 }
-    });
+            sample_next<kSampleU>(v);
+        }
+    }
     __syncthreads();
     SampleRow& R = a.rows[row];
-    for (int i = threadIdx.x; i < kSampleBins; i += kSampleT)
-        if (count[i]) {
-            atomicAdd(&R.count[i], count[i]);
-            if (mass[i]) atomicAdd(&R.mass[i], mass[i]);
-        }
+    for (int i = threadIdx.x; i < kSampleBins; i += kBinT) {
+        if (count[i]) atomicAdd(&R.count[i], count[i]);
+        if (mass[i]) atomicAdd(&R.mass[i], mass[i]);
+    }
 }
 
 /* p's share of a mass, one at least. */
@@ -294,124 +394,206 @@ __device__ __forceinline__ u64 sample_share(double p, u64 mass) {
     return t >= 1.0 ? (u64)t : 1;
 }
 
-template <bool BF16>
-__global__ __launch_bounds__(kSampleT) void sample_gather_kernel(SampleArgs a) {
-    constexpr int B = kSampleBins / kSampleT;      /* bins a lane */
-    __shared__ u64 su[kSampleT / 64];
-    __shared__ float s[kSampleT / 64];
-    __shared__ int kb, pb[2];
-    __shared__ u64 edge[2];                        /* mass above kb, above pb_lo */
-    __shared__ int count_k;
-    __shared__ u64 mass_kb;
-    const int64_t row = blockIdx.y;
-    float top, low;
-    sample_range<kSampleT>(a, row, s, &top, &low);
-    const SampleSet set = sample_set(a, row, top, low);
-    if (set.greedy || !sample_in(top)) return;
-    SampleRow& R = a.rows[row];
+/* From the bins' sums, a workgroup of T lanes. */
+template <int T>
+__device__ __forceinline__ void sample_cut(const SampleSet& set, const unsigned int* count, const u64* mass,
+                                           u64* su, SampleCut* C) {
+    constexpr int B = kSampleBins / T;             /* bins a lane */
+    u64 c[B], m[B], cs = 0, ms = 0, all, total;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        c[i] = count[B * threadIdx.x + i];
+        m[i] = mass[B * threadIdx.x + i];
+        cs += c[i];
+        ms += m[i];
+    }
+    u64 c0 = sample_block_scan<T>(cs, su, &all);
+    const u64 m0 = sample_block_scan<T>(ms, su, &total);
     if (threadIdx.x == 0) {
-        kb = pb[0] = pb[1] = kSampleBins;
-        edge[0] = edge[1] = mass_kb = 0;
-        count_k = 0;
-    }
-    if (set.use_k || set.use_p) {
-        u64 c[B], m[B], cs = 0, ms = 0, all, total;
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-            c[i] = R.count[B * threadIdx.x + i];
-            m[i] = R.mass[B * threadIdx.x + i];
-            cs += c[i];
-            ms += m[i];
-        }
-        u64 c0 = sample_block_scan<kSampleT>(cs, su, &all);
-        const u64 m0 = sample_block_scan<kSampleT>(ms, su, &total);
-        u64 mm = m0;
-        if (set.use_k && (u64)set.k < all) {
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                if (c0 < (u64)set.k && c0 + c[i] >= (u64)set.k) {
-                    kb = B * threadIdx.x + i;
-                    edge[0] = mm;
-                    mass_kb = m[i];
-                    count_k = (int)c0;
-                }
-                c0 += c[i];
-                mm += m[i];
-            }
-        }
-        __syncthreads();
-        if (set.use_p) {
-            /* the kept tokens' mass is known to within bin kb: the border of top-p to within these */
-            const u64 lo = sample_share(set.p, kb < kSampleBins ? edge[0] : total);
-            const u64 hi = sample_share(set.p, kb < kSampleBins ? edge[0] + mass_kb : total);
-            mm = m0;
-#pragma unroll
-            for (int i = 0; i < B; ++i) {
-                if (mm < lo && mm + m[i] >= lo) {
-                    pb[0] = B * threadIdx.x + i;
-                    edge[1] = mm;
-                }
-                if (mm < hi && mm + m[i] >= hi) pb[1] = B * threadIdx.x + i;
-                mm += m[i];
-            }
-        }
-        __syncthreads();
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        R.kb = kb;
-        R.pb_lo = pb[0];
-        R.pb_hi = pb[1];
-        R.mass_k = edge[0];
-        R.mass_p = edge[1];
-        R.count_k = count_k;
+        C->kb = C->pb_lo = C->pb_hi = kSampleBins;
+        C->count_k = 0;
+        C->mass_k = C->mass_p = C->mass_kb = 0;
+        C->total = total;
     }
     __syncthreads();
-    const int lk = kb, p0 = pb[0], p1 = pb[1], whole = lk < p0 ? lk : p0;   /* bins below `whole`: kept */
-    sample_walk<BF16>(a, [&](int seg, int64_t i0, float (*v)[4]) {
-        u64 sum = 0;
+    u64 mm = m0;
+    if (set.use_k && (u64)set.k <= all) {          /* (k of k listed ones are a cut of the row) */
 #pragma unroll
-        for (int j = 0; j < kSampleU; ++j)
+        for (int i = 0; i < B; ++i) {
+            if (c0 < (u64)set.k && c0 + c[i] >= (u64)set.k) {
+                C->kb = B * threadIdx.x + i;
+                C->mass_k = mm;
+                C->mass_kb = m[i];
+                C->count_k = (int)c0;
+            }
+            c0 += c[i];
+            mm += m[i];
+        }
+    }
+    __syncthreads();
+    if (set.use_p) {
+        /* the kept tokens' mass is known to within bin kb: the border of top-p to within these */
+        const u64 lo = sample_share(set.p, C->kb < kSampleBins ? C->mass_k : total);
+        const u64 hi = sample_share(set.p, C->kb < kSampleBins ? C->mass_k + C->mass_kb : total);
+        mm = m0;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            if (mm < lo && mm + m[i] >= lo) {
+                C->pb_lo = B * threadIdx.x + i;
+                C->mass_p = mm;
+            }
+            if (mm < hi && mm + m[i] >= hi) C->pb_hi = B * threadIdx.x + i;
+            mm += m[i];
+        }
+    }
+    __syncthreads();
+}
+/* Bins below this one are kept whole. */
+__device__ __forceinline__ int sample_whole(const SampleCut& C) { return C.kb < C.pb_lo ? C.kb : C.pb_lo; }
+/* Tokens of a border bin are listed. */
+__device__ __forceinline__ bool sample_border(const SampleCut& C, int b) {
+    return b == C.kb || (b >= C.pb_lo && b <= C.pb_hi);
+}
+/* Places for this lane's c entries (BITS bits) of a list: the first.  By the bits' ballots: no lane waits
+ * for another. */
+template <int BITS>
+__device__ __forceinline__ unsigned int sample_slots(unsigned int c, unsigned int* counter) {
+    unsigned int before = 0, all = 0;
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+        const u64 m = __ballot(c >> b & 1);
+        before += __builtin_amdgcn_mbcnt_hi((unsigned)(m >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)m, 0)) << b;
+        all += (unsigned)__builtin_popcountll(m) << b;
+    }
+    if (!all) return 0;
+    unsigned int at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(counter, all);
+    return __builtin_amdgcn_readfirstlane(at) + before;
+}
+__device__ __forceinline__ u64 sample_entry_of(float x, int64_t i) { return (u64)~sample_key(x) << 32 | (u64)i; }
+
+template <bool BF16>
+__global__ __launch_bounds__(kBinT) void sample_gather_kernel(SampleArgs a) {
+    __shared__ u64 su[kBinT / 64];
+    __shared__ float s[kBinT / 64];
+    __shared__ SampleCut cut;
+    __shared__ u64 sums[kSampleMaxSegs];
+    __shared__ u64 part[kBinList];                 /* listed by this workgroup: one atomic for them all */
+    __shared__ unsigned int n_part, part_at;
+    const SampleShare share = sample_share_out(a);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if ((int)blockIdx.x >= share.items) return;
+    const int64_t row = a.rows[blockIdx.x / share.parts].binned;
+    const int s0 = (int)blockIdx.x % share.parts * share.per;
+    const int s1 = s0 + share.per < a.segs ? s0 + share.per : a.segs;
+    SampleSet set = sample_set(a, row);
+    sample_range<kBinT>(a, row, s, &set);
+    if (!sample_in(set.top)) return;
+    SampleRow& R = a.rows[row];
+    if (threadIdx.x == 0) n_part = 0;
+    for (int i = threadIdx.x; i < s1 - s0; i += kBinT) sums[i] = 0;
+    sample_cut<kBinT>(set, R.count, R.mass, su, &cut);
+    const SampleCut C = cut;
+    if (s0 == 0 && threadIdx.x == 0) R.cut = C;
+    const int whole = sample_whole(C);
+    /* no token past bin `most` is kept or listed: a chunk whose largest logit lies there is not read */
+    const int most = C.kb < kSampleBins ? C.kb : C.pb_hi < kSampleBins ? C.pb_hi : kSampleBins - 1;
+    const uint8_t* x = sample_row(a.P, row);
+    for (int q = 4 * s0 + wave; q < 4 * s1; q += kBinWaves) {
+        const float* const cm = a.chunk_max + (row * 4 * a.segs + q) * (kSampleSegChunks / 4);
+        float v[kSampleU][4];
+#pragma unroll
+        for (int j = 0; j < kSampleU; ++j) {
+            const float m = cm[lane / 16 + 4 * j];
+            if (sample_in(m) && sample_bin(set, m) <= most) {
+                sample_ld4<BF16>(x, (int64_t)q * (kSampleSeg / 4) + 4 * (lane + 64 * j), a.P.V, v[j]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[j][i] = -__builtin_inff();
+            }
+        }
+        u64 sum = 0;
+#pragma unroll 1
+        for (int j = 0; j < kSampleU; ++j) {
+            unsigned int border = 0;       /* a bit a token */
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float x = v[j][i];
-                if (!sample_in(x)) continue;
-                const int b = sample_bin(set, x);
+                if (!sample_in(v[0][i])) continue;
+                const int b = sample_bin(set, v[0][i]);
                 if (b < whole) {
-                    const double w = sample_w(set, x);
+                    const double w = sample_w(set, v[0][i]);
                     if (w >= set.min_p) sum += sample_mass(w, a.shift);
-                } else if (b == lk || (b >= p0 && b <= p1)) {
-                    const unsigned int at = atomicAdd(&R.n_list, 1u);
-                    if (at < kSampleList)
-                        R.list[at] = (u64)~sample_key(x) << 32 | (u64)(i0 + 4 * kSampleT * j + i);
+                } else if (sample_border(C, b)) {
+                    border |= 1u << i;
                 }
             }
-        sum = sample_block_sum<kSampleT>(sum, su);
-        if (threadIdx.x == 0) a.seg_mass[row * a.segs + seg] = sum;
-    });
+            unsigned int at = sample_slots<3>(__builtin_popcount(border), &n_part);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (border >> i & 1) {
+                    const u64 e = sample_entry_of(v[0][i], (int64_t)q * (kSampleSeg / 4) + 4 * (lane + 64 * j) + i);
+                    if (at < kBinList) {
+                        part[at] = e;
+                    } else {               /* many equal logits */
+                        const unsigned int g = atomicAdd(&R.n_list, 1u);
+                        if (g < kSampleList) R.list[g] = e;
+                    }
+                    ++at;
+                }
+            sample_next<kSampleU>(v);
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        if (lane == 0 && sum) atomicAdd(&sums[q / 4 - s0], sum);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < s1 - s0; i += kBinT) a.seg_mass[row * a.segs + s0 + i] = sums[i];
+    const unsigned int n = n_part < kBinList ? n_part : kBinList;
+    if (threadIdx.x == 0 && n) part_at = atomicAdd(&R.n_list, n);
+    __syncthreads();
+    for (unsigned int i = threadIdx.x; i < n; i += kBinT)
+        if (part_at + i < kSampleList) R.list[part_at + i] = part[i];
 }
 
 constexpr int kPickT = 1024;
+/* Pass 4's LDS, in 8 bytes: the list [8192], the segments' masses [1024], 256 masses and counters (radix
+ * selection), the listed chunks' numbers [8192 / 2] */
+constexpr int kPickSeg = kSampleList, kPickMass = kPickSeg + kSampleMaxSegs, kPickCount = kPickMass + kSampleBins;
+constexpr int kPickWhich = kPickCount + kSampleBins / 2, kPickWords = kPickWhich + kSampleList / 2;
 
-/* Pass 4.  LDS: the list [8192], the segments' masses [1024], 256 counters and masses. */
 template <bool BF16>
 __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
     extern __shared__ __attribute__((aligned(16))) u64 smem[];
     u64* const list = smem;
-    u64* const segm = smem + kSampleList;
-    u64* const hmass = segm + kSampleMaxSegs;                     /* [256] */
-    unsigned int* const hcount = reinterpret_cast<unsigned int*>(hmass + 256);   /* [256] */
+    u64* const segm = smem + kPickSeg;
+    u64* const hmass = smem + kPickMass;                          /* [bins], or [256] of a radix pass */
+    unsigned int* const hcount = reinterpret_cast<unsigned int*>(smem + kPickCount);
     __shared__ u64 su[kPickT / 64];
     __shared__ float sf[kPickT / 64];
+    __shared__ SampleCut s_cut;
     __shared__ u64 s_a, s_b;
     __shared__ int s_i, s_j;
+    __shared__ unsigned int s_n, s_key;
     const int t = threadIdx.x;
     const int64_t row = blockIdx.x, V = a.P.V;
     const uint8_t* x = sample_row(a.P, row);
     int* const token = a.P.token + row * a.P.token_stride;
     float* const prob = a.P.prob ? a.P.prob + row * a.P.prob_stride : nullptr;
-    float top, low;
-    sample_range<kPickT>(a, row, sf, &top, &low);
-    const SampleSet set = sample_set(a, row, top, low);
+    /* the listed rows' chunk maxima, the first 4096 of them on their way before they are asked for */
+    const float* const cm = a.chunk_max + row * a.segs * kSampleSegChunks;
+    const int chunks = a.segs * kSampleSegChunks;
+    float cv[4];
+    auto load_chunks = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            cv[j] = i0 + t + kPickT * j < chunks ? cm[i0 + t + kPickT * j] : -__builtin_inff();
+    };
+    load_chunks(0);
+    SampleSet set = sample_set(a, row);
+    const float u = a.P.u[row * a.P.u_stride];
+    sample_range<kPickT>(a, row, sf, &set);
+    const float top = set.top;
+    const float* const q_max = a.q_max + row * 4 * a.segs;
     if (!sample_in(top)) {
         if (t == 0) {
             *token = -1;
@@ -422,8 +604,8 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
     if (set.greedy) {
         if (t == 0) s_i = a.segs;
         __syncthreads();
-        for (int i = t; i < a.segs; i += kPickT)
-            if (a.seg_max[row * a.segs + i] == top) atomicMin(&s_i, i);
+        for (int i = t; i < 4 * a.segs; i += kPickT)
+            if (q_max[i] == top) atomicMin(&s_i, i / 4);
         if (t == 0) s_j = kSampleSeg;
         __syncthreads();
         float v[4];
@@ -438,54 +620,253 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         }
         return;
     }
-    for (int i = t; i < a.segs; i += kPickT) segm[i] = a.seg_mass[row * a.segs + i];
     const SampleRow& R = a.rows[row];
-    const int kb = R.kb, pb_lo = R.pb_lo, pb_hi = R.pb_hi;
-    const bool cut_k = kb < kSampleBins, cut_p = pb_lo < kSampleBins;
+    /* top-k's border is in bins [kb_lo, C.kb] */
+    SampleCut C = {kSampleBins, kSampleBins, kSampleBins, 0, 0, 0, 0, 0};
+    int kb_lo = kSampleBins;
+    unsigned int n = 0;                            /* listed tokens */
+    if (set.plain) {
+        for (int i = t; i < a.segs; i += kPickT) {
+            double w = 0.0;
+#pragma unroll
+            for (int j = 4 * i; j < 4 * i + 4; ++j)
+                if (sample_in(q_max[j])) w += a.q_sum[row * 4 * a.segs + j] * sample_w(set, q_max[j]);
+            segm[i] = sample_mass(w, a.shift);
+        }
+    } else if (set.listed) {
+        /* top-k: k chunks have their largest logit in bins 0 .. last, so no token under the least of those
+         * is among the k.  min-p: none under max + T log(min_p) has w >= min_p (a millionth less for the
+         * roundings of log, exp and the products). */
+        int last = kSampleBins;
+        float least = -3.4028235e38f;              /* and no token under this one can be kept */
+        for (int i = t; i < a.segs; i += kPickT) segm[i] = 0;
+        for (int i = t; i < kSampleBins; i += kPickT) hcount[i] = 0;
+        if (t == 0) {
+            s_i = kSampleBins;                     /* fewer than k chunks */
+            s_j = 0;                               /* chunks */
+            s_n = 0;                               /* tokens */
+            s_key = 0xFFFFFFFFu;
+        }
+        __syncthreads();
+        if (set.use_k) {
+            for (int i0 = 0; i0 < chunks; i0 += 4 * kPickT) {
+                if (i0) load_chunks(i0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (sample_in(cv[j])) atomicAdd(&hcount[sample_bin(set, cv[j])], 1u);
+            }
+            if (chunks > 4 * kPickT) load_chunks(0);
+            __syncthreads();
+            const unsigned int c0 = hcount[2 * t], c1 = hcount[2 * t + 1];
+            u64 all;
+            const u64 c = sample_block_scan<kPickT>(c0 + c1, su, &all);
+            if (c < (u64)set.k && c + c0 + c1 >= (u64)set.k) s_i = c + c0 >= (u64)set.k ? 2 * t : 2 * t + 1;
+            hcount[2 * t] = hcount[2 * t + 1] = 0;
+            hmass[2 * t] = hmass[2 * t + 1] = 0;
+            __syncthreads();
+            last = s_i;
+        } else {
+            const double d = log(set.min_p) / set.inv_t;
+            const double l = (double)top + (d * 1.000001 - 1e-30);
+            least = l > -3.4028234e38 ? (float)l : least;
+        }
+        /* the chunks, then their tokens, 16 lanes a chunk */
+        unsigned int* const which = reinterpret_cast<unsigned int*>(smem + kPickWhich);
+        uint32_t low = 0xFFFFFFFFu;                /* as a key */
+        for (int i0 = 0; i0 < chunks; i0 += 4 * kPickT) {
+            unsigned int in = 0;
+            if (i0) load_chunks(i0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (cv[j] >= least && sample_bin(set, cv[j]) <= last) {
+                    in |= 1u << j;
+                    low = min(low, sample_key(cv[j]));
+                }
+            unsigned int at = sample_slots<3>(__builtin_popcount(in), reinterpret_cast<unsigned int*>(&s_j));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (in >> j & 1) {
+                    if (at < kSampleList) which[at] = (unsigned int)(i0 + t + kPickT * j);
+                    ++at;
+                }
+        }
+        if (last < kSampleBins) {
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) low = min(low, (uint32_t)__shfl_xor(low, off, 64));
+            if ((t & 63) == 0) atomicMin(&s_key, low);
+        }
+        __syncthreads();
+        if (last < kSampleBins) least = sample_value(s_key);
+        const int nc = s_j;
+        if (nc <= kSampleList) {
+            constexpr int U = 8;                   /* loads in flight a lane */
+            for (int c0 = t / 16; c0 - t / 16 < nc; c0 += kPickT / 16 * U) {
+                float v[U][4];
+                unsigned int in = 0;
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int c = c0 + kPickT / 16 * j;
+                    if (c < nc) {
+                        sample_ld4<BF16>(x, (int64_t)which[c] * kSampleChunk + 4 * (t & 15), V, v[j]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) v[j][i] = -__builtin_inff();
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) in += v[j][i] >= least;
+                unsigned int at = sample_slots<6>(in, &s_n);
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int c = c0 + kPickT / 16 * j;
+                    if (c >= nc) break;
+                    const unsigned int i0 = which[c] * kSampleChunk + 4 * (t & 15);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (v[j][i] >= least) {
+                            if (at < kSampleList) list[at] = sample_entry_of(v[j][i], i0 + i);
+                            ++at;
+                        }
+                }
+            }
+            __syncthreads();
+            n = s_n;
+            __syncthreads();
+        } else {
+            n = kSampleList + 1;
+        }
+        if (n <= kSampleList) {
+            /* the same cuts as from a whole row's bins, of the listed: what lies above the border bins
+             * is kept, the list is left with what lies in them */
+            if (set.use_k) {
+                for (int i = t; i < (int)n; i += kPickT) {
+                    const float v = sample_value(~(uint32_t)(list[i] >> 32));
+                    const int b = sample_bin(set, v);
+                    atomicAdd(&hcount[b], 1u);
+                    if (set.use_p) atomicAdd(&hmass[b], sample_mass(sample_w(set, v), a.shift));
+                }
+                __syncthreads();
+                sample_cut<kPickT>(set, hcount, hmass, su, &s_cut);
+                C = s_cut;
+            }
+            if (t == 0) s_n = 0;
+            const int whole = sample_whole(C);
+            for (int i0 = 0; i0 < (int)n; i0 += kPickT) {
+                const int i = i0 + t;
+                bool in = false;
+                u64 e = 0;
+                if (i < (int)n) {
+                    e = list[i];
+                    const float v = sample_value(~(uint32_t)(e >> 32));
+                    const int b = sample_bin(set, v);
+                    if (b < whole) {
+                        const double w = sample_w(set, v);
+                        if (w >= set.min_p) atomicAdd(&segm[(int)(uint32_t)e / kSampleSeg], sample_mass(w, a.shift));
+                    } else {
+                        in = sample_border(C, b);
+                    }
+                }
+                __syncthreads();                   /* the list is read up to here, and written up to here at most */
+                const unsigned int at = sample_slots<1>(in, &s_n);
+                if (in) list[at] = e;
+            }
+            __syncthreads();
+            n = s_n;
+            kb_lo = C.kb;
+        } else {
+            kb_lo = 0;
+            if (set.use_k) C.kb = kSampleBins - 1;
+            else kb_lo = kSampleBins;
+            if (set.use_p) {
+                C.pb_lo = 0;
+                C.pb_hi = kSampleBins - 1;
+            }
+        }
+    } else {
+        for (int i = t; i < a.segs; i += kPickT) segm[i] = a.seg_mass[row * a.segs + i];
+        C = R.cut;
+        kb_lo = C.kb;
+        n = R.n_list;
+        for (int i = t; i < (int)n && i < kSampleList; i += kPickT) list[i] = R.list[i];
+    }
+    const bool cut_k = C.kb < kSampleBins, cut_p = C.pb_lo < kSampleBins;
     /* the last kept token: its key, and its index among equal keys */
     uint32_t last_key = 0;
     int64_t last_idx = V;
-    if (cut_k || cut_p) {
-        const unsigned int n = R.n_list;
+    if (cut_k || cut_p || n > kSampleList) {
         if (n <= kSampleList) {
             int size = 2;
             while (size < (int)n) size *= 2;
-            for (int i = t; i < size; i += kPickT) list[i] = i < (int)n ? R.list[i] : ~(u64)0;
-            __syncthreads();
-            for (int k = 2; k <= size; k *= 2)                    /* bitonic, rising */
-                for (int j = k / 2; j > 0; j /= 2) {
-                    for (int i = t; i < size / 2; i += kPickT) {
-                        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
-                        const u64 p = list[lo], q = list[hi];
-                        if ((p > q) == ((lo & k) == 0)) {
-                            list[lo] = q;
-                            list[hi] = p;
+            /* Bitonic, rising.  Up to a token a lane in registers, by way of LDS only to another wave;
+             * past that in LDS, where a wave's 64 pairs at distance 64 or less are 128 tokens of its own
+             * and only wider steps need the barrier.  (480 tokens 7.5 us by barriers alone.) */
+            if (size <= kPickT) {
+                __syncthreads();
+                u64 e = t < (int)n ? list[t] : ~(u64)0;
+                for (int k = 2; k <= size; k *= 2)
+                    for (int j = k / 2; j > 0; j /= 2) {
+                        u64 o;
+                        if (j < 64) {
+                            o = __shfl_xor(e, j, 64);
+                        } else {
+                            __syncthreads();
+                            list[t] = e;
+                            __syncthreads();
+                            o = list[t ^ j];
+                        }
+                        const bool low = ((t & j) == 0) == ((t & k) == 0);
+                        e = (o < e) == low ? o : e;
+                    }
+                __syncthreads();
+                list[t] = e;
+            } else {
+                for (int i = (int)n + t; i < size; i += kPickT) list[i] = ~(u64)0;
+                __syncthreads();
+                for (int k = 2; k <= size; k *= 2)
+                    for (int j = k / 2; j > 0; j /= 2) {
+                        for (int i = t; i < size / 2; i += kPickT) {
+                            const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+                            const u64 p = list[lo], q = list[hi];
+                            if ((p > q) == ((lo & k) == 0)) {
+                                list[lo] = q;
+                                list[hi] = p;
+                            }
+                        }
+                        if (j > 64 || (j == 1 && k > 64)) {
+                            __syncthreads();
+                        } else {
+                            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                            __builtin_amdgcn_wave_barrier();
                         }
                     }
-                    __syncthreads();
-                }
+            }
+            __syncthreads();
             /* a lane has `each` tokens in a row of the sorted list */
             const int each = (size + kPickT - 1) / kPickT, e0 = t * each;
             int in_p = 0;                                         /* listed tokens of top-p's bins */
             u64 wk = 0, wp = 0;
             auto value = [&](int i) { return sample_value(~(uint32_t)(list[i] >> 32)); };
-            /* tokens of bin kb among the k; their positions start behind top-p's own bins */
-            const int need = cut_k ? set.k - R.count_k : 0;
+            const double w0 = e0 < (int)n ? sample_w(set, value(e0)) : 0.0;
+            auto weight = [&](int i) { return i == e0 ? w0 : sample_w(set, value(i)); };
+            /* tokens of bin C.kb among the k; their positions start behind top-p's own bins */
+            const int need = cut_k ? set.k - C.count_k : 0;
             int before_kb = 0;
             for (int i = e0; i < e0 + each && i < (int)n; ++i) {
                 const int b = sample_bin(set, value(i));
-                if (cut_p && b <= pb_hi) ++in_p;
-                if (cut_k && b < kb) ++before_kb;
+                if (cut_p && b <= C.pb_hi) ++in_p;
+                if (cut_k && b < kb_lo) ++before_kb;
             }
             u64 tmp;
             sample_block_scan<kPickT>((u64)in_p << 32 | (u64)before_kb, su, &tmp);
             in_p = (int)(tmp >> 32);
             before_kb = (int)(tmp & 0xFFFFFFFFu);
-            const int end_k = cut_k ? before_kb + need : (int)n;
+            const int end_k = cut_k && before_kb + need < (int)n ? before_kb + need : (int)n;
             int end = end_k;
             if (cut_p) {
                 for (int i = e0; i < e0 + each && i < (int)n; ++i) {
-                    const u64 w = sample_mass(sample_w(set, value(i)), a.shift);
+                    const u64 w = sample_mass(weight(i), a.shift);
                     if (cut_k && i >= before_kb && i < end_k) wk += w;
                     if (i < in_p) wp += w;
                 }
@@ -493,28 +874,23 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
                 mass_k = sample_block_sum<kPickT>(wk, su);
                 u64 run = sample_block_scan<kPickT>(wp, su, &all_p);
                 /* the mass that p is a share of: top-k's, or all */
-                u64 of = R.mass_k + mass_k;
-                if (!cut_k) {
-                    u64 m = 0;
-                    for (int i = t; i < kSampleBins; i += kPickT) m += R.mass[i];
-                    of = sample_block_sum<kPickT>(m, su);
-                }
+                const u64 of = cut_k ? C.mass_k + mass_k : C.total;
                 const u64 want = sample_share(set.p, of);
                 if (t == 0) s_i = in_p < end_k ? in_p : end_k;
                 __syncthreads();
-                run += R.mass_p;
+                run += C.mass_p;
                 for (int i = e0; i < e0 + each && i < in_p; ++i) {
                     if (run >= want) {                            /* enough before this one */
                         atomicMin(&s_i, i);
                         break;
                     }
-                    run += sample_mass(sample_w(set, value(i)), a.shift);
+                    run += sample_mass(weight(i), a.shift);
                 }
                 __syncthreads();
                 end = s_i;
             }
             for (int i = e0; i < e0 + each && i < end; ++i) {
-                const double w = sample_w(set, value(i));
+                const double w = weight(i);
                 if (w >= set.min_p) atomicAdd(&segm[(int)(uint32_t)list[i] / kSampleSeg], sample_mass(w, a.shift));
             }
             last_key = ~(uint32_t)(list[end - 1] >> 32);
@@ -609,27 +985,24 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             uint32_t key_k = 0;
             u64 keep_k = 0;
             if (cut_k) {
-                select(kb, kb, false, (u64)(set.k - R.count_k), &key_k, &above, &over, &same);
-                keep_k = (u64)(set.k - R.count_k) - above;
+                select(kb_lo, C.kb, false, (u64)(set.k - C.count_k), &key_k, &above, &over, &same);
+                keep_k = (u64)(set.k - C.count_k) - above;
+                if (keep_k > same) keep_k = same;  /* fewer than k tokens */
                 last_key = key_k;
                 keep = keep_k;
-                of = R.mass_k + over + keep * sample_mass(sample_w(set, sample_value(key_k)), a.shift);
+                of = C.mass_k + over + keep * sample_mass(sample_w(set, sample_value(key_k)), a.shift);
             }
             if (cut_p) {
-                if (!cut_k) {
-                    u64 m = 0;
-                    for (int i = t; i < kSampleBins; i += kPickT) m += R.mass[i];
-                    of = sample_block_sum<kPickT>(m, su);
-                }
-                const u64 want = sample_share(set.p, of) - R.mass_p;
-                select(pb_lo, pb_hi, true, want, &last_key, &above, &over, &same);
+                if (!cut_k) of = C.total;
+                const u64 want = sample_share(set.p, of) - C.mass_p;
+                select(C.pb_lo, C.pb_hi, true, want, &last_key, &above, &over, &same);
                 const u64 w = sample_mass(sample_w(set, sample_value(last_key)), a.shift);
                 keep = w ? (want - over + w - 1) / w : same;
                 if (keep > same) keep = same;
                 if (cut_k && last_key == key_k && keep > keep_k) keep = keep_k;
             }
-            last_idx = nth(last_key, keep);
-            const int whole = cut_p && pb_lo < kb ? pb_lo : kb;
+            if (cut_k || cut_p) last_idx = nth(last_key, keep);
+            const int whole = cut_p && C.pb_lo < kb_lo ? C.pb_lo : kb_lo;
             __syncthreads();
             for (int64_t i = 4 * t; i < V; i += 4 * kPickT) {
                 float v[4];
@@ -652,7 +1025,6 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
     u64 total;
     const u64 mine = t < a.segs ? segm[t] : 0;
     const u64 before = sample_block_scan<kPickT>(mine, su, &total);
-    const float u = a.P.u[row * a.P.u_stride];
     const double goal = __builtin_floor((u > 0.0f ? (double)u : 0.0) * (double)total);
     const u64 at = goal < (double)total ? (u64)goal : total - 1;
     const u64 r = at < total ? at : total - 1;
@@ -661,87 +1033,66 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         s_a = r - before;
     }
     __syncthreads();
-    float v[4];
-    const double whole_mass = (double)total * __longlong_as_double((long long)(1023 - a.shift) << 52);
-    if (r == 0) {
-        /* u at 0 or next to it, where masses under half of 2^-s decide: the running sum in f64, from
-         * the first token on (up to the first one that has a mass, at the latest) */
-        const double want = (u > 0.0f ? (double)u : 0.0) * whole_mass;
-        double done = 0.0;
-        for (int seg = 0; seg < a.segs; ++seg) {
-            const int64_t i1 = (int64_t)seg * kSampleSeg + 4 * t;
-            double wv[4], mine_d = 0.0;
-            sample_ld4<BF16>(x, i1, V, v);
+    /* Within the segment in f64: its kept tokens in order until their sum passes what is left of u's
+     * share, or the last one should a rounding leave none.  With u at 0 or next to it masses under half
+     * of 2^-s decide: from the first segment on, up to the first token that has a mass at the latest. */
+    const double unit = __longlong_as_double((long long)(1023 - a.shift) << 52);
+    const double whole_mass = (double)total * unit;
+    const bool first = r == 0;
+    const double rest = first ? (u > 0.0f ? (double)u : 0.0) * whole_mass : (double)s_a * unit;
+    double done = 0.0;
+    for (int seg = first ? 0 : s_i;; ++seg) {
+        const int64_t i0 = (int64_t)seg * kSampleSeg + 4 * t;
+        float v[4];
+        double w[4] = {0.0, 0.0, 0.0, 0.0}, sum = 0.0;
+        int any = -1;
+        sample_ld4<BF16>(x, i0, V, v);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t kk = sample_key(v[i]);
-                wv[i] = 0.0;
-                if (sample_in(v[i]) && (kk > last_key || (kk == last_key && i1 + i <= last_idx))) {
-                    wv[i] = sample_w(set, v[i]);
-                    if (!(wv[i] >= set.min_p)) wv[i] = 0.0;
-                }
-                mine_d += wv[i];
-            }
-            double in = mine_d;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t kk = sample_key(v[i]);
+            if (!sample_in(v[i]) || kk < last_key || (kk == last_key && i0 + i > last_idx)) continue;
+            w[i] = sample_w(set, v[i]);
+            if (!(w[i] >= set.min_p)) w[i] = 0.0;
+            if (w[i] > 0.0) any = 4 * t + i;
+            sum += w[i];
+        }
+        double in = sum;
 #pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const double o = __shfl_up(in, off, 64);
-                if ((t & 63) >= off) in += o;
-            }
-            __syncthreads();
-            if ((t & 63) == 63) su[t >> 6] = (u64)__double_as_longlong(in);
-            if (t == 0) s_j = kSampleSeg;
-            __syncthreads();
-            double run = done, seg_all = done;
-            for (int i = 0; i < kPickT / 64; ++i) {
-                if (i < t >> 6) run += __longlong_as_double((long long)su[i]);
-                seg_all += __longlong_as_double((long long)su[i]);
-            }
-            run += in - mine_d;
+        for (int off = 1; off < 64; off <<= 1) {
+            const double o = __shfl_up(in, off, 64);
+            if ((t & 63) >= off) in += o;
+        }
+        __syncthreads();                           /* s_i, s_a and the last segment's are read */
+        if ((t & 63) == 63) su[t >> 6] = (u64)__double_as_longlong(in);
+        if (t == 0) {
+            s_i = kSampleSeg;
+            s_j = -1;
+        }
+        __syncthreads();
+        double run = done + (in - sum);
+        for (int i = 0; i < kPickT / 64; ++i) {
+            const double o = __longlong_as_double((long long)su[i]);
+            if (i < t >> 6) run += o;
+            done += o;
+        }
+        int over = -1;                             /* the first past u's share: lanes are in index order */
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                run += wv[i];
-                if (wv[i] > 0.0 && run > want) {
-                    atomicMin(&s_j, 4 * t + i);
-                    break;
-                }
-            }
-            __syncthreads();
-            if (s_j < kSampleSeg) {
-                const int at_t = s_j >> 2, at_i = s_j & 3;
-                if (t == at_t) {
-                    *token = seg * kSampleSeg + s_j;
-                    if (prob) *prob = (float)((at_i == 0 ? wv[0] : at_i == 1 ? wv[1] : at_i == 2 ? wv[2] : wv[3]) / whole_mass);
-                }
-                return;
-            }
-            done = seg_all;
+        for (int i = 0; i < 4; ++i) {
+            run += w[i];
+            if (over < 0 && w[i] > 0.0 && run > rest) over = 4 * t + i;
+        }
+        const u64 m_over = __ballot(over >= 0), m_any = __ballot(any >= 0);
+        if (m_over && (t & 63) == __builtin_ctzll(m_over)) atomicMin(&s_i, over);
+        if (m_any && (t & 63) == 63 - __builtin_clzll(m_any)) atomicMax(&s_j, any);
+        __syncthreads();
+        if (first && s_i == kSampleSeg && seg + 1 < a.segs) continue;
+        const int pick = s_i < kSampleSeg ? s_i : s_j;
+        if (pick >= 0 && t == pick >> 2) {
+            *token = seg * kSampleSeg + pick;
+            const double wp = (pick & 3) == 0 ? w[0] : (pick & 3) == 1 ? w[1] : (pick & 3) == 2 ? w[2] : w[3];
+            if (prob) *prob = (float)(wp / whole_mass);
         }
         return;
-    }
-    const int64_t i0 = (int64_t)s_i * kSampleSeg + 4 * t;
-    const u64 rest = s_a;
-    u64 w[4], sum = 0, all;
-    double wd[4] = {0.0, 0.0, 0.0, 0.0};
-    sample_ld4<BF16>(x, i0, V, v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[i] = 0;
-        if (!sample_in(v[i])) continue;
-        const uint32_t kk = sample_key(v[i]);
-        if (kk < last_key || (kk == last_key && i0 + i > last_idx)) continue;
-        wd[i] = sample_w(set, v[i]);
-        if (wd[i] >= set.min_p) w[i] = sample_mass(wd[i], a.shift);
-        sum += w[i];
-    }
-    u64 run = sample_block_scan<kPickT>(sum, su, &all);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (run <= rest && rest < run + w[i]) {
-            *token = (int)(i0 + i);
-            if (prob) *prob = (float)(wd[i] / whole_mass);
-        }
-        run += w[i];
     }
 }
 
@@ -757,22 +1108,26 @@ static int sample_entry(const RadArgs* ra, RadStream s) {
     a.segs = (int)((V + kSampleSeg - 1) / kSampleSeg);
     a.rows = (SampleRow*)ra->scratch;
     a.seg_mass = (u64*)(a.rows + M);
-    a.seg_max = (float*)(a.seg_mass + M * a.segs);
-    a.seg_min = a.seg_max + M * a.segs;
+    a.q_sum = (double*)(a.seg_mass + M * a.segs);
+    a.q_max = (float*)(a.q_sum + 4 * M * a.segs);
+    a.q_min = a.q_max + 4 * M * a.segs;
+    a.chunk_max = a.q_min + 4 * M * a.segs;
     int bits = 0;                                  /* V <= 2^bits: V 2^(62 - bits) <= 2^62 */
     while (((int64_t)1 << bits) < V) ++bits;
     a.shift = 62 - bits;
-    /* a workgroup a segment while that makes no more than 2048 of them */
-    a.per = (int)((a.segs * M + 2047) / 2048);
+    a.per = (int)((a.segs * M + 2047) / 2048);      /* a workgroup a segment while that makes 2048 at most */
     if (a.per > a.segs) a.per = a.segs;
     const dim3 grid((unsigned)((a.segs + a.per - 1) / a.per), (unsigned)M);
-    const size_t lds = (kSampleList + kSampleMaxSegs + 256) * 8 + 256 * 4;
+    const int64_t shares = (int64_t)((a.segs + kBinLeast - 1) / kBinLeast) * M;
+    const dim3 bgrid((unsigned)(shares < kBinGrid ? shares : M > kBinGrid ? M : kBinGrid));
+    const size_t lds = kPickWords * 8;
     hipStream_t stream = (hipStream_t)s;
-#define R3D_SAMPLE(B_)                                                                        \
-    hipLaunchKernelGGL((sample_range_kernel<B_>), grid, dim3(kSampleT), 0, stream, a);          \
-    if (a.P.top_k || a.P.top_p)                                                                \
-        hipLaunchKernelGGL((sample_hist_kernel<B_>), grid, dim3(kSampleT), 0, stream, a);       \
-    hipLaunchKernelGGL((sample_gather_kernel<B_>), grid, dim3(kSampleT), 0, stream, a);         \
+#define R3D_SAMPLE(B_)                                                                          \
+    hipLaunchKernelGGL((sample_range_kernel<B_>), grid, dim3(kSampleT), 0, stream, a);            \
+    if (a.P.top_k || a.P.top_p) {                                                                \
+        hipLaunchKernelGGL((sample_hist_kernel<B_>), bgrid, dim3(kBinT), 0, stream, a);           \
+        hipLaunchKernelGGL((sample_gather_kernel<B_>), bgrid, dim3(kBinT), 0, stream, a);         \
+    }                                                                                            \
     hipLaunchKernelGGL((sample_pick_kernel<B_>), dim3((unsigned)M), dim3(kPickT), lds, stream, a)
     if (a.P.bf16) { R3D_SAMPLE(true); } else { R3D_SAMPLE(false); }
 #undef R3D_SAMPLE

@@ -22,7 +22,7 @@ static int column(const RadTensor* t, uint32_t dtype, int64_t M, bool out, int64
 
 int64_t sample_scratch_bytes(int64_t M, int64_t V) {
     const int64_t segs = (V + kSampleSeg - 1) / kSampleSeg;
-    return M * ((int64_t)sizeof(SampleRow) + segs * 16);
+    return M * ((int64_t)sizeof(SampleRow) + segs * (8 + 4 * 16 + 4 * kSampleSegChunks));
 }
 
 int plan_sample(const RadArgs* a, SamplePlan* P) {

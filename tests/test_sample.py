@@ -84,7 +84,7 @@ def test_scratch_hook():
     one = R.row_scratch_bytes(ROW, ops(M=1, V=4096))
     assert one > 0 and one % 8 == 0
     assert R.row_scratch_bytes(ROW, ops(M=7, V=4096)) == 7 * one
-    assert R.row_scratch_bytes(ROW, ops(M=1, V=4097)) == one + 16
+    assert R.row_scratch_bytes(ROW, ops(M=1, V=4097)) == one + 8 + 64 + 256
     o = ops()
     o._p[0].ival = 1 << 40
     assert R.row_scratch_bytes(ROW, o) == 0
