@@ -8,7 +8,7 @@
  * kept mass.  T <= 0 (or NaN) takes the lowest index of the maximum.  A row with nothing in it gives
  * token -1 and probability 0.
  *
- * Masses are 64-bit integers, w * 2^s to nearest with V 2^s < 2^63 (s = 44 at V = 262144), from an
+ * Masses are 64-bit integers, w * 2^s to nearest with V 2^s < 2^63, s <= 51 (44 at V = 262144), from an
  * exp in f64: integer sums do not depend on their order, so atomics may make them, a cut and the
  * search see the same numbers, and a run repeats bit for bit.  A border moves by about
  * 2^-s sqrt(V) / mass, 2^-35 at V = 262144, where f32 sums would move it by 2^-20 and pick a
@@ -31,10 +31,10 @@
  * Passes 2 and 3 are not launched without a top-k or top-p operand.
  *
  * Bound by the one read of the row in pass 1 and by the four launches' chains of dependent loads.
- * Measured on MI355X at V = 262144, f32: one row 21.6 us; 128 rows, each with settings of its own, 106 us
- * (of which pass 1's read of 134 MB 31 to 37 us, 3.6 to 4.4 TB/s; passes 2 and 3 for the 22 rows that have a
- * use for them 20 and 24, f64 exps; pass 4 32, of them 8 to list 1000 chunks).  With bins for every row, no chunks
- * and a sort that waited at a barrier for every step the same took 27.7 and 143 us. */
+ * Measured on MI355X at V = 262144, f32: one row 22 us; 128 rows, each with settings of its own, 94 us (of
+ * which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22 rows that have a use for
+ * them, 18 and 22; pass 4 29, of them 8 to list 1000 chunks).  With bins for every row, no chunks and a sort
+ * that waited at a barrier for every step the same took 27.7 and 143 us. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -127,7 +127,14 @@ __device__ __forceinline__ bool sample_in(float x) { return x > -__builtin_inff(
 __device__ __forceinline__ double sample_w(const SampleSet& s, float x) {
     return x == s.top ? 1.0 : sample_exp(((double)x - (double)s.top) * s.inv_t);
 }
+/* w 2^shift to nearest, w 2^shift < 2^52: in the low bits of w 2^shift + 2^52. */
 __device__ __forceinline__ u64 sample_mass(double w, int shift) {
+    const double big = 4503599627370496.0;
+    return (u64)__double_as_longlong(__builtin_fma(w, __longlong_as_double((long long)(1023 + shift) << 52), big)) -
+           (u64)__double_as_longlong(big);
+}
+/* The same to 2^63, for sums. */
+__device__ __forceinline__ u64 sample_mass_sum(double w, int shift) {
     return (u64)__builtin_rint(w * __longlong_as_double((long long)(1023 + shift) << 52));
 }
 __device__ __forceinline__ int sample_bin(const SampleSet& s, float x) {
@@ -185,10 +192,36 @@ __device__ __forceinline__ void sample_next(float (*v)[4]) {
         for (int i = 0; i < 4; ++i) v[j][i] = v[j + 1][i];
 }
 
+/* The largest over each 16 lanes, by rotations of the register (no lane waits for LDS). */
+__device__ __forceinline__ float sample_max16(float v) {
+#define R3D_ROTATE(N_) \
+    v = __builtin_fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x120 + N_, 15, 15, true)))
+    R3D_ROTATE(8); R3D_ROTATE(4); R3D_ROTATE(2); R3D_ROTATE(1);
+#undef R3D_ROTATE
+    return v;
+}
+
+/* The sum over this lane and the ones before it in the wave, by row shifts and broadcasts. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 sample_moved(u64 v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 15, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 15, false);
+    return (u64)hi << 32 | lo;
+}
+template <class V>
+__device__ __forceinline__ V sample_wave_scan(V v) {
+#define R3D_STEP(CTRL_, ROWS_) v += __builtin_bit_cast(V, sample_moved<CTRL_, ROWS_>(__builtin_bit_cast(u64, v)))
+    R3D_STEP(0x111, 15); R3D_STEP(0x112, 15); R3D_STEP(0x114, 15); R3D_STEP(0x118, 15);   /* within 16 lanes */
+    R3D_STEP(0x142, 10); R3D_STEP(0x143, 12);                       /* the 16 before, the 32 before */
+#undef R3D_STEP
+    return v;
+}
+
 template <int T>
 __device__ __forceinline__ float sample_block_max(float v, float* s) {
+    v = sample_max16(v);
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off, 64));
+    for (int off = 32; off >= 16; off >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off, 64));
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -198,10 +231,9 @@ __device__ __forceinline__ float sample_block_max(float v, float* s) {
 }
 template <int T>
 __device__ __forceinline__ u64 sample_block_sum(u64 v, u64* s) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    v = sample_wave_scan(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) s[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
 #pragma unroll
@@ -211,13 +243,8 @@ __device__ __forceinline__ u64 sample_block_sum(u64 v, u64* s) {
 /* The sum over the lanes before this one; *total over all. */
 template <int T>
 __device__ __forceinline__ u64 sample_block_scan(u64 v, u64* s, u64* total) {
-    u64 in = v;
+    const u64 in = sample_wave_scan(v);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const u64 o = __shfl_up(in, off, 64);
-        if (lane >= off) in += o;
-    }
     __syncthreads();
     if (lane == 63) s[wave] = in;
     __syncthreads();
@@ -294,15 +321,15 @@ __global__ __launch_bounds__(kSampleT) void sample_range_kernel(SampleArgs a) {
                 m = __builtin_fmaxf(m, v[j][i]);                      /* a NaN is passed over */
                 lo = __builtin_fminf(lo, sample_in(v[j][i]) ? v[j][i] : lo);
             }
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, off, 64));
+            m = sample_max16(m);
             if ((lane & 15) == 0) cm[lane / 16 + 4 * j] = m;
             hi = __builtin_fmaxf(hi, m);
         }
 #pragma unroll
         for (int off = 32; off >= 16; off >>= 1) hi = __builtin_fmaxf(hi, __shfl_xor(hi, off, 64));
+        lo = -sample_max16(-lo);
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) lo = __builtin_fminf(lo, __shfl_xor(lo, off, 64));
+        for (int off = 32; off >= 16; off >>= 1) lo = __builtin_fminf(lo, __shfl_xor(lo, off, 64));
         if (lane == 0) {
             a.q_max[row * 4 * a.segs + q] = hi;
             a.q_min[row * 4 * a.segs + q] = lo;
@@ -318,16 +345,15 @@ __global__ __launch_bounds__(kSampleT) void sample_range_kernel(SampleArgs a) {
                     if (sample_in(v[0][i])) sum += sample_w(here, v[0][i]);
                 sample_next<kSampleU>(v);
             }
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-            if (lane == 0) a.q_sum[row * 4 * a.segs + q] = sum;
+            sum = sample_wave_scan(sum);
+            if (lane == 63) a.q_sum[row * 4 * a.segs + q] = sum;
         }
     }
 }
 
 /* Passes 2 and 3, a wave a quarter of a segment at a time.  The binned rows are dealt out to
- * all workgroups, a row to as many as there are for it.  (A grid over every row's parts took 16 us of a
- * 26 us launch to start the workgroups of the 106 other rows of 128 and see them end.) */
+ * all workgroups, a row to as many as there are for it.  (Over every row's parts, where 22 of 128 rows
+ * have something to do, some CUs had two or three of those and others none: 26 us for 17.) */
 constexpr int kBinT = 1024, kBinWaves = kBinT / 64, kBinGrid = 256, kBinLeast = kBinWaves / 4;
 constexpr unsigned int kBinList = 2048;
 struct SampleShare {
@@ -542,9 +568,8 @@ __global__ __launch_bounds__(kBinT) void sample_gather_kernel(SampleArgs a) {
                 }
             sample_next<kSampleU>(v);
         }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        if (lane == 0 && sum) atomicAdd(&sums[q / 4 - s0], sum);
+        sum = sample_wave_scan(sum);
+        if (lane == 63 && sum) atomicAdd(&sums[q / 4 - s0], sum);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < s1 - s0; i += kBinT) a.seg_mass[row * a.segs + s0 + i] = sums[i];
@@ -631,7 +656,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
 #pragma unroll
             for (int j = 4 * i; j < 4 * i + 4; ++j)
                 if (sample_in(q_max[j])) w += a.q_sum[row * 4 * a.segs + j] * sample_w(set, q_max[j]);
-            segm[i] = sample_mass(w, a.shift);
+            segm[i] = sample_mass_sum(w, a.shift);
         }
     } else if (set.listed) {
         /* top-k: k chunks have their largest logit in bins 0 .. last, so no token under the least of those
@@ -1056,12 +1081,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             if (w[i] > 0.0) any = 4 * t + i;
             sum += w[i];
         }
-        double in = sum;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double o = __shfl_up(in, off, 64);
-            if ((t & 63) >= off) in += o;
-        }
+        const double in = sample_wave_scan(sum);
         __syncthreads();                           /* s_i, s_a and the last segment's are read */
         if ((t & 63) == 63) su[t >> 6] = (u64)__double_as_longlong(in);
         if (t == 0) {
@@ -1114,8 +1134,10 @@ static int sample_entry(const RadArgs* ra, RadStream s) {
     a.chunk_max = a.q_min + 4 * M * a.segs;
     int bits = 0;                                  /* V <= 2^bits: V 2^(62 - bits) <= 2^62 */
     while (((int64_t)1 << bits) < V) ++bits;
-    a.shift = 62 - bits;
-    a.per = (int)((a.segs * M + 2047) / 2048);      /* a workgroup a segment while that makes 2048 at most */
+    a.shift = 62 - bits < 51 ? 62 - bits : 51;
+    /* a workgroup a segment while that makes 16384 at most (128 rows of 64: 29 us; four a workgroup, which
+     * leaves a last round of few workgroups, 36) */
+    a.per = (int)((a.segs * M + 16383) / 16384);
     if (a.per > a.segs) a.per = a.segs;
     const dim3 grid((unsigned)((a.segs + a.per - 1) / a.per), (unsigned)M);
     const int64_t shares = (int64_t)((a.segs + kBinLeast - 1) / kBinLeast) * M;
