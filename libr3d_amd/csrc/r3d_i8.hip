@@ -30,7 +30,7 @@ static int i8_failed(const char* what, hipError_t e) {
 static int i8_launch_any(const I8Plan& P, hipStream_t stream) {
     const int tm = P.M <= 16 ? 1 : 2;
     const int64_t gx = (P.N + 127) / 128, gy = (P.M + 16 * tm - 1) / (16 * tm);
-    if (gy > 65535) return RAD_E_SHAPE;
+    if (gy > 65535) return RAD_E_UNSUPPORTED;
     const dim3 grid((unsigned)gx, (unsigned)gy), block(256);
 #define R3D_I8_ANY(TM_)                                                                       \
     hipLaunchKernelGGL((i8_any_kernel<TM_>), grid, block, 0, stream, P.A, P.SA, P.B, P.SB, P.Y, \

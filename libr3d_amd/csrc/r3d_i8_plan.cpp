@@ -93,6 +93,7 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
     /* the fast kernels move 16 bytes a lane and walk 256 rows with 32-bit offsets */
     P->ua = (K & 15) || (((uintptr_t)P->A | (uintptr_t)P->B) & 15) ||
             ((P->a_pitch | P->b_pitch) & 15) || P->a_pitch > (1 << 22) || P->b_pitch > (1 << 22);
+    if (P->ua && M > 65535 * 32) return RAD_E_UNSUPPORTED;     /* its grid's second axis */
     return RAD_OK;
 }
 
@@ -157,8 +158,8 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
         for (int64_t kc : {1, 2, 3, 4, 5, 6, 8, 12, 16, 24}) {
             if (kc > 1 && steps / kc < 3) break;
             const int64_t per = (steps + kc - 1) / kc;
-            if ((steps + per - 1) / per != kc || tiles * kc > 0x7FFFFFFF) continue;
-            if (kc > 1 && (tiles * kc > 4 * ncu || kc * P.M * P.N * 4 > scratch)) break;
+            if ((steps + per - 1) / per != kc || tiles * kc > 0x7FFFFF) continue;      /* 2^32 lanes a launch */
+            if (kc > 1 && (P.M > 65535 || tiles * kc > 4 * ncu || kc * P.M * P.N * 4 > scratch)) break;
             const int64_t ns = i8_tile_ns(c, P.M, P.N, P.K, per, kc, ncu);
             if (best && ns >= best) continue;
             best = ns;
@@ -260,6 +261,7 @@ int plan_i8_band(const RadArgs* a, int op, I8BandPlan* P) {
     P->eps = rad_args_getf_or(a, "eps", 1e-6);
     P->wadd = (float)rad_args_getf_or(a, "wadd", 0.0);
     if (!(P->eps >= 0.0)) return RAD_E_INVAL;
+    if (rows * i8_band_geom(rows, n).lanes > 0xFFFFFFFFLL) return RAD_E_UNSUPPORTED;   /* lanes a launch */
     return RAD_OK;
 }
 
