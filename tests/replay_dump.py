@@ -15,6 +15,9 @@ PRE state, and those are compared with the POST state the GPU wrote:
   logits_gemm_e4m3                                       the planes out of the captured
       joined head, the logits within the row's bound (its MFMA sums and the oracle's
       f32 chain: (140 + 2 ceil(K/256) + K) 2^-24 S), NaN classes equal
+  gemm_nt_q (i8a8), quant_act_i8, gated_quant_i8, rmsnorm_quant_i8, sample_logits
+      in float64 on their own (tests/replay_rows.py): the product bit for bit, codes and
+      scales within their roundings, tokens equal
 --device re-launches each capture through libr3d_gfx950.so on a GPU instead (operands
 rebuilt from PRE at the same offsets, the same parameters, tunables and scratch size) and
 requires the outputs to equal POST byte for byte: the kernels are deterministic.
@@ -373,6 +376,9 @@ def check_logits(c, O):
 def replay_oracle(c):
     import oracle as O
     from tests import gpu_util as gu       # the comparison helpers (numpy only here)
+    if c.row.endswith("_i8") or c.row.startswith("gemm_nt_q_i8a8") or c.row == "sample_logits":
+        from tests import replay_rows
+        return replay_rows.check(c)
     if c.row.startswith("gemm_nt_q_gated"):
         return check_gemm_gated(c, O, gu)
     if c.row.startswith("gemm_nt_q"):
