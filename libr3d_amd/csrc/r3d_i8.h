@@ -34,7 +34,7 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P);
 
 /* Which kernel a call takes, and its launch. */
 enum { I8_ANY = 0, I8_GEMV = 1, I8_TILE = 2 };
-enum { I8_T_256x256, I8_T_128x256, I8_T_128x128, I8_T_128x64, I8_T_64x64, I8_T_64x32, I8_TILES };
+enum { I8_T_256x256, I8_T_128x256, I8_T_128x192, I8_T_128x128, I8_T_128x96, I8_T_128x64, I8_T_64x64, I8_T_64x32, I8_TILES };
 
 struct I8Geom {
     int arm;

@@ -78,7 +78,9 @@ static int i8_launch_tile(const I8Plan& P, const I8Geom& g, int* part, hipStream
             hipLaunchKernelGGL(i8_wide_kernel, grid, dim3(512), (size_t)i8_tile_lds(256, 256, 2), stream, a);
             break;
         case I8_T_128x256: R3D_I8T(4, 4, 2, 4, 3); break;
+        case I8_T_128x192: R3D_I8T(2, 6, 4, 2, 3); break;
         case I8_T_128x128: R3D_I8T(2, 4, 4, 2, 4); break;
+        case I8_T_128x96: R3D_I8T(2, 6, 4, 1, 4); break;
         case I8_T_128x64: R3D_I8T(2, 4, 4, 1, 4); break;
         case I8_T_64x64: R3D_I8T(1, 4, 4, 1, 4); break;
         default: R3D_I8T(1, 2, 4, 1, 6); break;

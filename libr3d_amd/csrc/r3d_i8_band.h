@@ -10,10 +10,10 @@
  *   q    = rint(h * (1 / s)), to nearest even, within +-127
  *
  * h is quantised as it stands in f32 (the e4m3 producers beside these narrow it to bf16 first, as
- * the kernels that they follow do; here the narrowing would only move codes).  The 2^-126 keeps 1 / s finite.  The maximum is taken
- * over the magnitudes' bits, where an infinity is above every number and a NaN above that: a row
- * with a NaN has scale NaN and one with an infinity scale inf, both with codes 0, so the product
- * over the row is NaN and not a number that hides them.
+ * the kernels that they follow do; here the narrowing would only move codes).  The 2^-126 keeps 1 / s
+ * finite.  The maximum is taken over the magnitudes' bits, where an infinity is above every number and
+ * a NaN above that: a row with a NaN has scale NaN and one with an infinity scale inf, both with codes
+ * 0, so the product over the row is NaN and not a number that hides them.
  *
  * One workgroup a row, the row in registers (C chunks of 8 elements a lane) from the load to the
  * codes: every operand is read once and every result written once, which is all the traffic there

@@ -99,7 +99,10 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
 
 /* What a launch of a tile takes, in ns: least squares over 2426 shapes (M 5..2048, N 512..21504, K
  * 512..21504) and 4 to 40 launches of each, rows starting on 128-byte lines or not; the pick is 2.8 %
- * slower than the best of 17 tiles on average (geometric), 10 % at the ninth decile.
+ * slower than the best of 17 tiles on average (geometric), 10 % at the ninth decile.  192 and 96 tokens,
+ * from 10020 shapes of 33..2048 tokens, are for where they fill the compute units and powers of two do
+ * not: taken by 19 % of those shapes, 8 % faster there (512 x 5376 x 5376 27.5 -> 23.6 us, 1024 x 5376 x 5376
+ * 49.9 -> 41.8).
  *     a + max(ceil(units / ncu) * q * steps a unit, weights / rate) + the planes and their sum
  * rate: 5.2 TB/s, or what the units in flight stream, `one` bytes a us each where every weight byte
  * comes from memory (one tile of tokens), `more` where tiles of tokens share them in L2.  K off 128
@@ -111,7 +114,9 @@ struct I8Cost {
 static const I8Cost kI8Cost[I8_TILES] = {
     {256, 256, 1, 8107, 1065, 119, 30500, 48300},
     {128, 256, 1, 4835,  888, 120, 48300, 30600},
+    {128, 192, 1, 3428,  823, 115, 20000, 20000},
     {128, 128, 1, 4312,  474, 126, 46300, 18800},
+    {128,  96, 1, 3955,  443, 122, 74000, 36800},
     {128,  64, 1, 3351,  398, 123, 59300, 49200},
     { 64,  64, 2, 3147,  246, 120, 27400, 30500},
     { 64,  32, 2, 2896,  202, 111, 42700, 28700},

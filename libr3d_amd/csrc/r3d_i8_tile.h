@@ -4,9 +4,10 @@
  * 16 WNF x 16 WMF of them, v_mfma_i32_16x16x64_i8 with the weights as source A, so lane l's result
  * is four consecutive weight rows of one token.  K is walked 128 a step.  A step's operands go
  * straight from memory to LDS (buffer loads, 16 bytes a lane) into a ring of NST stages; each 1 KB
- * load is the image of one MFMA operand: 16 rows x 64 bytes, four lanes a row, the 16-byte piece
- * swizzled by (row / 2) % 4, so an operand read (ds_read_b128) touches every bank group once in any
- * 8 lanes.  Rows past the operands clamp to the last (their results are not stored); columns past K
+ * load is 8 rows of 128 bytes, so that it asks for whole cache lines (with 16 rows of half a line the
+ * loads were the bound), the 16-byte piece of a row at place piece ^ row
+ * % 8: an operand read (ds_read_b128) touches every bank group once in any 8 lanes.  Rows past the
+ * operands clamp to the last (their results are not stored); columns past K
  * (K % 128 = 16 .. 112) are asked for past the buffer's records and land as zeros.
  *
  * One barrier a step: it says both that the next step's stage has landed (each wave has waited for
@@ -16,6 +17,11 @@
  *
  * The sum is exact in i32, so K may be cut anywhere: with kc > 1 workgroup u takes K chunk
  * u / tiles of its tile and leaves an i32 plane, and i8_join_kernel adds the planes.
+ *
+ * Measured on MI355X (a 16384 x 16384 x 8192 product of the library's reaches 2.39 POP/s, a 1 GiB copy 5.14
+ * TB/s): M = 13 x 5376 x 21504 26 us, 4.4 TB/s, bound by the weights; M = 333 x 8187 x 5360 24 us, 1.2 POP/s:
+ * 256 tiles of 128 x 96, an eighth of them past the edges, and a K off 128 asks for two lines a row (the
+ * weights cold 31.8 us; K = 5376 24.2).  A step of a 128 x 128 tile takes 0.47 us a compute unit, 8.9 TOP/s of its 9.3.
  */
 #ifndef R3D_I8_TILE_H
 #define R3D_I8_TILE_H

@@ -11,8 +11,9 @@
  *   rmsnorm_quant_i8         prio 1000  n GE 1, dtype IN bf16               norm producer
  *   sample_logits            prio 1000  n_vocab GE 1, dtype IN f32 bf16     sampler
  *
- * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row, R3D_NO_SAMPLE the
- * sampler (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row, R3D_NO_SAMPLE the sampler
+ * (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is
+ * rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
