@@ -34,7 +34,10 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P);
 
 /* Which kernel a call takes, and its launch. */
 enum { I8_ANY = 0, I8_GEMV = 1, I8_TILE = 2 };
-enum { I8_T_256x256, I8_T_128x256, I8_T_128x192, I8_T_128x128, I8_T_128x96, I8_T_128x64, I8_T_64x64, I8_T_64x32, I8_TILES };
+enum {
+    I8_T_256x256, I8_T_128x256, I8_T_128x192, I8_T_128x128, I8_T_128x96, I8_T_128x64, I8_T_64x64,
+    I8_T_64x32, I8_T_32x32, I8_T_32x16, I8_TILES
+};
 
 struct I8Geom {
     int arm;
@@ -50,8 +53,9 @@ struct I8Geom {
 
 /* GEMV: the tokens in LDS, rows this many bytes apart */
 constexpr int64_t i8_gemv_row(int64_t K) { return ((K + 127) & ~(int64_t)127) + 16; }
-/* and at most this much of it.  Up to it the GEMV takes 0.65 to 0.98 of the tiles' time (M 1..8, 430
- * shapes, by M and 8 KB of tokens); with 56 KB and more, two workgroups a compute unit, 1.05 to 1.4 */
+/* and at most this much of it.  Up to it the GEMV takes 0.85 to 1.07 of the tiles' time at M 5..8 (2295
+ * shapes, by M and 8 KB of tokens; under 8 KB the 1.03 to 1.07), less below; with 56 KB and more, two
+ * workgroups a compute unit, 1.05 to 1.4 */
 constexpr int64_t kI8GemvLds = 48 * 1024;
 
 /* The launch that suits a shape on ncu compute units, with at most `scratch` bytes for planes. */

@@ -83,7 +83,9 @@ static int i8_launch_tile(const I8Plan& P, const I8Geom& g, int* part, hipStream
         case I8_T_128x96: R3D_I8T(2, 6, 4, 1, 4); break;
         case I8_T_128x64: R3D_I8T(2, 4, 4, 1, 4); break;
         case I8_T_64x64: R3D_I8T(1, 4, 4, 1, 4); break;
-        default: R3D_I8T(1, 2, 4, 1, 6); break;
+        case I8_T_64x32: R3D_I8T(1, 2, 4, 1, 6); break;
+        case I8_T_32x32: R3D_I8T(1, 2, 2, 1, 10); break;
+        default: R3D_I8T(1, 1, 2, 1, 8); break;
     }
 #undef R3D_I8T
     hipError_t e = hipGetLastError();

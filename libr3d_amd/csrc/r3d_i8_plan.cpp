@@ -1,6 +1,7 @@
 /* r3d_i8_plan.cpp -- host plans of the int8 rows (see r3d_i8.h). */
 #include "r3d_i8.h"
 
+#include <math.h>
 #include <stdio.h>
 #include <stdlib.h>
 #include <string.h>
@@ -97,40 +98,46 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
     return RAD_OK;
 }
 
-/* What a launch of a tile takes, in ns: least squares over 2426 shapes (M 5..2048, N 512..21504, K
- * 512..21504) and 4 to 40 launches of each, rows starting on 128-byte lines or not; the pick is 2.8 %
- * slower than the best of 17 tiles on average (geometric), 10 % at the ninth decile.  192 and 96 tokens,
- * from 10020 shapes of 33..2048 tokens, are for where they fill the compute units and powers of two do
- * not: taken by 19 % of those shapes, 8 % faster there (512 x 5376 x 5376 27.5 -> 23.6 us, 1024 x 5376 x 5376
- * 49.9 -> 41.8).
- *     a + max(ceil(units / ncu) * q * steps a unit, weights / rate) + the planes and their sum
- * rate: 5.2 TB/s, or what the units in flight stream, `one` bytes a us each where every weight byte
- * comes from memory (one tile of tokens), `more` where tiles of tokens share them in L2.  K off 128
- * starts rows inside lines, and a step of 128 bytes then takes two lines: q * mis / 100. */
+/* What a launch of a tile takes, in ns:
+ *     a + sqrt(work^2 + stream^2) + the planes and their sum
+ *     work: ceil(units / ncu) * q * steps a unit; K off 128 starts rows inside lines, and a step of 128
+ *           bytes then takes two lines: * mis / 100
+ *     stream: the weights at 6.12 TB/s, or at what the units in flight ask for, `one` bytes a us each
+ *           with one tile of tokens, `more` where tiles of tokens share them in L2
+ * Least squares over 5230 shapes (M 9..2048, N and K 512..21504) and 4 to 40 launches of each.  The pick is
+ * 1.6 % slower than the best launch on average (geometric), 7 % at the ninth decile; with the larger of
+ * work and stream in place of the root 2.8 % and 11 %.
+ * Powers of two alone leave compute units idle at common widths: tiles of 96 and 192 tokens are taken by a
+ * fifth of the shapes, 8 % faster there (512 x 5376 x 5376 27.5 -> 23.6 us, 1024 x 5376 x 5376 49.9 -> 41.8).
+ * Tiles of 32 weight rows cover few tokens in as many workgroups as two planes of 64 (13 x 8192 x 5376 12.8
+ * -> 10.3 us, 12 x 5376 x 4096 9.7 -> 7.9). */
 struct I8Cost {
     int bn, bm, resident;    /* workgroups a compute unit holds (LDS) */
     int a, q, mis, one, more;
 };
+constexpr int kI8Any = 1000000;                                     /* a unit's rate never the bound */
 static const I8Cost kI8Cost[I8_TILES] = {
-    {256, 256, 1, 8107, 1065, 119, 30500, 48300},
-    {128, 256, 1, 4835,  888, 120, 48300, 30600},
-    {128, 192, 1, 3428,  823, 115, 20000, 20000},
-    {128, 128, 1, 4312,  474, 126, 46300, 18800},
-    {128,  96, 1, 3955,  443, 122, 74000, 36800},
-    {128,  64, 1, 3351,  398, 123, 59300, 49200},
-    { 64,  64, 2, 3147,  246, 120, 27400, 30500},
-    { 64,  32, 2, 2896,  202, 111, 42700, 28700},
+    {256, 256, 1, 8244, 1034, 119, kI8Any, kI8Any},
+    {128, 256, 1, 4783,  852, 122, kI8Any, kI8Any},
+    {128, 192, 1, 3379,  776, 116, kI8Any,  21400},
+    {128, 128, 1, 4258,  445, 131, kI8Any, kI8Any},
+    {128,  96, 1, 3856,  422, 124, kI8Any, kI8Any},
+    {128,  64, 1, 3480,  343, 131, kI8Any, kI8Any},
+    { 64,  64, 2, 3242,  226, 123, kI8Any, kI8Any},
+    { 64,  32, 2, 3052,  175, 118, kI8Any, kI8Any},
+    { 32,  32, 2, 3319,  134, 112,  65500,  26700},
+    { 32,  16, 3, 3088,   96, 116,  43100,  19400},
 };
 
-static int64_t i8_tile_ns(const I8Cost& c, int64_t M, int64_t N, int64_t K, int64_t per, int64_t kc,
-                          int ncu) {
+static double i8_tile_ns(const I8Cost& c, int64_t M, int64_t N, int64_t K, int64_t per, int64_t kc,
+                         int ncu) {
     const int64_t gm = (M + c.bm - 1) / c.bm, units = (N + c.bn - 1) / c.bn * gm * kc;
-    const int64_t work = (units + ncu - 1) / ncu * c.q * per * (K % 128 ? c.mis : 100) / 100;
+    const double work = (double)((units + ncu - 1) / ncu) * c.q * per * (K % 128 ? c.mis / 100.0 : 1.0);
     const int64_t busy = units < c.resident * ncu ? units : c.resident * ncu;
     int64_t rate = busy * (gm == 1 ? c.one : c.more);               /* bytes a us */
-    if (rate > 5200000) rate = 5200000;
-    const int64_t stream = N * K * 1000 / rate;
-    return c.a + (work > stream ? work : stream) + (kc > 1 ? 2390 + kc * M * N * 18 / 10000 : 0);
+    if (rate > 6120000) rate = 6120000;
+    const double stream = (double)N * K * 1000 / rate;
+    return c.a + sqrt(work * work + stream * stream) + (kc > 1 ? 2260 + 1.83e-3 * kc * M * N : 0.0);
 }
 
 constexpr int64_t kI8MaxPlanes = (int64_t)1 << 28;                 /* bytes of planes, at most */
@@ -156,7 +163,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
         g->blocks = (rows + g->waves / kc - 1) / (g->waves / kc);
         return;
     }
-    int64_t best = 0;
+    double best = 0;
     for (int t = 0; t < I8_TILES; ++t) {
         const I8Cost& c = kI8Cost[t];
         const int64_t tiles = (P.N + c.bn - 1) / c.bn * ((P.M + c.bm - 1) / c.bm);
@@ -165,8 +172,8 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
             const int64_t per = (steps + kc - 1) / kc;
             if ((steps + per - 1) / per != kc || tiles * kc > 0x7FFFFF) continue;      /* 2^32 lanes a launch */
             if (kc > 1 && (P.M > 65535 || tiles * kc > 4 * ncu || kc * P.M * P.N * 4 > scratch)) break;
-            const int64_t ns = i8_tile_ns(c, P.M, P.N, P.K, per, kc, ncu);
-            if (best && ns >= best) continue;
+            const double ns = i8_tile_ns(c, P.M, P.N, P.K, per, kc, ncu);
+            if (best > 0 && ns >= best) continue;
             best = ns;
             g->arm = I8_TILE;
             g->tile = t;

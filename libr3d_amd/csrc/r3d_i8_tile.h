@@ -19,7 +19,7 @@
  * u / tiles of its tile and leaves an i32 plane, and i8_join_kernel adds the planes.
  *
  * Measured on MI355X (a 16384 x 16384 x 8192 product of the library's reaches 2.39 POP/s, a 1 GiB copy 5.14
- * TB/s): M = 13 x 5376 x 21504 26 us, 4.4 TB/s, bound by the weights; M = 333 x 8187 x 5360 24 us, 1.2 POP/s:
+ * TB/s): M = 13 x 5376 x 21504 23.3 us, 5.0 TB/s, bound by the weights; M = 333 x 8187 x 5360 24 us, 1.2 POP/s:
  * 256 tiles of 128 x 96, an eighth of them past the edges, and a K off 128 asks for two lines a row (the
  * weights cold 31.8 us; K = 5376 24.2).  A step of a 128 x 128 tile takes 0.47 us a compute unit, 8.9 TOP/s of its 9.3.
  */
