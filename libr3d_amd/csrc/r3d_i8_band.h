@@ -17,8 +17,10 @@
  *
  * One workgroup a row, the row in registers (C chunks of 8 elements a lane) from the load to the
  * codes: every operand is read once and every result written once, which is all the traffic there
- * is; the kernels are bound by it (us, and all bytes a second: norm with its residual 2048 x 5376
- * 21.8, 3.5 TB/s, 4096 x 5376 36.3, 4.2; gated 2048 x 21504 40, 5.5; quant 2048 x 4096 6.4, 3.9; a
+ * is; the kernels are bound by it (us of a kernel trace, and all bytes a second: norm with its residual
+ * 2048 x 5376 19.5, 4.0 TB/s; gated 2048 x 21504 44.8, 4.9; quant 2048 x 4096 6.0, 4.2; four rows, where the
+ * chain of one row counts, 4.2, 6.6 and 2.4; with the two reductions over a wave by way of LDS 20.0, 46.9
+ * and 6.4; 4.6, 6.8 and 2.6; a
  * large copy reaches 5.1).  Operands move in 16-byte accesses at element alignment
  * (gfx950's global memory takes them anywhere), so no pitch or base needs a kernel of its own; the
  * last n % 8 elements go one by one.  A row past the registers (C = 0) is walked twice. */
@@ -27,6 +29,7 @@
 
 #include "r3d_device.h"
 #include "r3d_i8.h"
+#include "r3d_wave.h"
 
 namespace r3d {
 
@@ -141,11 +144,7 @@ __device__ __forceinline__ void i8_gated8(const I8Raw<BF16>& g, const I8Raw<BF16
 
 /* The largest of a workgroup's values, or their sum, on every lane; `s` holds one a wave. */
 __device__ __forceinline__ uint32_t i8_block_max(uint32_t v, uint32_t* s) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const uint32_t o = __shfl_xor(v, off, 64);
-        v = v > o ? v : o;
-    }
+    v = r3d_wave_max(v);
     const int nw = blockDim.x >> 6;
     if (nw == 1) return v;
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
@@ -155,8 +154,7 @@ __device__ __forceinline__ uint32_t i8_block_max(uint32_t v, uint32_t* s) {
     return r;
 }
 __device__ __forceinline__ double i8_block_sum(double v, double* s) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    v = r3d_wave_sum(v);
     const int nw = blockDim.x >> 6;
     if (nw == 1) return v;
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;

@@ -43,6 +43,7 @@
 #include "r3d_dump.h"
 #include "r3d_plan.h"
 #include "r3d_sample.h"
+#include "r3d_wave.h"
 
 namespace r3d {
 
@@ -192,34 +193,9 @@ __device__ __forceinline__ void sample_next(float (*v)[4]) {
         for (int i = 0; i < 4; ++i) v[j][i] = v[j + 1][i];
 }
 
-/* The largest over each 16 lanes, by rotations of the register (no lane waits for LDS). */
-__device__ __forceinline__ float sample_max16(float v) {
-#define R3D_ROTATE(N_) \
-    v = __builtin_fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x120 + N_, 15, 15, true)))
-    R3D_ROTATE(8); R3D_ROTATE(4); R3D_ROTATE(2); R3D_ROTATE(1);
-#undef R3D_ROTATE
-    return v;
-}
-
-/* The sum over this lane and the ones before it in the wave, by row shifts and broadcasts. */
-template <int CTRL, int ROWS>
-__device__ __forceinline__ u64 sample_moved(u64 v) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 15, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 15, false);
-    return (u64)hi << 32 | lo;
-}
-template <class V>
-__device__ __forceinline__ V sample_wave_scan(V v) {
-#define R3D_STEP(CTRL_, ROWS_) v += __builtin_bit_cast(V, sample_moved<CTRL_, ROWS_>(__builtin_bit_cast(u64, v)))
-    R3D_STEP(0x111, 15); R3D_STEP(0x112, 15); R3D_STEP(0x114, 15); R3D_STEP(0x118, 15);   /* within 16 lanes */
-    R3D_STEP(0x142, 10); R3D_STEP(0x143, 12);                       /* the 16 before, the 32 before */
-#undef R3D_STEP
-    return v;
-}
-
 template <int T>
 __device__ __forceinline__ float sample_block_max(float v, float* s) {
-    v = sample_max16(v);
+    v = r3d_max16(v);
 #pragma unroll
     for (int off = 32; off >= 16; off >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off, 64));
     __syncthreads();
@@ -231,7 +207,7 @@ __device__ __forceinline__ float sample_block_max(float v, float* s) {
 }
 template <int T>
 __device__ __forceinline__ u64 sample_block_sum(u64 v, u64* s) {
-    v = sample_wave_scan(v);
+    v = r3d_wave_scan(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 63) s[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -243,7 +219,7 @@ __device__ __forceinline__ u64 sample_block_sum(u64 v, u64* s) {
 /* The sum over the lanes before this one; *total over all. */
 template <int T>
 __device__ __forceinline__ u64 sample_block_scan(u64 v, u64* s, u64* total) {
-    const u64 in = sample_wave_scan(v);
+    const u64 in = r3d_wave_scan(v);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     __syncthreads();
     if (lane == 63) s[wave] = in;
@@ -321,13 +297,13 @@ __global__ __launch_bounds__(kSampleT) void sample_range_kernel(SampleArgs a) {
                 m = __builtin_fmaxf(m, v[j][i]);                      /* a NaN is passed over */
                 lo = __builtin_fminf(lo, sample_in(v[j][i]) ? v[j][i] : lo);
             }
-            m = sample_max16(m);
+            m = r3d_max16(m);
             if ((lane & 15) == 0) cm[lane / 16 + 4 * j] = m;
             hi = __builtin_fmaxf(hi, m);
         }
 #pragma unroll
         for (int off = 32; off >= 16; off >>= 1) hi = __builtin_fmaxf(hi, __shfl_xor(hi, off, 64));
-        lo = -sample_max16(-lo);
+        lo = -r3d_max16(-lo);
 #pragma unroll
         for (int off = 32; off >= 16; off >>= 1) lo = __builtin_fminf(lo, __shfl_xor(lo, off, 64));
         if (lane == 0) {
@@ -345,7 +321,7 @@ __global__ __launch_bounds__(kSampleT) void sample_range_kernel(SampleArgs a) {
                     if (sample_in(v[0][i])) sum += sample_w(here, v[0][i]);
                 sample_next<kSampleU>(v);
             }
-            sum = sample_wave_scan(sum);
+            sum = r3d_wave_scan(sum);
             if (lane == 63) a.q_sum[row * 4 * a.segs + q] = sum;
         }
     }
@@ -568,7 +544,7 @@ __global__ __launch_bounds__(kBinT) void sample_gather_kernel(SampleArgs a) {
                 }
             sample_next<kSampleU>(v);
         }
-        sum = sample_wave_scan(sum);
+        sum = r3d_wave_scan(sum);
         if (lane == 63 && sum) atomicAdd(&sums[q / 4 - s0], sum);
     }
     __syncthreads();
@@ -1081,7 +1057,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             if (w[i] > 0.0) any = 4 * t + i;
             sum += w[i];
         }
-        const double in = sample_wave_scan(sum);
+        const double in = r3d_wave_scan(sum);
         __syncthreads();                           /* s_i, s_a and the last segment's are read */
         if ((t & 63) == 63) su[t >> 6] = (u64)__double_as_longlong(in);
         if (t == 0) {
