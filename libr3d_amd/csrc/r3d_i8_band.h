@@ -20,8 +20,8 @@
  * is; the kernels are bound by it (us of a kernel trace, and all bytes a second: norm with its residual
  * 2048 x 5376 19.5, 4.0 TB/s; gated 2048 x 21504 44.8, 4.9; quant 2048 x 4096 6.0, 4.2; four rows, where the
  * chain of one row counts, 4.2, 6.6 and 2.4; with the two reductions over a wave by way of LDS 20.0, 46.9
- * and 6.4; 4.6, 6.8 and 2.6; a
- * large copy reaches 5.1).  Operands move in 16-byte accesses at element alignment
+ * and 6.4; 4.6, 6.8 and 2.6;
+ * a large copy reaches 5.1).  Operands move in 16-byte accesses at element alignment
  * (gfx950's global memory takes them anywhere), so no pitch or base needs a kernel of its own; the
  * last n % 8 elements go one by one.  A row past the registers (C = 0) is walked twice. */
 #ifndef R3D_I8_BAND_H
