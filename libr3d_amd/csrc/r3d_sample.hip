@@ -31,10 +31,10 @@
  * Passes 2 and 3 are not launched without a top-k or top-p operand.
  *
  * Bound by the one read of the row in pass 1 and by the four launches' chains of dependent loads.
- * Measured on MI355X at V = 262144, f32: one row 22 us; 128 rows, each with settings of its own, 94 us (of
- * which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22 rows that have a use for
- * them, 18 and 22; pass 4 29, of them 8 to list 1000 chunks).  With bins for every row, no chunks and a sort
- * that waited at a barrier for every step the same took 27.7 and 143 us. */
+ * Measured on MI355X at V = 262144, f32: one row 13 to 22 us by its settings; 128 rows, each with settings of
+ * its own, 89 us (of which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22 rows
+ * that have a use for them, 18 and 22; pass 4 27, of them 8 to list 1000 chunks).  With bins for every row,
+ * no chunks and a sort that waited at a barrier for every step the same took 27.7 and 143 us. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -738,7 +738,9 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         } else {
             n = kSampleList + 1;
         }
-        if (n <= kSampleList) {
+        /* few tokens are all sorted (50: 1.3 us for the bins' 4.3; 205: 3.8 and twice the exps); of more, or
+         * with min-p alone, only those that lie at a cut */
+        if (n <= kSampleList && !(set.use_k && n <= 128)) {
             /* the same cuts as from a whole row's bins, of the listed: what lies above the border bins
              * is kept, the list is left with what lies in them */
             if (set.use_k) {
@@ -800,10 +802,25 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         if (n <= kSampleList) {
             int size = 2;
             while (size < (int)n) size *= 2;
-            /* Bitonic, rising.  Up to a token a lane in registers, by way of LDS only to another wave;
-             * past that in LDS, where a wave's 64 pairs at distance 64 or less are 128 tokens of its own
-             * and only wider steps need the barrier.  (480 tokens 7.5 us by barriers alone.) */
-            if (size <= kPickT) {
+            /* Rising.  Up to 256 tokens each counts those before it (a lane a token, the list read by all
+             * lanes alike: 88 take 1.2 us less than bitonic steps do, 205 in all 3.8 us).  Past that bitonic: up to a token
+             * a lane in registers, by way of LDS only to another wave; past that in LDS, where a wave's 64
+             * pairs at distance 64 or less are 128 tokens of its own and only wider steps need the barrier
+             * (480 tokens 7.5 us by barriers alone, 5 so). */
+            if (n <= 256) {
+                __syncthreads();
+                const u64 e = list[t & 255];
+                int before = 0;
+                if ((t & ~63) < (int)n) {
+                    int i = 0;
+                    for (; i + 8 <= (int)n; i += 8)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) before += list[i + j] < e;
+                    for (; i < (int)n; ++i) before += list[i] < e;
+                }
+                __syncthreads();
+                if (t < (int)n) list[before] = e;
+            } else if (size <= kPickT) {
                 __syncthreads();
                 u64 e = t < (int)n ? list[t] : ~(u64)0;
                 for (int k = 2; k <= size; k *= 2)
