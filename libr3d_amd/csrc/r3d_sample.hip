@@ -193,45 +193,35 @@ __device__ __forceinline__ void sample_next(float (*v)[4]) {
         for (int i = 0; i < 4; ++i) v[j][i] = v[j + 1][i];
 }
 
+/* Over a workgroup of T lanes, up to 16 waves: their own results meet in 16 lanes of every wave. */
 template <int T>
 __device__ __forceinline__ float sample_block_max(float v, float* s) {
+    const int lane = threadIdx.x & 63;
     v = r3d_max16(v);
 #pragma unroll
     for (int off = 32; off >= 16; off >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off, 64));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+    if (lane == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < T / 64; ++i) v = __builtin_fmaxf(v, s[i]);
-    return v;
-}
-template <int T>
-__device__ __forceinline__ u64 sample_block_sum(u64 v, u64* s) {
-    v = r3d_wave_scan(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 63) s[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int i = 0; i < T / 64; ++i) v += s[i];
-    return v;
+    return r3d_max16(s[lane & (T / 64 - 1)]);
 }
 /* The sum over the lanes before this one; *total over all. */
-template <int T>
-__device__ __forceinline__ u64 sample_block_scan(u64 v, u64* s, u64* total) {
-    const u64 in = r3d_wave_scan(v);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <int T, class V>
+__device__ __forceinline__ V sample_block_scan(V v, V* s, V* total) {
+    const V in = r3d_wave_scan(v);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     __syncthreads();
     if (lane == 63) s[wave] = in;
     __syncthreads();
-    u64 before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < T / 64; ++i) {
-        if (i < wave) before += s[i];
-        all += s[i];
-    }
-    *total = all;
-    return before + in - v;
+    const V waves = r3d_scan16(s[lane & (T / 64 - 1)]);
+    *total = r3d_lane(waves, T / 64 - 1);
+    return (wave ? r3d_lane(waves, wave - 1) : V(0)) + (in - v);
+}
+template <int T>
+__device__ __forceinline__ u64 sample_block_sum(u64 v, u64* s) {
+    u64 total;
+    sample_block_scan<T>(v, s, &total);
+    return total;
 }
 
 /* The row's largest and least logit from its quarters', into the set. */
@@ -660,7 +650,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             __syncthreads();
             const unsigned int c0 = hcount[2 * t], c1 = hcount[2 * t + 1];
             u64 all;
-            const u64 c = sample_block_scan<kPickT>(c0 + c1, su, &all);
+            const u64 c = sample_block_scan<kPickT>((u64)(c0 + c1), su, &all);
             if (c < (u64)set.k && c + c0 + c1 >= (u64)set.k) s_i = c + c0 >= (u64)set.k ? 2 * t : 2 * t + 1;
             hcount[2 * t] = hcount[2 * t + 1] = 0;
             hmass[2 * t] = hmass[2 * t + 1] = 0;
@@ -692,8 +682,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
                 }
         }
         if (last < kSampleBins) {
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) low = min(low, (uint32_t)__shfl_xor(low, off, 64));
+            low = ~r3d_wave_max(~low);
             if ((t & 63) == 0) atomicMin(&s_key, low);
         }
         __syncthreads();
@@ -1074,20 +1063,14 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             if (w[i] > 0.0) any = 4 * t + i;
             sum += w[i];
         }
-        const double in = r3d_wave_scan(sum);
-        __syncthreads();                           /* s_i, s_a and the last segment's are read */
-        if ((t & 63) == 63) su[t >> 6] = (u64)__double_as_longlong(in);
+        __syncthreads();                           /* s_i and s_a are read, and the last segment's */
         if (t == 0) {
             s_i = kSampleSeg;
             s_j = -1;
         }
-        __syncthreads();
-        double run = done + (in - sum);
-        for (int i = 0; i < kPickT / 64; ++i) {
-            const double o = __longlong_as_double((long long)su[i]);
-            if (i < t >> 6) run += o;
-            done += o;
-        }
+        double all;
+        double run = done + sample_block_scan<kPickT>(sum, reinterpret_cast<double*>(su), &all);
+        done += all;
         int over = -1;                             /* the first past u's share: lanes are in index order */
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -24,20 +24,28 @@ __device__ __forceinline__ uint64_t r3d_moved(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 template <class V>
-__device__ __forceinline__ V r3d_wave_scan(V v) {
+__device__ __forceinline__ V r3d_scan16(V v) {                      /* within each 16 lanes */
 #define R3D_STEP(CTRL_, ROWS_) v += __builtin_bit_cast(V, r3d_moved<CTRL_, ROWS_>(__builtin_bit_cast(uint64_t, v)))
-    R3D_STEP(0x111, 15); R3D_STEP(0x112, 15); R3D_STEP(0x114, 15); R3D_STEP(0x118, 15);   /* within 16 lanes */
+    R3D_STEP(0x111, 15); R3D_STEP(0x112, 15); R3D_STEP(0x114, 15); R3D_STEP(0x118, 15);
+    return v;
+}
+template <class V>
+__device__ __forceinline__ V r3d_wave_scan(V v) {
+    v = r3d_scan16(v);
     R3D_STEP(0x142, 10); R3D_STEP(0x143, 12);                       /* the 16 before, the 32 before */
 #undef R3D_STEP
     return v;
 }
+/* Lane i's, i uniform. */
+template <class V>
+__device__ __forceinline__ V r3d_lane(V v, int i) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, i), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), i);
+    return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+}
 
 /* The sum, or the largest, over all lanes of the wave, on every lane. */
-__device__ __forceinline__ double r3d_wave_sum(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, r3d_wave_scan(v));
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), 63);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
+__device__ __forceinline__ double r3d_wave_sum(double v) { return r3d_lane(r3d_wave_scan(v), 63); }
 __device__ __forceinline__ uint32_t r3d_wave_max(uint32_t v) {
 #define R3D_STEP(CTRL_, ROWS_) \
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL_, ROWS_, 15, false))
