@@ -154,6 +154,10 @@ __device__ __forceinline__ const uint8_t* sample_row(const SamplePlan& P, int64_
     return P.logits + row * P.pitch * (P.bf16 ? 2 : 4);
 }
 
+template <bool BF16>
+__device__ __forceinline__ float sample_ld1(const uint8_t* x, int64_t i) {
+    return BF16 ? r3d_bf16_to_f32(reinterpret_cast<const uint16_t*>(x)[i]) : reinterpret_cast<const float*>(x)[i];
+}
 /* Four logits from index i on; -inf past V. */
 template <bool BF16>
 __device__ __forceinline__ void sample_ld4(const uint8_t* x, int64_t i, int64_t V, float* v) {
@@ -173,9 +177,7 @@ __device__ __forceinline__ void sample_ld4(const uint8_t* x, int64_t i, int64_t 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             v[j] = -__builtin_inff();
-            if (i + j < V)
-                v[j] = BF16 ? r3d_bf16_to_f32(reinterpret_cast<const uint16_t*>(x)[i + j])
-                            : reinterpret_cast<const float*>(x)[i + j];
+            if (i + j < V) v[j] = sample_ld1<BF16>(x, i + j);
         }
     }
 }
@@ -689,7 +691,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         if (last < kSampleBins) least = sample_value(s_key);
         const int nc = s_j;
         if (nc <= kSampleList) {
-            constexpr int U = 8;                   /* loads in flight a lane */
+            constexpr int U = 8;                   /* loads in flight a lane: 32 tokens, a bit each */
             for (int c0 = t / 16; c0 - t / 16 < nc; c0 += kPickT / 16 * U) {
                 float v[U][4];
                 unsigned int in = 0;
@@ -706,23 +708,25 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
 #pragma unroll
                 for (int j = 0; j < U; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) in += v[j][i] >= least;
-                unsigned int at = sample_slots<6>(in, &s_n);
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    const int c = c0 + kPickT / 16 * j;
-                    if (c >= nc) break;
-                    const unsigned int i0 = which[c] * kSampleChunk + 4 * (t & 15);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (v[j][i] >= least) {
-                            if (at < kSampleList) list[at] = sample_entry_of(v[j][i], i0 + i);
-                            ++at;
-                        }
+                    for (int i = 0; i < 4; ++i) in = 2 * in + (v[j][i] >= least);       /* the first token in bit 31 */
+                unsigned int at = sample_slots<6>(__builtin_popcount(in), &s_n);
+                while (in) {
+                    const int k = __builtin_clz(in);
+                    in &= ~(0x80000000u >> k);
+                    if (at < kSampleList)
+                        list[at] = which[c0 + kPickT / 16 * (k >> 2)] * kSampleChunk + 4 * (t & 15) + (k & 3);
+                    ++at;
                 }
             }
             __syncthreads();
             n = s_n;
+            /* (entries only now, a lane each: made where a token is found they would take as many steps of a
+             * wave as it has tokens in flight) */
+            if (n <= kSampleList)
+                for (int i = t; i < (int)n; i += kPickT) {
+                    const int64_t at = (int64_t)list[i];
+                    list[i] = sample_entry_of(sample_ld1<BF16>(x, at), at);
+                }
             __syncthreads();
         } else {
             n = kSampleList + 1;
