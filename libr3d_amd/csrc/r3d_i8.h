@@ -53,9 +53,8 @@ struct I8Geom {
 
 /* GEMV: the tokens in LDS, rows this many bytes apart */
 constexpr int64_t i8_gemv_row(int64_t K) { return ((K + 127) & ~(int64_t)127) + 16; }
-/* and at most this much of it.  Up to it the GEMV takes 0.85 to 1.07 of the tiles' time at M 5..8 (2295
- * shapes, by M and 8 KB of tokens; under 8 KB the 1.03 to 1.07), less below; with 56 KB and more, two
- * workgroups a compute unit, 1.05 to 1.4 */
+/* and at most this much of it: with 56 KB and more, two workgroups a compute unit, the GEMV takes 1.05 to
+ * 1.4 of the tiles' time */
 constexpr int64_t kI8GemvLds = 48 * 1024;
 
 /* The launch that suits a shape on ncu compute units, with at most `scratch` bytes for planes. */

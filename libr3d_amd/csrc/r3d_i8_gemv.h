@@ -10,12 +10,12 @@
  * 1 KB of weights, which HBM brings a compute unit in 80.
  *
  * The tokens lie in LDS (staged once, beside the first weight loads in flight): read from L2 next to
- * every weight line instead they cost 23.1 us where this takes 20.5 (M = 1, N = 21504, K = 5376).
+ * every weight line instead they cost 23.1 us where this takes 20.2 (M = 1, N = 21504, K = 5376).
  * Weight lines go from memory to registers, D ahead.  Rows past N are past the buffer's records and
  * columns past K are asked for there; both read 0.  The chunks of a row block are waves of one
  * workgroup, joined through LDS; the sums are integers, so no order changes a result.
  *
- * M = 1, N = 21504, K = 5376: 20.5 us, 5.65 TB/s.  Of D = 2, 3, 4, 6, 8, of 8 or 16 rows and of 4, 8
+ * M = 1, N = 21504, K = 5376: 20.2 us, 5.7 TB/s.  Of D = 2, 3, 4, 6, 8, of 8 or 16 rows and of 4, 8
  * or 16 waves a workgroup, D = 4 with 8 rows and 4 waves is the best over 274 shapes (7 % off the
  * best of all of them at each shape; the next, D = 3 and D = 6, 9 %).
  */

@@ -140,6 +140,16 @@ static double i8_tile_ns(const I8Cost& c, int64_t M, int64_t N, int64_t K, int64
     return c.a + sqrt(work * work + stream * stream) + (kc > 1 ? 2260 + 1.83e-3 * kc * M * N : 0.0);
 }
 
+/* The GEMV's time in the same terms, work growing with the tokens: over 13494 shapes of 1..8 tokens the
+ * cheaper of it and a tile is 1.0 % slower than the best launch, the GEMV wherever it fits 3.4 % (8 x 8192 x
+ * 5376 12.1 -> 10.4 us on tiles of 32 rows; up to 3 tokens it is the faster one nearly everywhere). */
+static double i8_gemv_ns(int64_t M, int64_t N, int64_t K, int ncu) {
+    const double lines = (double)((N + 7) / 8) * ((K + 127) / 128) / ncu;
+    const double work = 11.8 * (1.0 + 0.0841 * M) * lines * (K % 128 ? 1.73 : 1.0);
+    const double stream = (double)N * K * 1000 / 6120000;
+    return 3610 + 32 * M + sqrt(work * work + stream * stream);
+}
+
 constexpr int64_t kI8MaxPlanes = (int64_t)1 << 28;                 /* bytes of planes, at most */
 
 void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
@@ -147,6 +157,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
     if (P.ua) return;
     if (ncu <= 0) ncu = 256;
     const int64_t steps = (P.K + 127) / 128;
+    double best = 0;
     if (P.M <= 8 && P.M * i8_gemv_row(P.K) <= kI8GemvLds) {
         /* 8 weight rows a wave; K over waves until about 1600 of them stream (the K chunks of a row
          * block are waves of one workgroup), two lines a wave at least */
@@ -161,9 +172,8 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
         g->per = (int)((steps + kc - 1) / kc);
         g->waves = kc > 4 ? kc : 4;
         g->blocks = (rows + g->waves / kc - 1) / (g->waves / kc);
-        return;
+        best = i8_gemv_ns(P.M, P.N, P.K, ncu);
     }
-    double best = 0;
     for (int t = 0; t < I8_TILES; ++t) {
         const I8Cost& c = kI8Cost[t];
         const int64_t tiles = (P.N + c.bn - 1) / c.bn * ((P.M + c.bm - 1) / c.bm);
@@ -183,6 +193,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
             g->kc = (int)kc;
             g->per = (int)per;
             g->blocks = tiles * kc;
+            g->waves = 0;
         }
     }
 }
