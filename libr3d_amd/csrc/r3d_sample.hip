@@ -31,10 +31,11 @@
  * Passes 2 and 3 are not launched without a top-k or top-p operand.
  *
  * Bound by the one read of the row in pass 1 and by the four launches' chains of dependent loads.
- * Measured on MI355X at V = 262144, f32: one row 13 to 22 us by its settings; 128 rows, each with settings of
- * its own, 89 us (of which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22 rows
- * that have a use for them, 18 and 22; pass 4 27, of them 8 to list 1000 chunks).  With bins for every row,
- * no chunks and a sort that waited at a barrier for every step the same took 27.7 and 143 us. */
+ * Measured on MI355X at V = 262144, f32: one row 13 to 20 us by its settings; 128 rows, each with settings of
+ * its own, 86 to 90 us (of which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22
+ * to 30 rows that have a use for them, 16 to 20 and 19 to 25; pass 4 23, of them 6 to list 1000 chunks).  With
+ * bins for every row, no chunks and a sort that waited at a barrier for every step the same took 27.7 and
+ * 143 us. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -101,8 +102,9 @@ __device__ __forceinline__ SampleSet sample_set(const SampleArgs& a, int64_t row
 }
 
 /* exp(z) for z <= 0, within 2^-50: z = n ln 2 + r, |r| <= ln 2 / 2, the series of exp(r) to r^12
- * (r^13 / 13! < 2^-52), times 2^n.  Past the least f64 (and for NaN) 0. */
+ * (r^13 / 13! < 2^-52), times 2^n.  Past the least f64 (and for NaN, which the maximum passes over) 0. */
 __device__ __forceinline__ double sample_exp(double z) {
+    z = __builtin_fmax(z, -1100.0);
     const double n = __builtin_rint(z * 1.4426950408889634);
     double r = __builtin_fma(n, -0.6931471824645996, z);          /* ln 2 in f32 (n times it is exact), */
     r = __builtin_fma(n, 1.904654299957768e-09, r);                /* and what is left of it */
@@ -119,7 +121,6 @@ __device__ __forceinline__ double sample_exp(double z) {
     e = __builtin_fma(e, r, 0.5);
     e = __builtin_fma(e, r, 1.0);
     e = __builtin_fma(e, r, 1.0);
-    if (!(z > -746.0)) return 0.0;
     return __builtin_amdgcn_ldexp(e, (int)n);
 }
 
