@@ -550,8 +550,8 @@ __global__ __launch_bounds__(kBinT) void sample_gather_kernel(SampleArgs a) {
 }
 
 constexpr int kPickT = 1024;
-/* Pass 4's LDS, in 8 bytes: the list [8192], the segments' masses [1024], 256 masses and counters (radix
- * selection), the listed chunks' numbers [8192 / 2] */
+/* Pass 4's LDS, in 8 bytes: the list [8192], the segments' masses [1024], the bins' masses [2048] and counters
+ * [2048 / 2] (or a radix pass's), the listed chunks' numbers [8192 / 2] */
 constexpr int kPickSeg = kSampleList, kPickMass = kPickSeg + kSampleMaxSegs, kPickCount = kPickMass + kSampleBins;
 constexpr int kPickWhich = kPickCount + kSampleBins / 2, kPickWords = kPickWhich + kSampleList / 2;
 
@@ -629,8 +629,8 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         }
     } else if (set.listed) {
         /* top-k: k chunks have their largest logit in bins 0 .. last, so no token under the least of those
-         * is among the k.  min-p: none under max + T log(min_p) has w >= min_p (a millionth less for the
-         * roundings of log, exp and the products). */
+         * is among the k.  min-p: none under max + T log(min_p) has w >= min_p (the logarithm a millionth
+         * and 1e-14 less, for its rounding and those of exp, which makes a 1 of everything above -2^-54). */
         int last = kSampleBins;
         float least = -3.4028235e38f;              /* and no token under this one can be kept */
         for (int i = t; i < a.segs; i += kPickT) segm[i] = 0;
@@ -660,8 +660,7 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             __syncthreads();
             last = s_i;
         } else {
-            const double d = log(set.min_p) / set.inv_t;
-            const double l = (double)top + (d * 1.000001 - 1e-30);
+            const double l = (double)top + (log(set.min_p) * 1.000001 - 1e-14) / set.inv_t;
             least = l > -3.4028234e38 ? (float)l : least;
         }
         /* the chunks, then their tokens, 16 lanes a chunk */
@@ -775,7 +774,6 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
         } else {
             kb_lo = 0;
             if (set.use_k) C.kb = kSampleBins - 1;
-            else kb_lo = kSampleBins;
             if (set.use_p) {
                 C.pb_lo = 0;
                 C.pb_hi = kSampleBins - 1;
@@ -797,10 +795,10 @@ __global__ __launch_bounds__(kPickT) void sample_pick_kernel(SampleArgs a) {
             int size = 2;
             while (size < (int)n) size *= 2;
             /* Rising.  Up to 256 tokens each counts those before it (a lane a token, the list read by all
-             * lanes alike: 88 take 1.2 us less than bitonic steps do, 205 in all 3.8 us).  Past that bitonic: up to a token
-             * a lane in registers, by way of LDS only to another wave; past that in LDS, where a wave's 64
-             * pairs at distance 64 or less are 128 tokens of its own and only wider steps need the barrier
-             * (480 tokens 7.5 us by barriers alone, 5 so). */
+             * lanes alike: 88 take 1.2 us less than bitonic steps do, 205 in all 3.8 us).  Past that
+             * bitonic: up to a token a lane in registers, by way of LDS only to another wave; past that in
+             * LDS, where a wave's 64 pairs at distance 64 or less are 128 tokens of its own and only wider
+             * steps need the barrier (480 tokens 7.5 us by barriers alone, 5 so). */
             if (n <= 256) {
                 __syncthreads();
                 const u64 e = list[t & 255];

@@ -2,6 +2,7 @@
 at which the kernel changes how it orders a list, rows that hold about k tokens.  Against the same float64
 sampler; at 2^22 tokens a mass is off by up to 2^-41, a border by some 2^-29 of the mass, and the uniform
 numbers (24 bits, generic) do not lie within that of one."""
+import numpy as np
 import pytest
 import torch
 
@@ -54,3 +55,30 @@ def test_about_k_tokens_present(gpu):
     check(gpu, x, u, k=k)
     check(gpu, x, u, k=k, p=[0.999999, 0.5, 0.9] * 4)
     check(gpu, x, u, k=[60, 5000, 4999] * 4, p=[0.999999, 0.5, 0.9, 1.0] * 3)
+
+
+def test_min_p_of_one_at_high_temperatures(gpu, monkeypatch):
+    """A weight that rounds to 1 in float64 is not below min_p = 1, however far its logit lies below the
+    largest.  numpy's exp is off by one in the last place there (exp(-4.7e-17) is 1 - 4.7e-17, nearer to 1
+    than to 1 - 2^-53 = 1 - 1.11e-16, and comes out as the latter), so under 2^-30 the sampler it is held
+    against takes 1 + z, which z^2 / 2 < 2^-61 moves by less than 2^-8 of a last place."""
+    exp = np.exp
+    monkeypatch.setattr(np, "exp", lambda z: np.where(np.abs(z) < 2.0 ** -30, 1.0 + z, exp(z)))
+    g = torch.Generator().manual_seed(9)
+    M, V = 8, 9000
+    x, u = 3 * torch.randn(M, V, generator=g), torch.rand(M, generator=g)
+    T = [1e20, 1e17, 1e30, 3e38, 1.0, 1e4, 1e8, float("inf")]
+    for m in (1.0, 2.0, 1 - 2.0 ** -24, 0.5):
+        check(gpu, x, u, T=T, m=[m] * M)
+        check(gpu, x, u, T=T, m=[m] * M, k=[300, 9000, 1, 0] * 2)
+        check(gpu, x, u, T=T, m=[m] * M, p=[0.9] * M)
+
+
+@pytest.mark.parametrize("V", [8192, 8193, 20000, 300000])
+def test_min_p_that_keeps_more_than_a_list(gpu, V):
+    g = torch.Generator().manual_seed(V)
+    M = 6
+    x, u = 0.1 * torch.randn(M, V, generator=g), torch.rand(M, generator=g)
+    check(gpu, x, u, m=[0.3, 0.5, 0.7, 0.8, 0.05, 1e-30])
+    check(gpu, x, u, m=[1e-30] * M, T=[0.01, 0.1, 1.0, 10.0, 0.02, 0.003])
+    check(gpu, torch.zeros(M, V), u, m=[0.3, 0.5, 0.7, 1.0, 0.05, 1e-30])
