@@ -69,24 +69,29 @@ static int i8_launch_tile(const I8Plan& P, const I8Geom& g, int* part, hipStream
                        (int)P.b_pitch, (int)((P.M + g.bm - 1) / g.bm), (int)g.tiles, g.kc, g.per,
                        P.sa_stride, P.sb_stride, P.y_pitch};
     const dim3 grid((unsigned)g.blocks);
-#define R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_)                                                 \
-    hipLaunchKernelGGL((i8_tile_kernel<WNF_, WMF_, WVN_, WVM_, NST_>), grid,                    \
+#define R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, OFF_)                                           \
+    hipLaunchKernelGGL((i8_tile_kernel<WNF_, WMF_, WVN_, WVM_, NST_, OFF_>), grid,              \
                        dim3(64 * WVN_ * WVM_),                                                 \
                        (size_t)i8_tile_lds(16 * WNF_ * WVN_, 16 * WMF_ * WVM_, NST_), stream, a)
+#define R3D_I8T2(WNF_, WMF_, WVN_, WVM_, NST_, ONST_)                                         \
+    if (P.off) { R3D_I8T(WNF_, WMF_, WVN_, WVM_, ONST_, true); }                                \
+    else { R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, false); }                                      \
+    break
     switch (g.tile) {
         case I8_T_256x256:
             hipLaunchKernelGGL(i8_wide_kernel, grid, dim3(512), (size_t)i8_tile_lds(256, 256, 2), stream, a);
             break;
-        case I8_T_128x256: R3D_I8T(4, 4, 2, 4, 3); break;
-        case I8_T_128x192: R3D_I8T(2, 6, 4, 2, 3); break;
-        case I8_T_128x128: R3D_I8T(2, 4, 4, 2, 4); break;
-        case I8_T_128x96: R3D_I8T(2, 6, 4, 1, 4); break;
-        case I8_T_128x64: R3D_I8T(2, 4, 4, 1, 4); break;
-        case I8_T_64x64: R3D_I8T(1, 4, 4, 1, 4); break;
-        case I8_T_64x32: R3D_I8T(1, 2, 4, 1, 6); break;
-        case I8_T_32x32: R3D_I8T(1, 2, 2, 1, 10); break;
-        default: R3D_I8T(1, 1, 2, 1, 8); break;
+        case I8_T_128x256: R3D_I8T(4, 4, 2, 4, 3, false); break;
+        case I8_T_128x192: R3D_I8T(2, 6, 4, 2, 3, false); break;
+        case I8_T_128x128: R3D_I8T2(2, 4, 4, 2, 4, 5);
+        case I8_T_128x96: R3D_I8T2(2, 6, 4, 1, 4, 5);
+        case I8_T_128x64: R3D_I8T2(2, 4, 4, 1, 4, 5);
+        case I8_T_64x64: R3D_I8T2(1, 4, 4, 1, 4, 5);
+        case I8_T_64x32: R3D_I8T2(1, 2, 4, 1, 6, 6);
+        case I8_T_32x32: R3D_I8T2(1, 2, 2, 1, 10, 10);
+        default: R3D_I8T2(1, 1, 2, 1, 8, 8);
     }
+#undef R3D_I8T2
 #undef R3D_I8T
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && g.kc > 1) {

@@ -94,14 +94,15 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
     /* the fast kernels move 16 bytes a lane and walk 256 rows with 32-bit offsets */
     P->ua = (K & 15) || (((uintptr_t)P->A | (uintptr_t)P->B) & 15) ||
             ((P->a_pitch | P->b_pitch) & 15) || P->a_pitch > (1 << 22) || P->b_pitch > (1 << 22);
+    P->off = (((uintptr_t)P->A | (uintptr_t)P->B) & 127) || ((P->a_pitch | P->b_pitch) & 127);
     if (P->ua && M > 65535 * 32) return RAD_E_UNSUPPORTED;     /* its grid's second axis */
     return RAD_OK;
 }
 
 /* What a launch of a tile takes, in ns:
  *     a + sqrt(work^2 + stream^2) + the planes and their sum
- *     work: ceil(units / ncu) * q * steps a unit; K off 128 starts rows inside lines, and a step of 128
- *           bytes then takes two lines: * mis / 100
+ *     work: ceil(units / ncu) * q * steps a unit; rows that begin inside lines (a base or a pitch off 128):
+ *           * off / 100 (4000 launches of each tile over 22167 such shapes)
  *     stream: the weights at 6.12 TB/s, or at what the units in flight ask for, `one` bytes a us each
  *           with one tile of tokens, `more` where tiles of tokens share them in L2
  * Least squares over 5230 shapes (M 9..2048, N and K 512..21504) and 4 to 40 launches of each.  The pick is
@@ -113,41 +114,40 @@ int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
  * -> 10.3 us, 12 x 5376 x 4096 9.7 -> 7.9). */
 struct I8Cost {
     int bn, bm, resident;    /* workgroups a compute unit holds (LDS) */
-    int a, q, mis, one, more;
+    int a, q, off, one, more;
 };
 constexpr int kI8Any = 1000000;                                     /* a unit's rate never the bound */
 static const I8Cost kI8Cost[I8_TILES] = {
-    {256, 256, 1, 8244, 1034, 119, kI8Any, kI8Any},
+    {256, 256, 1, 8244, 1034, 121, kI8Any, kI8Any},
     {128, 256, 1, 4783,  852, 122, kI8Any, kI8Any},
-    {128, 192, 1, 3379,  776, 116, kI8Any,  21400},
-    {128, 128, 1, 4258,  445, 131, kI8Any, kI8Any},
-    {128,  96, 1, 3856,  422, 124, kI8Any, kI8Any},
-    {128,  64, 1, 3480,  343, 131, kI8Any, kI8Any},
-    { 64,  64, 2, 3242,  226, 123, kI8Any, kI8Any},
-    { 64,  32, 2, 3052,  175, 118, kI8Any, kI8Any},
-    { 32,  32, 2, 3319,  134, 112,  65500,  26700},
-    { 32,  16, 3, 3088,   96, 116,  43100,  19400},
+    {128, 192, 1, 3379,  776, 122, kI8Any,  21400},
+    {128, 128, 1, 4258,  445, 110, kI8Any, kI8Any},
+    {128,  96, 1, 3856,  422, 111, kI8Any, kI8Any},
+    {128,  64, 1, 3480,  343, 109, kI8Any, kI8Any},
+    { 64,  64, 2, 3242,  226, 116, kI8Any, kI8Any},
+    { 64,  32, 2, 3052,  175, 121, kI8Any, kI8Any},
+    { 32,  32, 2, 3319,  134, 130,  65500,  26700},
+    { 32,  16, 3, 3088,   96, 130,  43100,  19400},
 };
 
-static double i8_tile_ns(const I8Cost& c, int64_t M, int64_t N, int64_t K, int64_t per, int64_t kc,
-                         int ncu) {
-    const int64_t gm = (M + c.bm - 1) / c.bm, units = (N + c.bn - 1) / c.bn * gm * kc;
-    const double work = (double)((units + ncu - 1) / ncu) * c.q * per * (K % 128 ? c.mis / 100.0 : 1.0);
+static double i8_tile_ns(const I8Cost& c, const I8Plan& P, int64_t per, int64_t kc, int ncu) {
+    const int64_t M = P.M, N = P.N, gm = (M + c.bm - 1) / c.bm, units = (N + c.bn - 1) / c.bn * gm * kc;
+    const double work = (double)((units + ncu - 1) / ncu) * c.q * per * (P.off ? c.off / 100.0 : 1.0);
     const int64_t busy = units < c.resident * ncu ? units : c.resident * ncu;
     int64_t rate = busy * (gm == 1 ? c.one : c.more);               /* bytes a us */
     if (rate > 6120000) rate = 6120000;
-    const double stream = (double)N * K * 1000 / rate;
+    const double stream = (double)N * P.K * 1000 / rate;
     return c.a + sqrt(work * work + stream * stream) + (kc > 1 ? 2260 + 1.83e-3 * kc * M * N : 0.0);
 }
 
 /* The GEMV's time in the same terms, work growing with the tokens: over 13494 shapes of 1..8 tokens the
  * cheaper of it and a tile is 1.0 % slower than the best launch, the GEMV wherever it fits 3.4 % (8 x 8192 x
  * 5376 12.1 -> 10.4 us on tiles of 32 rows; up to 3 tokens it is the faster one nearly everywhere). */
-static double i8_gemv_ns(int64_t M, int64_t N, int64_t K, int ncu) {
-    const double lines = (double)((N + 7) / 8) * ((K + 127) / 128) / ncu;
-    const double work = 11.8 * (1.0 + 0.0841 * M) * lines * (K % 128 ? 1.73 : 1.0);
-    const double stream = (double)N * K * 1000 / 6120000;
-    return 3610 + 32 * M + sqrt(work * work + stream * stream);
+static double i8_gemv_ns(const I8Plan& P, int ncu) {
+    const double lines = (double)((P.N + 7) / 8) * ((P.K + 127) / 128) / ncu;
+    const double work = 11.8 * (1.0 + 0.0841 * P.M) * lines;
+    const double stream = (double)P.N * P.K * 1000 / 6120000 * (P.off ? 1.3 : 1.0);
+    return 3610 + 32 * P.M + sqrt(work * work + stream * stream);
 }
 
 constexpr int64_t kI8MaxPlanes = (int64_t)1 << 28;                 /* bytes of planes, at most */
@@ -172,7 +172,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
         g->per = (int)((steps + kc - 1) / kc);
         g->waves = kc > 4 ? kc : 4;
         g->blocks = (rows + g->waves / kc - 1) / (g->waves / kc);
-        best = i8_gemv_ns(P.M, P.N, P.K, ncu);
+        best = i8_gemv_ns(P, ncu);
     }
     for (int t = 0; t < I8_TILES; ++t) {
         const I8Cost& c = kI8Cost[t];
@@ -182,7 +182,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
             const int64_t per = (steps + kc - 1) / kc;
             if ((steps + per - 1) / per != kc || tiles * kc > 0x7FFFFF) continue;      /* 2^32 lanes a launch */
             if (kc > 1 && (P.M > 65535 || tiles * kc > 4 * ncu || kc * P.M * P.N * 4 > scratch)) break;
-            const double ns = i8_tile_ns(c, P.M, P.N, P.K, per, kc, ncu);
+            const double ns = i8_tile_ns(c, P, per, kc, ncu);
             if (best > 0 && ns >= best) continue;
             best = ns;
             g->arm = I8_TILE;
@@ -211,6 +211,7 @@ int64_t i8_scratch_bytes(const RadArgs* a, int ncu) {
     P.M = M;
     P.N = N;
     P.K = K;
+    P.off = (K & 127) != 0;
     I8Geom g;
     i8_geom(P, ncu, kI8MaxPlanes, &g);
     return g.arm == I8_TILE && g.kc > 1 ? (int64_t)g.kc * M * N * 4 : 0;

@@ -10,6 +10,14 @@
  * operands clamp to the last (their results are not stored); columns past K
  * (K % 128 = 16 .. 112) are asked for past the buffer's records and land as zeros.
  *
+ * Rows that begin inside lines (a base or a pitch off 128 bytes; both are multiples of 16 here) would take
+ * two lines a step each.  OFF loads whole lines all the same: a row's lines lie in the ring as they do in
+ * memory, its pieces counted from its own beginning, and a step reads the last of them from the stage
+ * after.  That asks for one stage more to have landed (M = 64 x 21504 x 5360 37.4 -> 27.7 us, 128 49.6 -> 33.5,
+ * 333 82 -> 58; at K = 5376, where nothing asks for it, 1 to 9 % more).  The tiles of 192 and 256 tokens have no
+ * LDS for that stage and take the two
+ * lines.
+ *
  * One barrier a step: it says both that the next step's stage has landed (each wave has waited for
  * its own loads) and that the stage before this one is read, whose slot then takes the loads of
  * NST - 1 steps ahead.  A wave reads the operands of one half step while the products of the other
@@ -42,11 +50,12 @@ struct I8TileArgs {
     int64_t sa_stride, sb_stride, y_pitch;
 };
 
-template <int WNF, int WMF, int WVN, int WVM, int NST>
+template <int WNF, int WMF, int WVN, int WVM, int NST, bool OFF>
 __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
     constexpr int WV = WVN * WVM, BN = 16 * WNF * WVN, BM = 16 * WMF * WVM;
     constexpr int WLD = BN / 8 / WV, ALD = BM / 8 / WV, LOADS = WLD + ALD;   /* 1 KB loads a wave */
     static_assert(WLD * WV * 8 == BN && ALD * WV * 8 == BM, "whole loads a wave");
+    static_assert(NST >= 3 + OFF, "the stages a step reads, and one to load");
     constexpr int AOFF = BN * 128, STAGE = (BN + BM) * 128;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63;
@@ -70,31 +79,43 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
     const int kend = k0 + P.cst * 128 < P.K ? k0 + P.cst * 128 : P.K;
     const int steps = (kend - k0 + 127) >> 7;
 
-    const __amdgpu_buffer_rsrc_t rB = r3d_rsrc(P.B + n0 * P.b_pitch, (P.N - 1 - n0) * (int64_t)P.b_pitch + P.K);
-    const __amdgpu_buffer_rsrc_t rA = r3d_rsrc(P.A + m0 * P.a_pitch, (P.M - 1 - m0) * (int64_t)P.a_pitch + P.K);
+    /* (OFF: a row's first line begins before the row; the records begin a line earlier, for offsets from
+     * 0 on, and nothing is asked for there) */
+    constexpr int LEAD = OFF ? 128 : 0;
+    const __amdgpu_buffer_rsrc_t rB =
+        r3d_rsrc(P.B + n0 * P.b_pitch - LEAD, (P.N - 1 - n0) * (int64_t)P.b_pitch + P.K + LEAD);
+    const __amdgpu_buffer_rsrc_t rA =
+        r3d_rsrc(P.A + m0 * P.a_pitch - LEAD, (P.M - 1 - m0) * (int64_t)P.a_pitch + P.K + LEAD);
     /* image j: rows 8 j .. + 7 of 128 bytes, a line a row; lane (row lr, place) fetches the 16-byte
-     * piece place ^ lr */
-    const int lr = lane >> 3, col = 16 * ((lane & 7) ^ lr);
+     * piece place ^ lr of the row's own count, which lies `shift` pieces on in its line */
+    const int lr = lane >> 3;
+    auto shift = [](const uint8_t* base, int pitch, int r) {
+        return OFF ? (int)(((uintptr_t)base >> 4) + (uint32_t)r * (uint32_t)(pitch >> 4)) & 7 : 0;
+    };
+    auto column = [&](int sh) { return 16 * (((((lane & 7) ^ lr) + sh) & 7) - sh); };
+    const int wcol = column(shift(P.B, P.b_pitch, lr)), acol = column(shift(P.A, P.a_pitch, lr));
     uint32_t woff[WLD], aoff[ALD];
 #pragma unroll
     for (int i = 0; i < WLD; ++i) {
         const int64_t n = n0 + 8 * (wave + WV * i) + lr;
-        woff[i] = (uint32_t)(((n < P.N ? n : P.N - 1) - n0) * P.b_pitch + col);
+        woff[i] = (uint32_t)(((n < P.N ? n : P.N - 1) - n0) * P.b_pitch + wcol + LEAD);
     }
 #pragma unroll
     for (int i = 0; i < ALD; ++i) {
         const int64_t m = m0 + 8 * (wave + WV * i) + lr;
-        aoff[i] = (uint32_t)(((m < P.M ? m : P.M - 1) - m0) * P.a_pitch + col);
+        aoff[i] = (uint32_t)(((m < P.M ? m : P.M - 1) - m0) * P.a_pitch + acol + LEAD);
     }
     auto issue = [&](int s, uint8_t* st) __attribute__((always_inline)) {
         const int k = k0 + 128 * s;
-        const bool ok = col < kend - k;                         /* past the end: zeros */
+        /* outside the chunk's columns: zeros */
+        const bool wok = (uint32_t)(128 * s + wcol) < (uint32_t)(kend - k0);
+        const bool aok = (uint32_t)(128 * s + acol) < (uint32_t)(kend - k0);
 #pragma unroll
         for (int i = 0; i < WLD; ++i)
-            r3d_buf_lds<16>(rB, st + 1024 * (wave + WV * i), ok ? woff[i] : 0x80000000u, k);
+            r3d_buf_lds<16>(rB, st + 1024 * (wave + WV * i), wok ? woff[i] : 0x80000000u, k);
 #pragma unroll
         for (int i = 0; i < ALD; ++i)
-            r3d_buf_lds<16>(rA, st + AOFF + 1024 * (wave + WV * i), ok ? aoff[i] : 0x80000000u, k);
+            r3d_buf_lds<16>(rA, st + AOFF + 1024 * (wave + WV * i), aok ? aoff[i] : 0x80000000u, k);
     };
 
     r3d_i32x4 acc[WNF][WMF];
@@ -106,14 +127,18 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
     /* fragments of one half step (64 of K): half 0 and half 1 each have a register set, read while
      * the other half's products run */
     r3d_i32x4 wf[2][WNF], xf[2][WMF];
-    auto read = [&](const uint8_t* st, int h) __attribute__((always_inline)) {
+    /* (OFF: the pieces past the end of the row's line are in the next stage) */
+    const int wsh = shift(P.B, P.b_pitch, li) + q, ash = shift(P.A, P.a_pitch, li) + q;
+    auto read = [&](int now, int then, int h) __attribute__((always_inline)) {
         const int rd = h ? rd1 : rd0;
+        const uint8_t* const sw = smem + STAGE * (OFF && wsh + 4 * h >= 8 ? then : now) + rd;
+        const uint8_t* const sx = smem + STAGE * (OFF && ash + 4 * h >= 8 ? then : now) + AOFF + rd;
 #pragma unroll
         for (int a = 0; a < WNF; ++a)
-            wf[h][a] = *reinterpret_cast<const r3d_i32x4*>(st + 2048 * (wn * WNF + a) + rd);
+            wf[h][a] = *reinterpret_cast<const r3d_i32x4*>(sw + 2048 * (wn * WNF + a));
 #pragma unroll
         for (int b = 0; b < WMF; ++b)
-            xf[h][b] = *reinterpret_cast<const r3d_i32x4*>(st + AOFF + 2048 * (wm * WMF + b) + rd);
+            xf[h][b] = *reinterpret_cast<const r3d_i32x4*>(sx + 2048 * (wm * WMF + b));
     };
     auto products = [&](int h) __attribute__((always_inline)) {
 #pragma unroll
@@ -132,16 +157,17 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
     };
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) issue(s, smem + STAGE * s);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(LOADS * (NST - 2)) : "memory");
-    read(smem, 0);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"(LOADS * (NST - 2 - OFF)) : "memory");
+    read(0, 1, 0);
     int slot = 0;
     for (int s = 0; s < steps; ++s) {
         const int next = slot + 1 == NST ? 0 : slot + 1, last = slot == 0 ? NST - 1 : slot - 1;
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LOADS * (NST - 3)) : "memory");
+        const int after = next + 1 == NST ? 0 : next + 1;
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(LOADS * (NST - 3 - OFF)) : "memory");
         issue(s + NST - 1, smem + STAGE * last);                /* the slot read one step ago */
-        read(smem + STAGE * slot, 1);
+        read(slot, next, 1);
         products(0);
-        read(smem + STAGE * next, 0);
+        read(next, after, 0);
         products(1);
         slot = next;
     }
