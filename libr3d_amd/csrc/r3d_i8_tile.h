@@ -15,8 +15,7 @@
  * memory, its pieces counted from its own beginning, and a step reads the last of them from the stage
  * after.  That asks for one stage more to have landed (M = 64 x 21504 x 5360 37.4 -> 27.7 us, 128 49.6 -> 33.5,
  * 333 82 -> 58; at K = 5376, where nothing asks for it, 1 to 9 % more).  The tiles of 192 and 256 tokens have no
- * LDS for that stage and take the two
- * lines.
+ * LDS for that stage and take the two lines.
  *
  * One barrier a step: it says both that the next step's stage has landed (each wave has waited for
  * its own loads) and that the stage before this one is read, whose slot then takes the loads of
@@ -27,9 +26,9 @@
  * u / tiles of its tile and leaves an i32 plane, and i8_join_kernel adds the planes.
  *
  * Measured on MI355X (a 16384 x 16384 x 8192 product of the library's reaches 2.39 POP/s, a 1 GiB copy 5.14
- * TB/s): M = 13 x 5376 x 21504 23.3 us, 5.0 TB/s, bound by the weights; M = 333 x 8187 x 5360 24 us, 1.2 POP/s:
- * 256 tiles of 128 x 96, an eighth of them past the edges, and a K off 128 asks for two lines a row (the
- * weights cold 31.8 us; K = 5376 24.2).  A step of a 128 x 128 tile takes 0.47 us a compute unit, 8.9 TOP/s of its 9.3.
+ * TB/s): M = 13 x 5376 x 21504 23.3 us, 5.0 TB/s, bound by the weights; M = 333 x 8187 x 5360 22.6 us, 1.3 POP/s:
+ * 256 tiles of 128 x 96, an eighth of them past the edges.  A step of a 128 x 128 tile takes 0.45 us a
+ * compute unit, 9.3 TOP/s of the 9.3 that the library's product leaves each.
  */
 #ifndef R3D_I8_TILE_H
 #define R3D_I8_TILE_H
