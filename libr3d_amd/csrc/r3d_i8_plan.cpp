@@ -301,7 +301,7 @@ I8BandGeom i8_band_geom(int64_t rows, int64_t n) {
      * Few rows, or short ones: as few chunks as some 768 lanes allow.  Many long rows: two to four,
      * the fewest idle lanes, three where they tie. */
     if (nc <= 256 || rows * nc < 400000) {
-        const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : nc <= 3072 ? 3 : 4;
+        const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : lanes(3) <= 1024 ? 3 : 4;
         return I8BandGeom{lanes(c), c};
     }
     int best = 0;
