@@ -250,6 +250,17 @@ def ext_rows():
     return _rows(lib().r3d_gfx950_ext_kernel_count(), lib().r3d_gfx950_ext_kernel_at)
 
 
+_TABLES = (None, [])
+
+
+def _all_rows():
+    """Both tables' rows, read once a library: they are fixed at its registration."""
+    global _TABLES
+    if _TABLES[0] is not lib():
+        _TABLES = (lib(), rows() + ext_rows())
+    return _TABLES[1]
+
+
 def _rows(count, at):
     out = []
     for i in range(count):
@@ -310,13 +321,13 @@ def _holds(c, query):
 def resolve(op, query):
     """Highest-priority registered row of `op` whose constraints all hold, or None."""
     best = None
-    for r in rows() + ext_rows():
+    for r in _all_rows():
         if r["op"] != op:
             continue
         if all(_holds(c, query) for c in r["constraints"]):
             if best is None or r["priority"] > best["priority"]:
                 best = r
-    return best
+    return None if best is None else dict(best)
 
 
 class GemmOperands:
@@ -903,7 +914,7 @@ def sample_logits(logits, u, token, prob=None, *, n_vocab, temperature=None, top
 
 def row_launcher(row_name):
     """The named row's launch pointer as a callable f(ops, stream) -> status."""
-    for r in rows() + ext_rows():
+    for r in _all_rows():
         if r["name"] == row_name:
             fn = LaunchFn(r["launch"])
 
@@ -915,7 +926,7 @@ def row_launcher(row_name):
 
 def row_scratch_bytes(row_name, ops):
     """The named row's scratch hook on `ops` (bytes; 0 when the row has no hook)."""
-    for r in rows() + ext_rows():
+    for r in _all_rows():
         if r["name"] == row_name:
             if not r.get("scratch"):
                 return 0
