@@ -870,30 +870,43 @@ def quant_act_fp8(x, q, scale, *, n, group=128, stream=None):
     return launch_row("quant_act_fp8_act", ops, stream)
 
 
-def _launch_on(row_name, ops, stream):
+def _one_gpu(*tensors):
+    """The GPU that the operands lie on; host tensors, or two devices', would reach a kernel as
+    addresses that it cannot read."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1 or next(iter(devices)).type != "cuda":
+        raise ValueError("operands have to lie on one GPU, not on %s" % sorted(str(d) for d in devices))
+    return next(iter(devices))
+
+
+def _launch_on(row_name, ops, stream, device):
     import torch
-    if stream is None:
-        stream = torch.cuda.current_stream().cuda_stream
-    return launch_row(row_name, ops, stream)
+    with torch.cuda.device(device):
+        if stream is None:
+            stream = torch.cuda.current_stream(device).cuda_stream
+        return launch_row(row_name, ops, stream)
 
 
 def quant_act_i8(x, q, scale, *, n, stream=None):
     """Launch the quant_act_i8 row on `stream` (default the current torch stream); its status."""
-    return _launch_on("quant_act_i8", QuantActI8Operands(x, q, scale, n=n), stream)
+    device = _one_gpu(x, q, scale)
+    return _launch_on("quant_act_i8", QuantActI8Operands(x, q, scale, n=n), stream, device)
 
 
 def gated_quant_i8(gate_up, q, scale, out=None, *, n, act=None, stream=None):
     """Launch the gated_quant_i8 row on `stream` (default the current torch stream); its status."""
-    return _launch_on("gated_quant_i8", GatedQuantI8Operands(gate_up, q, scale, out, n=n, act=act), stream)
+    device = _one_gpu(gate_up, q, scale, out)
+    return _launch_on("gated_quant_i8", GatedQuantI8Operands(gate_up, q, scale, out, n=n, act=act), stream, device)
 
 
 def rmsnorm_quant_i8(x, residual, w, q, scale, out=None, *, n, residual_out=None, eps=1e-6,
                      wadd=None, stream=None):
     """Launch the rmsnorm_quant_i8 row on `stream` (default the current torch stream); its
     status."""
+    device = _one_gpu(x, residual, w, q, scale, out, residual_out)
     ops = RmsNormQuantI8Operands(x, residual, w, q, scale, out, n=n, residual_out=residual_out,
                                  eps=eps, wadd=wadd)
-    return _launch_on("rmsnorm_quant_i8", ops, stream)
+    return _launch_on("rmsnorm_quant_i8", ops, stream, device)
 
 
 def sample_logits(logits, u, token, prob=None, *, n_vocab, temperature=None, top_k=None, top_p=None,
@@ -901,15 +914,16 @@ def sample_logits(logits, u, token, prob=None, *, n_vocab, temperature=None, top
     """Launch the sample_logits row on `stream` (a raw hipStream_t int, default the current torch
     stream), with launch scratch of the size its hook asks for; its status."""
     import torch
+    device = _one_gpu(logits, u, token, prob, temperature, top_k, top_p, min_p)
     ops = SampleOperands(logits, u, token, prob, n_vocab=n_vocab, temperature=temperature, top_k=top_k,
                          top_p=top_p, min_p=min_p)
     need = row_scratch_bytes("sample_logits", ops)
     if need > 0:
         # from the launch stream's pool, as gemm_nt_q's: freed on return
-        own = None if stream is None else torch.cuda.ExternalStream(stream, device=logits.device)
-        with torch.cuda.stream(own):
-            ops.set_scratch(torch.empty(need, dtype=torch.uint8, device=logits.device), need)
-    return _launch_on("sample_logits", ops, stream)
+        own = None if stream is None else torch.cuda.ExternalStream(stream, device=device)
+        with torch.cuda.device(device), torch.cuda.stream(own):
+            ops.set_scratch(torch.empty(need, dtype=torch.uint8, device=device), need)
+    return _launch_on("sample_logits", ops, stream, device)
 
 
 def row_launcher(row_name):
@@ -950,6 +964,9 @@ def gemm_nt_q(a, a_scale, b, b_scale, y, *, dtype, N, K, group=None, stream=None
     current torch stream), with launch scratch of the size the row's hook asks for.
     Returns (status, row name)."""
     import torch
+    if dtype == "i8a8" and _one_gpu(a, a_scale, b, b_scale, y).index != torch.cuda.current_device():
+        with torch.cuda.device(y.device):
+            return gemm_nt_q(a, a_scale, b, b_scale, y, dtype=dtype, N=N, K=K, group=group, stream=stream, row=row)
     ops = GemmOperands(a, a_scale, b, b_scale, y, dtype=dtype, N=N, K=K, group=group)
     M = y.numel() // N
     if row is None:
