@@ -879,6 +879,19 @@ def _one_gpu(*tensors):
     return next(iter(devices))
 
 
+def _scratch(need, device, stream):
+    """Launch scratch of `need` bytes from the pool of the stream that the launch goes to (a raw
+    hipStream_t int; None: the current one): it is freed when the call returns, and whatever takes
+    the memory next must come after the launch.  A raw 0 is the default stream; torch would make a new
+    stream of its own of it, whose pool is not ordered behind the launch."""
+    import torch
+    own = None
+    if stream is not None:
+        own = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.device(device), torch.cuda.stream(own):
+        return torch.empty(need, dtype=torch.uint8, device=device)
+
+
 def _launch_on(row_name, ops, stream, device):
     import torch
     with torch.cuda.device(device):
@@ -913,16 +926,12 @@ def sample_logits(logits, u, token, prob=None, *, n_vocab, temperature=None, top
                   min_p=None, stream=None):
     """Launch the sample_logits row on `stream` (a raw hipStream_t int, default the current torch
     stream), with launch scratch of the size its hook asks for; its status."""
-    import torch
     device = _one_gpu(logits, u, token, prob, temperature, top_k, top_p, min_p)
     ops = SampleOperands(logits, u, token, prob, n_vocab=n_vocab, temperature=temperature, top_k=top_k,
                          top_p=top_p, min_p=min_p)
     need = row_scratch_bytes("sample_logits", ops)
     if need > 0:
-        # from the launch stream's pool, as gemm_nt_q's: freed on return
-        own = None if stream is None else torch.cuda.ExternalStream(stream, device=device)
-        with torch.cuda.device(device), torch.cuda.stream(own):
-            ops.set_scratch(torch.empty(need, dtype=torch.uint8, device=device), need)
+        ops.set_scratch(_scratch(need, device, stream), need)
     return _launch_on("sample_logits", ops, stream, device)
 
 
@@ -978,11 +987,7 @@ def gemm_nt_q(a, a_scale, b, b_scale, y, *, dtype, N, K, group=None, stream=None
         row = r["name"]
     need = row_scratch_bytes(row, ops)
     if need > 0:                        # the row's hook sized it, as an engine's arena would
-        # from the launch stream's pool: it is freed on return, and whatever takes the memory
-        # next must come after the launch
-        own = None if stream is None else torch.cuda.ExternalStream(stream, device=y.device)
-        with torch.cuda.stream(own):
-            ops.set_scratch(torch.empty(need, dtype=torch.uint8, device=y.device), need)
+        ops.set_scratch(_scratch(need, y.device, stream), need)
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
     return launch_row(row, ops, stream), row
