@@ -249,8 +249,9 @@ const RadKernelInfo* r3d_gfx950_ext_kernel_at(int i);
 int r3d_rad_gemm_nt_q_i8(const RadArgs* a, RadStream s);
 int r3d_rad_gemm_nt_q_i8_decode(const RadArgs* a, RadStream s);
 /* Both rows' scratch hook: kc * M * N * 4 bytes of i32 planes where K is best split over
- * workgroups (at N, K and M = numel(y) / N; without y the M parameter, else 128), else 0; at most
- * 256 MiB.  Optional, as for the other tile rows: with less, or off 16 bytes, K takes as few chunks
+ * workgroups, else 0; at most 256 MiB.  Of a whole call its operands' alignment and pitches count, as they do
+ * at the launch; with some of them absent: N, K and M = numel(y) / N (without y the M parameter, else 128),
+ * as of dense operands on lines.  Optional, as for the other tile rows: with less, or off 16 bytes, K takes as few chunks
  * as fit.  Calls that share one buffer are ordered on one stream. */
 int64_t r3d_rad_gemm_nt_q_i8_scratch(const RadArgs* a);
 

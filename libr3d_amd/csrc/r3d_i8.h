@@ -61,7 +61,8 @@ constexpr int64_t kI8GemvLds = 48 * 1024;
 /* The launch that suits a shape on ncu compute units, with at most `scratch` bytes for planes. */
 void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g);
 
-/* The planes that a call's best launch wants: kc M N 4 bytes, 0 for none (the row's scratch hook). */
+/* The planes that a call's best launch wants: kc M N 4 bytes, 0 for none (the row's scratch hook).  Operands that
+ * are given are planned as the launch plans them. */
 int64_t i8_scratch_bytes(const RadArgs* a, int ncu);
 
 /* Codes out of a band producer, one scale a row. */

@@ -200,21 +200,26 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
 
 int64_t i8_scratch_bytes(const RadArgs* a, int ncu) {
     I8Plan P{};
-    long long N = 0, K = 0, M = 0;
-    if (!rad_args_geti(a, "N", &N) || !rad_args_geti(a, "K", &K) || N <= 0 || K <= 0 || N > kDimMax ||
-        K > kI8MaxK)
-        return 0;
-    const RadTensor* Y = rad_arg_in(a, 4);
-    if (Y) M = rad_tensor_numel(Y) / N;
-    else if (!rad_args_geti(a, "M", &M)) M = 128;
-    if (M <= 0 || M > kDimMax || (K & 15)) return 0;
-    P.M = M;
-    P.N = N;
-    P.K = K;
-    P.off = (K & 127) != 0;
+    if (plan_i8(a, 0, &P) != RAD_OK) {
+        /* not a whole call yet: dense operands on lines */
+        long long N = 0, K = 0, M = 0;
+        P = I8Plan{};
+        if (!rad_args_geti(a, "N", &N) || !rad_args_geti(a, "K", &K) || N <= 0 || K <= 0 || N > kDimMax ||
+            K > kI8MaxK)
+            return 0;
+        const RadTensor* Y = rad_arg_in(a, 4);
+        if (Y) M = rad_tensor_numel(Y) / N;
+        else if (!rad_args_geti(a, "M", &M)) M = 128;
+        if (M <= 0 || M > kDimMax) return 0;
+        P.M = M;
+        P.N = N;
+        P.K = K;
+        P.ua = (K & 15) != 0;
+        P.off = (K & 127) != 0;
+    }
     I8Geom g;
     i8_geom(P, ncu, kI8MaxPlanes, &g);
-    return g.arm == I8_TILE && g.kc > 1 ? (int64_t)g.kc * M * N * 4 : 0;
+    return g.arm == I8_TILE && g.kc > 1 ? (int64_t)g.kc * P.M * P.N * 4 : 0;
 }
 
 int plan_i8_band(const RadArgs* a, int op, I8BandPlan* P) {
