@@ -233,8 +233,8 @@ int r3d_gfx950_mfma_valu_probe(int nv, int lag3, int iters, void* work, int64_t*
  * set that radiance's other plugins declare (int8: gemm_nt_q at i8a8 and its producers; a
  * sampler), in the same structures, resolved and launched the same way.  A loader compares the schemas of
  * rad_kernel_schema_at with other plugins', so these are listed apart; an engine that knows the ops
- * reads them here.  R3D_NO_I8, R3D_NO_I8_DEC and R3D_NO_SAMPLE hide rows at registration.  gemm_nt_q's schema is
- * rad_kernel_schema_at's. */
+ * reads them here.  R3D_NO_I8, R3D_NO_I8_DEC and R3D_NO_SAMPLE hide rows at registration (R3D_NO_I8_DEC: the
+ * decode row, and no int8 call takes its GEMV).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 int r3d_gfx950_ext_schema_count(void);
 const RadOpSchema* r3d_gfx950_ext_schema_at(int i);
 int r3d_gfx950_ext_kernel_count(void);

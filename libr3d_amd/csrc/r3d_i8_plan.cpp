@@ -158,7 +158,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
     if (ncu <= 0) ncu = 256;
     const int64_t steps = (P.K + 127) / 128;
     double best = 0;
-    if (P.M <= 8 && P.M * i8_gemv_row(P.K) <= kI8GemvLds) {
+    if (P.M <= 8 && P.M * i8_gemv_row(P.K) <= kI8GemvLds && !env_no_i8_dec()) {
         /* 8 weight rows a wave; K over waves until about 1600 of them stream (the K chunks of a row
          * block are waves of one workgroup), two lines a wave at least */
         const int64_t rows = (P.N + 7) / 8;

@@ -5,15 +5,15 @@
  *
  * Rows (resolver: as in r3d_rows.cpp):
  *   gemm_nt_q_i8a8           prio 1000  dtype IN i8a8                     int8 GEMM, any M
- *   gemm_nt_q_i8a8_decode    prio 1100  + M LE 16                          int8 decode GEMV
+ *   gemm_nt_q_i8a8_decode    prio 1100  + M LE 16                          the same, decode band
  *   quant_act_i8             prio 1000  n GE 1, dtype IN f32 bf16           activation producer
  *   gated_quant_i8           prio 1000  n GE 1, dtype IN f32 bf16           gated producer
  *   rmsnorm_quant_i8         prio 1000  n GE 1, dtype IN bf16               norm producer
  *   sample_logits            prio 1000  n_vocab GE 1, dtype IN f32 bf16     sampler
  *
- * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row, R3D_NO_SAMPLE the sampler
- * (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is
- * rad_kernel_schema_at's. */
+ * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row (and turns off its GEMV in the other
+ * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler (presence-tested, read once; hidden at
+ * registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
@@ -128,8 +128,8 @@ enum { kPrioTile = 1000, kPrioDecode = 1100 };
 
 const RadKernelInfo kRows[] = {
     {"gemm_nt_q_i8a8", "gemm_nt_q", "gemm",
-     "int8 GEMM on gfx950 matrix cores: LDS tiles of 64 x 32 to 256 x 256 (a GEMV up to M = 8), summed "
-     "exactly in i32, one scale a token and one an output channel applied once; K split over "
+     "int8 GEMM on gfx950 matrix cores: LDS tiles of 32 x 16 to 256 x 256 (up to M = 8 a GEMV where that "
+     "is the faster one), summed exactly in i32, one scale a token and one an output channel applied once; K split over "
      "workgroups into i32 planes in launch scratch where tiles leave compute units idle",
      "K up to 131071 (the sum stays in i32); operands at any alignment and pitch (K, bases and "
      "pitches off 16 bytes: dword loads); M derives from numel(y)/N; scratch optional",
@@ -138,8 +138,9 @@ const RadKernelInfo kRows[] = {
      RAD_DOMAIN_DEVICE, kPrioTile, cI8, 1, nullptr, 0, nullptr, nullptr, nullptr,
      r3d_rad_gemm_nt_q_i8, r3d_rad_gemm_nt_q_i8_scratch, nullptr, nullptr, nullptr, nullptr},
     {"gemm_nt_q_i8a8_decode", "gemm_nt_q", "gemm",
-     "int8 decode-band product on gfx950 matrix cores: up to M = 8 a wave 8 weight rows, whole lines "
-     "from memory to registers, the tokens in LDS; above, or with long tokens, LDS tiles",
+     "int8 decode-band product on gfx950 matrix cores: up to M = 8 a GEMV (a wave 8 weight rows, whole lines "
+     "from memory to registers, the tokens in LDS) or LDS tiles, whichever its cost makes the faster one; "
+     "above, LDS tiles",
      "M <= 16; else as gemm_nt_q_i8a8",
      "as gemm_nt_q_i8a8",
      RAD_DOMAIN_DEVICE, kPrioDecode, cI8Decode, 2, nullptr, 0, nullptr, nullptr, nullptr,
