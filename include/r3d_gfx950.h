@@ -196,7 +196,8 @@ int r3d_rad_gemm_nt_q_mxfp4a16_noalloc(const RadArgs* a, RadStream s);
  * plan on `a` and writes the chosen arm and launch geometry (or the refusal) into buf.
  * Launches nothing and copies nothing from the device: a logits head's header is read in
  * place when the blob is host-accessible, else taken from the copy an earlier launch
- * cached (RAD_E_UNSUPPORTED when there is none).  Returns the plan's status code. */
+ * cached (RAD_E_UNSUPPORTED when there is none).  Plans for 256 compute units, a whole card; a launch for those
+ * that its device has.  Returns the plan's status code. */
 int r3d_gfx950_describe(const char* row, const RadArgs* a, char* buf, int len);
 
 /* Diagnostic with no counterpart in the reference: one stage of a gemm_nt_q_mxfp4a16 call
@@ -262,8 +263,9 @@ int64_t r3d_rad_gemm_nt_q_i8_scratch(const RadArgs* a);
  *   rmsnorm_quant_i8   (x bf16, residual? bf16, w bf16/f32 [n], q, scale, out?, residual_out?):
  *                      r = bf16(residual + x) to residual_out (given together; residual_out may be
  *                      the memory of residual or of x), then (r / rms) * (w + wadd) in f32
- * scale = max(amax / 127, 2^-126), 1 for a row of zeros; q to nearest even.  A row with a NaN or
- * an infinity has that as its scale and codes 0.  Params n, dtype (x's), eps, wadd, act; M =
+ * scale = max(amax / 127, 2^-126), 1 for a row of zeros; q to nearest even.  A row of which these values (x,
+ * act(gate) * up, the normed ones) hold a NaN, or else an infinity, has that as its scale and codes 0; an infinity
+ * in rmsnorm_quant_i8's x, or -inf as silu's gate, makes a NaN of them.  Params n, dtype (x's), eps, wadd, act; M =
  * numel(x) / n.  out (bf16/f32 [M, n]) carries the values that the codes are of.  RAD_OK,
  * RAD_E_INVAL for a missing operand, RAD_E_DTYPE / RAD_E_SHAPE / RAD_E_STRIDE / RAD_E_UNSUPPORTED
  * (act) for refused ones, RAD_E_DEVICE.  Asynchronous on `s`. */
@@ -280,7 +282,8 @@ int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
  * index order whose running mass passes u times the kept mass.  NaN and -inf logits are not there;
  * a row of them gives token -1, prob 0.  n_vocab <= 4194304, M <= 65535.  Launch scratch of the size
  * the hook gives, 16-byte aligned, is required (else RAD_E_UNSUPPORTED); calls that share it are
- * ordered on one stream.  RAD_E_INVAL / RAD_E_DTYPE / RAD_E_SHAPE / RAD_E_STRIDE for refused operands,
+ * ordered on one stream.  A cut among more than 8192 equal logits is slow (2 to 4 ms for some 20 us a row of
+ * 262144): mask with -inf, not with a finite number, where top_k may ask for more tokens than are allowed.  RAD_E_INVAL / RAD_E_DTYPE / RAD_E_SHAPE / RAD_E_STRIDE for refused operands,
  * RAD_E_DEVICE for a failed launch.  Asynchronous on `s`; results do not depend on the run. */
 int r3d_rad_sample_logits(const RadArgs* a, RadStream s);
 int64_t r3d_rad_sample_logits_scratch(const RadArgs* a);

@@ -12,14 +12,15 @@
  * h is quantised as it stands in f32 (the e4m3 producers beside these narrow it to bf16 first, as
  * the kernels that they follow do; here the narrowing would only move codes).  The 2^-126 keeps 1 / s
  * finite.  The maximum is taken over the magnitudes' bits, where an infinity is above every number and
- * a NaN above that: a row with a NaN has scale NaN and one with an infinity scale inf, both with codes
- * 0, so the product over the row is NaN and not a number that hides them.
+ * a NaN above that: a row whose h has a NaN has scale NaN and one with an infinity scale inf, both with codes
+ * 0, so the product over the row is NaN and not a number that hides them.  (h of a norm over an infinity is NaN,
+ * inf * (1 / inf); so is that of silu at -inf, -inf * 0.)
  *
  * One workgroup a row, the row in registers (C chunks of 8 elements a lane) from the load to the
  * codes: every operand is read once and every result written once, which is all the traffic there
  * is; the kernels are bound by it (us of a kernel trace, and all bytes a second: norm with its residual
  * 2048 x 5376 19.5, 4.0 TB/s; gated 2048 x 21504 44.8, 4.9; quant 2048 x 4096 6.0, 4.2; four rows, where the
- * chain of one row counts, 4.2, 6.6 and 2.4; with the two reductions over a wave by way of LDS 20.0, 46.9
+ * chain of one row counts, 4.2, 6.6 and 2.4; f32 in gated 78.7, quant 8.0; the norm alone 12.5; with the two reductions over a wave by way of LDS 20.0, 46.9
  * and 6.4; 4.6, 6.8 and 2.6;
  * a large copy reaches 5.1).  Operands move in 16-byte accesses at element alignment
  * (gfx950's global memory takes them anywhere), so no pitch or base needs a kernel of its own; the
@@ -100,7 +101,8 @@ __device__ __forceinline__ void i8_st8(uint8_t* row, int64_t i, int64_t n, const
     }
 }
 
-/* sigmoid(g) = 1 / (1 + exp(-g)) in f32, within 3 ulp: exp2 of the product's high part (its
+/* sigmoid(g) = 1 / (1 + exp(-g)) in f32, within 3 ulp where that is a normal number (g over -87.3; under that
+ * it may be 0, off by less than 2^-126): exp2 of the product's high part (its
  * rounding error times ln 2 is a factor on top, which keeps large |g| exact) and a reciprocal with
  * one Newton step.  Past 100 exp is inf and the result 0, as 1 / (1 + inf). */
 __device__ __forceinline__ float i8_sigmoid(float g) {

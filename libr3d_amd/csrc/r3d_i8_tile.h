@@ -26,9 +26,9 @@
  * u / tiles of its tile and leaves an i32 plane, and i8_join_kernel adds the planes.
  *
  * Measured on MI355X (a 16384 x 16384 x 8192 product of the library's reaches 2.39 POP/s, a 1 GiB copy 5.14
- * TB/s): M = 13 x 5376 x 21504 23.3 us, 5.0 TB/s, bound by the weights; M = 333 x 8187 x 5360 22.6 us, 1.3 POP/s:
- * 256 tiles of 128 x 96, an eighth of them past the edges.  A step of a 128 x 128 tile takes 0.45 us a
- * compute unit, 9.3 TOP/s of the 9.3 that the library's product leaves each.
+ * TB/s): M = 13 x 5376 x 21504 23.3 to 24.3 us, 5.0 TB/s, bound by the weights; M = 333 x 8187 x 5360 22.6 to 23.8 us,
+ * 1.3 POP/s: 256 tiles of 128 x 96, an eighth of them past the edges.  A step of a 128 x 128 tile takes 0.45 us a
+ * compute unit, 9.3 TOP/s of the 9.3 that the library's product leaves each; one of 128 x 96 0.42, 7.5 TOP/s.
  */
 #ifndef R3D_I8_TILE_H
 #define R3D_I8_TILE_H

@@ -13,7 +13,8 @@
  * matrix work at a time (sched_barrier: left to itself the compiler gathers the reads at the end of
  * the step).  A wave raises its priority over its products.
  *
- * 2048 x 21504 x 5376: 214 us, 2.2 POP/s (one barrier a step on 16 x 16 x 64 products 267; loads of
+ * 2048 x 21504 x 5376: 213 to 222 us in calls one after the other, 2.1 to 2.2 POP/s; in kernel traces 210 at
+ * best and 250 to 261 in the median (when it was 214: one barrier a step on 16 x 16 x 64 products 267; loads of
  * 16 rows x half lines 225).  The chip's power bounds it, not a unit: the same launch over zeros takes
  * 153 us, and torch's library product of the same codes 216 to 256. */
 #ifndef R3D_I8_WIDE_H

@@ -31,11 +31,16 @@
  * Passes 2 and 3 are not launched without a top-k or top-p operand.
  *
  * Bound by the one read of the row in pass 1 and by the four launches' chains of dependent loads.
- * Measured on MI355X at V = 262144, f32: one row 13 to 20 us by its settings; 128 rows, each with settings of
- * its own, 86 to 90 us (of which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22
- * to 30 rows that have a use for them, 16 to 20 and 19 to 25; pass 4 23, of them 6 to list 1000 chunks).  With
- * bins for every row, no chunks and a sort that waited at a barrier for every step the same took 27.7 and
- * 143 us. */
+ * Measured on MI355X at V = 262144, f32: one row 8 us greedy, 13 without a cut, 15 with min-p, 21, 22 and 26 with a
+ * top-k of 50, 200 and 1000 (of those 12, 14 and 19 in pass 4), 47 with top-p alone; 128 rows, each with settings of
+ * its own, 86 to 92 us (of which pass 1's read of 134 MB 29 us, 4.6 TB/s; passes 2 and 3, f64 exps for the 22
+ * to 30 rows that have a use for them, 16 to 20 and 19 to 25; pass 4 23, of them 6 to list 1000 chunks).  bf16: the
+ * same within a tenth (pass 1 25, pass 4 27).  With bins for every row, no chunks and a sort that waited at a
+ * barrier for every step one row took 27.7 and 128 143 us.
+ * The radix selection over the row takes 2.2 ms (2.5 with top-p as well, 4.1 so over a row of equal logits): some
+ * eight sweeps by one workgroup, half of them with an exp and two atomics a token, nearly all at one address.  A mask
+ * of a finite number leads there where a small top-k asks for more tokens than are allowed; one of -inf does
+ * not. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
