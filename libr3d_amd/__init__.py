@@ -26,6 +26,7 @@ __all__ = [
     "relayout_head", "unrelayout_head", "ext_rows", "ext_schemas", "QuantActI8Operands",
     "GatedQuantI8Operands", "RmsNormQuantI8Operands", "quant_act_i8", "gated_quant_i8",
     "rmsnorm_quant_i8", "SampleOperands", "sample_logits",
+    "GemmEpiOperands", "gemm_nt_epi",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -669,6 +670,26 @@ class RmsNormQuantI8Operands(_Args):
                          ([("M", M)] if M is not None else []))
 
 
+class GemmEpiOperands(_Args):
+    """One gemm_nt_epi call: y = act(S * a . b^T + bias) + residual.
+
+    dtype "bf16": a bf16/int16 [M, K], b bf16/int16 [N, K], no scales (S = 1); "i8a8": a int8 [M, K] with
+    a_scale float32 [M] or [M, 1], b int8 [N, K] with b_scale float32 [N] or [N, 1] (S their product)
+    bias       optional float32 or bf16/int16 [N]
+    residual   optional float32 or bf16/int16 [M, N]; may be y
+    y          float32 or bf16/int16 [M, N] out
+    act        "none" (default), "relu", "silu", "sigmoid", "gelu" or "gelu_tanh"
+    Launch scratch of row_scratch_bytes(row, ops) bytes (set_scratch) lets K be split; it is optional.
+    """
+
+    def __init__(self, a, b, y, *, dtype, N, K, a_scale=None, b_scale=None, bias=None, residual=None, act=None, M=None):
+        ops = [(a, "BF16"), (a_scale, "F32"), (b, "BF16"), (b_scale, "F32"), (bias, "F32"), (residual, "BF16"),
+               (y, "BF16")]
+        super().__init__([(t, _type(t, dt), None, None) for t, dt in ops],
+                         [("N", N), ("K", K), ("dtype", dtype)] + ([("act", act)] if act is not None else []) +
+                         ([("M", M)] if M is not None else []))
+
+
 class LogitsOperands(_Args):
     """One logits_gemm call (src/r3d_gemm_logits.hip:144-226).
 
@@ -892,6 +913,11 @@ def _scratch(need, device, stream):
         return torch.empty(need, dtype=torch.uint8, device=device)
 
 
+def _device(device):
+    import torch
+    return torch.cuda.device(device)
+
+
 def _launch_on(row_name, ops, stream, device):
     import torch
     with torch.cuda.device(device):
@@ -933,6 +959,22 @@ def sample_logits(logits, u, token, prob=None, *, n_vocab, temperature=None, top
     if need > 0:
         ops.set_scratch(_scratch(need, device, stream), need)
     return _launch_on("sample_logits", ops, stream, device)
+
+
+def gemm_nt_epi(a, b, y, *, dtype, N, K, a_scale=None, b_scale=None, bias=None, residual=None, act=None, stream=None):
+    """Launch gemm_nt_epi's row of `dtype` ("bf16" or "i8a8") on `stream` (a raw hipStream_t int, default the current
+    torch stream), with launch scratch of the size its hook asks for; its status."""
+    device = _one_gpu(a, b, y, a_scale, b_scale, bias, residual)
+    ops = GemmEpiOperands(a, b, y, dtype=dtype, N=N, K=K, a_scale=a_scale, b_scale=b_scale, bias=bias, residual=residual,
+                          act=act)
+    row = resolve("gemm_nt_epi", {"dtype": dtype, "M": y.numel() // N if N else 0, "N": N, "K": K})
+    if row is None:
+        return RAD_E_UNSUPPORTED
+    with _device(device):
+        need = row_scratch_bytes(row["name"], ops)
+    if need > 0:
+        ops.set_scratch(_scratch(need, device, stream), need)
+    return _launch_on(row["name"], ops, stream, device)
 
 
 def row_launcher(row_name):

@@ -1,0 +1,60 @@
+/* r3d_act_dev.h -- the activations of r3d_act.h on the device, in f32. */
+#ifndef R3D_ACT_DEV_H
+#define R3D_ACT_DEV_H
+
+#include <hip/hip_runtime.h>
+
+#include "r3d_act.h"
+
+namespace r3d {
+
+/* sigmoid(g) = 1 / (1 + exp(-g)) in f32, within 3 ulp where that is a normal number (g over -87.3; under that
+ * it may be 0, off by less than 2^-126): exp2 of the product's high part (its
+ * rounding error times ln 2 is a factor on top, which keeps large |g| exact) and a reciprocal with
+ * one Newton step.  Past 100 exp is inf and the result 0, as 1 / (1 + inf). */
+__device__ __forceinline__ float i8_sigmoid(float g) {
+    const float x = __builtin_fminf(__builtin_fmaxf(-g, -100.0f), 100.0f);
+    const float t = x * 1.44269504f;
+    const float lo = __builtin_fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    const float d = 1.0f + __builtin_fmaf(e, lo * 0.693147181f, e);
+    float r = __builtin_amdgcn_rcpf(d);
+    r = d < 3.0e38f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : 0.0f;
+    return g != g ? g : r;
+}
+
+/* One activation over W values; `act` is the same on every lane, so one branch is taken.
+ *   gelu       v Phi(v) = v erfc(-v / sqrt 2) / 2: erfc keeps the lower tail, where 1 + erf cancels
+ *   gelu_tanh  v (1 + tanh(u)) / 2 with u = sqrt(2 / pi) (v + 0.044715 v^3), which is v sigmoid(2 u)
+ * A NaN stays one; silu and both gelus of -inf are NaN (-inf * 0). */
+template <int W>
+__device__ __forceinline__ void act_values(int act, float* v) {
+    switch (act) {
+        case ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+            break;
+        case ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] *= i8_sigmoid(v[i]);
+            break;
+        case ACT_SIGMOID:
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = i8_sigmoid(v[i]);
+            break;
+        case ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = 0.5f * v[i] * erfcf(v[i] * -0.707106781f);
+            break;
+        case ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+                v[i] *= i8_sigmoid(1.59576912f * __builtin_fmaf(0.044715f * v[i] * v[i], v[i], v[i]));
+            break;
+        default: break;
+    }
+}
+
+}  // namespace r3d
+
+#endif /* R3D_ACT_DEV_H */

@@ -65,6 +65,9 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g);
  * are given are planned as the launch plans them. */
 int64_t i8_scratch_bytes(const RadArgs* a, int ncu);
 
+/* The bytes of planes that the best launch of a plan wants. */
+int64_t i8_planes_bytes(const I8Plan& P, int ncu);
+
 /* Codes out of a band producer, one scale a row. */
 struct I8BandPlan {
     const uint8_t* x;        /* the activation, or gate_up [rows, 2n] */

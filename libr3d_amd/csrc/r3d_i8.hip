@@ -12,20 +12,10 @@
 #include "r3d_i8.h"
 #include "r3d_i8_any.h"
 #include "r3d_i8_band.h"
-#include "r3d_i8_gemv.h"
-#include "r3d_i8_tile.h"
-#include "r3d_i8_wide.h"
+#include "r3d_i8_launch.h"
 #include "r3d_plan.h"
 
 namespace r3d {
-
-bool chip_ok();                  /* r3d_gemm.hip */
-int cu_count();
-
-static int i8_failed(const char* what, hipError_t e) {
-    fprintf(stderr, "libr3d_gfx950: %s launch FAILED (%s)\n", what, hipGetErrorName(e));
-    return RAD_E_DEVICE;
-}
 
 static int i8_launch_any(const I8Plan& P, hipStream_t stream) {
     const int tm = P.M <= 16 ? 1 : 2;
@@ -42,67 +32,6 @@ static int i8_launch_any(const I8Plan& P, hipStream_t stream) {
     return e == hipSuccess ? RAD_OK : i8_failed("i8a8 any-alignment GEMM", e);
 }
 
-static int i8_launch_gemv(const I8Plan& P, const I8Geom& g, hipStream_t stream) {
-    int64_t lds = P.M * i8_gemv_row(P.K);
-    if (g.kc > 1 && lds < (int64_t)g.waves * 256) lds = g.waves * 256;    /* the chunks' join */
-    if (P.M < 1 || P.M > 8 || lds > kI8GemvLds || g.kc < 1 || g.waves % g.kc ||
-        g.blocks > 0x7FFFFFFF || (int64_t)g.kc * g.per * 128 < P.K)
-        return RAD_E_UNSUPPORTED;
-    const I8GemvArgs a{P.A, P.B, P.SA, P.SB, P.Y, (int)P.M, (int)P.N, (int)P.K, (int)P.a_pitch,
-                       (int)P.b_pitch, g.kc, g.per, P.sa_stride, P.sb_stride, P.y_pitch};
-    const dim3 grid((unsigned)g.blocks), block((unsigned)(64 * g.waves));
-    if (g.waves == 4)
-        hipLaunchKernelGGL((i8_gemv_kernel<4>), grid, block, (size_t)lds, stream, a);
-    else if (g.waves == 8)
-        hipLaunchKernelGGL((i8_gemv_kernel<8>), grid, block, (size_t)lds, stream, a);
-    else
-        return RAD_E_UNSUPPORTED;
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? RAD_OK : i8_failed("i8a8 GEMV", e);
-}
-
-static int i8_launch_tile(const I8Plan& P, const I8Geom& g, int* part, hipStream_t stream) {
-    if (g.blocks > 0x7FFFFFFF || (int64_t)g.kc * g.per * 128 < P.K || (g.kc > 1 && !part) ||
-        (g.kc > 1 && P.M > 65535))
-        return RAD_E_UNSUPPORTED;
-    const I8TileArgs a{P.A, P.B, P.SA, P.SB, P.Y, part, (int)P.M, (int)P.N, (int)P.K, (int)P.a_pitch,
-                       (int)P.b_pitch, (int)((P.M + g.bm - 1) / g.bm), (int)g.tiles, g.kc, g.per,
-                       P.sa_stride, P.sb_stride, P.y_pitch};
-    const dim3 grid((unsigned)g.blocks);
-#define R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, OFF_)                                           \
-    hipLaunchKernelGGL((i8_tile_kernel<WNF_, WMF_, WVN_, WVM_, NST_, OFF_>), grid,              \
-                       dim3(64 * WVN_ * WVM_),                                                 \
-                       (size_t)i8_tile_lds(16 * WNF_ * WVN_, 16 * WMF_ * WVM_, NST_), stream, a)
-#define R3D_I8T2(WNF_, WMF_, WVN_, WVM_, NST_, ONST_)                                         \
-    if (P.off) { R3D_I8T(WNF_, WMF_, WVN_, WVM_, ONST_, true); }                                \
-    else { R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, false); }                                      \
-    break
-    switch (g.tile) {
-        case I8_T_256x256:
-            hipLaunchKernelGGL(i8_wide_kernel, grid, dim3(512), (size_t)i8_tile_lds(256, 256, 2), stream, a);
-            break;
-        case I8_T_128x256: R3D_I8T(4, 4, 2, 4, 3, false); break;
-        case I8_T_128x192: R3D_I8T(2, 6, 4, 2, 3, false); break;
-        case I8_T_128x128: R3D_I8T2(2, 4, 4, 2, 4, 5);
-        case I8_T_128x96: R3D_I8T2(2, 6, 4, 1, 4, 5);
-        case I8_T_128x64: R3D_I8T2(2, 4, 4, 1, 4, 5);
-        case I8_T_64x64: R3D_I8T2(1, 4, 4, 1, 4, 5);
-        case I8_T_64x32: R3D_I8T2(1, 2, 4, 1, 6, 6);
-        case I8_T_32x32: R3D_I8T2(1, 2, 2, 1, 10, 10);
-        default: R3D_I8T2(1, 1, 2, 1, 8, 8);
-    }
-#undef R3D_I8T2
-#undef R3D_I8T
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess && g.kc > 1) {
-        hipLaunchKernelGGL(i8_join_kernel, dim3((unsigned)((P.N + 255) / 256), (unsigned)P.M), dim3(64), 0,
-                           stream, part, P.SA, P.SB, P.Y, g.kc, (int)P.M, (int)P.N, P.sa_stride,
-                           P.sb_stride, P.y_pitch);
-        e = hipGetLastError();
-    }
-    return e == hipSuccess ? RAD_OK : i8_failed("i8a8 GEMM", e);
-}
-
 /* Scratch is optional: without it, or with less than the hook asks for or off 16 bytes, K stays in
  * as few chunks as its planes fit. */
 static int i8_entry(const RadArgs* a, RadStream s, bool decode) {
@@ -115,9 +44,15 @@ static int i8_entry(const RadArgs* a, RadStream s, bool decode) {
     I8Geom g;
     i8_geom(P, cu_count(), sc ? a->scratch_bytes : 0, &g);
     hipStream_t stream = (hipStream_t)s;
-    if (g.arm == I8_GEMV) return i8_launch_gemv(P, g, stream);
-    if (g.arm == I8_TILE) return i8_launch_tile(P, g, (int*)a->scratch, stream);
-    return i8_launch_any(P, stream);
+    if (g.arm == I8_GEMV) return i8_launch_gemv<I8Ops>(P, g, nullptr, stream);
+    if (g.arm != I8_TILE) return i8_launch_any(P, stream);
+    const int lrc = i8_launch_tile<I8Ops>(P, g, a->scratch, nullptr, stream);
+    if (lrc != RAD_OK || g.kc == 1) return lrc;
+    hipLaunchKernelGGL(i8_join_kernel, dim3((unsigned)((P.N + 255) / 256), (unsigned)P.M), dim3(64), 0,
+                       stream, (const int*)a->scratch, P.SA, P.SB, P.Y, g.kc, (int)P.M, (int)P.N, P.sa_stride,
+                       P.sb_stride, P.y_pitch);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? RAD_OK : i8_failed("i8a8 GEMM", e);
 }
 
 static int i8_band_entry(const RadArgs* a, RadStream s, int op) {

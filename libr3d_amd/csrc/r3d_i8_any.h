@@ -37,6 +37,29 @@ __device__ __forceinline__ r3d_i32x4 i8_keep(r3d_i32x4 v, int left) {
     return v;
 }
 
+/* What a product's kernels are made for: the matrix instructions over 16-byte operand pieces (64 int8
+ * codes or 32 bf16 of K in the four lanes of a row: the same bytes in the same lanes), their sums, and what
+ * happens to these.  I8Ops is gemm_nt_q at i8a8; gemm_nt_epi's are in r3d_epi_dev.h. */
+struct I8GemvArgs;
+struct I8TileArgs;
+typedef int r3d_i32x16 __attribute__((ext_vector_type(16)));
+struct I8Ops {
+    typedef int Sum;
+    typedef r3d_i32x4 Acc4;
+    typedef r3d_i32x16 Acc16;
+    typedef I8GemvArgs GemvArgs;
+    typedef I8TileArgs TileArgs;
+    static constexpr bool kScaled = true;       /* a scale a token and one a weight row */
+    static constexpr bool kZeroBoth = false;    /* a zero times whatever lies past K may be no zero */
+    static constexpr bool kEpi = false;         /* bias, activation, residual */
+    static __device__ __forceinline__ Acc4 mfma16(r3d_i32x4 w, r3d_i32x4 x, Acc4 c) {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Acc16 mfma32(r3d_i32x4 w, r3d_i32x4 x, Acc16 c) {
+        return __builtin_amdgcn_mfma_i32_32x32x32_i8(w, x, c, 0, 0, 0);
+    }
+};
+
 template <int TM>
 __global__ __launch_bounds__(256) void i8_any_kernel(
     const uint8_t* __restrict__ A, const float* __restrict__ SA, const uint8_t* __restrict__ B,

@@ -28,6 +28,7 @@
 #ifndef R3D_I8_BAND_H
 #define R3D_I8_BAND_H
 
+#include "r3d_act_dev.h"
 #include "r3d_device.h"
 #include "r3d_i8.h"
 #include "r3d_wave.h"
@@ -99,21 +100,6 @@ __device__ __forceinline__ void i8_st8(uint8_t* row, int64_t i, int64_t n, const
         for (int j = 0; j < 8; ++j)
             if (i + j < n) reinterpret_cast<float*>(row)[i + j] = v[j];
     }
-}
-
-/* sigmoid(g) = 1 / (1 + exp(-g)) in f32, within 3 ulp where that is a normal number (g over -87.3; under that
- * it may be 0, off by less than 2^-126): exp2 of the product's high part (its
- * rounding error times ln 2 is a factor on top, which keeps large |g| exact) and a reciprocal with
- * one Newton step.  Past 100 exp is inf and the result 0, as 1 / (1 + inf). */
-__device__ __forceinline__ float i8_sigmoid(float g) {
-    const float x = __builtin_fminf(__builtin_fmaxf(-g, -100.0f), 100.0f);
-    const float t = x * 1.44269504f;
-    const float lo = __builtin_fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-    const float e = __builtin_amdgcn_exp2f(t);
-    const float d = 1.0f + __builtin_fmaf(e, lo * 0.693147181f, e);
-    float r = __builtin_amdgcn_rcpf(d);
-    r = d < 3.0e38f ? __builtin_fmaf(__builtin_fmaf(-d, r, 1.0f), r, r) : 0.0f;
-    return g != g ? g : r;
 }
 
 /* bf16(residual + x), also to element i of the row at ro on. */

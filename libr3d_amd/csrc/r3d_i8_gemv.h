@@ -23,6 +23,7 @@
 #define R3D_I8_GEMV_H
 
 #include "r3d_device.h"
+#include "r3d_epi_dev.h"
 #include "r3d_i8_any.h"
 
 namespace r3d {
@@ -36,6 +37,7 @@ __device__ __forceinline__ r3d_i32x4 i8_buf16(__amdgpu_buffer_rsrc_t r, uint32_t
                               __builtin_amdgcn_raw_buffer_load_b128(r, (int)voff, (int)soff, NT));
 }
 
+/* A and B in bytes, K a row's bytes */
 struct I8GemvArgs {
     const uint8_t* A;
     const uint8_t* B;
@@ -46,8 +48,8 @@ struct I8GemvArgs {
     int64_t sa_stride, sb_stride, y_pitch;
 };
 
-template <int W>
-__global__ __launch_bounds__(64 * W) void i8_gemv_kernel(I8GemvArgs P) {
+template <class T, int W>
+__global__ __launch_bounds__(64 * W) void i8_gemv_kernel(typename T::GemvArgs P) {
     constexpr int D = 4, SB = 4;
     extern __shared__ __attribute__((aligned(16))) uint8_t s_a[];   /* [M][lp]; then [W][16] i32x4 */
     const int lane = threadIdx.x & 63;
@@ -80,7 +82,7 @@ __global__ __launch_bounds__(64 * W) void i8_gemv_kernel(I8GemvArgs P) {
     const bool mine = c == 0 && lane < 32 && (lane & 8) == 0;
     const int ml = lane & 7, nl = 4 * ((lane >> 4) & 1);
     float sb[4], sa = 0.0f;
-    if (mine) {
+    if (T::kScaled && mine) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t n = n0 + nl + i;
@@ -89,7 +91,8 @@ __global__ __launch_bounds__(64 * W) void i8_gemv_kernel(I8GemvArgs P) {
         if (ml < P.M) sa = P.SA[ml * P.sa_stride];
     }
 
-    r3d_i32x4 w[D], acc = {0, 0, 0, 0};
+    r3d_i32x4 w[D];
+    typename T::Acc4 acc = {0, 0, 0, 0};
     auto load = [&](int s) __attribute__((always_inline)) {
         const int k = (l0 + s) * 128;
         return i8_buf16<2>(rB, 16 * chunk < k1 - k ? wo : kI8Oob, k);   /* zeros past the chunk's end */
@@ -111,8 +114,9 @@ __global__ __launch_bounds__(64 * W) void i8_gemv_kernel(I8GemvArgs P) {
 #pragma unroll
         for (int d = 0; d < D; ++d) {
             const int k = (l0 + s + d) * 128;                   /* past K the weights are zeros */
-            const r3d_i32x4 x = *reinterpret_cast<const r3d_i32x4*>(xa + (k < lp - 16 ? k : 0));
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[d], x, acc, 0, 0, 0);
+            r3d_i32x4 x = *reinterpret_cast<const r3d_i32x4*>(xa + (k < lp - 16 ? k : 0));
+            if (T::kZeroBoth && s + d >= steps) x = r3d_i32x4{0, 0, 0, 0};
+            acc = T::mfma16(w[d], x, acc);
             w[d] = load(s + D + d);
         }
     }
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(64 * W) void i8_gemv_kernel(I8GemvArgs P) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[i] += __shfl(acc[i], (lane + 40) & 63, 64);
     if (P.kc > 1) {
-        r3d_i32x4* const s_part = reinterpret_cast<r3d_i32x4*>(s_a);
+        typename T::Acc4* const s_part = reinterpret_cast<typename T::Acc4*>(s_a);
         const int slot = (lane >> 4) * 8 + ml;                  /* 16 lanes hold the results */
         __syncthreads();                                        /* the tokens are read */
         if (c > 0 && lane < 32 && (lane & 8) == 0) s_part[wave * 16 + slot] = acc;
@@ -130,10 +134,15 @@ __global__ __launch_bounds__(64 * W) void i8_gemv_kernel(I8GemvArgs P) {
     }
     const int64_t n = n0 + nl;
     if (!mine || ml >= P.M || n >= P.N) return;
-    uint16_t* y = P.Y + ml * P.y_pitch + n;
     float v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i8_out(acc[i], sa, sb[i]);
+    for (int i = 0; i < 4; ++i) v[i] = T::kScaled ? i8_out(acc[i], sa, sb[i]) : (float)acc[i];
+    if constexpr (T::kEpi) {
+        epi_values<4>(P.e, v, ml, n, P.N);
+        epi_store<4>(P.e, P.Y, P.y_pitch, v, ml, n, P.N);
+        return;
+    }
+    uint16_t* y = P.Y + ml * P.y_pitch + n;
     if (n + 4 <= P.N) {
         *reinterpret_cast<r3d_u32x2_u2*>(y) =
             r3d_u32x2_u2{r3d_pack_bf16x2(v[0], v[1]), r3d_pack_bf16x2(v[2], v[3])};

@@ -7,44 +7,10 @@
 #include <string.h>
 
 #include "rad_plugin.h"
+#include "r3d_operands.h"
 #include "r3d_plan.h"
 
 namespace r3d {
-
-static const int64_t kDimMax = 0x7FFFFFFLL;
-
-static bool pitch_ok(int64_t p) { return p >= 0 && p <= (int64_t(1) << 40); }
-
-/* One f32 a row: rank 1 [rows], or rank 2 [rows, 1]; the stride may be 0 (one scale for all). */
-static int scale_column(const RadTensor* t, int64_t rows, int64_t* stride) {
-    if (t->dtype != RAD_F32) return RAD_E_UNSUPPORTED;
-    if ((t->rank != 1 && t->rank != 2) || (t->rank == 2 && t->shape[1] != 1)) return RAD_E_SHAPE;
-    if (t->shape[0] < rows) return RAD_E_SHAPE;
-    *stride = t->stride[0];
-    return pitch_ok(*stride) ? RAD_OK : RAD_E_STRIDE;
-}
-
-/* The pitch of a [rows, cols] operand whose rows lie anywhere: rank 2 with its own row stride,
- * or higher ranks whose outer axes are dense; rank 1 is one row. */
-static int rows_of(const RadTensor* t, int64_t rows, int64_t cols, int64_t* pitch) {
-    const long long n = rad_tensor_numel(t);
-    if (n < 0 || rows > INT64_MAX / cols || n < rows * cols) return RAD_E_SHAPE;
-    if (t->rank == 1) {
-        if (rows != 1 || n != cols) return RAD_E_SHAPE;
-        if (t->stride[0] != 1) return RAD_E_STRIDE;
-        *pitch = cols;
-        return RAD_OK;
-    }
-    if (t->rank < 2 || t->shape[t->rank - 1] != cols) return RAD_E_SHAPE;
-    if (t->stride[t->rank - 1] != 1) return RAD_E_STRIDE;
-    for (int i = 0; i + 2 < (int)t->rank; ++i) {
-        int64_t span = 0;
-        if (__builtin_mul_overflow(t->shape[i + 1], t->stride[i + 1], &span) || t->stride[i] != span)
-            return RAD_E_STRIDE;
-    }
-    *pitch = t->stride[t->rank - 2];
-    return pitch_ok(*pitch) ? RAD_OK : RAD_E_STRIDE;
-}
 
 int plan_i8(const RadArgs* a, int64_t m_max, I8Plan* P) {
     const RadTensor* A  = rad_arg_in(a, 0);
@@ -217,6 +183,10 @@ int64_t i8_scratch_bytes(const RadArgs* a, int ncu) {
         P.ua = (K & 15) != 0;
         P.off = (K & 127) != 0;
     }
+    return i8_planes_bytes(P, ncu);
+}
+
+int64_t i8_planes_bytes(const I8Plan& P, int ncu) {
     I8Geom g;
     i8_geom(P, ncu, kI8MaxPlanes, &g);
     return g.arm == I8_TILE && g.kc > 1 ? (int64_t)g.kc * P.M * P.N * 4 : 0;

@@ -34,23 +34,25 @@
 #define R3D_I8_TILE_H
 
 #include "r3d_device.h"
+#include "r3d_epi_dev.h"
 #include "r3d_i8_any.h"
 
 namespace r3d {
 
+/* A and B in bytes, K a row's bytes */
 struct I8TileArgs {
     const uint8_t* A;
     const uint8_t* B;
     const float* SA;
     const float* SB;
     uint16_t* Y;
-    int* part;                       /* kc > 1: i32 [kc][M][N] */
+    void* part;                      /* kc > 1: i32 (or f32, of bf16) [kc][M][N] */
     int M, N, K, a_pitch, b_pitch, grid_m, tiles, kc, cst;
     int64_t sa_stride, sb_stride, y_pitch;
 };
 
-template <int WNF, int WMF, int WVN, int WVM, int NST, bool OFF>
-__global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
+template <class T, int WNF, int WMF, int WVN, int WVM, int NST, bool OFF>
+__global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(typename T::TileArgs P) {
     constexpr int WV = WVN * WVM, BN = 16 * WNF * WVN, BM = 16 * WMF * WVM;
     constexpr int WLD = BN / 8 / WV, ALD = BM / 8 / WV, LOADS = WLD + ALD;   /* 1 KB loads a wave */
     static_assert(WLD * WV * 8 == BN && ALD * WV * 8 == BM, "whole loads a wave");
@@ -117,11 +119,11 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
             r3d_buf_lds<16>(rA, st + AOFF + 1024 * (wave + WV * i), aok ? aoff[i] : 0x80000000u, k);
     };
 
-    r3d_i32x4 acc[WNF][WMF];
+    typename T::Acc4 acc[WNF][WMF];
 #pragma unroll
     for (int a = 0; a < WNF; ++a)
 #pragma unroll
-        for (int b = 0; b < WMF; ++b) acc[a][b] = r3d_i32x4{0, 0, 0, 0};
+        for (int b = 0; b < WMF; ++b) acc[a][b] = typename T::Acc4{0, 0, 0, 0};
     const int rd0 = 128 * li + 16 * (q ^ (li & 7)), rd1 = 128 * li + 16 * ((4 + q) ^ (li & 7));
     /* fragments of one half step (64 of K): half 0 and half 1 each have a register set, read while
      * the other half's products run */
@@ -144,7 +146,7 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
         for (int b = 0; b < WMF; ++b)
 #pragma unroll
             for (int a = 0; a < WNF; ++a)
-                acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[h][a], xf[h][b], acc[a][b], 0, 0, 0);
+                acc[a][b] = T::mfma16(wf[h][a], xf[h][b], acc[a][b]);
         /* a read between every so many products */
         constexpr int PER = WNF * WMF / (WNF + WMF) > 0 ? WNF * WMF / (WNF + WMF) : 1;
 #pragma unroll
@@ -173,7 +175,8 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            /* the loads past the end, before LDS goes */
 
     if (P.kc > 1) {
-        int* const part = P.part + (int64_t)kci * P.M * P.N;
+        typedef typename T::Sum Sum;
+        Sum* const part = reinterpret_cast<Sum*>(P.part) + (int64_t)kci * P.M * P.N;
 #pragma unroll
         for (int b = 0; b < WMF; ++b) {
             const int64_t m = m0 + 16 * (wm * WMF + b) + li;
@@ -181,9 +184,9 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
 #pragma unroll
             for (int a = 0; a < WNF; ++a) {
                 const int64_t n = n0 + 16 * (wn * WNF + a) + 4 * q;
-                typedef int i32x4_u4 __attribute__((ext_vector_type(4), aligned(4)));
+                typedef Sum sumx4_u4 __attribute__((ext_vector_type(4), aligned(4)));
                 if (n + 4 <= P.N) {
-                    *reinterpret_cast<i32x4_u4*>(part + m * P.N + n) = acc[a][b];
+                    *reinterpret_cast<sumx4_u4*>(part + m * P.N + n) = acc[a][b];
                 } else {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -191,6 +194,19 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
                 }
             }
         }
+        return;
+    }
+    if constexpr (T::kEpi) {
+        static_assert(BM * epi_row(BN) <= NST * STAGE, "the sums in the ring's place");
+        __syncthreads();                                        /* every wave is done with the ring */
+#pragma unroll
+        for (int b = 0; b < WMF; ++b)
+#pragma unroll
+            for (int a = 0; a < WNF; ++a)
+                *reinterpret_cast<typename T::Acc4*>(smem + (16 * (wm * WMF + b) + li) * epi_row(BN) +
+                                                     4 * (16 * (wn * WNF + a) + 4 * q)) = acc[a][b];
+        __syncthreads();
+        epi_tile<T, BN, 64 * WV>(P, smem, BM, m0, n0);
         return;
     }
     /* the bf16 tile through LDS, a token's row 32 bytes off a multiple of 128, then 16 bytes a lane */
@@ -211,7 +227,7 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(I8TileArgs P) {
         const float sa = P.SA[(m < P.M ? m : P.M - 1) * P.sa_stride];
 #pragma unroll
         for (int a = 0; a < WNF; ++a) {
-            const r3d_i32x4 v = acc[a][b];
+            const typename T::Acc4 v = acc[a][b];
             *reinterpret_cast<uint2*>(smem + ml * YP + 2 * (16 * (wn * WNF + a) + 4 * q)) =
                 make_uint2(r3d_pack_bf16x2(i8_out(v[0], sa, sb[a][0]), i8_out(v[1], sa, sb[a][1])),
                            r3d_pack_bf16x2(i8_out(v[2], sa, sb[a][2]), i8_out(v[3], sa, sb[a][3])));
@@ -240,7 +256,7 @@ constexpr int i8_tile_lds(int bn, int bm, int nst) {
 }
 
 /* Y of kc i32 planes: four columns a lane, (ceil(N / 256) , M) workgroups of 64. */
-__global__ __launch_bounds__(64) void i8_join_kernel(const int* __restrict__ part, const float* __restrict__ SA,
+static __global__ __launch_bounds__(64) void i8_join_kernel(const int* __restrict__ part, const float* __restrict__ SA,
                                                      const float* __restrict__ SB, uint16_t* __restrict__ Y,
                                                      int kc, int M, int N, int64_t sa_stride,
                                                      int64_t sb_stride, int64_t y_pitch) {

@@ -24,9 +24,8 @@
 
 namespace r3d {
 
-typedef int r3d_i32x16 __attribute__((ext_vector_type(16)));
-
-__global__ __launch_bounds__(512) void i8_wide_kernel(I8TileArgs P) {
+template <class T>
+__global__ __launch_bounds__(512) void i8_wide_kernel(typename T::TileArgs P) {
     constexpr int BN = 256, BM = 256, AOFF = BN * 128, STAGE = (BN + BM) * 128;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63;
@@ -76,7 +75,7 @@ __global__ __launch_bounds__(512) void i8_wide_kernel(I8TileArgs P) {
         }
     };
 
-    r3d_i32x16 acc[2][4];
+    typename T::Acc16 acc[2][4];
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
@@ -103,7 +102,7 @@ __global__ __launch_bounds__(512) void i8_wide_kernel(I8TileArgs P) {
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
-                    acc[a][b] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[a][p], xf[b & 1][p], acc[a][b], 0, 0, 0);
+                    acc[a][b] = T::mfma32(wf[a][p], xf[b & 1][p], acc[a][b]);
                     if (b == 3) read_w(nxt, a, p);
                 }
                 __builtin_amdgcn_s_setprio(0);
@@ -161,8 +160,9 @@ __global__ __launch_bounds__(512) void i8_wide_kernel(I8TileArgs P) {
 
     /* lane l's element i of a 32 x 32 result is weight row 8 (i / 4) + 4 (l / 32) + i % 4, token l % 32 */
     if (P.kc > 1) {
-        int* const part = P.part + (int64_t)kci * P.M * P.N;
-        typedef int i32x4_u4 __attribute__((ext_vector_type(4), aligned(4)));
+        typedef typename T::Sum Sum;
+        Sum* const part = reinterpret_cast<Sum*>(P.part) + (int64_t)kci * P.M * P.N;
+        typedef Sum sumx4_u4 __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int64_t m = m0 + 128 * wm + 32 * b + lj;
@@ -173,14 +173,37 @@ __global__ __launch_bounds__(512) void i8_wide_kernel(I8TileArgs P) {
                 for (int g = 0; g < 4; ++g) {
                     const int64_t n = n0 + 64 * wn + 32 * a + 8 * g + 4 * lh;
                     if (n + 4 <= P.N) {
-                        *reinterpret_cast<i32x4_u4*>(part + m * P.N + n) =
-                            i32x4_u4{acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+                        *reinterpret_cast<sumx4_u4*>(part + m * P.N + n) =
+                            sumx4_u4{acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
                     } else {
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             if (n + i < P.N) part[m * P.N + n + i] = acc[a][b][4 * g + i];
                     }
                 }
+        }
+        return;
+    }
+    if constexpr (T::kEpi) {
+        /* half the tokens at a time: the sums of all would take 256 KB */
+        static_assert(128 * epi_row(BN) <= i8_tile_lds(BN, BM, 2), "the sums in the ring's place");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __syncthreads();                                    /* the ring, or the half before, is read */
+#pragma unroll
+            for (int b2 = 0; b2 < 2; ++b2)
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const typename T::Acc16& v = acc[a][2 * h + b2];
+                        *reinterpret_cast<typename T::Acc4*>(smem + (64 * wm + 32 * b2 + lj) * epi_row(BN) +
+                                                             4 * (64 * wn + 32 * a + 8 * g + 4 * lh)) =
+                            typename T::Acc4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+                    }
+            __syncthreads();
+            epi_tile<T, BN, 512>(P, smem, 64, m0 + 64 * h, n0);
+            epi_tile<T, BN, 512>(P, smem + 64 * epi_row(BN), 64, m0 + 128 + 64 * h, n0);
         }
         return;
     }

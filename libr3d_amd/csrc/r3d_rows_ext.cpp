@@ -10,14 +10,17 @@
  *   gated_quant_i8           prio 1000  n GE 1, dtype IN f32 bf16           gated producer
  *   rmsnorm_quant_i8         prio 1000  n GE 1, dtype IN bf16               norm producer
  *   sample_logits            prio 1000  n_vocab GE 1, dtype IN f32 bf16     sampler
+ *   gemm_nt_epi_bf16         prio 1000  dtype IN bf16                     product with an epilogue
+ *   gemm_nt_epi_i8a8         prio 1000  dtype IN i8a8                     the same over int8 codes
  *
  * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row (and turns off its GEMV in the other
- * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler (presence-tested, read once; hidden at
- * registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler, R3D_NO_EPI gemm_nt_epi's rows (presence-tested,
+ * read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
 #include "rad_abi.h"
+#include "r3d_epi.h"
 #include "r3d_i8.h"
 #include "r3d_sample.h"
 
@@ -30,6 +33,10 @@ int r3d_rad_gated_quant_i8(const RadArgs* a, RadStream s);
 int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
 int r3d_rad_sample_logits(const RadArgs* a, RadStream s);
 int64_t r3d_rad_sample_logits_scratch(const RadArgs* a);
+int r3d_rad_gemm_nt_epi_bf16(const RadArgs* a, RadStream s);
+int64_t r3d_rad_gemm_nt_epi_bf16_scratch(const RadArgs* a);
+int r3d_rad_gemm_nt_epi_i8(const RadArgs* a, RadStream s);
+int64_t r3d_rad_gemm_nt_epi_i8_scratch(const RadArgs* a);
 }
 
 namespace {
@@ -89,6 +96,23 @@ const RadOperandSpec kSampleOperands[] = {
     {"prob", RAD_OPD_OUT, 1},
 };
 
+const RadParamSpec kEpiParams[] = {
+    {"M", RAD_P_INT, RAD_DERIVED, 0},
+    {"N", RAD_P_INT, RAD_REQUIRED, 0},
+    {"K", RAD_P_INT, RAD_REQUIRED, 0},
+    {"dtype", RAD_P_STR, RAD_REQUIRED, 0},
+    {"act", RAD_P_STR, RAD_OPTIONAL, 0},
+};
+const RadOperandSpec kEpiOperands[] = {
+    {"a", RAD_OPD_IN, 0},
+    {"a_scale", RAD_OPD_IN, 1},
+    {"b", RAD_OPD_WEIGHT, 0},
+    {"b_scale", RAD_OPD_WEIGHT, 1},
+    {"bias", RAD_OPD_WEIGHT, 1},
+    {"residual", RAD_OPD_IN, 1},
+    {"y", RAD_OPD_OUT, 0},
+};
+
 const RadOpSchema kSchemas[] = {
     {"quant_act_i8", kQuantParams, 3, kQuantOperands, 3,
      "symmetric int8 quantisation of an activation with one f32 scale a row, amax/127."},
@@ -102,6 +126,9 @@ const RadOpSchema kSchemas[] = {
      "one token a row of logits from a uniform number u in [0, 1): softmax at the row's temperature, "
      "top-k, top-p of those, min-p of those, then the first kept token in index order whose running "
      "mass passes u times the kept mass; prob is its share of that mass."},
+    {"gemm_nt_epi", kEpiParams, 5, kEpiOperands, 7,
+     "y = act(S * a . b^T + bias) + residual, rounded once: S = 1 at bf16, a_scale * b_scale at i8a8; act none "
+     "(default), relu, silu, sigmoid, gelu or gelu_tanh; y may be the residual's memory."},
 };
 
 const RadConstraint cI8[] = {
@@ -121,6 +148,10 @@ const RadConstraint cSample[] = {
 };
 const RadConstraint cNorm[] = {
     {"n", RAD_C_GE, 1, nullptr},
+    {"dtype", RAD_C_IN, 0, "bf16"},
+};
+
+const RadConstraint cEpiBf16[] = {
     {"dtype", RAD_C_IN, 0, "bf16"},
 };
 
@@ -172,10 +203,26 @@ const RadKernelInfo kRows[] = {
      "f32/bf16 logits, f32 u, temperature, top_p, min_p, i32 top_k, i32 token, optional f32 prob",
      RAD_DOMAIN_DEVICE, kPrioTile, cSample, 2, nullptr, 0, nullptr, nullptr, nullptr,
      r3d_rad_sample_logits, r3d_rad_sample_logits_scratch, nullptr, nullptr, nullptr, nullptr},
+    {"gemm_nt_epi_bf16", "gemm_nt_epi", "gemm",
+     "bf16 product with bias, activation and residual applied to its f32 sums: up to M = 8 a GEMV or LDS tiles, above "
+     "LDS tiles of 32 x 16 to 256 x 256, K split over workgroups into f32 planes in launch scratch where tiles leave "
+     "compute units idle",
+     "K up to 1048576; operands at any alignment and pitch (row bytes, bases and pitches off 16 bytes: dword loads); "
+     "M derives from numel(y)/N; scratch optional",
+     "bf16 a and b, f32/bf16 bias [N], residual [M, N] and y",
+     RAD_DOMAIN_DEVICE, kPrioTile, cEpiBf16, 1, nullptr, 0, nullptr, nullptr, nullptr,
+     r3d_rad_gemm_nt_epi_bf16, r3d_rad_gemm_nt_epi_bf16_scratch, nullptr, nullptr, nullptr, nullptr},
+    {"gemm_nt_epi_i8a8", "gemm_nt_epi", "gemm",
+     "int8 product (gemm_nt_q_i8a8's) with bias, activation and residual applied to its scaled f32 values",
+     "K up to 131071; else as gemm_nt_epi_bf16",
+     "int8 a with f32 a_scale [M] or [M, 1], int8 b with f32 b_scale [N] or [N, 1], f32/bf16 bias, residual and y",
+     RAD_DOMAIN_DEVICE, kPrioTile, cI8, 1, nullptr, 0, nullptr, nullptr, nullptr,
+     r3d_rad_gemm_nt_epi_i8, r3d_rad_gemm_nt_epi_i8_scratch, nullptr, nullptr, nullptr, nullptr},
 };
 
 bool row_hidden(const RadKernelInfo& k) {
     if (!strcmp(k.name, "sample_logits")) return r3d::env_no_sample();
+    if (!strcmp(k.op, "gemm_nt_epi")) return r3d::env_no_epi();
     if (!strcmp(k.name, "gemm_nt_q_i8a8_decode")) return r3d::env_no_i8() || r3d::env_no_i8_dec();
     return r3d::env_no_i8();
 }
