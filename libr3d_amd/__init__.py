@@ -26,7 +26,7 @@ __all__ = [
     "relayout_head", "unrelayout_head", "ext_rows", "ext_schemas", "QuantActI8Operands",
     "GatedQuantI8Operands", "RmsNormQuantI8Operands", "quant_act_i8", "gated_quant_i8",
     "rmsnorm_quant_i8", "SampleOperands", "sample_logits",
-    "GemmEpiOperands", "gemm_nt_epi",
+    "GemmEpiOperands", "gemm_nt_epi", "RmsNormBlockOperands", "rmsnorm_block",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -690,6 +690,30 @@ class GemmEpiOperands(_Args):
                          ([("M", M)] if M is not None else []))
 
 
+class RmsNormBlockOperands(_Args):
+    """One rmsnorm_block call: h = res_scale * residual + gate * norm(x; w_post), then norm(h; w_pre).
+
+    x             float32 or bf16/int16 [M, n]
+    residual      optional bf16/int16 [M, n];  residual_out optional bf16/int16 [M, n] out: h
+    w_post, w_pre optional float32 or bf16/int16 [n] (without w_post x goes on as it is)
+    gate          optional, of the weights' type: [n], [M, 1] or [M, n]
+    out           optional float32 or bf16/int16 [M, n] out: norm(h; w_pre)
+    q, scale      optional codes of it: int8 [M, n] with float32 [M] or [M, 1], or uint8 / float8_e4m3fn [M, n] with
+                  float32 [M, ceil(n / 128)]
+    residual_out and out may be the memory of x, residual or gate.
+    """
+
+    def __init__(self, x, *, n, residual=None, w_post=None, gate=None, w_pre=None, residual_out=None, out=None, q=None,
+                 scale=None, eps=1e-6, wadd=None, res_scale=None, group=None, M=None):
+        ops = [(x, "BF16"), (residual, "BF16"), (w_post, "BF16"), (gate, "BF16"), (w_pre, "BF16"), (residual_out, "BF16"),
+               (out, "BF16"), (q, "I8"), (scale, "F32")]
+        super().__init__([(t, _type(t, dt), None, None) for t, dt in ops],
+                         [("n", n), ("eps", float(eps)), ("dtype", "f32" if _type(x, "") == "F32" else "bf16")] +
+                         ([("wadd", float(wadd))] if wadd is not None else []) +
+                         ([("res_scale", float(res_scale))] if res_scale is not None else []) +
+                         ([("group", group)] if group is not None else []) + ([("M", M)] if M is not None else []))
+
+
 class LogitsOperands(_Args):
     """One logits_gemm call (src/r3d_gemm_logits.hip:144-226).
 
@@ -975,6 +999,15 @@ def gemm_nt_epi(a, b, y, *, dtype, N, K, a_scale=None, b_scale=None, bias=None, 
     if need > 0:
         ops.set_scratch(_scratch(need, device, stream), need)
     return _launch_on(row["name"], ops, stream, device)
+
+
+def rmsnorm_block(x, *, n, residual=None, w_post=None, gate=None, w_pre=None, residual_out=None, out=None, q=None,
+                  scale=None, eps=1e-6, wadd=None, res_scale=None, group=None, stream=None):
+    """Launch the rmsnorm_block row on `stream` (default the current torch stream); its status."""
+    device = _one_gpu(x, residual, w_post, gate, w_pre, residual_out, out, q, scale)
+    ops = RmsNormBlockOperands(x, n=n, residual=residual, w_post=w_post, gate=gate, w_pre=w_pre, residual_out=residual_out,
+                               out=out, q=q, scale=scale, eps=eps, wadd=wadd, res_scale=res_scale, group=group)
+    return _launch_on("rmsnorm_block", ops, stream, device)
 
 
 def row_launcher(row_name):

@@ -1,0 +1,162 @@
+/* r3d_block_plan.cpp -- host plan of rmsnorm_block (see r3d_block.h). */
+#include "r3d_block.h"
+
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+
+#include "rad_plugin.h"
+#include "r3d_operands.h"
+
+namespace r3d {
+
+int plan_block(const RadArgs* a, BlockPlan* P) {
+    const RadTensor* x  = rad_arg_in(a, 0);
+    const RadTensor* rs = rad_arg_in(a, 1);
+    const RadTensor* wp = rad_arg_in(a, 2);
+    const RadTensor* g  = rad_arg_in(a, 3);
+    const RadTensor* wn = rad_arg_in(a, 4);
+    const RadTensor* ro = rad_arg_in(a, 5);
+    const RadTensor* o  = rad_arg_in(a, 6);
+    const RadTensor* q  = rad_arg_in(a, 7);
+    const RadTensor* sc = rad_arg_in(a, 8);
+    if (!x || (q == nullptr) != (sc == nullptr) || (!ro && !o && !q)) return RAD_E_INVAL;
+    if ((wn == nullptr) != (!o && !q)) return RAD_E_INVAL;      /* a norm with no result, or a result with no norm */
+    if (x->dtype != RAD_BF16 && x->dtype != RAD_F32) return RAD_E_DTYPE;
+    const char* dt = rad_args_gets(a, "dtype");                 /* names x's type, if given */
+    if (dt && strcmp(dt, x->dtype == RAD_BF16 ? "bf16" : "f32") != 0) return RAD_E_DTYPE;
+    if ((rs && rs->dtype != RAD_BF16) || (ro && ro->dtype != RAD_BF16)) return RAD_E_DTYPE;
+    if (o && o->dtype != RAD_BF16 && o->dtype != RAD_F32) return RAD_E_DTYPE;
+    if (sc && sc->dtype != RAD_F32) return RAD_E_DTYPE;
+    P->codes = !q ? BLOCK_NO_CODES : q->dtype == RAD_I8 ? BLOCK_I8
+             : q->dtype == RAD_F8E4M3 || q->dtype == RAD_U8 ? BLOCK_E4M3 : -1;
+    if (P->codes < 0) return RAD_E_DTYPE;
+    uint32_t wt = RAD_BF16;                                     /* one type for the weights and the gate */
+    bool any = false;
+    for (const RadTensor* t : {wp, g, wn}) {
+        if (!t) continue;
+        if ((t->dtype != RAD_F32 && t->dtype != RAD_BF16) || (any && t->dtype != wt)) return RAD_E_DTYPE;
+        wt = t->dtype;
+        any = true;
+    }
+    long long v = 0;
+    if (!rad_args_geti(a, "n", &v) || v <= 0 || v > kDimMax) return RAD_E_SHAPE;
+    const int64_t n = v;
+    if (n > kBlockMaxN) return RAD_E_UNSUPPORTED;
+    if (rad_args_geti(a, "group", &v) && v > 0 && v != (P->codes == BLOCK_E4M3 ? 128 : n)) return RAD_E_UNSUPPORTED;
+    const long long xn = rad_tensor_numel(x);
+    if (xn <= 0 || xn % n) return RAD_E_SHAPE;
+    const int64_t rows = xn / n;
+    if (rows > 0x7FFFFFFF) return RAD_E_SHAPE;
+    int rc = rows_of(x, rows, n, &P->x_pitch);
+    if (!rc && rs) rc = rows_of(rs, rows, n, &P->r_pitch);
+    if (!rc && ro) rc = rows_of(ro, rows, n, &P->ro_pitch);
+    if (!rc && o) rc = rows_of(o, rows, n, &P->o_pitch);
+    if (!rc && q) rc = rows_of(q, rows, n, &P->q_pitch);
+    if (!rc && sc) {
+        if (P->codes == BLOCK_I8) rc = scale_column(sc, rows, &P->s_pitch);
+        else rc = rows_of(sc, rows, (n + 127) / 128, &P->s_pitch);
+    }
+    if (rc) return rc;
+    for (const RadTensor* t : {wp, wn}) {
+        if (t && (t->rank != 1 || t->shape[0] != n)) return RAD_E_SHAPE;
+        if (t && t->stride[0] != 1) return RAD_E_STRIDE;
+    }
+    P->gate_kind = BLOCK_NO_GATE;
+    if (g) {
+        if (g->rank == 1 && g->shape[0] == n) {
+            if (g->stride[0] != 1) return RAD_E_STRIDE;
+            P->gate_kind = BLOCK_GATE_ROWS;
+            P->g_pitch = 0;
+        } else if (g->rank == 2 && g->shape[1] == 1 && n > 1) {
+            if (g->shape[0] != rows) return RAD_E_SHAPE;
+            P->gate_kind = BLOCK_GATE_TOKEN;
+            P->g_pitch = g->stride[0];
+            if (!pitch_ok(P->g_pitch)) return RAD_E_STRIDE;
+        } else {
+            if (g->rank < 2) return RAD_E_SHAPE;
+            P->gate_kind = BLOCK_GATE_ROWS;
+            if ((rc = rows_of(g, rows, n, &P->g_pitch))) return rc;
+        }
+    }
+    /* outputs whose rows overlap would race */
+    const int64_t s_cols = P->codes == BLOCK_E4M3 ? (n + 127) / 128 : 1;
+    if (rows > 1 && ((ro && P->ro_pitch < n) || (o && P->o_pitch < n) || (q && P->q_pitch < n) ||
+                     (sc && P->s_pitch < s_cols)))
+        return RAD_E_STRIDE;
+    for (const RadTensor* t : {x, rs, wp, g, wn, ro, o, sc})
+        if (misaligned(t)) return RAD_E_STRIDE;
+    /* an output may be x's, the residual's or the gate's own elements (a lane reads them before it writes);
+     * any other overlap would be read after it is written */
+    const int xb = elt_bytes(x->dtype), wb = elt_bytes(wt);
+    struct { const RadTensor* t; Span s; } outs[4] = {
+        {ro, {ro ? ro->data : nullptr, rows, n, P->ro_pitch, 2}},
+        {o, {o ? o->data : nullptr, rows, n, P->o_pitch, o ? elt_bytes(o->dtype) : 0}},
+        {q, {q ? q->data : nullptr, rows, n, P->q_pitch, 1}},
+        {sc, {sc ? sc->data : nullptr, rows, s_cols, P->s_pitch, 4}}};
+    for (int i = 0; i < 4; ++i) {
+        if (!outs[i].t) continue;
+        if (spans_clash(outs[i].s, Span{x->data, rows, n, P->x_pitch, xb})) return RAD_E_INVAL;
+        if (rs && spans_clash(outs[i].s, Span{rs->data, rows, n, P->r_pitch, 2})) return RAD_E_INVAL;
+        if (g && spans_clash(outs[i].s, Span{g->data, rows, P->gate_kind == BLOCK_GATE_TOKEN ? 1 : n, P->g_pitch, wb}))
+            return RAD_E_INVAL;
+        for (const RadTensor* w : {wp, wn})
+            if (w && spans_meet(outs[i].s, Span{w->data, 1, n, n, wb})) return RAD_E_INVAL;
+        for (int j = 0; j < i; ++j)
+            if (outs[j].t && spans_meet(outs[i].s, outs[j].s)) return RAD_E_INVAL;
+    }
+    auto bytes = [](const RadTensor* t) { return t ? (uint8_t*)t->data : nullptr; };
+    P->x = bytes(x);
+    P->res = bytes(rs);
+    P->w_post = bytes(wp);
+    P->gate = bytes(g);
+    P->w_pre = bytes(wn);
+    P->res_out = bytes(ro);
+    P->out = bytes(o);
+    P->q = bytes(q);
+    P->scale = (float*)bytes(sc);
+    P->x_bf16 = x->dtype == RAD_BF16;
+    P->w_bf16 = wt == RAD_BF16;
+    P->out_bf16 = o && o->dtype == RAD_BF16;
+    P->rows = rows;
+    P->n = n;
+    P->eps = rad_args_getf_or(a, "eps", 1e-6);
+    P->wadd = (float)rad_args_getf_or(a, "wadd", 0.0);
+    P->res_scale = (float)rad_args_getf_or(a, "res_scale", 1.0);
+    if (!(P->eps >= 0.0)) return RAD_E_INVAL;
+    if (rows * block_geom(rows, n).lanes > 0xFFFFFFFFLL) return RAD_E_UNSUPPORTED;   /* lanes a launch */
+    return RAD_OK;
+}
+
+BlockGeom block_geom(int64_t rows, int64_t n) {
+    const int64_t nc = (n + 7) / 8;
+    auto lanes = [&](int c) { return (int)(((nc + c - 1) / c + 63) / 64 * 64); };
+    if (nc <= 256 || rows * nc < 400000) {
+        const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : lanes(3) <= 1024 ? 3 : 4;
+        return BlockGeom{lanes(c), c};
+    }
+    int best = 0;
+    for (int c : {3, 2, 4})
+        if (lanes(c) <= 1024 && (!best || lanes(c) * c < lanes(best) * best)) best = c;
+    return BlockGeom{lanes(best), best};
+}
+
+int describe_block(const char* row, const RadArgs* a, char* buf, int len) {
+    if (strcmp(row, "rmsnorm_block")) return -1;
+    BlockPlan P{};
+    const int rc = plan_block(a, &P);
+    if (rc) { snprintf(buf, (size_t)len, "refused rc=%d (plan)", rc); return rc; }
+    static const char* const kGate[] = {"none", "rows", "token"};
+    static const char* const kCodes[] = {"none", "i8", "e4m3"};
+    const BlockGeom g = block_geom(P.rows, P.n);
+    snprintf(buf, (size_t)len, "arm=band op=rmsnorm_block x=%s w=%s rows=%lld n=%lld lanes=%d chunks=%d post=%d "
+             "residual=%d gate=%s pre=%d residual_out=%d out=%s codes=%s", P.x_bf16 ? "bf16" : "f32",
+             P.w_bf16 ? "bf16" : "f32", (long long)P.rows, (long long)P.n, g.lanes, g.chunks, P.w_post != nullptr,
+             P.res != nullptr, kGate[P.gate_kind], P.w_pre != nullptr, P.res_out != nullptr,
+             P.out ? (P.out_bf16 ? "bf16" : "f32") : "none", kCodes[P.codes]);
+    return RAD_OK;
+}
+
+bool env_no_block() { static const bool v = getenv("R3D_NO_BLOCK_NORM") != nullptr; return v; }
+
+}  // namespace r3d

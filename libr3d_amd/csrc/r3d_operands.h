@@ -66,20 +66,25 @@ struct Span {
     int size;                /* bytes an element */
 };
 
-/* Whether an output's memory overlaps an input's other than by being the same elements at the same places
- * (each lane reads its elements before it writes them).  Column ranges of rows a pitch apart do not overlap. */
-inline bool spans_clash(const Span& out, const Span& in) {
-    const uintptr_t a = (uintptr_t)out.data, b = (uintptr_t)in.data;
-    const uintptr_t ae = a + (uintptr_t)(((out.rows - 1) * out.pitch + out.cols) * out.size);
-    const uintptr_t be = b + (uintptr_t)(((in.rows - 1) * in.pitch + in.cols) * in.size);
+/* Whether two operands' rows have an element's memory in common.  Column ranges of rows that lie a common
+ * pitch apart are told from each other; of other pairs it is enough that what they span overlaps. */
+inline bool spans_meet(const Span& u, const Span& v) {
+    const uintptr_t a = (uintptr_t)u.data, b = (uintptr_t)v.data;
+    const uintptr_t ae = a + (uintptr_t)(((u.rows - 1) * u.pitch + u.cols) * u.size);
+    const uintptr_t be = b + (uintptr_t)(((v.rows - 1) * v.pitch + v.cols) * v.size);
     if (ae <= b || be <= a) return false;
-    const bool alike = out.size == in.size && (out.pitch == in.pitch || (out.rows == 1 && in.rows == 1));
-    if (!alike) return true;
-    if (a == b) return out.cols != in.cols;
-    if (out.rows == 1 || out.pitch <= 0) return true;
-    const uintptr_t p = (uintptr_t)out.pitch * (uintptr_t)out.size;
-    const uintptr_t d = b > a ? (b - a) % p : p - (a - b) % p;      /* where in an output's row the input's begin */
-    return d < (uintptr_t)out.cols * (uintptr_t)out.size || d + (uintptr_t)in.cols * (uintptr_t)in.size > p;
+    const uintptr_t p = (uintptr_t)u.pitch * (uintptr_t)u.size;
+    if (u.rows == 1 || v.rows == 1 || !p || p != (uintptr_t)v.pitch * (uintptr_t)v.size) return true;
+    const uintptr_t d = b >= a ? (b - a) % p : (p - (a - b) % p) % p;   /* where in u's row v's begins */
+    return d < (uintptr_t)u.cols * (uintptr_t)u.size || d + (uintptr_t)v.cols * (uintptr_t)v.size > p;
+}
+
+/* Whether an output's memory overlaps an input's other than by being the same elements at the same places,
+ * which is no harm where a lane reads its elements before it writes them. */
+inline bool spans_clash(const Span& out, const Span& in) {
+    const bool same = out.data == in.data && out.size == in.size && out.cols == in.cols &&
+                      (out.pitch == in.pitch || (out.rows == 1 && in.rows == 1));
+    return !same && spans_meet(out, in);
 }
 
 }  // namespace r3d

@@ -7,6 +7,7 @@
 
 #include "rad_planes.h"
 #include "rad_plugin.h"
+#include "r3d_block.h"
 #include "r3d_epi.h"
 #include "r3d_i8.h"
 #include "r3d_sample.h"
@@ -1459,6 +1460,7 @@ int describe(const char* row, const RadArgs* a, char* buf, int len) {
     if (const int rc = describe_i8(row, a, buf, len); rc >= 0) return rc;
     if (const int rc = describe_sample(row, a, buf, len); rc >= 0) return rc;
     if (const int rc = describe_epi(row, a, buf, len); rc >= 0) return rc;
+    if (const int rc = describe_block(row, a, buf, len); rc >= 0) return rc;
     if (strstr(row, "quant_act_fp8") != nullptr) {
         QuantPlan Q{};
         const int rc = plan_quant_act_fp8(a, &Q);

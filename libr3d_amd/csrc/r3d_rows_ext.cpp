@@ -12,14 +12,16 @@
  *   sample_logits            prio 1000  n_vocab GE 1, dtype IN f32 bf16     sampler
  *   gemm_nt_epi_bf16         prio 1000  dtype IN bf16                     product with an epilogue
  *   gemm_nt_epi_i8a8         prio 1000  dtype IN i8a8                     the same over int8 codes
+ *   rmsnorm_block            prio 1000  n GE 1, dtype IN f32 bf16           norms, gate and residual between blocks
  *
  * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row (and turns off its GEMV in the other
- * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler, R3D_NO_EPI gemm_nt_epi's rows (presence-tested,
- * read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler, R3D_NO_EPI gemm_nt_epi's rows, R3D_NO_BLOCK_NORM
+ * rmsnorm_block (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
 #include "rad_abi.h"
+#include "r3d_block.h"
 #include "r3d_epi.h"
 #include "r3d_i8.h"
 #include "r3d_sample.h"
@@ -37,6 +39,7 @@ int r3d_rad_gemm_nt_epi_bf16(const RadArgs* a, RadStream s);
 int64_t r3d_rad_gemm_nt_epi_bf16_scratch(const RadArgs* a);
 int r3d_rad_gemm_nt_epi_i8(const RadArgs* a, RadStream s);
 int64_t r3d_rad_gemm_nt_epi_i8_scratch(const RadArgs* a);
+int r3d_rad_rmsnorm_block(const RadArgs* a, RadStream s);
 }
 
 namespace {
@@ -113,6 +116,27 @@ const RadOperandSpec kEpiOperands[] = {
     {"y", RAD_OPD_OUT, 0},
 };
 
+const RadParamSpec kBlockParams[] = {
+    {"M", RAD_P_INT, RAD_REQUIRED, 0},
+    {"n", RAD_P_INT, RAD_REQUIRED, 0},
+    {"eps", RAD_P_F64, RAD_REQUIRED, 0},
+    {"dtype", RAD_P_STR, RAD_REQUIRED, 0},
+    {"wadd", RAD_P_F64, RAD_OPTIONAL, 0},
+    {"res_scale", RAD_P_F64, RAD_OPTIONAL, 0},
+    {"group", RAD_P_INT, RAD_OPTIONAL, 0},
+};
+const RadOperandSpec kBlockOperands[] = {
+    {"x", RAD_OPD_IN, 0},
+    {"residual", RAD_OPD_IN, 1},
+    {"w_post", RAD_OPD_WEIGHT, 1},
+    {"gate", RAD_OPD_IN, 1},
+    {"w_pre", RAD_OPD_WEIGHT, 1},
+    {"residual_out", RAD_OPD_OUT, 1},
+    {"out", RAD_OPD_OUT, 1},
+    {"q", RAD_OPD_OUT, 1},
+    {"scale", RAD_OPD_OUT, 1},
+};
+
 const RadOpSchema kSchemas[] = {
     {"quant_act_i8", kQuantParams, 3, kQuantOperands, 3,
      "symmetric int8 quantisation of an activation with one f32 scale a row, amax/127."},
@@ -129,6 +153,10 @@ const RadOpSchema kSchemas[] = {
     {"gemm_nt_epi", kEpiParams, 5, kEpiOperands, 7,
      "y = act(S * a . b^T + bias) + residual, rounded once: S = 1 at bf16, a_scale * b_scale at i8a8; act none "
      "(default), relu, silu, sigmoid, gelu or gelu_tanh; y may be the residual's memory."},
+    {"rmsnorm_block", kBlockParams, 7, kBlockOperands, 9,
+     "h = res_scale * residual + gate * norm(x; w_post), to residual_out in bf16, then norm(h; w_pre) of the f32 h: to out, "
+     "and to q as int8 codes with one scale a row or e4m3 codes with one a group of 128; norm is the RMS norm times "
+     "w + wadd, x itself without w_post; gate a value a channel [n], a token [M, 1] or an element [M, n]."},
 };
 
 const RadConstraint cI8[] = {
@@ -218,11 +246,21 @@ const RadKernelInfo kRows[] = {
      "int8 a with f32 a_scale [M] or [M, 1], int8 b with f32 b_scale [N] or [N, 1], f32/bf16 bias, residual and y",
      RAD_DOMAIN_DEVICE, kPrioTile, cI8, 1, nullptr, 0, nullptr, nullptr, nullptr,
      r3d_rad_gemm_nt_epi_i8, r3d_rad_gemm_nt_epi_i8_scratch, nullptr, nullptr, nullptr, nullptr},
+    {"rmsnorm_block", "rmsnorm_block", "quant",
+     "the norm after a block, its gate, the residual's scale and addition, and the norm before the next block with its "
+     "quantiser, in one pass: a workgroup a row, the row in registers, sums of squares in f64",
+     "n up to 32768; any alignment and pitch; residual_out and out may be x's, the residual's or the gate's memory; q with "
+     "scale; w_pre with out or q",
+     "bf16/f32 x, bf16 residual and residual_out, w_post, gate and w_pre of one type (bf16/f32), bf16/f32 out, int8 q with "
+     "f32 scale [M] or [M, 1], e4m3 q with f32 scale [M, ceil(n / 128)]",
+     RAD_DOMAIN_DEVICE, kPrioTile, cBand, 2, nullptr, 0, nullptr, nullptr, nullptr,
+     r3d_rad_rmsnorm_block, nullptr, nullptr, nullptr, nullptr, nullptr},
 };
 
 bool row_hidden(const RadKernelInfo& k) {
     if (!strcmp(k.name, "sample_logits")) return r3d::env_no_sample();
     if (!strcmp(k.op, "gemm_nt_epi")) return r3d::env_no_epi();
+    if (!strcmp(k.name, "rmsnorm_block")) return r3d::env_no_block();
     if (!strcmp(k.name, "gemm_nt_q_i8a8_decode")) return r3d::env_no_i8() || r3d::env_no_i8_dec();
     return r3d::env_no_i8();
 }
