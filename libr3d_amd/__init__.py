@@ -27,6 +27,7 @@ __all__ = [
     "GatedQuantI8Operands", "RmsNormQuantI8Operands", "quant_act_i8", "gated_quant_i8",
     "rmsnorm_quant_i8", "SampleOperands", "sample_logits",
     "GemmEpiOperands", "gemm_nt_epi", "RmsNormBlockOperands", "rmsnorm_block",
+    "MoeLayerOperands", "moe_layer",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -714,6 +715,45 @@ class RmsNormBlockOperands(_Args):
                          ([("group", group)] if group is not None else []) + ([("M", M)] if M is not None else []))
 
 
+class MoeLayerOperands(_Args):
+    """One moe_layer call.
+
+    x        bf16/int16 [M, n], M up to 64;  logits float32 or bf16/int16 [M, E]: the router's
+    gate_up  [E, 2f, n] (f gate rows, then f up rows) and down [E, n, f] by dtype:
+             "bf16"   bf16/int16, no scales
+             "i8"     int8, with gate_up_scale float32 [E, 2f] and down_scale float32 [E, n] ([..., 1] too)
+             "mxfp4"  uint8 [E, rows, K / 2] of packed e2m1 (low nibble = even column), with scales uint8 E8M0
+                      [E, rows, K / 32]
+    y        float32 or bf16/int16 [M, n] out
+    ids, weights   optional int32 and float32 [M, top_k] out: the choice (-1: none) and its weights
+    act      "silu" (default) or another of gemm_nt_epi's;  score "softmax" (default) or "sigmoid";  renorm 1 (default):
+             weights divided by the chosen ones' sum;  weight_scale times each weight
+    The launch needs scratch of row_scratch_bytes("moe_layer", ops) bytes (set_scratch).
+    """
+
+    def __init__(self, x, logits, gate_up, down, y, *, dtype, n, f, E, top_k, gate_up_scale=None, down_scale=None, ids=None,
+                 weights=None, act=None, score=None, renorm=None, weight_scale=None, M=None):
+        def codes(w, default):
+            if w is None or dtype != "mxfp4":
+                return w, _type(w, default), None, None
+            if _type(w, "U8") != "U8":
+                return w, _type(w, default), None, None            # the row refuses it
+            # FP4 counts nibbles
+            return w, "FP4E2M1", list(w.shape[:-1]) + [2 * w.shape[-1]], [2 * v for v in w.stride()[:-1]] + [w.stride()[-1]]
+
+        def scale(s):
+            kind = _type(s, "F32")
+            return s, "E8M0" if dtype == "mxfp4" and kind == "U8" else kind, None, None
+        ops = [(x, _type(x, "BF16"), None, None), (logits, _type(logits, "F32"), None, None), codes(gate_up, "BF16"),
+               scale(gate_up_scale), codes(down, "BF16"), scale(down_scale)]
+        ops += [(t, _type(t, dt), None, None) for t, dt in ((y, "BF16"), (ids, "I32"), (weights, "F32"))]
+        super().__init__(ops, [("n", n), ("f", f), ("E", E), ("top_k", top_k), ("dtype", dtype)] +
+                         ([("act", act)] if act is not None else []) + ([("score", score)] if score is not None else []) +
+                         ([("renorm", int(renorm))] if renorm is not None else []) +
+                         ([("weight_scale", float(weight_scale))] if weight_scale is not None else []) +
+                         ([("M", M)] if M is not None else []))
+
+
 class LogitsOperands(_Args):
     """One logits_gemm call (src/r3d_gemm_logits.hip:144-226).
 
@@ -1008,6 +1048,20 @@ def rmsnorm_block(x, *, n, residual=None, w_post=None, gate=None, w_pre=None, re
     ops = RmsNormBlockOperands(x, n=n, residual=residual, w_post=w_post, gate=gate, w_pre=w_pre, residual_out=residual_out,
                                out=out, q=q, scale=scale, eps=eps, wadd=wadd, res_scale=res_scale, group=group)
     return _launch_on("rmsnorm_block", ops, stream, device)
+
+
+def moe_layer(x, logits, gate_up, down, y, *, dtype, n, f, E, top_k, gate_up_scale=None, down_scale=None, ids=None,
+              weights=None, act=None, score=None, renorm=None, weight_scale=None, stream=None):
+    """Launch the moe_layer row on `stream` (a raw hipStream_t int, default the current torch stream), with launch
+    scratch of the size its hook asks for; its status."""
+    device = _one_gpu(x, logits, gate_up, down, y, gate_up_scale, down_scale, ids, weights)
+    ops = MoeLayerOperands(x, logits, gate_up, down, y, dtype=dtype, n=n, f=f, E=E, top_k=top_k,
+                           gate_up_scale=gate_up_scale, down_scale=down_scale, ids=ids, weights=weights, act=act,
+                           score=score, renorm=renorm, weight_scale=weight_scale)
+    need = row_scratch_bytes("moe_layer", ops)
+    if need > 0:
+        ops.set_scratch(_scratch(need, device, stream), need)
+    return _launch_on("moe_layer", ops, stream, device)
 
 
 def row_launcher(row_name):

@@ -27,7 +27,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 SOURCES = ["r3d_gemm.hip", "r3d_logits.hip", "r3d_noalloc.hip", "r3d_plan.cpp", "r3d_rows.cpp",
            "r3d_dump.cpp", "r3d_head.cpp", "r3d_probe.hip", "r3d_i8.hip", "r3d_i8_plan.cpp",
            "r3d_rows_ext.cpp", "r3d_sample.hip", "r3d_sample_plan.cpp", "r3d_epi.hip", "r3d_epi_plan.cpp",
-           "r3d_block.hip", "r3d_block_plan.cpp"]
+           "r3d_block.hip", "r3d_block_plan.cpp", "r3d_moe.hip", "r3d_moe_plan.cpp"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",

@@ -1,0 +1,73 @@
+/* r3d_moe.h -- host-side plan of moe_layer: a mixture-of-experts layer for a few tokens, in two kernels.
+ *     choice   the top_k largest router logits of a token, by falling logit, ties to the lower index
+ *     weights  softmax over the logits, or a sigmoid of each; of the chosen ones' sum where renorm; times weight_scale
+ *     h        weight * act(W_gate x) * (W_up x)          the chosen expert's f rows each
+ *     y        the chosen experts' W_down h, added up
+ * Expert planes in bf16, in int8 with one f32 scale a row, or in e2m1 with one E8M0 scale a row and 32 columns.
+ * Pure host C++. */
+#ifndef R3D_MOE_H
+#define R3D_MOE_H
+
+#include <stdint.h>
+#include "rad_abi.h"
+
+namespace r3d {
+
+enum { MOE_BF16 = 0, MOE_I8, MOE_FP4 };
+
+constexpr int kMoeMaxM = 64;            /* an expert's tokens are a 64-bit mask */
+constexpr int kMoeMaxE = 512;           /* a lane of the first kernel's workgroups an expert */
+constexpr int kMoeMaxK = 16;            /* choices a token */
+constexpr int64_t kMoeMaxN = 1 << 19;   /* n and f: h of all pairs stays under 2^30 bytes */
+constexpr int kMoeMaxPairs = kMoeMaxM * kMoeMaxK;
+
+/* What the first kernel leaves for the second at the head of the scratch; h follows. */
+struct MoeTable {
+    int32_t jobs;                       /* groups of an expert's tokens, in the experts' order */
+    int32_t pad[3];
+    uint32_t job[kMoeMaxPairs];         /* expert | first slot << 9 | tokens << 20 */
+    uint8_t tok[kMoeMaxPairs];          /* a slot's token */
+};
+
+struct MoePlan {
+    const uint8_t* x;                   /* bf16 [M, n] */
+    const uint8_t* logits;              /* f32 or bf16 [M, E] */
+    const uint8_t* gu;                  /* [E, 2f, n]: gate rows, then up rows */
+    const uint8_t* gus;
+    const uint8_t* dn;                  /* [E, n, f] */
+    const uint8_t* dns;
+    uint8_t* y;                         /* bf16 or f32 [M, n] */
+    int32_t* ids;                       /* [M, top_k], or null */
+    float* weights;                     /* [M, top_k], or null */
+    int64_t M, n, f, E, top_k;
+    /* bytes, or scales' elements */
+    int64_t x_pitch, l_pitch, y_pitch, gu_expert, gu_pitch, dn_expert, dn_pitch;
+    int64_t gus_expert, gus_pitch, dns_expert, dns_pitch, i_pitch, w_pitch;
+    int enc, l_bf16, y_bf16, act, sigmoid, renorm;
+    float weight_scale;
+};
+
+int plan_moe(const RadArgs* a, MoePlan* P);
+
+/* Launch shapes of the two kernels on ncu compute units. */
+struct MoeGeom {
+    int ct;                             /* 8 ct tokens of an expert a job */
+    int kc;                             /* up: waves that share a block of 8 rows, K cut between them */
+    int64_t up_blocks;
+    int rt;                             /* down: 8 rt rows of y a workgroup */
+    int64_t down_blocks;
+};
+void moe_geom(const MoePlan& P, int ncu, MoeGeom* g);
+
+/* Bytes of scratch that a call needs (the row's hook; 0 where the sizes are not given). */
+int64_t moe_scratch_bytes(const RadArgs* a);
+int64_t moe_scratch(const MoePlan& P);
+
+/* describe() for this row; -1 when `row` is another. */
+int describe_moe(const char* row, const RadArgs* a, char* buf, int len);
+
+bool env_no_moe();
+
+}  // namespace r3d
+
+#endif /* R3D_MOE_H */

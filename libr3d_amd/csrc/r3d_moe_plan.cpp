@@ -1,0 +1,212 @@
+/* r3d_moe_plan.cpp -- host plan of moe_layer (see r3d_moe.h). */
+#include "r3d_moe.h"
+
+#include <math.h>
+#include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
+
+#include "rad_plugin.h"
+#include "r3d_act.h"
+#include "r3d_operands.h"
+
+namespace r3d {
+
+/* The strides of an [E, rows, cols] operand, its last axis dense. */
+static int planes_of(const RadTensor* t, int64_t E, int64_t rows, int64_t cols, int64_t* expert, int64_t* pitch) {
+    if (t->rank != 3 || t->shape[0] != E || t->shape[1] != rows || t->shape[2] != cols) return RAD_E_SHAPE;
+    if (t->stride[2] != 1) return RAD_E_STRIDE;
+    *expert = t->stride[0];
+    *pitch = t->stride[1];
+    return pitch_ok(*expert) && pitch_ok(*pitch) ? RAD_OK : RAD_E_STRIDE;
+}
+
+/* A plane of codes and its scales. */
+struct Experts {
+    const RadTensor* w;
+    const RadTensor* s;
+    int64_t expert, pitch, s_expert, s_pitch;
+};
+
+static int plan_experts(int enc, int64_t E, int64_t rows, int64_t cols, Experts* X) {
+    static const uint32_t kType[] = {RAD_BF16, RAD_I8, RAD_FP4E2M1};
+    if (X->w->dtype != kType[enc]) return RAD_E_DTYPE;
+    if ((enc == MOE_BF16) != (X->s == nullptr)) return RAD_E_INVAL;
+    if (X->s && X->s->dtype != (enc == MOE_I8 ? RAD_F32 : RAD_E8M0)) return RAD_E_DTYPE;
+    int rc = planes_of(X->w, E, rows, cols, &X->expert, &X->pitch);
+    if (rc) return rc;
+    if (enc == MOE_FP4 && ((X->expert | X->pitch) & 1)) return RAD_E_STRIDE;      /* nibbles: whole bytes */
+    X->expert = enc == MOE_BF16 ? 2 * X->expert : enc == MOE_FP4 ? X->expert / 2 : X->expert;
+    X->pitch = enc == MOE_BF16 ? 2 * X->pitch : enc == MOE_FP4 ? X->pitch / 2 : X->pitch;
+    const int64_t row = enc == MOE_BF16 ? 2 * cols : enc == MOE_FP4 ? cols / 2 : cols;
+    /* 16 bytes a lane: whole pieces on their own alignment, an expert's plane under 32-bit offsets */
+    if ((row | X->expert | X->pitch) & 15 || (uintptr_t)X->w->data & 15) return RAD_E_UNSUPPORTED;
+    if (X->pitch > (int64_t(1) << 31) / rows || (rows - 1) * X->pitch + row > 0x7FFFFFFF) return RAD_E_UNSUPPORTED;
+    if (enc == MOE_I8) {
+        if (X->s->rank == 3) {                                       /* [E, rows, 1] */
+            if (X->s->shape[0] != E || X->s->shape[1] != rows || X->s->shape[2] != 1) return RAD_E_SHAPE;
+        } else if (X->s->rank != 2 || X->s->shape[0] != E || X->s->shape[1] != rows) {
+            return RAD_E_SHAPE;
+        }
+        if (X->s->stride[1] != 1) return RAD_E_STRIDE;
+        X->s_expert = X->s->stride[0];
+        if (!pitch_ok(X->s_expert)) return RAD_E_STRIDE;
+    } else if (enc == MOE_FP4) {
+        if ((rc = planes_of(X->s, E, rows, cols / 32, &X->s_expert, &X->s_pitch))) return rc;
+        if (X->s_pitch > (int64_t(1) << 31) / rows) return RAD_E_UNSUPPORTED;
+    }
+    return RAD_OK;
+}
+
+int plan_moe(const RadArgs* a, MoePlan* P) {
+    const RadTensor* x  = rad_arg_in(a, 0);
+    const RadTensor* lg = rad_arg_in(a, 1);
+    const RadTensor* y  = rad_arg_in(a, 6);
+    const RadTensor* id = rad_arg_in(a, 7);
+    const RadTensor* wt = rad_arg_in(a, 8);
+    Experts up{rad_arg_in(a, 2), rad_arg_in(a, 3), 0, 0, 0, 0}, down{rad_arg_in(a, 4), rad_arg_in(a, 5), 0, 0, 0, 0};
+    if (!x || !lg || !up.w || !down.w || !y) return RAD_E_INVAL;
+    const char* dt = rad_args_gets(a, "dtype");
+    P->enc = !dt ? -1 : !strcmp(dt, "bf16") ? MOE_BF16 : !strcmp(dt, "i8") ? MOE_I8 : !strcmp(dt, "mxfp4") ? MOE_FP4 : -1;
+    if (P->enc < 0) return RAD_E_UNSUPPORTED;
+    if (x->dtype != RAD_BF16 || (lg->dtype != RAD_F32 && lg->dtype != RAD_BF16) ||
+        (y->dtype != RAD_F32 && y->dtype != RAD_BF16) || (id && id->dtype != RAD_I32) || (wt && wt->dtype != RAD_F32))
+        return RAD_E_DTYPE;
+    const char* act = rad_args_gets(a, "act");
+    P->act = act ? act_by_name(act) : ACT_SILU;
+    const char* score = rad_args_gets(a, "score");
+    P->sigmoid = score && !strcmp(score, "sigmoid");
+    if (P->act < 0 || (score && !P->sigmoid && strcmp(score, "softmax"))) return RAD_E_UNSUPPORTED;
+    long long n = 0, f = 0, E = 0, k = 0, v = 0;
+    if (!rad_args_geti(a, "n", &n) || !rad_args_geti(a, "f", &f) || !rad_args_geti(a, "E", &E) ||
+        !rad_args_geti(a, "top_k", &k) || n <= 0 || f <= 0 || E <= 0 || k <= 0 || n > kDimMax || f > kDimMax || k > E)
+        return RAD_E_SHAPE;
+    if (E > kMoeMaxE || k > kMoeMaxK || n > kMoeMaxN || f > kMoeMaxN) return RAD_E_UNSUPPORTED;
+    /* whole 16-byte pieces of codes (plan_experts), and 8 rows of an expert a wave */
+    if ((n | f) & (P->enc == MOE_FP4 ? 31 : P->enc == MOE_I8 ? 15 : 7)) return RAD_E_UNSUPPORTED;
+    const long long yn = rad_tensor_numel(y);
+    if (yn <= 0 || yn % n) return RAD_E_SHAPE;
+    const int64_t M = yn / n;
+    if (M > kMoeMaxM) return RAD_E_UNSUPPORTED;
+    int rc = rows_of(x, M, n, &P->x_pitch);
+    if (!rc) rc = rows_of(lg, M, E, &P->l_pitch);
+    if (!rc) rc = rows_of(y, M, n, &P->y_pitch);
+    if (!rc && id) rc = rows_of(id, M, k, &P->i_pitch);
+    if (!rc && wt) rc = rows_of(wt, M, k, &P->w_pitch);
+    if (!rc) rc = plan_experts(P->enc, E, 2 * f, n, &up);
+    if (!rc) rc = plan_experts(P->enc, E, n, f, &down);
+    if (rc) return rc;
+    if (M > 1 && (P->y_pitch < n || (id && P->i_pitch < k) || (wt && P->w_pitch < k))) return RAD_E_STRIDE;
+    for (const RadTensor* t : {x, lg, up.s, down.s, y, id, wt})
+        if (misaligned(t)) return RAD_E_STRIDE;
+    P->x_pitch *= 2;
+    if ((uintptr_t)x->data & 15 || (M > 1 && (P->x_pitch & 15 || P->x_pitch > (1 << 24)))) return RAD_E_UNSUPPORTED;
+    if (M == 1) P->x_pitch = 2 * n;                             /* a single row has no next one */
+    /* y is written when x and the logits are read, but by other workgroups than read them */
+    const Span outs[3] = {{y->data, M, n, P->y_pitch, elt_bytes(y->dtype)},
+                          {id ? id->data : nullptr, M, k, P->i_pitch, 4}, {wt ? wt->data : nullptr, M, k, P->w_pitch, 4}};
+    const Span ins[2] = {{x->data, M, n, P->x_pitch / 2, 2}, {lg->data, M, E, P->l_pitch, elt_bytes(lg->dtype)}};
+    for (int i = 0; i < 3; ++i) {
+        if (!outs[i].data) continue;
+        for (int j = 0; j < i; ++j)
+            if (outs[j].data && spans_meet(outs[i], outs[j])) return RAD_E_INVAL;
+        if (i == 0) continue;                                   /* the second kernel reads neither x nor logits */
+        for (const Span& in : ins)
+            if (spans_meet(outs[i], in)) return RAD_E_INVAL;
+    }
+    P->x = (const uint8_t*)x->data;
+    P->logits = (const uint8_t*)lg->data;
+    P->l_bf16 = lg->dtype == RAD_BF16;
+    P->gu = (const uint8_t*)up.w->data;
+    P->gus = up.s ? (const uint8_t*)up.s->data : nullptr;
+    P->dn = (const uint8_t*)down.w->data;
+    P->dns = down.s ? (const uint8_t*)down.s->data : nullptr;
+    P->gu_expert = up.expert;
+    P->gu_pitch = up.pitch;
+    P->gus_expert = up.s_expert;
+    P->gus_pitch = up.s_pitch;
+    P->dn_expert = down.expert;
+    P->dn_pitch = down.pitch;
+    P->dns_expert = down.s_expert;
+    P->dns_pitch = down.s_pitch;
+    P->y = (uint8_t*)y->data;
+    P->y_bf16 = y->dtype == RAD_BF16;
+    P->ids = id ? (int32_t*)id->data : nullptr;
+    P->weights = wt ? (float*)wt->data : nullptr;
+    P->M = M;
+    P->n = n;
+    P->f = f;
+    P->E = E;
+    P->top_k = k;
+    P->renorm = !rad_args_geti(a, "renorm", &v) || v != 0;
+    P->weight_scale = (float)rad_args_getf_or(a, "weight_scale", 1.0);
+    return RAD_OK;
+}
+
+/* Experts that someone chose, were the choices spread evenly. */
+static double moe_read(const MoePlan& P) {
+    return (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
+}
+
+void moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
+    if (ncu <= 0) ncu = 256;
+    const int64_t pairs = P.M * P.top_k, most = P.E < pairs ? P.E : pairs;
+    const double read = moe_read(P), each = (double)pairs / read;
+    g->ct = P.M <= 8 || each <= 6 ? 1 : each <= 12 ? 2 : 4;
+    const int64_t jobs = most + (pairs - most) / (8 * g->ct);   /* at most */
+    const int64_t fb = P.f / 8;
+    const double width = P.enc == MOE_BF16 ? 64 : P.enc == MOE_I8 ? 128 : 256;
+    const double lines = ceil((double)P.n / width);
+    /* waves that stream: enough of them, two lines each at least */
+    g->kc = 1;
+    while (g->kc < 8 && read * fb * g->kc < 16 * ncu && lines / (2 * g->kc) >= 2) g->kc *= 2;
+    const int64_t units = jobs * fb, wg = (units + 8 / g->kc - 1) / (8 / g->kc);
+    g->up_blocks = wg < 4 * ncu ? wg : 4 * ncu;
+    g->rt = 1;
+    g->down_blocks = (P.n / 8 + g->rt - 1) / g->rt;
+}
+
+int64_t moe_scratch(const MoePlan& P) {
+    return (int64_t)sizeof(MoeTable) + P.M * P.top_k * P.f * 2 * (P.y_bf16 ? 1 : 2);
+}
+
+int64_t moe_scratch_bytes(const RadArgs* a) {
+    MoePlan P{};
+    if (plan_moe(a, &P) == RAD_OK) return moe_scratch(P);
+    long long n = 0, f = 0, k = 0, M = 0;                       /* not a whole call yet: y in f32 */
+    if (!rad_args_geti(a, "n", &n) || !rad_args_geti(a, "f", &f) || !rad_args_geti(a, "top_k", &k) || n <= 0 || f <= 0 ||
+        k <= 0 || n > kMoeMaxN || f > kMoeMaxN || k > kMoeMaxK)
+        return 0;
+    const RadTensor* y = rad_arg_in(a, 6);
+    if (y) M = rad_tensor_numel(y) / n;
+    else if (!rad_args_geti(a, "M", &M)) M = kMoeMaxM;
+    if (M <= 0 || M > kMoeMaxM) return 0;
+    P.M = M;
+    P.f = f;
+    P.top_k = k;
+    P.y_bf16 = 0;
+    return moe_scratch(P);
+}
+
+int describe_moe(const char* row, const RadArgs* a, char* buf, int len) {
+    if (strcmp(row, "moe_layer")) return -1;
+    MoePlan P{};
+    const int rc = plan_moe(a, &P);
+    if (rc) { snprintf(buf, (size_t)len, "refused rc=%d (plan)", rc); return rc; }
+    if (!a->scratch || (uintptr_t)a->scratch & 15 || a->scratch_bytes < moe_scratch(P)) {
+        snprintf(buf, (size_t)len, "refused rc=%d (scratch)", RAD_E_UNSUPPORTED);
+        return RAD_E_UNSUPPORTED;
+    }
+    static const char* const kEnc[] = {"bf16", "i8", "mxfp4"};
+    MoeGeom g;
+    moe_geom(P, 256, &g);
+    snprintf(buf, (size_t)len, "arm=moe enc=%s M=%lld n=%lld f=%lld E=%lld top_k=%lld score=%s renorm=%d act=%d y=%s ct=%d "
+             "kc=%d up_blocks=%lld rt=%d down_blocks=%lld", kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
+             (long long)P.E, (long long)P.top_k, P.sigmoid ? "sigmoid" : "softmax", P.renorm, P.act,
+             P.y_bf16 ? "bf16" : "f32", g.ct, g.kc, (long long)g.up_blocks, g.rt, (long long)g.down_blocks);
+    return RAD_OK;
+}
+
+bool env_no_moe() { static const bool v = getenv("R3D_NO_MOE") != nullptr; return v; }
+
+}  // namespace r3d

@@ -10,6 +10,7 @@
 #include "r3d_block.h"
 #include "r3d_epi.h"
 #include "r3d_i8.h"
+#include "r3d_moe.h"
 #include "r3d_sample.h"
 #include "r3d_gemv_layout.h"
 #include "r3d_prefill_layout.h"
@@ -1461,6 +1462,7 @@ int describe(const char* row, const RadArgs* a, char* buf, int len) {
     if (const int rc = describe_sample(row, a, buf, len); rc >= 0) return rc;
     if (const int rc = describe_epi(row, a, buf, len); rc >= 0) return rc;
     if (const int rc = describe_block(row, a, buf, len); rc >= 0) return rc;
+    if (const int rc = describe_moe(row, a, buf, len); rc >= 0) return rc;
     if (strstr(row, "quant_act_fp8") != nullptr) {
         QuantPlan Q{};
         const int rc = plan_quant_act_fp8(a, &Q);

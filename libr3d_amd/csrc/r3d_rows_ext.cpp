@@ -12,11 +12,12 @@
  *   sample_logits            prio 1000  n_vocab GE 1, dtype IN f32 bf16     sampler
  *   gemm_nt_epi_bf16         prio 1000  dtype IN bf16                     product with an epilogue
  *   gemm_nt_epi_i8a8         prio 1000  dtype IN i8a8                     the same over int8 codes
+ *   moe_layer                prio 1000  dtype IN bf16 i8 mxfp4, M LE 64     mixture-of-experts layer
  *   rmsnorm_block            prio 1000  n GE 1, dtype IN f32 bf16           norms, gate and residual between blocks
  *
  * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row (and turns off its GEMV in the other
  * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler, R3D_NO_EPI gemm_nt_epi's rows, R3D_NO_BLOCK_NORM
- * rmsnorm_block (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * rmsnorm_block, R3D_NO_MOE moe_layer (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
@@ -24,6 +25,7 @@
 #include "r3d_block.h"
 #include "r3d_epi.h"
 #include "r3d_i8.h"
+#include "r3d_moe.h"
 #include "r3d_sample.h"
 
 extern "C" {
@@ -40,6 +42,8 @@ int64_t r3d_rad_gemm_nt_epi_bf16_scratch(const RadArgs* a);
 int r3d_rad_gemm_nt_epi_i8(const RadArgs* a, RadStream s);
 int64_t r3d_rad_gemm_nt_epi_i8_scratch(const RadArgs* a);
 int r3d_rad_rmsnorm_block(const RadArgs* a, RadStream s);
+int r3d_rad_moe_layer(const RadArgs* a, RadStream s);
+int64_t r3d_rad_moe_layer_scratch(const RadArgs* a);
 }
 
 namespace {
@@ -137,6 +141,30 @@ const RadOperandSpec kBlockOperands[] = {
     {"scale", RAD_OPD_OUT, 1},
 };
 
+const RadParamSpec kMoeParams[] = {
+    {"M", RAD_P_INT, RAD_REQUIRED, 0},
+    {"n", RAD_P_INT, RAD_REQUIRED, 0},
+    {"f", RAD_P_INT, RAD_REQUIRED, 0},
+    {"E", RAD_P_INT, RAD_REQUIRED, 0},
+    {"top_k", RAD_P_INT, RAD_REQUIRED, 0},
+    {"dtype", RAD_P_STR, RAD_REQUIRED, 0},
+    {"act", RAD_P_STR, RAD_OPTIONAL, 0},
+    {"score", RAD_P_STR, RAD_OPTIONAL, 0},
+    {"renorm", RAD_P_INT, RAD_OPTIONAL, 0},
+    {"weight_scale", RAD_P_F64, RAD_OPTIONAL, 0},
+};
+const RadOperandSpec kMoeOperands[] = {
+    {"x", RAD_OPD_IN, 0},
+    {"logits", RAD_OPD_IN, 0},
+    {"gate_up", RAD_OPD_WEIGHT, 0},
+    {"gate_up_scale", RAD_OPD_WEIGHT, 1},
+    {"down", RAD_OPD_WEIGHT, 0},
+    {"down_scale", RAD_OPD_WEIGHT, 1},
+    {"y", RAD_OPD_OUT, 0},
+    {"ids", RAD_OPD_OUT, 1},
+    {"weights", RAD_OPD_OUT, 1},
+};
+
 const RadOpSchema kSchemas[] = {
     {"quant_act_i8", kQuantParams, 3, kQuantOperands, 3,
      "symmetric int8 quantisation of an activation with one f32 scale a row, amax/127."},
@@ -157,6 +185,10 @@ const RadOpSchema kSchemas[] = {
      "h = res_scale * residual + gate * norm(x; w_post), to residual_out in bf16, then norm(h; w_pre) of the f32 h: to out, "
      "and to q as int8 codes with one scale a row or e4m3 codes with one a group of 128; norm is the RMS norm times "
      "w + wadd, x itself without w_post; gate a value a channel [n], a token [M, 1] or an element [M, n]."},
+    {"moe_layer", kMoeParams, 10, kMoeOperands, 9,
+     "each token's top_k experts by falling router logit (ties to the lower index; NaN and -inf are not there), weights by "
+     "softmax over the logits (default) or sigmoid, of the chosen ones' sum unless renorm is 0, times weight_scale; y = the "
+     "sum of weight * down(act(gate x) * up x) in f32; ids (-1: none) and weights as chosen."},
 };
 
 const RadConstraint cI8[] = {
@@ -179,6 +211,10 @@ const RadConstraint cNorm[] = {
     {"dtype", RAD_C_IN, 0, "bf16"},
 };
 
+const RadConstraint cMoe[] = {
+    {"dtype", RAD_C_IN, 0, "bf16 i8 mxfp4"},
+    {"M", RAD_C_LE, 64, nullptr},
+};
 const RadConstraint cEpiBf16[] = {
     {"dtype", RAD_C_IN, 0, "bf16"},
 };
@@ -255,12 +291,22 @@ const RadKernelInfo kRows[] = {
      "f32 scale [M] or [M, 1], e4m3 q with f32 scale [M, ceil(n / 128)]",
      RAD_DOMAIN_DEVICE, kPrioTile, cBand, 2, nullptr, 0, nullptr, nullptr, nullptr,
      r3d_rad_rmsnorm_block, nullptr, nullptr, nullptr, nullptr, nullptr},
+    {"moe_layer", "moe_layer", "gemm",
+     "a mixture-of-experts layer for up to 64 tokens in two kernels: choice and gate/up products with their activation, then "
+     "down products and the weighted sum; the chosen experts' planes are streamed once, codes become bf16 in registers",
+     "E up to 512, top_k up to 16, n and f multiples of 8 (bf16), 16 (i8) or 32 (mxfp4); x and the code planes on 16 "
+     "bytes; launch scratch of the size the hook asks for (16-byte aligned) required",
+     "bf16 x, f32/bf16 logits [M, E], gate_up [E, 2f, n] (gate rows, then up) and down [E, n, f] in bf16, in int8 with f32 "
+     "scales [E, rows], or in e2m1 with E8M0 scales [E, rows, K / 32]; f32/bf16 y, i32 ids and f32 weights [M, top_k]",
+     RAD_DOMAIN_DEVICE, kPrioTile, cMoe, 2, nullptr, 0, nullptr, nullptr, nullptr,
+     r3d_rad_moe_layer, r3d_rad_moe_layer_scratch, nullptr, nullptr, nullptr, nullptr},
 };
 
 bool row_hidden(const RadKernelInfo& k) {
     if (!strcmp(k.name, "sample_logits")) return r3d::env_no_sample();
     if (!strcmp(k.op, "gemm_nt_epi")) return r3d::env_no_epi();
     if (!strcmp(k.name, "rmsnorm_block")) return r3d::env_no_block();
+    if (!strcmp(k.name, "moe_layer")) return r3d::env_no_moe();
     if (!strcmp(k.name, "gemm_nt_q_i8a8_decode")) return r3d::env_no_i8() || r3d::env_no_i8_dec();
     return r3d::env_no_i8();
 }
