@@ -1,4 +1,4 @@
-/* r3d_moe.h -- host-side plan of moe_layer: a mixture-of-experts layer for a few tokens, in two kernels.
+/* r3d_moe.h -- host-side plan of moe_layer: a mixture-of-experts layer for a few tokens, in three kernels.
  *     choice   the top_k largest router logits of a token, by falling logit, ties to the lower index
  *     weights  softmax over the logits, or a sigmoid of each; of the chosen ones' sum where renorm; times weight_scale
  *     h        weight * act(W_gate x) * (W_up x)          the chosen expert's f rows each
@@ -16,17 +16,18 @@ namespace r3d {
 enum { MOE_BF16 = 0, MOE_I8, MOE_FP4 };
 
 constexpr int kMoeMaxM = 64;            /* an expert's tokens are a 64-bit mask */
-constexpr int kMoeMaxE = 512;           /* a lane of the first kernel's workgroups an expert */
+constexpr int kMoeMaxE = 512;           /* a lane of a workgroup an expert */
 constexpr int kMoeMaxK = 16;            /* choices a token */
 constexpr int64_t kMoeMaxN = 1 << 19;   /* n and f: h of all pairs stays under 2^30 bytes */
 constexpr int kMoeMaxPairs = kMoeMaxM * kMoeMaxK;
 
-/* What the first kernel leaves for the second at the head of the scratch; h follows. */
+/* What the first kernel leaves for the others at the head of the scratch; h and the slots' sums follow.  A slot is a
+ * chosen (token, expert), in the experts' order. */
 struct MoeTable {
     int32_t jobs;                       /* groups of an expert's tokens, in the experts' order */
     int32_t pad[3];
     uint32_t job[kMoeMaxPairs];         /* expert | first slot << 9 | tokens << 20 */
-    uint8_t tok[kMoeMaxPairs];          /* a slot's token */
+    int16_t slot[kMoeMaxPairs];         /* by (token, choice); -1: none */
 };
 
 struct MoePlan {
@@ -49,19 +50,18 @@ struct MoePlan {
 
 int plan_moe(const RadArgs* a, MoePlan* P);
 
-/* Launch shapes of the two kernels on ncu compute units. */
+/* The launch on ncu compute units: tokens a job (in 8 ct columns), rows of them that LDS holds in each kernel. */
 struct MoeGeom {
-    int ct;                             /* 8 ct tokens of an expert a job */
-    int kc;                             /* up: waves that share a block of 8 rows, K cut between them */
-    int64_t up_blocks;
-    int rt;                             /* down: 8 rt rows of y a workgroup */
-    int64_t down_blocks;
+    int ct, width, up_rows, down_rows;
+    int64_t blocks;
 };
-void moe_geom(const MoePlan& P, int ncu, MoeGeom* g);
+/* false: LDS does not hold a single row */
+bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g);
 
 /* Bytes of scratch that a call needs (the row's hook; 0 where the sizes are not given). */
 int64_t moe_scratch_bytes(const RadArgs* a);
 int64_t moe_scratch(const MoePlan& P);
+int64_t moe_h_bytes(const MoePlan& P);
 
 /* describe() for this row; -1 when `row` is another. */
 int describe_moe(const char* row, const RadArgs* a, char* buf, int len);

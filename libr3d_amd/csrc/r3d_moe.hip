@@ -8,18 +8,24 @@
  * bf16's range infinite), so the sums are f32 sums of exact products.
  *
  *   up    every workgroup makes the same choice from the logits for itself (a few hundred cycles a token and wave,
- *         which costs less than a kernel of its own before this one), so that it knows the jobs: an expert and up
- *         to 8 CT of its tokens.  Units of (job, 8 of f) go round the workgroups; a unit's gate and up rows are KC
- *         waves', K cut between them.  h leaves with its weight, to slot (job's first + token).
- *   down  a workgroup owns 8 RT rows of y, its waves the jobs' lines in equal runs; a wave adds each job's rows to
- *         its own sums in LDS by token, and the waves' sums are added in their order.  Nothing is added in an order
- *         that changes from run to run.
+ *         which costs less than a kernel of its own before this one), so that it knows the jobs: an expert and some
+ *         of its tokens.  A unit is a job's 8 gate and 8 up rows of f; h leaves with its weight, to its token's slot.
+ *   down  a unit is a job's 16 rows of n; its sums leave to its tokens' slots in f32.
+ *   sum   y of each token's slots, in the order of its choice: nothing is added in an order that changes from run to run.
  *
- * h is bf16 where y is: its rounding (2^-9 of each of f terms at most, of random sign) is under y's own.  Where y is f32 it
- * is two bf16 numbers, high and low, 2^-17 together. */
+ * up and down are one kernel: the units lie in a row, and each workgroup, one a compute unit, takes an equal run of
+ * them; of a run's lines each of its 16 waves takes an equal run again, and what it leaves of a unit to the next wave
+ * meets through LDS.  The tokens' rows of a run's jobs are in LDS, where the waves read them beside their weights'
+ * loads, and the line's loads are the only ones in the stream: with the tokens read from memory too, the
+ * address unit was busy 9 cycles of 10 at 2.5 TB/s (64 tokens, 128 e2m1 experts).
+ *
+ * h is kept as the sum of two bf16 numbers where y is bf16 and of three where it is f32 (2^-16 and 2^-24 of it at most), so
+ * that of the roundings on the way y's own counts: the products of the parts cost matrix cycles, which idle here. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
+
+#include <type_traits>
 
 #include "r3d_act_dev.h"
 #include "r3d_device.h"
@@ -30,29 +36,21 @@
 
 namespace r3d {
 
-struct MoeUpArgs {
-    const uint8_t* x;
-    const uint8_t* logits;
+struct MoeArgs {
+    const uint8_t* x;                   /* up: the tokens; down: h */
     const uint8_t* w;
     const uint8_t* ws;
     MoeTable* table;
-    uint16_t* h;
-    uint16_t* h_lo;                     /* null: h is bf16 alone */
+    void* out;                          /* up: h, bf16 [parts][pairs][f]; down: sums, f32 [pairs][n] */
+    int M, K, rows, pairs, x_pitch, w_pitch, job_rows;   /* K columns of `rows` rows (gate rows, or rows of y) */
+    int64_t w_expert, ws_expert, ws_pitch;
+    /* up */
+    const uint8_t* logits;
     int32_t* ids;
     float* weights;
-    int M, n, f, E, top_k, x_pitch, w_pitch, kc, act, sigmoid, renorm, l_bf16;
-    int64_t w_expert, ws_expert, ws_pitch, l_pitch, i_pitch, wt_pitch;
+    int64_t l_pitch, i_pitch, wt_pitch;
+    int E, top_k, width, parts, act, sigmoid, renorm, l_bf16;
     float weight_scale;
-};
-struct MoeDownArgs {
-    const uint8_t* h;
-    const uint8_t* h_lo;
-    const uint8_t* w;
-    const uint8_t* ws;
-    const MoeTable* table;
-    uint8_t* y;
-    int M, n, f, pairs, w_pitch, y_bf16;
-    int64_t w_expert, ws_expert, ws_pitch, y_pitch;
 };
 
 /* 16 bytes of codes: how many weights, and 16-byte pieces of bf16 that these become */
@@ -91,7 +89,8 @@ __device__ __forceinline__ void moe_bf16(r3d_i32x4 w, uint32_t scale, r3d_i32x4 
 
 /* ------------------------------------------------------------------------------ the choice */
 
-constexpr int kMoeThreads = 512, kMoeWaves = 8;
+constexpr int kMoeWaves = 16, kMoeThreads = 64 * kMoeWaves;
+constexpr int kMoeUnits = 128;          /* units whose scales lie in LDS at a time */
 
 struct MoeChoice {                      /* in LDS, the same in every workgroup */
     uint64_t mask[kMoeMaxE];            /* an expert's tokens */
@@ -109,7 +108,7 @@ struct MoeChoice {                      /* in LDS, the same in every workgroup *
  * numbers in the same order, 0 for what is not there (NaN, -inf); each round takes the wave's largest, of equals the
  * first lane's first. */
 template <int J>
-__device__ __forceinline__ void moe_choose(const MoeUpArgs& P, MoeChoice& S, int t) {
+__device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t) {
     const int lane = threadIdx.x & 63;
     float v[J];
     uint32_t key[J];
@@ -176,11 +175,10 @@ __device__ __forceinline__ void moe_choose(const MoeUpArgs& P, MoeChoice& S, int
     }
 }
 
-/* Choices of every token, then the experts' slots and jobs.  All lanes of the workgroup. */
-template <int CT>
-__device__ __forceinline__ void moe_plan(const MoeUpArgs& P, MoeChoice& S) {
+/* Choices of every token, then the experts' slots and jobs, `width` tokens each.  All lanes of the workgroup. */
+__device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    S.mask[tid] = 0;
+    if (tid < kMoeMaxE) S.mask[tid] = 0;
     for (int t = wave; t < P.M; t += kMoeWaves) {
         if (P.E <= 64) moe_choose<1>(P, S, t);
         else if (P.E <= 128) moe_choose<2>(P, S, t);
@@ -188,75 +186,51 @@ __device__ __forceinline__ void moe_plan(const MoeUpArgs& P, MoeChoice& S) {
         else moe_choose<8>(P, S, t);
     }
     __syncthreads();
-    const int pairs = P.M * P.top_k;
-    for (int i = tid; i < pairs; i += kMoeThreads) {
-        const int e = S.id[i];
-        if (e >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&S.mask[e]), 1ull << (i / P.top_k));
-    }
+    /* a lane a (token, choice) from here on, and an expert */
+    const int t = tid < P.pairs ? tid / P.top_k : 0, e = tid < P.pairs ? S.id[tid] : -1;
+    if (e >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&S.mask[e]), 1ull << t);
     __syncthreads();
-    /* a lane an expert: slots and jobs before it */
-    const int cnt = __popcll(S.mask[tid]), nj = (cnt + 8 * CT - 1) / (8 * CT);
-    const uint64_t own = (uint64_t)nj << 32 | (uint32_t)cnt;
+    const int cnt = tid < kMoeMaxE ? __popcll(S.mask[tid]) : 0, nj = (cnt + P.width - 1) / P.width;
+    const uint64_t own = (uint64_t)nj << 32 | (uint32_t)cnt;         /* slots and jobs before an expert's */
     uint64_t upto = r3d_wave_scan(own);
     if (lane == 63) S.scan[wave] = upto;
     __syncthreads();
     uint64_t all = 0;
-    for (int i = 0; i < kMoeWaves; ++i) {
+#pragma unroll
+    for (int i = 0; i < kMoeMaxE / 64; ++i) {
         if (i == wave) upto += all;
         all += S.scan[i];
     }
-    const int slot = (int)(uint32_t)(upto - own), j0 = (int)((upto - own) >> 32);
-    S.first[tid] = (uint16_t)slot;
-    for (int j = 0; j < nj; ++j) {
-        const int left = cnt - 8 * CT * j;
-        S.job[j0 + j] = (uint32_t)tid | (uint32_t)(slot + 8 * CT * j) << 9 | (uint32_t)(left < 8 * CT ? left : 8 * CT) << 20;
+    if (tid < kMoeMaxE) {
+        const int slot = (int)(uint32_t)(upto - own), j0 = (int)((upto - own) >> 32);
+        S.first[tid] = (uint16_t)slot;
+        for (int j = 0; j < nj; ++j) {
+            const int left = cnt - P.width * j;
+            S.job[j0 + j] = (uint32_t)tid | (uint32_t)(slot + P.width * j) << 9 | (uint32_t)(left < P.width ? left : P.width) << 20;
+        }
     }
     if (tid == 0) S.jobs = (int)(all >> 32);
     __syncthreads();
-    for (int i = tid; i < pairs; i += kMoeThreads) {
-        const int e = S.id[i], t = i / P.top_k;
-        if (e < 0) continue;
-        const int at = S.first[e] + __popcll(S.mask[e] & ((1ull << t) - 1));
-        S.tok[at] = (uint8_t)t;
-        S.slot_w[at] = S.w[i];
+    int slot = -1;
+    if (e >= 0) {
+        slot = S.first[e] + __popcll(S.mask[e] & ((1ull << t) - 1));
+        S.tok[slot] = (uint8_t)t;
+        S.slot_w[slot] = S.w[tid];
     }
     __syncthreads();
     if (blockIdx.x == 0) {
-        for (int i = tid; i < kMoeMaxPairs; i += kMoeThreads) {
-            if (i < S.jobs) P.table->job[i] = S.job[i];
-            if (i < pairs) {
-                P.table->tok[i] = S.tok[i];
-                if (P.ids) P.ids[i / P.top_k * P.i_pitch + i % P.top_k] = S.id[i];
-                if (P.weights) P.weights[i / P.top_k * P.wt_pitch + i % P.top_k] = S.w[i];
-            }
+        if (tid < S.jobs) P.table->job[tid] = S.job[tid];
+        if (tid < P.pairs) {
+            const int i = tid - t * P.top_k;
+            P.table->slot[tid] = (int16_t)slot;
+            if (P.ids) P.ids[t * P.i_pitch + i] = e;
+            if (P.weights) P.weights[t * P.wt_pitch + i] = S.w[tid];
         }
         if (tid == 0) P.table->jobs = S.jobs;
     }
 }
 
 /* ------------------------------------------------------------------------------ products */
-
-/* One line of 8 rows of R planes' blocks and of 8 CT columns, on its way. */
-template <int ENC, int R, int CT, int XH>
-struct MoeStep {
-    r3d_i32x4 w[R];
-    uint32_t s[R];                                              /* e2m1: the piece's scale */
-    r3d_i32x4 x[CT][XH * MoeCodes<ENC>::X];
-};
-
-template <int ENC, int R, int CT, int XH>
-__device__ __forceinline__ void moe_products(const MoeStep<ENC, R, CT, XH>& st, r3d_f32x4 (&acc)[R][CT]) {
-    constexpr int X = MoeCodes<ENC>::X;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        r3d_i32x4 b[X];
-        moe_bf16<ENC>(st.w[r], st.s[r], b);
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
-#pragma unroll
-            for (int i = 0; i < XH * X; ++i) acc[r][c] = moe_mfma(b[i % X], st.x[c][i], acc[r][c]);
-    }
-}
 
 /* The sum of a result's two halves, (0, 0) and (1, 1), 40 lanes apart: lanes 0-7 and 16-23 then hold rows
  * 4 (lane / 16) .. + 3 of column lane % 8. */
@@ -267,265 +241,290 @@ __device__ __forceinline__ r3d_f32x4 moe_halves(r3d_f32x4 a) {
     return a;
 }
 
-template <int ENC, int CT>
-__global__ __launch_bounds__(kMoeThreads) void moe_up_kernel(MoeUpArgs P) {
-    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X, D = CT == 1 ? 4 : 2;
-    __shared__ MoeChoice S;
-    __shared__ r3d_f32x4 s_part[kMoeWaves][CT][2][16];
-    moe_plan<CT>(P, S);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int r8 = lane & 7, piece = ((lane >> 3) & 1) | ((lane >> 4) << 1);
-    const int fb = P.f >> 3, units = S.jobs * fb, kc = P.kc, upw = kMoeWaves / kc;
-    const int sub = i8_uniform(wave / kc), c = wave - sub * kc;
-    const int pieces = P.n / N, lines = (pieces + 7) >> 3, per = (lines + kc - 1) / kc;
-    const int l0 = c * per, l1 = l0 + per < lines ? l0 + per : lines;
-    const __amdgpu_buffer_rsrc_t rX = r3d_rsrc(P.x, (int64_t)(P.M - 1) * P.x_pitch + 2 * (int64_t)P.n);
-    const int64_t plane = (int64_t)(2 * P.f - 1) * P.w_pitch + (int64_t)pieces * 16;
+/* LDS that a row of K columns in XH parts takes: whole 1 KB loads, and 16 bytes off a multiple of 128 so that
+ * eight tokens' pieces meet no bank twice. */
+constexpr int moe_row(int64_t K, int parts) { return (int)(parts * ((2 * K + 1023) / 1024) * 1024 + 16); }
 
-    for (int u0 = blockIdx.x * upw; u0 < units; u0 += gridDim.x * upw) {
-        const int u = u0 + sub, live = u < units;
-        const int jb = i8_uniform(live ? u / fb : 0), b0 = 8 * (live ? u - jb * fb : 0);
-        const uint32_t job = i8_uniform(S.job[jb]);
-        const int e = job & 511, slot0 = (job >> 9) & 2047, cnt = live ? job >> 20 : 0;
-        if (live) {
-            const __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w + e * P.w_expert, plane);
-            const __amdgpu_buffer_rsrc_t rS = r3d_rsrc(ENC == MOE_FP4 ? P.ws + e * P.ws_expert : nullptr,
-                                                       ENC == MOE_FP4 ? (2 * P.f - 1) * P.ws_pitch + pieces : 0);
-            const uint32_t wo[2] = {(uint32_t)((b0 + r8) * P.w_pitch + 16 * piece),
-                                    (uint32_t)((P.f + b0 + r8) * P.w_pitch + 16 * piece)};
-            const uint32_t so[2] = {(uint32_t)((b0 + r8) * P.ws_pitch + piece),
-                                    (uint32_t)((P.f + b0 + r8) * P.ws_pitch + piece)};
-            uint32_t xo[CT];
-#pragma unroll
-            for (int t = 0; t < CT; ++t)
-                xo[t] = 8 * t + r8 < cnt ? (uint32_t)(S.tok[slot0 + 8 * t + r8] * P.x_pitch + 16 * X * piece) : kI8Oob;
-            MoeStep<ENC, 2, CT, 1> ring[D];
-            auto load = [&](MoeStep<ENC, 2, CT, 1>& st, int l) __attribute__((always_inline)) {
-                const bool in = l < l1 && 8 * l + piece < pieces;
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    st.w[r] = i8_buf16<2>(rW, in ? wo[r] : kI8Oob, 128 * l);
-                    if (ENC == MOE_FP4)
-                        st.s[r] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rS, (int)(in ? so[r] : kI8Oob), 8 * l, 0);
-                }
-#pragma unroll
-                for (int t = 0; t < CT; ++t)
-#pragma unroll
-                    for (int i = 0; i < X; ++i)
-                        st.x[t][i] = i8_buf16<0>(rX, in ? xo[t] + 16 * i : kI8Oob, 128 * X * l);
-            };
-            r3d_f32x4 acc[2][CT];
-#pragma unroll
-            for (int t = 0; t < CT; ++t) acc[0][t] = acc[1][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int d = 0; d < D; ++d) load(ring[d], l0 + d);
-            for (int l = l0; l < l1; l += D) {
-#pragma unroll
-                for (int d = 0; d < D; ++d) {
-                    moe_products(ring[d], acc);
-                    load(ring[d], l + D + d);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < CT; ++t)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const r3d_f32x4 v = moe_halves(acc[r][t]);
-                    if (lane < 32 && !(lane & 8)) s_part[wave][t][r][(lane >> 4) * 8 + r8] = v;
-                }
-        }
-        __syncthreads();
-        if (live && c == 0 && lane < 16 * CT) {
-            /* lane (t, half, column): rows 4 half .. + 3 of token 8 t + column */
-            const int t = lane >> 4, half = (lane >> 3) & 1, col = 8 * t + (lane & 7);
-            r3d_f32x4 g = s_part[wave][t][0][lane & 15], w = s_part[wave][t][1][lane & 15];
-            for (int o = 1; o < kc; ++o) {
-                g += s_part[wave + o][t][0][lane & 15];
-                w += s_part[wave + o][t][1][lane & 15];
-            }
-            if (col < cnt) {
-                const int row = b0 + 4 * half, slot = slot0 + col;
-                float a[4], v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    a[i] = g[i];
-                    v[i] = w[i];
-                    if (ENC == MOE_I8) {
-                        const float* s = reinterpret_cast<const float*>(P.ws) + e * P.ws_expert + row + i;
-                        a[i] *= s[0];
-                        v[i] *= s[P.f];
-                    }
-                }
-                act_values<4>(P.act, a);
-                const float wt = S.slot_w[slot];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[i] = a[i] * v[i] * wt;
-                const uint32_t h0 = r3d_pack_bf16x2(a[0], a[1]), h1 = r3d_pack_bf16x2(a[2], a[3]);
-                *reinterpret_cast<uint2*>(P.h + (int64_t)slot * P.f + row) = make_uint2(h0, h1);
-                if (P.h_lo) {
-                    float lo[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t d = i < 2 ? h0 : h1;
-                        const float hi = __uint_as_float(i & 1 ? d & 0xFFFF0000u : d << 16);
-                        lo[i] = __builtin_fabsf(hi) < __builtin_inff() ? a[i] - hi : 0.0f;   /* inf - inf; NaN is in hi */
-                    }
-                    *reinterpret_cast<uint2*>(P.h_lo + (int64_t)slot * P.f + row) =
-                        make_uint2(r3d_pack_bf16x2(lo[0], lo[1]), r3d_pack_bf16x2(lo[2], lo[3]));
-                }
-            }
-        }
-        __syncthreads();
-    }
-}
-
-/* XH 2: h in two parts */
-template <int ENC, int CT, int RT, int XH>
-__global__ __launch_bounds__(kMoeThreads) void moe_down_kernel(MoeDownArgs P) {
-    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X, D = CT * RT * XH == 1 ? 4 : 2;
-    __shared__ uint32_t s_job[kMoeMaxPairs];
-    __shared__ uint8_t s_tok[kMoeMaxPairs];
-    extern __shared__ __attribute__((aligned(16))) float s_y[];     /* [waves][M][8 RT] */
+template <int ENC, int CT, int XH, bool UP>
+__global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
+    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X, D = 4;
+    struct Jobs {
+        uint32_t job[kMoeMaxPairs];
+    };
+    __shared__ typename std::conditional<UP, MoeChoice, Jobs>::type S;
+    __shared__ r3d_f32x4 s_part[kMoeWaves][2][2][CT][16];            /* a wave's last unit and its first, where shared */
+    __shared__ __attribute__((aligned(16))) float s_scale[ENC == MOE_I8 ? kMoeUnits * 16 : 1];
+    extern __shared__ __attribute__((aligned(16))) uint8_t s_x[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int jobs = P.table->jobs;
-    /* past the table's own entries: what lies there is not used */
-    *reinterpret_cast<uint2*>(s_job + 2 * tid) = *reinterpret_cast<const uint2*>(P.table->job + 2 * tid);
-    *reinterpret_cast<uint16_t*>(s_tok + 2 * tid) = *reinterpret_cast<const uint16_t*>(P.table->tok + 2 * tid);
-    for (int i = tid; i < kMoeWaves * P.M * 8 * RT; i += kMoeThreads) s_y[i] = 0.0f;
-    __syncthreads();
+    int jobs;
+    if constexpr (UP) {
+        moe_plan(P, S);
+        jobs = i8_uniform(S.jobs);
+    } else {
+        jobs = P.table->jobs;
+        S.job[tid] = P.table->job[tid];                              /* what lies past the jobs is not used */
+        __syncthreads();
+    }
     const int r8 = lane & 7, piece = ((lane >> 3) & 1) | ((lane >> 4) << 1);
-    const int pieces = P.f / N, lines = (pieces + 7) >> 3;
-    const int64_t total = (int64_t)jobs * lines;
-    const int s0 = (int)(total * wave / kMoeWaves), s1 = (int)(total * (wave + 1) / kMoeWaves);
-    const int row0 = blockIdx.x * 8 * RT;
-    float* const ys = s_y + wave * P.M * 8 * RT;
-    const int64_t plane = (int64_t)(P.n - 1) * P.w_pitch + (int64_t)pieces * 16;
-    const int64_t h_bytes = (int64_t)P.pairs * P.f * 2;
-    const __amdgpu_buffer_rsrc_t rH = r3d_rsrc(P.h, h_bytes);
-    const __amdgpu_buffer_rsrc_t rL = r3d_rsrc(XH == 2 ? P.h_lo : P.h, XH == 2 ? h_bytes : 0);
-    uint32_t wo[RT], so[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {                                    /* rows past n are past the plane: zeros */
-        wo[r] = (uint32_t)(row0 + 8 * r + r8) * (uint32_t)P.w_pitch + 16 * piece;
-        so[r] = (uint32_t)((row0 + 8 * r + r8) * P.ws_pitch + piece);
-    }
-    struct Ring {
-        MoeStep<ENC, RT, CT, XH> st;
-        r3d_f32x4 scale[RT];                                          /* int8: of the job's rows, with its last line */
-    } ring[D];
-    /* the run that loads walk, D steps ahead of the products */
-    int lj = lines ? s0 / lines : 0, ll = s0 - lj * lines;
-    __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w, 0), rS = rW;
-    uint32_t xo[CT];
-    int64_t sc_at = 0;
-    auto enter = [&](int j) __attribute__((always_inline)) {
-        const uint32_t job = i8_uniform(s_job[j]);
-        const int64_t e = job & 511;
-        const int slot0 = (job >> 9) & 2047, cnt = job >> 20;
-        rW = r3d_rsrc(P.w + e * P.w_expert, plane);
-        if (ENC == MOE_FP4) rS = r3d_rsrc(P.ws + e * P.ws_expert, (P.n - 1) * P.ws_pitch + pieces);
-        if (ENC == MOE_I8) sc_at = e * P.ws_expert;
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-            xo[t] = 8 * t + r8 < cnt ? (uint32_t)((slot0 + 8 * t + r8) * P.f * 2 + 16 * X * piece) : kI8Oob;
-    };
-    auto load = [&](Ring& g, int s) __attribute__((always_inline)) {
-        const bool run = s < s1;
-        if (run && (ll == 0 || s == s0)) enter(lj);
-        const bool in = run && 8 * ll + piece < pieces;
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            g.st.w[r] = i8_buf16<2>(rW, in ? wo[r] : kI8Oob, 128 * ll);
-            if (ENC == MOE_FP4)
-                g.st.s[r] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rS, (int)(in ? so[r] : kI8Oob), 8 * ll, 0);
+    const bool mine = lane < 32 && !(lane & 8);                      /* holds results (moe_halves) */
+    const int row4 = 4 * ((lane >> 4) & 1);
+    const int nb = UP ? P.rows >> 3 : (P.rows + 15) >> 4;            /* units a job */
+    const int pieces = P.K / N, lines = (pieces + 7) >> 3, cpr = (2 * P.K + 1023) >> 10;
+    const int row_lds = moe_row(P.K, XH), part_lds = cpr * 1024;
+    /* a run an XCD, so that its L2 sees few jobs' tokens */
+    const int G = gridDim.x, per = G >> 3, rem = G & 7, xcd = blockIdx.x & 7;
+    const int g = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const int64_t units = (int64_t)jobs * nb;
+    const int u_end = i8_uniform((int)(units * (g + 1) / G));
+    const int64_t x_rows = UP ? P.M : P.pairs;
+    const int64_t x_bytes = (x_rows - 1) * P.x_pitch + 2 * (int64_t)P.K;
+    const int64_t plane = (int64_t)((UP ? 2 * P.rows : P.rows) - 1) * P.w_pitch + (int64_t)pieces * 16;
+    const int64_t s_plane = (int64_t)((UP ? 2 * P.rows : P.rows) - 1) * P.ws_pitch + pieces;
+
+    for (int u = i8_uniform((int)(units * g / G)); u < u_end;) {
+        /* as many units of the run as LDS holds the tokens (and the scales) of */
+        const int j0 = i8_uniform(u / nb), slot_base = i8_uniform((S.job[j0] >> 9) & 2047);
+        int end = u, held = 0;
+        for (int j = j0; end < u_end && end - u < (ENC == MOE_I8 ? kMoeUnits : 1 << 30); ++j) {
+            const uint32_t job = i8_uniform(S.job[j]);
+            const int upto = (int)((job >> 9) & 2047) + (int)(job >> 20) - slot_base;
+            if (upto > P.job_rows) break;
+            held = upto;
+            end = (j + 1) * nb < u_end ? (j + 1) * nb : u_end;
         }
-#pragma unroll
-        for (int t = 0; t < CT; ++t)
-#pragma unroll
-            for (int i = 0; i < X; ++i) {
-                g.st.x[t][i] = i8_buf16<0>(rH, in ? xo[t] + 16 * i : kI8Oob, 128 * X * ll);
-                if (XH == 2) g.st.x[t][(XH - 1) * X + i] = i8_buf16<0>(rL, in ? xo[t] + 16 * i : kI8Oob, 128 * X * ll);
-            }
-        if (ENC == MOE_I8 && run && (ll == lines - 1 || s == s1 - 1)) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                int at = row0 + 8 * r + 4 * ((lane >> 4) & 1);
-                at = at + 4 <= P.n ? at : 0;
-                g.scale[r] = *reinterpret_cast<const r3d_f32x4_u4*>(reinterpret_cast<const float*>(P.ws) + sc_at + at);
+        if (ENC == MOE_I8 && end - u > kMoeUnits) end = u + kMoeUnits;
+        for (int c = wave; c < held * XH * cpr; c += kMoeWaves) {
+            const int r = i8_uniform(c / (XH * cpr)), rest = c - r * XH * cpr, p = i8_uniform(rest / cpr), k = rest - p * cpr;
+            const __amdgpu_buffer_rsrc_t rX = r3d_rsrc(P.x + p * (x_rows * P.x_pitch), x_bytes);
+            int row;
+            if constexpr (UP) row = i8_uniform(S.tok[slot_base + r]);
+            else row = slot_base + r;
+            const uint32_t at = 1024 * k + 16 * lane;                /* past the row's end: zeros */
+            r3d_buf_lds<16>(rX, s_x + r * row_lds + p * part_lds + 1024 * k,
+                            at < 2 * (uint32_t)P.K ? (uint32_t)row * (uint32_t)P.x_pitch + at : kI8Oob, 0);
+        }
+        if constexpr (ENC == MOE_I8) {
+            for (int i = tid; i < 16 * (end - u); i += kMoeThreads) {
+                const int un = u + (i >> 4), j = un / nb, blk = un - j * nb, r = i & 15;
+                int row = UP ? (r >> 3) * P.rows + 8 * blk + (r & 7) : 16 * blk + r;
+                if (!UP && row >= P.rows) row = P.rows - 1;
+                s_scale[i] = reinterpret_cast<const float*>(P.ws)[(int64_t)(S.job[j] & 511) * P.ws_expert + row];
             }
         }
-        if (++ll == lines) {
-            ll = 0;
-            ++lj;
-        }
-    };
-    r3d_f32x4 acc[RT][CT];
+        /* this wave's lines */
+        const int64_t total = (int64_t)(end - u) * lines;
+        const int a = i8_uniform((int)(total * wave / kMoeWaves)), b = i8_uniform((int)(total * (wave + 1) / kMoeWaves));
+        struct Line {
+            r3d_i32x4 w[2];
+            uint32_t s[2];                                           /* e2m1: the pieces' scales */
+        } ring[D];
+        const int ua = i8_uniform(a / lines);
+        int ll = a - ua * lines, lj = i8_uniform((u + ua) / nb), lb = u + ua - lj * nb;   /* where loads are */
+        int cl = ll, cj = lj, cb = lb, cu = ua;                      /* where products are */
+        __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w, 0), rS = rW;
+        uint32_t w_at[2] = {0, 0}, s_at[2] = {0, 0};
+        bool both = true;
+        auto load = [&](Line& st, int s) __attribute__((always_inline)) {
+            const bool run = s < b;
+            if (run && (ll == 0 || s == a)) {                        /* a unit's first line here */
+                const int64_t e = i8_uniform(S.job[lj]) & 511;
+                rW = r3d_rsrc(P.w + e * P.w_expert, plane);
+                if (ENC == MOE_FP4) rS = r3d_rsrc(P.ws + e * P.ws_expert, s_plane);
+                const uint32_t r0 = (UP ? 8 : 16) * lb, r1 = UP ? r0 + P.rows : r0 + 8;
+                both = UP || (int)r1 < P.rows;
+                w_at[0] = r0 * (uint32_t)P.w_pitch;
+                w_at[1] = r1 * (uint32_t)P.w_pitch;
+                s_at[0] = r0 * (uint32_t)P.ws_pitch;
+                s_at[1] = r1 * (uint32_t)P.ws_pitch;
+            }
+            const bool in = run && 8 * ll + piece < pieces;
+            const uint32_t wo = (uint32_t)(r8 * P.w_pitch + 16 * piece), so = (uint32_t)(r8 * P.ws_pitch + piece);
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int t = 0; t < CT; ++t) acc[r][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    int cj = lj, cl = ll;
-    if (s0 < s1) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) load(ring[d], s0 + d);
-    }
-    for (int s = s0; s < s1; s += D) {
+            for (int r = 0; r < 2; ++r) {
+                const bool ok = in && (r == 0 || both);
+                st.w[r] = i8_buf16<2>(rW, ok ? wo : kI8Oob, w_at[r] + 128 * ll);
+                if (ENC == MOE_FP4)
+                    st.s[r] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rS, (int)(ok ? so : kI8Oob), (int)(s_at[r] + 8 * ll), 0);
+            }
+            if (++ll == lines) {
+                ll = 0;
+                if (++lb == nb) {
+                    lb = 0;
+                    ++lj;
+                }
+            }
+        };
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            if (s + d < s1) {
-                moe_products(ring[d].st, acc);
-                if (++cl == lines || s + d + 1 == s1) {               /* the job's end, or the run's */
-                    const uint32_t job = i8_uniform(s_job[cj]);
-                    const int slot0 = (job >> 9) & 2047, cnt = job >> 20;
+            load(ring[d], a + d);
+            __builtin_amdgcn_sched_barrier(0);                       /* in this order everywhere: a line waits for its own */
+        }
+        __syncthreads();
+
+        int slot0 = 0, cnt = 0;
+        uint32_t xa[CT];
+        auto job_of = [&](int j) __attribute__((always_inline)) {
+            const uint32_t job = i8_uniform(S.job[j]);
+            slot0 = (job >> 9) & 2047;
+            cnt = job >> 20;
+#pragma unroll
+            for (int t = 0; t < CT; ++t)                             /* a column without a token repeats the first one's */
+                xa[t] = (slot0 - slot_base + (8 * t + r8 < cnt ? 8 * t + r8 : 0)) * row_lds + 16 * X * piece;
+        };
+        if (a < b) job_of(cj);
+        r3d_f32x4 acc[2][CT];
+        auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < CT; ++t) acc[0][t] = acc[1][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        };
+        /* a whole unit's results, on the lanes that hold them */
+        auto finish = [&](int un, int blk) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                const int col = 8 * t + r8;
+                if (!mine || col >= cnt) continue;
+                const int64_t slot = slot0 + col;
+                r3d_f32x4 v[2] = {acc[0][t], acc[1][t]};
+                if constexpr (ENC == MOE_I8) {
+                    v[0] *= *reinterpret_cast<const r3d_f32x4*>(&s_scale[16 * un + row4]);
+                    v[1] *= *reinterpret_cast<const r3d_f32x4*>(&s_scale[16 * un + 8 + row4]);
+                }
+                if constexpr (UP) {
+                    float h[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+                    act_values<4>(P.act, h);
+                    const float wt = S.slot_w[slot];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) h[i] = h[i] * v[1][i] * wt;
+                    uint16_t* to = static_cast<uint16_t*>(P.out) + slot * P.rows + 8 * blk + row4;
+                    for (int p = 0; p < P.parts; ++p) {
+                        const uint32_t h0 = r3d_pack_bf16x2(h[0], h[1]), h1 = r3d_pack_bf16x2(h[2], h[3]);
+                        *reinterpret_cast<uint2*>(to + (int64_t)p * P.pairs * P.rows) = make_uint2(h0, h1);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {                /* what is left of it; nothing of inf and NaN */
+                            const uint32_t d = i < 2 ? h0 : h1;
+                            const float hi = __uint_as_float(i & 1 ? d & 0xFFFF0000u : d << 16);
+                            h[i] = __builtin_fabsf(hi) < __builtin_inff() ? h[i] - hi : 0.0f;
+                        }
+                    }
+                } else {
+                    float* const to = static_cast<float*>(P.out) + slot * P.rows + 16 * blk + row4;
+                    *reinterpret_cast<r3d_f32x4*>(to) = v[0];
+                    if (16 * blk + 8 < P.rows) *reinterpret_cast<r3d_f32x4*>(to + 8) = v[1];
+                }
+            }
+        };
+        clear();
+        bool whole = cl == 0;                                        /* this wave has the unit from its first line on */
+        for (int s = a; s < b; s += D) {
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                if (s + d < b) {
+                    r3d_i32x4 w0[X], w1[X];
+                    moe_bf16<ENC>(ring[d].w[0], ring[d].s[0], w0);
+                    moe_bf16<ENC>(ring[d].w[1], ring[d].s[1], w1);
 #pragma unroll
                     for (int t = 0; t < CT; ++t)
 #pragma unroll
-                        for (int r = 0; r < RT; ++r) {
-                            r3d_f32x4 v = moe_halves(acc[r][t]);
-                            acc[r][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                            if (ENC == MOE_I8) v *= ring[d].scale[r];
-                            if (lane < 32 && !(lane & 8) && 8 * t + r8 < cnt) {
-                                /* a token comes once a job: no two lanes meet */
-                                r3d_f32x4* const to = reinterpret_cast<r3d_f32x4*>(
-                                    ys + s_tok[slot0 + 8 * t + r8] * 8 * RT + 8 * r + 4 * (lane >> 4));
-                                *to += v;
+                        for (int i = 0; i < XH * X; ++i) {
+                            const r3d_i32x4 x = *reinterpret_cast<const r3d_i32x4*>(
+                                s_x + xa[t] + i / X * part_lds + 128 * X * cl + 16 * (i % X));
+                            acc[0][t] = moe_mfma(w0[i % X], x, acc[0][t]);
+                            acc[1][t] = moe_mfma(w1[i % X], x, acc[1][t]);
+                        }
+                    if (++cl == lines || s + d + 1 == b) {           /* the unit's end, or the run's */
+#pragma unroll
+                        for (int t = 0; t < CT; ++t) {
+                            acc[0][t] = moe_halves(acc[0][t]);
+                            acc[1][t] = moe_halves(acc[1][t]);
+                        }
+                        if (whole && cl == lines) {
+                            finish(cu, cb);
+                        } else if (mine) {
+#pragma unroll
+                            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                                for (int r = 0; r < 2; ++r) s_part[wave][whole ? 0 : 1][r][t][2 * row4 + r8] = acc[r][t];
+                        }
+                        if (cl == lines) {
+                            clear();
+                            whole = true;
+                            cl = 0;
+                            ++cu;
+                            if (++cb == nb) {
+                                cb = 0;
+                                if (s + d + 1 < b) job_of(++cj);
                             }
                         }
-                    cl = 0;
-                    ++cj;
+                    }
                 }
+                load(ring[d], s + D + d);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            load(ring[d], s + D + d);
         }
+        __syncthreads();
+        if (a < b && cl > 0 && whole) {                              /* begun here, ended by the waves after */
+            const int stop = (cu + 1) * lines;
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    r3d_f32x4 v = s_part[wave][0][r][t][(2 * row4 + r8) & 15];
+                    for (int o = wave + 1; o < kMoeWaves; ++o) {
+                        const int ao = (int)(total * o / kMoeWaves);
+                        if (ao >= stop) break;
+                        if (ao < (int)(total * (o + 1) / kMoeWaves)) v += s_part[o][1][r][t][(2 * row4 + r8) & 15];
+                    }
+                    acc[r][t] = v;
+                }
+            finish(cu, cb);
+        }
+        u = end;
+        if (u < u_end) __syncthreads();                              /* the scales are read */
     }
-    __syncthreads();
-    for (int i = tid; i < P.M * 8 * RT; i += kMoeThreads) {
-        const int m = i / (8 * RT), row = row0 + i % (8 * RT);
-        float v = s_y[i];
-        for (int w = 1; w < kMoeWaves; ++w) v += s_y[w * P.M * 8 * RT + i];
-        if (row >= P.n) continue;
-        if (P.y_bf16) reinterpret_cast<uint16_t*>(P.y)[m * P.y_pitch + row] = r3d_bf16_rne(v);
-        else reinterpret_cast<float*>(P.y)[m * P.y_pitch + row] = v;
+}
+
+/* y of the slots' sums: four columns a lane, (ceil(n / 1024), M) workgroups of 256. */
+__global__ __launch_bounds__(256) void moe_sum_kernel(const float* __restrict__ sums, const MoeTable* __restrict__ table,
+                                                      void* y, int64_t y_pitch, int n, int top_k, int y_bf16) {
+    const int m = blockIdx.y, c = 4 * (blockIdx.x * 256 + threadIdx.x);
+    if (c >= n) return;                                              /* n is a multiple of 8 */
+    r3d_f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < top_k; ++i) {
+        const int slot = table->slot[m * top_k + i];
+        if (slot >= 0) v += *reinterpret_cast<const r3d_f32x4*>(sums + (int64_t)slot * n + c);
     }
+    if (y_bf16)
+        *reinterpret_cast<r3d_u32x2_u2*>(static_cast<uint16_t*>(y) + m * y_pitch + c) =
+            r3d_u32x2_u2{r3d_pack_bf16x2(v[0], v[1]), r3d_pack_bf16x2(v[2], v[3])};
+    else
+        *reinterpret_cast<r3d_f32x4_u4*>(static_cast<float*>(y) + m * y_pitch + c) = v;
 }
 
 template <int ENC, int CT>
 static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStream_t stream) {
     MoeTable* const table = static_cast<MoeTable*>(scratch);
-    uint16_t* const h = reinterpret_cast<uint16_t*>(table + 1);
-    uint16_t* const lo = P.y_bf16 ? nullptr : h + P.M * P.top_k * P.f;
-    const MoeUpArgs u{P.x, P.logits, P.gu, P.gus, table, h, lo, P.ids, P.weights, (int)P.M, (int)P.n, (int)P.f, (int)P.E,
-                      (int)P.top_k, (int)P.x_pitch, (int)P.gu_pitch, g.kc, P.act, P.sigmoid, P.renorm, P.l_bf16,
-                      P.gu_expert, P.gus_expert, P.gus_pitch, P.l_pitch, P.i_pitch, P.w_pitch, P.weight_scale};
-    hipLaunchKernelGGL((moe_up_kernel<ENC, CT>), dim3((unsigned)g.up_blocks), dim3(kMoeThreads), 0, stream, u);
+    const int64_t pairs = P.M * P.top_k;
+    const int parts = P.y_bf16 ? 2 : 3;
+    uint8_t* const h = reinterpret_cast<uint8_t*>(table + 1);
+    float* const sums = reinterpret_cast<float*>(h + moe_h_bytes(P));
+    MoeArgs u{P.x, P.gu, P.gus, table, h, (int)P.M, (int)P.n, (int)P.f, (int)pairs, (int)P.x_pitch, (int)P.gu_pitch,
+              g.up_rows, P.gu_expert, P.gus_expert, P.gus_pitch, P.logits, P.ids, P.weights, P.l_pitch, P.i_pitch,
+              P.w_pitch, (int)P.E, (int)P.top_k, g.width, parts, P.act, P.sigmoid, P.renorm, P.l_bf16, P.weight_scale};
+    hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 1, true>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
+                       (size_t)g.up_rows * moe_row(P.n, 1), stream, u);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) {
-        const MoeDownArgs d{(const uint8_t*)h, (const uint8_t*)lo, P.dn, P.dns, table, P.y, (int)P.M, (int)P.n, (int)P.f,
-                            (int)(P.M * P.top_k), (int)P.dn_pitch, P.y_bf16, P.dn_expert, P.dns_expert, P.dns_pitch, P.y_pitch};
-        const size_t lds = (size_t)(kMoeWaves * P.M * 8) * 4;
-        const dim3 grid((unsigned)g.down_blocks);
-        if (lo) hipLaunchKernelGGL((moe_down_kernel<ENC, CT, 1, 2>), grid, dim3(kMoeThreads), lds, stream, d);
-        else hipLaunchKernelGGL((moe_down_kernel<ENC, CT, 1, 1>), grid, dim3(kMoeThreads), lds, stream, d);
+        MoeArgs d{h, P.dn, P.dns, table, sums, (int)P.M, (int)P.f, (int)P.n, (int)pairs, (int)(2 * P.f), (int)P.dn_pitch,
+                  g.down_rows, P.dn_expert, P.dns_expert, P.dns_pitch};
+        const size_t lds = (size_t)g.down_rows * moe_row(P.f, parts);
+        const dim3 grid((unsigned)g.blocks), block(kMoeThreads);
+        if (P.y_bf16) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 2, false>), grid, block, lds, stream, d);
+        else hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 3, false>), grid, block, lds, stream, d);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) {
+        hipLaunchKernelGGL(moe_sum_kernel, dim3((unsigned)((P.n + 1023) / 1024), (unsigned)P.M), dim3(256), 0, stream, sums,
+                           table, P.y, P.y_pitch, (int)P.n, (int)P.top_k, P.y_bf16);
         e = hipGetLastError();
     }
     return e == hipSuccess ? RAD_OK : i8_failed("moe_layer", e);
@@ -539,11 +538,11 @@ static int moe_entry(const RadArgs* a, RadStream s) {
     if (!a->scratch || (uintptr_t)a->scratch & 15 || a->scratch_bytes < moe_scratch(P)) return RAD_E_UNSUPPORTED;
     if (!chip_ok()) return RAD_E_UNSUPPORTED;
     MoeGeom g;
-    moe_geom(P, cu_count(), &g);
+    if (!moe_geom(P, cu_count(), &g)) return RAD_E_UNSUPPORTED;
     hipStream_t t = (hipStream_t)s;
-#define R3D_MOE(ENC_)                                                              \
-    return g.ct == 1 ? moe_launch<ENC_, 1>(P, g, a->scratch, t)                     \
-         : g.ct == 2 ? moe_launch<ENC_, 2>(P, g, a->scratch, t) : moe_launch<ENC_, 4>(P, g, a->scratch, t)
+#define R3D_MOE(ENC_)                                          \
+    return g.ct == 1 ? moe_launch<ENC_, 1>(P, g, a->scratch, t) \
+                     : moe_launch<ENC_, 2>(P, g, a->scratch, t)
     if (P.enc == MOE_BF16) R3D_MOE(MOE_BF16);
     if (P.enc == MOE_I8) R3D_MOE(MOE_I8);
     R3D_MOE(MOE_FP4);

@@ -143,31 +143,39 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
     return RAD_OK;
 }
 
-/* Experts that someone chose, were the choices spread evenly. */
-static double moe_read(const MoePlan& P) {
-    return (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
+/* LDS a workgroup: 160 KB, less its tables, the waves' shared units and int8's scales */
+static int64_t moe_lds(const MoePlan& P, int ct, bool up) {
+    return 160 * 1024 - (up ? 21 : 5) * 1024 - 16 * 1024 * ct - (P.enc == MOE_I8 ? 8 * 1024 : 0);
 }
 
-void moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
+bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
     if (ncu <= 0) ncu = 256;
-    const int64_t pairs = P.M * P.top_k, most = P.E < pairs ? P.E : pairs;
-    const double read = moe_read(P), each = (double)pairs / read;
-    g->ct = P.M <= 8 || each <= 6 ? 1 : each <= 12 ? 2 : 4;
-    const int64_t jobs = most + (pairs - most) / (8 * g->ct);   /* at most */
-    const int64_t fb = P.f / 8;
-    const double width = P.enc == MOE_BF16 ? 64 : P.enc == MOE_I8 ? 128 : 256;
-    const double lines = ceil((double)P.n / width);
-    /* waves that stream: enough of them, two lines each at least */
-    g->kc = 1;
-    while (g->kc < 8 && read * fb * g->kc < 16 * ncu && lines / (2 * g->kc) >= 2) g->kc *= 2;
-    const int64_t units = jobs * fb, wg = (units + 8 / g->kc - 1) / (8 / g->kc);
-    g->up_blocks = wg < 4 * ncu ? wg : 4 * ncu;
-    g->rt = 1;
-    g->down_blocks = (P.n / 8 + g->rt - 1) / g->rt;
+    const int64_t pairs = P.M * P.top_k;
+    const int64_t up = (2 * P.n + 1023) / 1024 * 1024 + 16;
+    const int64_t down = (P.y_bf16 ? 2 : 3) * ((2 * P.f + 1023) / 1024 * 1024) + 16;
+    /* experts with more than 8 tokens are read once for 16 of them, where LDS holds these */
+    const double read = (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
+    g->ct = (double)pairs / read > 6 && moe_lds(P, 2, true) / up >= 16 && moe_lds(P, 2, false) / down >= 16 ? 2 : 1;
+    int64_t ur = moe_lds(P, g->ct, true) / up, dr = moe_lds(P, g->ct, false) / down;
+    if (ur > pairs) ur = pairs;
+    if (dr > pairs) dr = pairs;
+    int64_t width = 8 * g->ct;
+    if (width > ur) width = ur;
+    if (width > dr) width = dr;
+    if (width < 1) return false;
+    g->width = (int)width;
+    g->up_rows = (int)ur;
+    g->down_rows = (int)dr;
+    g->blocks = ncu;
+    return true;
+}
+
+int64_t moe_h_bytes(const MoePlan& P) {
+    return (P.M * P.top_k * P.f * 2 * (P.y_bf16 ? 2 : 3) + 15) / 16 * 16;
 }
 
 int64_t moe_scratch(const MoePlan& P) {
-    return (int64_t)sizeof(MoeTable) + P.M * P.top_k * P.f * 2 * (P.y_bf16 ? 1 : 2);
+    return (int64_t)sizeof(MoeTable) + moe_h_bytes(P) + P.M * P.top_k * P.n * 4;
 }
 
 int64_t moe_scratch_bytes(const RadArgs* a) {
@@ -182,6 +190,7 @@ int64_t moe_scratch_bytes(const RadArgs* a) {
     else if (!rad_args_geti(a, "M", &M)) M = kMoeMaxM;
     if (M <= 0 || M > kMoeMaxM) return 0;
     P.M = M;
+    P.n = n;
     P.f = f;
     P.top_k = k;
     P.y_bf16 = 0;
@@ -199,11 +208,14 @@ int describe_moe(const char* row, const RadArgs* a, char* buf, int len) {
     }
     static const char* const kEnc[] = {"bf16", "i8", "mxfp4"};
     MoeGeom g;
-    moe_geom(P, 256, &g);
+    if (!moe_geom(P, 256, &g)) {
+        snprintf(buf, (size_t)len, "refused rc=%d (LDS)", RAD_E_UNSUPPORTED);
+        return RAD_E_UNSUPPORTED;
+    }
     snprintf(buf, (size_t)len, "arm=moe enc=%s M=%lld n=%lld f=%lld E=%lld top_k=%lld score=%s renorm=%d act=%d y=%s ct=%d "
-             "kc=%d up_blocks=%lld rt=%d down_blocks=%lld", kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
+             "width=%d up_rows=%d down_rows=%d blocks=%lld", kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
              (long long)P.E, (long long)P.top_k, P.sigmoid ? "sigmoid" : "softmax", P.renorm, P.act,
-             P.y_bf16 ? "bf16" : "f32", g.ct, g.kc, (long long)g.up_blocks, g.rt, (long long)g.down_blocks);
+             P.y_bf16 ? "bf16" : "f32", g.ct, g.width, g.up_rows, g.down_rows, (long long)g.blocks);
     return RAD_OK;
 }
 

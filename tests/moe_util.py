@@ -50,13 +50,13 @@ def choose(logits, top_k, score="softmax", renorm=1, weight_scale=1.0):
 
 
 def exact(x, logits, gate_up, down, dtype, f, top_k, gate_up_scale=None, down_scale=None, act="silu", score="softmax",
-          renorm=1, weight_scale=1.0, split=False):
+          renorm=1, weight_scale=1.0, parts=2):
     """(ids, weights, weights' relative tolerance, y, y's tolerance but for its own rounding).
 
     Sums of exact products as in epi_util.exact: K / 32 + 64 roundings of at most a step of sum |w x|.  h = act(g) u w
-    passes the errors of its three factors on and takes three roundings.  Then it is rounded to bf16, as the formula
-    here does it too: where h's error lets it fall to either of two neighbours, their distance is the tolerance; or
-    split in two bf16 numbers (2^-16).  y is the sum over the top_k f terms."""
+    passes the errors of its three factors on and takes three roundings.  Then it is kept as the sum of two bf16
+    numbers (2^-16 of it) where y is bf16, of three (2^-24) where y is f32.  y is the sum over the choices of sums of
+    parts * f / 32 results."""
     dev = x.device
     ids, weights, rel = choose(logits.cpu(), top_k, score, renorm, weight_scale)
     y = torch.zeros(x.shape, dtype=torch.float64, device=dev)
@@ -75,17 +75,12 @@ def exact(x, logits, gate_up, down, dtype, f, top_k, gate_up_scale=None, down_sc
         ea = 1.13 * eu[:, :f] + 16 * U * g.abs().clamp_min(1.0 if act == "sigmoid" else 0.0)
         h = a * u * w
         eh = ((u * w).abs() * ea + (a * w).abs() * eu[:, f:] + (a * u).abs() * ew) * 1.01 + 4 * U * h.abs()
-        if split:
-            eh = eh + 2.0 ** -16 * h.abs() + 2.0 ** -133
-        else:
-            lo, hi = (h - eh).float().bfloat16().double(), (h + eh).float().bfloat16().double()
-            h = h.float().bfloat16().double()
-            eh = hi - lo
+        eh = eh + 2.0 ** (-8 * parts) * h.abs() + 2.0 ** -133
         D = plane(down[e], None if down_scale is None else down_scale[e], dtype)
         y.index_add_(0, m, h @ D.T)
         err.index_add_(0, m, eh @ D.abs().T)
         size.index_add_(0, m, h.abs() @ D.abs().T)
-    err = err + (top_k * f / 32 + 80) * 2.0 ** -23 * size
+    err = err + (parts * f / 32 + 64 + top_k) * 2.0 ** -23 * size
     return ids, weights, rel, y, err
 
 

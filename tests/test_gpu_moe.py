@@ -61,7 +61,7 @@ def run(dev, dtype, M, n, f, E, k, y="bf16", seed=0, logits=None, extra=0, pad=0
     assert R.launch_row("moe_layer", ops, torch.cuda.current_stream().cuda_stream) == R.RAD_OK
     torch.cuda.synchronize()
     on = {m: None if v is None else v.to(dev) for m, v in t.items()}
-    want = U.exact(**on, dtype=dtype, f=f, top_k=k, split=y == "f32", **par)
+    want = U.exact(**on, dtype=dtype, f=f, top_k=k, parts=3 if y == "f32" else 2, **par)
     use = U.check((Y.t, I.t, W.t), want)
     assert all(b.around() for b in (X, Y, I, W, L, S))
     return use
@@ -177,7 +177,7 @@ def test_scales_at_their_ends(gpu):
     on = {m: None if v is None else v.to(gpu) for m, v in t.items()}
     y = torch.empty(3, 64, device=gpu)
     assert R.moe_layer(y=y, dtype="mxfp4", n=64, f=32, E=2, top_k=1, **on) == R.RAD_OK
-    _, _, _, want, err = U.exact(**on, dtype="mxfp4", f=32, top_k=1, split=True)
+    _, _, _, want, err = U.exact(**on, dtype="mxfp4", f=32, top_k=1, parts=3)
     rest = [i for i in range(64) if i not in (6, 7)]
     U.E.check(y[:, rest], want[:, rest], err[:, rest])
     assert y[:, 6].isnan().all() and not y[:, 7].isfinite().any()
@@ -186,7 +186,7 @@ def test_scales_at_their_ends(gpu):
     t["down_scale"][0, 5], t["down_scale"][0, 6], t["down_scale"][0, 7] = 0.0, float("nan"), float("inf")
     on = {m: None if v is None else v.to(gpu) for m, v in t.items()}
     assert R.moe_layer(y=y, dtype="i8", n=64, f=32, E=2, top_k=1, **on) == R.RAD_OK
-    _, _, _, want, err = U.exact(**on, dtype="i8", f=32, top_k=1, split=True)
+    _, _, _, want, err = U.exact(**on, dtype="i8", f=32, top_k=1, parts=3)
     U.E.check(y[:, rest], want[:, rest], err[:, rest])
     assert y[:, 6].isnan().all() and not y[:, 7].isfinite().any()
 
@@ -201,11 +201,11 @@ def test_tokens_do_not_meet(gpu):
     t["x"][7, 100], t["x"][2, 255] = float("nan"), float("inf")
     t["gate_up"][5, 3, 9], t["down"][5, 200, 0] = float("nan"), float("inf")
     on = {m: None if v is None else v.to(gpu) for m, v in t.items()}
-    for kind, split in ((torch.float32, True), (torch.bfloat16, False)):
+    for kind, parts in ((torch.float32, 3), (torch.bfloat16, 2)):
         y = torch.empty(M, n, dtype=kind, device=gpu)
         assert R.moe_layer(y=y, dtype="bf16", n=n, f=f, E=E, top_k=2, **on) == R.RAD_OK
         rows = [m for m in range(M) if m not in (2, 4, 7)]
-        _, _, _, want, err = U.exact(**on, dtype="bf16", f=f, top_k=2, split=split)
+        _, _, _, want, err = U.exact(**on, dtype="bf16", f=f, top_k=2, parts=parts)
         U.E.check(y[rows], want[rows], err[rows])
         assert y[7].isnan().all() and not y[2].isfinite().any() and not y[4].isfinite().any()
 
@@ -223,7 +223,7 @@ def test_streams_and_graph(gpu):
             ops = R.MoeLayerOperands(y=y, ids=ids, weights=w, dtype=dtype, n=n, f=f, E=E, top_k=k, **on)
             ops.set_scratch(torch.full((R.row_scratch_bytes("moe_layer", ops),), 0xA5, dtype=torch.uint8, device=gpu))
             return y, ids, w, ops
-        want = U.exact(**on, dtype=dtype, f=f, top_k=k, split=True)
+        want = U.exact(**on, dtype=dtype, f=f, top_k=k, parts=3)
         two = [(torch.cuda.Stream(), bound()) for _ in range(2)]
         torch.cuda.synchronize()
         for s, b in two:
@@ -242,7 +242,7 @@ def test_streams_and_graph(gpu):
             y.fill_(-1)
             graph.replay()
             torch.cuda.synchronize()
-            U.check((y, ids, w), U.exact(**on, dtype=dtype, f=f, top_k=k, split=True))
+            U.check((y, ids, w), U.exact(**on, dtype=dtype, f=f, top_k=k, parts=3))
             again = torch.zeros_like(y)
             assert R.moe_layer(y=again, dtype=dtype, n=n, f=f, E=E, top_k=k, **on) == R.RAD_OK
             torch.cuda.synchronize()
