@@ -2,8 +2,8 @@
  *
  * Few tokens choose among many experts, so the chosen experts' planes are the work: each is to be read once, and
  * HBM bounds it.  A wave takes 8 rows of a plane as i8_gemv_kernel does (r3d_i8_gemv.h): a 16-byte load a lane
- * brings a 128-byte line of each, and v_mfma_f32_16x16x32_bf16 is fed with (row i % 8, pieces of parity i / 8)
- * against (token j % 8, parity j / 8), of whose 16 x 16 results those with i / 8 = j / 8 are wanted.  Codes become
+ * brings a 128-byte line of each, and v_mfma_f32_16x16x32_bf16 is fed with (row i / 2, pieces of parity i % 2)
+ * against (token j / 2, parity j % 2), of whose 16 x 16 results those with i % 2 = j % 2 are wanted.  Codes become
  * bf16 in registers: int8 and e2m1 with its E8M0 scale are exact there (E8M0 0 is 2^-127, 255 NaN, and what leaves
  * bf16's range infinite), so the sums are f32 sums of exact products.
  *
@@ -232,13 +232,13 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
 
 /* ------------------------------------------------------------------------------ products */
 
-/* The sum of a result's two halves, (0, 0) and (1, 1), 40 lanes apart: lanes 0-7 and 16-23 then hold rows
- * 4 (lane / 16) .. + 3 of column lane % 8. */
-__device__ __forceinline__ r3d_f32x4 moe_halves(r3d_f32x4 a) {
-    const int from = ((threadIdx.x & 63) + 40) & 63;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] += __shfl(a[i], from, 64);
-    return a;
+/* Of a 16 x 16 result, whose lane (i / 4, j) holds rows i .. i + 3: the sum of both parities of row 2 (lane / 16) + lane % 2
+ * and token lane / 2 % 8, one value a lane.  The even lane of a pair has wanted values in elements 0 and 2, the odd one
+ * in 1 and 3; each sends the other's. */
+__device__ __forceinline__ float moe_value(r3d_f32x4 a) {
+    const bool odd = threadIdx.x & 1;
+    const float send = odd ? a[1] : a[2], keep = odd ? a[3] : a[0];
+    return keep + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(send), 0xB1, 15, 15, true));
 }
 
 /* LDS that a row of K columns in XH parts takes: whole 1 KB loads, and 16 bytes off a multiple of 128 so that
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         uint32_t job[kMoeMaxPairs];
     };
     __shared__ typename std::conditional<UP, MoeChoice, Jobs>::type S;
-    __shared__ r3d_f32x4 s_part[kMoeWaves][2][2][CT][16];            /* a wave's last unit and its first, where shared */
+    __shared__ float s_part[kMoeWaves][2][2][CT][64];            /* a wave's last unit and its first, where shared */
     __shared__ __attribute__((aligned(16))) float s_scale[ENC == MOE_I8 ? kMoeUnits * 16 : 1];
     extern __shared__ __attribute__((aligned(16))) uint8_t s_x[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -265,9 +265,8 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         S.job[tid] = P.table->job[tid];                              /* what lies past the jobs is not used */
         __syncthreads();
     }
-    const int r8 = lane & 7, piece = ((lane >> 3) & 1) | ((lane >> 4) << 1);
-    const bool mine = lane < 32 && !(lane & 8);                      /* holds results (moe_halves) */
-    const int row4 = 4 * ((lane >> 4) & 1);
+    const int r8 = (lane >> 1) & 7, piece = (lane & 1) | (lane >> 4) << 1;   /* row, or column, and 16-byte piece of a line */
+    const int row1 = piece;                                          /* row of the lane's result (moe_value) */
     const int nb = UP ? P.rows >> 3 : (P.rows + 15) >> 4;            /* units a job */
     const int pieces = P.K / N, lines = (pieces + 7) >> 3, cpr = (2 * P.K + 1023) >> 10;
     const int row_lds = moe_row(P.K, XH), part_lds = cpr * 1024;
@@ -321,15 +320,27 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         const int ua = i8_uniform(a / lines);
         int ll = a - ua * lines, lj = i8_uniform((u + ua) / nb), lb = u + ua - lj * nb;   /* where loads are */
         int cl = ll, cj = lj, cb = lb, cu = ua;                      /* where products are */
-        __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w, 0), rS = rW;
+        __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w, 0);
+        const uint8_t* s_base = P.ws;
         uint32_t w_at[2] = {0, 0}, s_at[2] = {0, 0};
         bool both = true;
+        /* A line's scales are 8 bytes of each row, a byte a lane; byte loads take the address unit a lane each, so
+         * a lane loads the four bytes that its own is of (at any alignment), or the plane's last four. */
+        const uint32_t s_row = (uint32_t)(r8 * P.ws_pitch), s_last = (uint32_t)s_plane - 4;
+        auto scale_at = [&](uint32_t at, int l) __attribute__((always_inline)) {
+            const uint32_t o = at + s_row + 8 * l + (piece & 4);
+            return o < s_last ? o : s_last;
+        };
+        auto scale_of = [&](uint32_t four, uint32_t at, int l) __attribute__((always_inline)) {
+            const uint32_t o = at + s_row + 8 * l + piece;           /* past the row: 2^-127 of its zeros, not the next row's */
+            return 8 * l + piece < pieces ? (four >> (8 * (o - scale_at(at, l)) & 31)) & 0xFFu : 0u;
+        };
         auto load = [&](Line& st, int s) __attribute__((always_inline)) {
             const bool run = s < b;
             if (run && (ll == 0 || s == a)) {                        /* a unit's first line here */
                 const int64_t e = i8_uniform(S.job[lj]) & 511;
                 rW = r3d_rsrc(P.w + e * P.w_expert, plane);
-                if (ENC == MOE_FP4) rS = r3d_rsrc(P.ws + e * P.ws_expert, s_plane);
+                if (ENC == MOE_FP4) s_base = P.ws + e * P.ws_expert;
                 const uint32_t r0 = (UP ? 8 : 16) * lb, r1 = UP ? r0 + P.rows : r0 + 8;
                 both = UP || (int)r1 < P.rows;
                 w_at[0] = r0 * (uint32_t)P.w_pitch;
@@ -338,13 +349,15 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 s_at[1] = r1 * (uint32_t)P.ws_pitch;
             }
             const bool in = run && 8 * ll + piece < pieces;
-            const uint32_t wo = (uint32_t)(r8 * P.w_pitch + 16 * piece), so = (uint32_t)(r8 * P.ws_pitch + piece);
+            const uint32_t wo = (uint32_t)(r8 * P.w_pitch + 16 * piece);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const bool ok = in && (r == 0 || both);
                 st.w[r] = i8_buf16<2>(rW, ok ? wo : kI8Oob, w_at[r] + 128 * ll);
-                if (ENC == MOE_FP4)
-                    st.s[r] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rS, (int)(ok ? so : kI8Oob), (int)(s_at[r] + 8 * ll), 0);
+                if (ENC == MOE_FP4) {
+                    typedef uint32_t u32_u1 __attribute__((aligned(1)));
+                    st.s[r] = *reinterpret_cast<const u32_u1*>(s_base + scale_at(s_at[r], ll));
+                }
             }
             if (++ll == lines) {
                 ll = 0;
@@ -372,44 +385,39 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 xa[t] = (slot0 - slot_base + (8 * t + r8 < cnt ? 8 * t + r8 : 0)) * row_lds + 16 * X * piece;
         };
         if (a < b) job_of(cj);
+        uint32_t c_at[2] = {(uint32_t)((UP ? 8 : 16) * cb) * (uint32_t)P.ws_pitch, 0};
+        c_at[1] = c_at[0] + (uint32_t)(UP ? P.rows : 8) * (uint32_t)P.ws_pitch;
         r3d_f32x4 acc[2][CT];
         auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < CT; ++t) acc[0][t] = acc[1][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         };
-        /* a whole unit's results, on the lanes that hold them */
-        auto finish = [&](int un, int blk) __attribute__((always_inline)) {
+        /* a whole unit's results */
+        auto finish = [&](int un, int blk, const float (&val)[2][CT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
                 const int col = 8 * t + r8;
-                if (!mine || col >= cnt) continue;
-                const int64_t slot = slot0 + col;
-                r3d_f32x4 v[2] = {acc[0][t], acc[1][t]};
+                const int64_t slot = slot0 + (col < cnt ? col : 0);
+                float v[2] = {val[0][t], val[1][t]};
                 if constexpr (ENC == MOE_I8) {
-                    v[0] *= *reinterpret_cast<const r3d_f32x4*>(&s_scale[16 * un + row4]);
-                    v[1] *= *reinterpret_cast<const r3d_f32x4*>(&s_scale[16 * un + 8 + row4]);
+                    v[0] *= s_scale[16 * un + row1];
+                    v[1] *= s_scale[16 * un + 8 + row1];
                 }
                 if constexpr (UP) {
-                    float h[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
-                    act_values<4>(P.act, h);
-                    const float wt = S.slot_w[slot];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) h[i] = h[i] * v[1][i] * wt;
-                    uint16_t* to = static_cast<uint16_t*>(P.out) + slot * P.rows + 8 * blk + row4;
+                    act_values<1>(P.act, v);
+                    float h = v[0] * v[1] * S.slot_w[slot];
+                    uint16_t* const to = static_cast<uint16_t*>(P.out) + slot * P.rows + 8 * blk + row1;
                     for (int p = 0; p < P.parts; ++p) {
-                        const uint32_t h0 = r3d_pack_bf16x2(h[0], h[1]), h1 = r3d_pack_bf16x2(h[2], h[3]);
-                        *reinterpret_cast<uint2*>(to + (int64_t)p * P.pairs * P.rows) = make_uint2(h0, h1);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {                /* what is left of it; nothing of inf and NaN */
-                            const uint32_t d = i < 2 ? h0 : h1;
-                            const float hi = __uint_as_float(i & 1 ? d & 0xFFFF0000u : d << 16);
-                            h[i] = __builtin_fabsf(hi) < __builtin_inff() ? h[i] - hi : 0.0f;
-                        }
+                        const float other = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(h), 0xB1, 15, 15, true));
+                        const uint32_t d = r3d_pack_bf16x2(h, other);
+                        if (!(lane & 1) && col < cnt) *reinterpret_cast<uint32_t*>(to + (int64_t)p * P.pairs * P.rows) = d;
+                        const float hi = __uint_as_float(d << 16);   /* what is left of h; nothing of inf and NaN */
+                        h = __builtin_fabsf(hi) < __builtin_inff() ? h - hi : 0.0f;
                     }
-                } else {
-                    float* const to = static_cast<float*>(P.out) + slot * P.rows + 16 * blk + row4;
-                    *reinterpret_cast<r3d_f32x4*>(to) = v[0];
-                    if (16 * blk + 8 < P.rows) *reinterpret_cast<r3d_f32x4*>(to + 8) = v[1];
+                } else if (col < cnt) {
+                    float* const to = static_cast<float*>(P.out) + slot * P.rows + 16 * blk + row1;
+                    to[0] = v[0];
+                    if (16 * blk + 8 < P.rows) to[8] = v[1];
                 }
             }
         };
@@ -420,8 +428,8 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
             for (int d = 0; d < D; ++d) {
                 if (s + d < b) {
                     r3d_i32x4 w0[X], w1[X];
-                    moe_bf16<ENC>(ring[d].w[0], ring[d].s[0], w0);
-                    moe_bf16<ENC>(ring[d].w[1], ring[d].s[1], w1);
+                    moe_bf16<ENC>(ring[d].w[0], ENC == MOE_FP4 ? scale_of(ring[d].s[0], c_at[0], cl) : 0, w0);
+                    moe_bf16<ENC>(ring[d].w[1], ENC == MOE_FP4 ? scale_of(ring[d].s[1], c_at[1], cl) : 0, w1);
 #pragma unroll
                     for (int t = 0; t < CT; ++t)
 #pragma unroll
@@ -432,18 +440,19 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                             acc[1][t] = moe_mfma(w1[i % X], x, acc[1][t]);
                         }
                     if (++cl == lines || s + d + 1 == b) {           /* the unit's end, or the run's */
+                        float val[2][CT];
 #pragma unroll
                         for (int t = 0; t < CT; ++t) {
-                            acc[0][t] = moe_halves(acc[0][t]);
-                            acc[1][t] = moe_halves(acc[1][t]);
+                            val[0][t] = moe_value(acc[0][t]);
+                            val[1][t] = moe_value(acc[1][t]);
                         }
                         if (whole && cl == lines) {
-                            finish(cu, cb);
-                        } else if (mine) {
+                            finish(cu, cb, val);
+                        } else {
 #pragma unroll
                             for (int t = 0; t < CT; ++t)
 #pragma unroll
-                                for (int r = 0; r < 2; ++r) s_part[wave][whole ? 0 : 1][r][t][2 * row4 + r8] = acc[r][t];
+                                for (int r = 0; r < 2; ++r) s_part[wave][whole ? 0 : 1][r][t][lane] = val[r][t];
                         }
                         if (cl == lines) {
                             clear();
@@ -453,6 +462,10 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                             if (++cb == nb) {
                                 cb = 0;
                                 if (s + d + 1 < b) job_of(++cj);
+                            }
+                            if (ENC == MOE_FP4) {
+                                c_at[0] = (uint32_t)((UP ? 8 : 16) * cb) * (uint32_t)P.ws_pitch;
+                                c_at[1] = c_at[0] + (uint32_t)(UP ? P.rows : 8) * (uint32_t)P.ws_pitch;
                             }
                         }
                     }
@@ -464,19 +477,20 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         __syncthreads();
         if (a < b && cl > 0 && whole) {                              /* begun here, ended by the waves after */
             const int stop = (cu + 1) * lines;
+            float val[2][CT];
 #pragma unroll
             for (int t = 0; t < CT; ++t)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    r3d_f32x4 v = s_part[wave][0][r][t][(2 * row4 + r8) & 15];
+                    float v = s_part[wave][0][r][t][lane];
                     for (int o = wave + 1; o < kMoeWaves; ++o) {
                         const int ao = (int)(total * o / kMoeWaves);
                         if (ao >= stop) break;
-                        if (ao < (int)(total * (o + 1) / kMoeWaves)) v += s_part[o][1][r][t][(2 * row4 + r8) & 15];
+                        if (ao < (int)(total * (o + 1) / kMoeWaves)) v += s_part[o][1][r][t][lane];
                     }
-                    acc[r][t] = v;
+                    val[r][t] = v;
                 }
-            finish(cu, cb);
+            finish(cu, cb, val);
         }
         u = end;
         if (u < u_end) __syncthreads();                              /* the scales are read */
