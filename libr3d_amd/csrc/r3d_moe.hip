@@ -36,20 +36,32 @@
 
 namespace r3d {
 
+/* u / d for a d that the host knows (any u, d >= 1), without the forty instructions of a division */
+struct MoeDiv {
+    uint32_t d, m;                      /* m = (2^32 - 1) / d, rounded down: the quotient is short by one at most */
+    __device__ __forceinline__ uint32_t of(uint32_t u) const {
+        const uint32_t q = __umulhi(u, m);
+        return q + (u - q * d >= d ? 1u : 0u);
+    }
+};
+
 struct MoeArgs {
+    MoeTable* table;
+    const uint8_t* logits;              /* up: null for down */
+    int64_t l_pitch;
+    int M, E, top_k, l_bf16, K, rows, pairs, x_pitch;    /* K columns of `rows` rows (gate rows, or rows of y) */
     const uint8_t* x;                   /* up: the tokens; down: h */
     const uint8_t* w;
     const uint8_t* ws;
-    MoeTable* table;
     void* out;                          /* up: h, bf16 [parts][pairs][f]; down: sums, f32 [pairs][n] */
-    int M, K, rows, pairs, x_pitch, w_pitch, job_rows;   /* K columns of `rows` rows (gate rows, or rows of y) */
     int64_t w_expert, ws_expert, ws_pitch;
+    int w_pitch, job_rows, lines, cpr;  /* 128-byte lines a row of the plane, 1 KB loads a part of a token's row */
+    MoeDiv unit, line, grid, choice;    /* by units a job, lines, workgroups, top_k */
     /* up */
-    const uint8_t* logits;
     int32_t* ids;
     float* weights;
-    int64_t l_pitch, i_pitch, wt_pitch;
-    int E, top_k, width, parts, act, sigmoid, renorm, l_bf16;
+    int64_t i_pitch, wt_pitch;
+    int width, parts, act, sigmoid, renorm;
     float weight_scale;
 };
 
@@ -94,7 +106,6 @@ constexpr int kMoeUnits = 128;          /* units whose scales lie in LDS at a ti
 
 struct MoeChoice {                      /* in LDS, the same in every workgroup */
     uint64_t mask[kMoeMaxE];            /* an expert's tokens */
-    uint64_t scan[kMoeWaves];
     float w[kMoeMaxPairs];              /* by (token, choice) */
     float slot_w[kMoeMaxPairs];         /* by slot */
     uint32_t job[kMoeMaxPairs];
@@ -112,13 +123,23 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t
     const int lane = threadIdx.x & 63;
     float v[J];
     uint32_t key[J];
+    if (P.l_bf16) {
+        const uint16_t* const row = reinterpret_cast<const uint16_t*>(P.logits) + t * P.l_pitch;
+        uint32_t raw[J];                                         /* every load before a use of one */
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            raw[j] = 0xFF80u;
+            if (J * lane + j < P.E) raw[j] = row[J * lane + j];
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) v[j] = __uint_as_float(raw[j] << 16);
+    } else {
+        const float* const row = reinterpret_cast<const float*>(P.logits) + t * P.l_pitch;
+#pragma unroll
+        for (int j = 0; j < J; ++j) v[j] = J * lane + j < P.E ? row[J * lane + j] : -__builtin_inff();
+    }
 #pragma unroll
     for (int j = 0; j < J; ++j) {
-        const int e = J * lane + j;
-        v[j] = -__builtin_inff();
-        if (e < P.E)
-            v[j] = P.l_bf16 ? r3d_bf16_to_f32(reinterpret_cast<const uint16_t*>(P.logits)[t * P.l_pitch + e])
-                            : reinterpret_cast<const float*>(P.logits)[t * P.l_pitch + e];
         const uint32_t u = __float_as_uint(v[j] + 0.0f);                 /* -0 is 0 */
         key[j] = v[j] > -__builtin_inff() ? u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u) : 0u;
     }
@@ -172,6 +193,7 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t
     if (lane < P.top_k) {
         S.id[t * P.top_k + lane] = (int16_t)id;
         S.w[t * P.top_k + lane] = there ? p / total * P.weight_scale : 0.0f;
+        if (there) atomicOr(reinterpret_cast<unsigned long long*>(&S.mask[id]), 1ull << t);
     }
 }
 
@@ -179,6 +201,7 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t
 __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid < kMoeMaxE) S.mask[tid] = 0;
+    __syncthreads();
     for (int t = wave; t < P.M; t += kMoeWaves) {
         if (P.E <= 64) moe_choose<1>(P, S, t);
         else if (P.E <= 128) moe_choose<2>(P, S, t);
@@ -186,31 +209,31 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
         else moe_choose<8>(P, S, t);
     }
     __syncthreads();
-    /* a lane a (token, choice) from here on, and an expert */
-    const int t = tid < P.pairs ? tid / P.top_k : 0, e = tid < P.pairs ? S.id[tid] : -1;
-    if (e >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&S.mask[e]), 1ull << t);
-    __syncthreads();
-    const int cnt = tid < kMoeMaxE ? __popcll(S.mask[tid]) : 0, nj = (cnt + P.width - 1) / P.width;
-    const uint64_t own = (uint64_t)nj << 32 | (uint32_t)cnt;         /* slots and jobs before an expert's */
-    uint64_t upto = r3d_wave_scan(own);
-    if (lane == 63) S.scan[wave] = upto;
-    __syncthreads();
-    uint64_t all = 0;
+    if (wave == 0) {                                             /* a lane eight experts: slots and jobs before each */
+        uint32_t cnt[8], nj[8];
+        uint64_t own = 0;
 #pragma unroll
-    for (int i = 0; i < kMoeMaxE / 64; ++i) {
-        if (i == wave) upto += all;
-        all += S.scan[i];
-    }
-    if (tid < kMoeMaxE) {
-        const int slot = (int)(uint32_t)(upto - own), j0 = (int)((upto - own) >> 32);
-        S.first[tid] = (uint16_t)slot;
-        for (int j = 0; j < nj; ++j) {
-            const int left = cnt - P.width * j;
-            S.job[j0 + j] = (uint32_t)tid | (uint32_t)(slot + P.width * j) << 9 | (uint32_t)(left < P.width ? left : P.width) << 20;
+        for (int i = 0; i < 8; ++i) {
+            cnt[i] = __popcll(S.mask[8 * lane + i]);
+            nj[i] = cnt[i] <= (uint32_t)P.width ? (cnt[i] > 0) : (cnt[i] + P.width - 1) / P.width;
+            own += (uint64_t)nj[i] << 32 | cnt[i];
+        }
+        const uint64_t upto = r3d_wave_scan(own);
+        uint32_t slot = (uint32_t)(upto - own), j = (uint32_t)((upto - own) >> 32);
+        if (lane == 63) S.jobs = (int)(upto >> 32);
+        for (int i = 0; i < 8; ++i) {
+            S.first[8 * lane + i] = (uint16_t)slot;
+            for (uint32_t left = cnt[i]; left > 0; ++j) {
+                const uint32_t n = left < (uint32_t)P.width ? left : P.width;
+                S.job[j] = (uint32_t)(8 * lane + i) | (slot + cnt[i] - left) << 9 | n << 20;
+                left -= n;
+            }
+            slot += cnt[i];
         }
     }
-    if (tid == 0) S.jobs = (int)(all >> 32);
     __syncthreads();
+    /* a lane a (token, choice) */
+    const int t = tid < P.pairs ? (int)P.choice.of(tid) : 0, e = tid < P.pairs ? S.id[tid] : -1;
     int slot = -1;
     if (e >= 0) {
         slot = S.first[e] + __popcll(S.mask[e] & ((1ull << t) - 1));
@@ -247,7 +270,8 @@ constexpr int moe_row(int64_t K, int parts) { return (int)(parts * ((2 * K + 102
 
 template <int ENC, int CT, int XH, bool UP>
 __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
-    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X, D = 4;
+    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X;
+    constexpr int L = ENC == MOE_FP4 ? 4 : 1, D = ENC == MOE_FP4 ? 2 : 4;   /* lines a step, steps in flight */
     struct Jobs {
         uint32_t job[kMoeMaxPairs];
     };
@@ -258,31 +282,34 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int jobs;
     if constexpr (UP) {
+        /* the arguments' loads go out here, beside the logits', and not where each is first used */
+        asm volatile("" ::"s"(P.x), "s"(P.w), "s"(P.ws), "s"(P.w_expert), "s"(P.w_pitch), "s"(P.line.m), "s"(P.choice.m));
         moe_plan(P, S);
         jobs = i8_uniform(S.jobs);
     } else {
+        const uint32_t job = P.table->job[tid];                      /* what lies past the jobs is not used */
         jobs = P.table->jobs;
-        S.job[tid] = P.table->job[tid];                              /* what lies past the jobs is not used */
+        asm volatile("" ::"s"(P.x), "s"(P.w), "s"(P.ws), "s"(P.w_expert), "s"(P.w_pitch), "s"(P.line.m), "s"(P.grid.m));
+        S.job[tid] = job;
         __syncthreads();
     }
     const int r8 = (lane >> 1) & 7, piece = (lane & 1) | (lane >> 4) << 1;   /* row, or column, and 16-byte piece of a line */
     const int row1 = piece;                                          /* row of the lane's result (moe_value) */
-    const int nb = UP ? P.rows >> 3 : (P.rows + 15) >> 4;            /* units a job */
-    const int pieces = P.K / N, lines = (pieces + 7) >> 3, cpr = (2 * P.K + 1023) >> 10;
-    const int row_lds = moe_row(P.K, XH), part_lds = cpr * 1024;
+    const int nb = P.unit.d, lines = P.lines, pieces = P.K / N;      /* units a job */
+    const int part_lds = P.cpr * 1024, row_lds = XH * part_lds + 16;
     /* a run an XCD, so that its L2 sees few jobs' tokens */
-    const int G = gridDim.x, per = G >> 3, rem = G & 7, xcd = blockIdx.x & 7;
-    const int g = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
-    const int64_t units = (int64_t)jobs * nb;
-    const int u_end = i8_uniform((int)(units * (g + 1) / G));
+    const uint32_t G = P.grid.d, per = G >> 3, rem = G & 7, xcd = blockIdx.x & 7;
+    const uint32_t g = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
+    const uint32_t units = (uint32_t)jobs * nb;                      /* times G under 2^32: moe_geom */
+    const int u_end = i8_uniform((int)P.grid.of(units * (g + 1)));
     const int64_t x_rows = UP ? P.M : P.pairs;
     const int64_t x_bytes = (x_rows - 1) * P.x_pitch + 2 * (int64_t)P.K;
     const int64_t plane = (int64_t)((UP ? 2 * P.rows : P.rows) - 1) * P.w_pitch + (int64_t)pieces * 16;
     const int64_t s_plane = (int64_t)((UP ? 2 * P.rows : P.rows) - 1) * P.ws_pitch + pieces;
 
-    for (int u = i8_uniform((int)(units * g / G)); u < u_end;) {
+    for (int u = i8_uniform((int)P.grid.of(units * g)); u < u_end;) {
         /* as many units of the run as LDS holds the tokens (and the scales) of */
-        const int j0 = i8_uniform(u / nb), slot_base = i8_uniform((S.job[j0] >> 9) & 2047);
+        const int j0 = i8_uniform((int)P.unit.of(u)), slot_base = i8_uniform((S.job[j0] >> 9) & 2047);
         int end = u, held = 0;
         for (int j = j0; end < u_end && end - u < (ENC == MOE_I8 ? kMoeUnits : 1 << 30); ++j) {
             const uint32_t job = i8_uniform(S.job[j]);
@@ -292,52 +319,38 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
             end = (j + 1) * nb < u_end ? (j + 1) * nb : u_end;
         }
         if (ENC == MOE_I8 && end - u > kMoeUnits) end = u + kMoeUnits;
-        for (int c = wave; c < held * XH * cpr; c += kMoeWaves) {
-            const int r = i8_uniform(c / (XH * cpr)), rest = c - r * XH * cpr, p = i8_uniform(rest / cpr), k = rest - p * cpr;
-            const __amdgpu_buffer_rsrc_t rX = r3d_rsrc(P.x + p * (x_rows * P.x_pitch), x_bytes);
-            int row;
-            if constexpr (UP) row = i8_uniform(S.tok[slot_base + r]);
-            else row = slot_base + r;
-            const uint32_t at = 1024 * k + 16 * lane;                /* past the row's end: zeros */
-            r3d_buf_lds<16>(rX, s_x + r * row_lds + p * part_lds + 1024 * k,
-                            at < 2 * (uint32_t)P.K ? (uint32_t)row * (uint32_t)P.x_pitch + at : kI8Oob, 0);
-        }
         if constexpr (ENC == MOE_I8) {
             for (int i = tid; i < 16 * (end - u); i += kMoeThreads) {
-                const int un = u + (i >> 4), j = un / nb, blk = un - j * nb, r = i & 15;
+                const int un = u + (i >> 4), j = P.unit.of(un), blk = un - j * nb, r = i & 15;
                 int row = UP ? (r >> 3) * P.rows + 8 * blk + (r & 7) : 16 * blk + r;
                 if (!UP && row >= P.rows) row = P.rows - 1;
                 s_scale[i] = reinterpret_cast<const float*>(P.ws)[(int64_t)(S.job[j] & 511) * P.ws_expert + row];
             }
         }
-        /* this wave's lines */
-        const int64_t total = (int64_t)(end - u) * lines;
-        const int a = i8_uniform((int)(total * wave / kMoeWaves)), b = i8_uniform((int)(total * (wave + 1) / kMoeWaves));
-        struct Line {
-            r3d_i32x4 w[2];
-            uint32_t s[2];                                           /* e2m1: the pieces' scales */
+        /* this wave's lines, L a step and a unit's last ones fewer */
+        const int total = (end - u) * lines;                         /* times 16 under 2^31: moe_geom */
+        const int a = i8_uniform(total * wave / kMoeWaves), b = i8_uniform(total * (wave + 1) / kMoeWaves);
+        int tokens = 0;                                              /* of the rows to be held, a lane each */
+        if constexpr (UP) tokens = lane < held ? S.tok[slot_base + lane] : 0;
+        struct Step {
+            r3d_i32x4 w[L][2];
+            uint32_t s[2];                                           /* e2m1: four scales of the row's 32, the piece's number's */
         } ring[D];
-        const int ua = i8_uniform(a / lines);
-        int ll = a - ua * lines, lj = i8_uniform((u + ua) / nb), lb = u + ua - lj * nb;   /* where loads are */
-        int cl = ll, cj = lj, cb = lb, cu = ua;                      /* where products are */
+        const int ua = i8_uniform((int)P.line.of(a));
+        int ll = a - ua * lines, lj = i8_uniform((int)P.unit.of(u + ua)), lb = u + ua - lj * nb, left = b - a;   /* where loads are */
+        int cl = ll, cj = lj, cb = lb, cu = ua, todo = left;         /* where products are */
         __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w, 0);
         const uint8_t* s_base = P.ws;
         uint32_t w_at[2] = {0, 0}, s_at[2] = {0, 0};
-        bool both = true;
-        /* A line's scales are 8 bytes of each row, a byte a lane; byte loads take the address unit a lane each, so
-         * a lane loads the four bytes that its own is of (at any alignment), or the plane's last four. */
+        bool both = true, entered = false;
+        /* A line's scales are 8 bytes of each row, a byte a lane.  Loads of a byte a lane from 8 rows a line fetch the
+         * rows' lines anew each time (the stream has long left the L1), so a step loads its 32 bytes at once, four a lane at
+         * any alignment, the plane's last four in place of some that lie past it; a lane's byte is then another lane's. */
         const uint32_t s_row = (uint32_t)(r8 * P.ws_pitch), s_last = (uint32_t)s_plane - 4;
-        auto scale_at = [&](uint32_t at, int l) __attribute__((always_inline)) {
-            const uint32_t o = at + s_row + 8 * l + (piece & 4);
-            return o < s_last ? o : s_last;
-        };
-        auto scale_of = [&](uint32_t four, uint32_t at, int l) __attribute__((always_inline)) {
-            const uint32_t o = at + s_row + 8 * l + piece;           /* past the row: 2^-127 of its zeros, not the next row's */
-            return 8 * l + piece < pieces ? (four >> (8 * (o - scale_at(at, l)) & 31)) & 0xFFu : 0u;
-        };
-        auto load = [&](Line& st, int s) __attribute__((always_inline)) {
-            const bool run = s < b;
-            if (run && (ll == 0 || s == a)) {                        /* a unit's first line here */
+        auto load = [&](Step& st) __attribute__((always_inline)) {
+            const int n = left < lines - ll ? left : lines - ll;     /* 0: the wave's lines are done */
+            if (n > 0 && (ll == 0 || !entered)) {                    /* a unit's first line here */
+                entered = true;
                 const int64_t e = i8_uniform(S.job[lj]) & 511;
                 rW = r3d_rsrc(P.w + e * P.w_expert, plane);
                 if (ENC == MOE_FP4) s_base = P.ws + e * P.ws_expert;
@@ -348,18 +361,26 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 s_at[0] = r0 * (uint32_t)P.ws_pitch;
                 s_at[1] = r1 * (uint32_t)P.ws_pitch;
             }
-            const bool in = run && 8 * ll + piece < pieces;
             const uint32_t wo = (uint32_t)(r8 * P.w_pitch + 16 * piece);
+            if (ENC == MOE_FP4) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const bool ok = in && (r == 0 || both);
-                st.w[r] = i8_buf16<2>(rW, ok ? wo : kI8Oob, w_at[r] + 128 * ll);
-                if (ENC == MOE_FP4) {
+                for (int r = 0; r < 2; ++r) {
                     typedef uint32_t u32_u1 __attribute__((aligned(1)));
-                    st.s[r] = *reinterpret_cast<const u32_u1*>(s_base + scale_at(s_at[r], ll));
+                    const uint32_t o = s_at[r] + s_row + 8 * ll + 4 * piece;
+                    st.s[r] = *reinterpret_cast<const u32_u1*>(s_base + (o < s_last ? o : s_last));
                 }
             }
-            if (++ll == lines) {
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const bool in = i < n && 8 * (ll + i) + piece < pieces;
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    st.w[i][r] = i8_buf16<2>(rW, in && (r == 0 || both) ? wo : kI8Oob, w_at[r] + 128 * (ll + i));
+            }
+            const int m = n < L ? n : L;
+            left -= m;
+            ll += m;
+            if (ll == lines) {
                 ll = 0;
                 if (++lb == nb) {
                     lb = 0;
@@ -369,8 +390,30 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         };
 #pragma unroll
         for (int d = 0; d < D; ++d) {
-            load(ring[d], a + d);
-            __builtin_amdgcn_sched_barrier(0);                       /* in this order everywhere: a line waits for its own */
+            load(ring[d]);
+            __builtin_amdgcn_sched_barrier(0);                       /* in this order everywhere: a step waits for its own */
+        }
+        /* behind the weights' loads, and with no read of LDS among them, which would wait for them all */
+        for (int c = wave; c < XH * P.cpr; c += kMoeWaves) {         /* the tokens: 1 KB of a part of each row a turn */
+            int p = 0, k = c;
+            if (XH > 1 && k >= P.cpr) {
+                k -= P.cpr;
+                p = 1;
+            }
+            if (XH > 2 && k >= P.cpr) {
+                k -= P.cpr;
+                p = 2;
+            }
+            const __amdgpu_buffer_rsrc_t rX = r3d_rsrc(P.x + p * (x_rows * P.x_pitch), x_bytes);
+            const uint32_t at = 1024 * k + 16 * lane;                /* past the row's end: zeros */
+            const bool in = at < 2 * (uint32_t)P.K;
+            for (int r = 0; r < held; ++r) {
+                int row;
+                if constexpr (UP) row = __builtin_amdgcn_readlane(tokens, r & 63);
+                else row = slot_base + r;
+                r3d_buf_lds<16>(rX, s_x + r * row_lds + p * part_lds + 1024 * k,
+                                in ? (uint32_t)row * (uint32_t)P.x_pitch + at : kI8Oob, 0);
+            }
         }
         __syncthreads();
 
@@ -385,6 +428,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 xa[t] = (slot0 - slot_base + (8 * t + r8 < cnt ? 8 * t + r8 : 0)) * row_lds + 16 * X * piece;
         };
         if (a < b) job_of(cj);
+        const int s_from = 4 * ((lane >> 5) | r8 << 1);              /* plus 16 lanes a line */
         uint32_t c_at[2] = {(uint32_t)((UP ? 8 : 16) * cb) * (uint32_t)P.ws_pitch, 0};
         c_at[1] = c_at[0] + (uint32_t)(UP ? P.rows : 8) * (uint32_t)P.ws_pitch;
         r3d_f32x4 acc[2][CT];
@@ -423,23 +467,44 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         };
         clear();
         bool whole = cl == 0;                                        /* this wave has the unit from its first line on */
-        for (int s = a; s < b; s += D) {
+        while (todo > 0) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
-                if (s + d < b) {
-                    r3d_i32x4 w0[X], w1[X];
-                    moe_bf16<ENC>(ring[d].w[0], ENC == MOE_FP4 ? scale_of(ring[d].s[0], c_at[0], cl) : 0, w0);
-                    moe_bf16<ENC>(ring[d].w[1], ENC == MOE_FP4 ? scale_of(ring[d].s[1], c_at[1], cl) : 0, w1);
+                if (todo > 0) {
+                    int n = todo < lines - cl ? todo : lines - cl;
+                    n = n < L ? n : L;
 #pragma unroll
-                    for (int t = 0; t < CT; ++t)
+                    for (int i = 0; i < L; ++i) {
+                        if (i >= n) break;
+                        uint32_t scale[2] = {0, 0};
+                        if constexpr (ENC == MOE_FP4) {
 #pragma unroll
-                        for (int i = 0; i < XH * X; ++i) {
-                            const r3d_i32x4 x = *reinterpret_cast<const r3d_i32x4*>(
-                                s_x + xa[t] + i / X * part_lds + 128 * X * cl + 16 * (i % X));
-                            acc[0][t] = moe_mfma(w0[i % X], x, acc[0][t]);
-                            acc[1][t] = moe_mfma(w1[i % X], x, acc[1][t]);
+                            for (int r = 0; r < 2; ++r) {
+                                /* byte 8 i + piece of the step's, in the dword of piece 2 i + piece / 4 */
+                                const uint32_t four = (uint32_t)__builtin_amdgcn_ds_bpermute(s_from + 64 * i, (int)ring[d].s[r]);
+                                const uint32_t o = c_at[r] + s_row + 8 * (cl + i) + (piece & 4);
+                                const uint32_t back = o < s_last ? 0 : o - s_last;
+                                scale[r] = __builtin_amdgcn_ubfe(four, 8 * (back + (piece & 3)), 8);
+                                /* past the row: 2^-127 of its zeros, not the next row's */
+                                scale[r] = 8 * (cl + i) + piece < pieces ? scale[r] : 0u;
+                            }
                         }
-                    if (++cl == lines || s + d + 1 == b) {           /* the unit's end, or the run's */
+                        r3d_i32x4 w0[X], w1[X];
+                        moe_bf16<ENC>(ring[d].w[i][0], scale[0], w0);
+                        moe_bf16<ENC>(ring[d].w[i][1], scale[1], w1);
+#pragma unroll
+                        for (int t = 0; t < CT; ++t)
+#pragma unroll
+                            for (int k = 0; k < XH * X; ++k) {
+                                const r3d_i32x4 x = *reinterpret_cast<const r3d_i32x4*>(
+                                    s_x + xa[t] + k / X * part_lds + 128 * X * (cl + i) + 16 * (k % X));
+                                acc[0][t] = moe_mfma(w0[k % X], x, acc[0][t]);
+                                acc[1][t] = moe_mfma(w1[k % X], x, acc[1][t]);
+                            }
+                    }
+                    cl += n;
+                    todo -= n;
+                    if (cl == lines || todo == 0) {                  /* the unit's end, or the run's */
                         float val[2][CT];
 #pragma unroll
                         for (int t = 0; t < CT; ++t) {
@@ -461,7 +526,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                             ++cu;
                             if (++cb == nb) {
                                 cb = 0;
-                                if (s + d + 1 < b) job_of(++cj);
+                                if (todo > 0) job_of(++cj);
                             }
                             if (ENC == MOE_FP4) {
                                 c_at[0] = (uint32_t)((UP ? 8 : 16) * cb) * (uint32_t)P.ws_pitch;
@@ -470,7 +535,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                         }
                     }
                 }
-                load(ring[d], s + D + d);
+                load(ring[d]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -484,9 +549,9 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 for (int r = 0; r < 2; ++r) {
                     float v = s_part[wave][0][r][t][lane];
                     for (int o = wave + 1; o < kMoeWaves; ++o) {
-                        const int ao = (int)(total * o / kMoeWaves);
+                        const int ao = total * o / kMoeWaves;
                         if (ao >= stop) break;
-                        if (ao < (int)(total * (o + 1) / kMoeWaves)) v += s_part[o][1][r][t][lane];
+                        if (ao < total * (o + 1) / kMoeWaves) v += s_part[o][1][r][t][lane];
                     }
                     val[r][t] = v;
                 }
@@ -521,15 +586,20 @@ static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStre
     const int parts = P.y_bf16 ? 2 : 3;
     uint8_t* const h = reinterpret_cast<uint8_t*>(table + 1);
     float* const sums = reinterpret_cast<float*>(h + moe_h_bytes(P));
-    MoeArgs u{P.x, P.gu, P.gus, table, h, (int)P.M, (int)P.n, (int)P.f, (int)pairs, (int)P.x_pitch, (int)P.gu_pitch,
-              g.up_rows, P.gu_expert, P.gus_expert, P.gus_pitch, P.logits, P.ids, P.weights, P.l_pitch, P.i_pitch,
-              P.w_pitch, (int)P.E, (int)P.top_k, g.width, parts, P.act, P.sigmoid, P.renorm, P.l_bf16, P.weight_scale};
+    const auto div = [](int64_t d) { return MoeDiv{(uint32_t)d, (uint32_t)(0xFFFFFFFFu / (uint32_t)d)}; };
+    const auto lines = [](int64_t K) { return (K / MoeCodes<ENC>::N + 7) / 8; };
+    const auto loads = [](int64_t K) { return (int)((2 * K + 1023) / 1024); };
+    const MoeArgs u{table, P.logits, P.l_pitch, (int)P.M, (int)P.E, (int)P.top_k, P.l_bf16, (int)P.n, (int)P.f, (int)pairs,
+                    (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up_rows,
+                    (int)lines(P.n), loads(P.n), div(P.f / 8), div(lines(P.n)), div(g.blocks), div(P.top_k), P.ids, P.weights,
+                    P.i_pitch, P.w_pitch, g.width, parts, P.act, P.sigmoid, P.renorm, P.weight_scale};
     hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 1, true>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
                        (size_t)g.up_rows * moe_row(P.n, 1), stream, u);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) {
-        MoeArgs d{h, P.dn, P.dns, table, sums, (int)P.M, (int)P.f, (int)P.n, (int)pairs, (int)(2 * P.f), (int)P.dn_pitch,
-                  g.down_rows, P.dn_expert, P.dns_expert, P.dns_pitch};
+        const MoeArgs d{table, nullptr, 0, (int)P.M, (int)P.E, (int)P.top_k, 0, (int)P.f, (int)P.n, (int)pairs, (int)(2 * P.f),
+                        h, P.dn, P.dns, sums, P.dn_expert, P.dns_expert, P.dns_pitch, (int)P.dn_pitch, g.down_rows,
+                        (int)lines(P.f), loads(P.f), div((P.n + 15) / 16), div(lines(P.f)), div(g.blocks), div(P.top_k)};
         const size_t lds = (size_t)g.down_rows * moe_row(P.f, parts);
         const dim3 grid((unsigned)g.blocks), block(kMoeThreads);
         if (P.y_bf16) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 2, false>), grid, block, lds, stream, d);

@@ -157,8 +157,9 @@ bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
     const double read = (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
     g->ct = (double)pairs / read > 6 && moe_lds(P, 2, true) / up >= 16 && moe_lds(P, 2, false) / down >= 16 ? 2 : 1;
     int64_t ur = moe_lds(P, g->ct, true) / up, dr = moe_lds(P, g->ct, false) / down;
-    if (ur > pairs) ur = pairs;
-    if (dr > pairs) dr = pairs;
+    const int64_t most = pairs < 64 ? pairs : 64;               /* rows whose tokens lie in a wave's lanes */
+    if (ur > most) ur = most;
+    if (dr > most) dr = most;
     int64_t width = 8 * g->ct;
     if (width > ur) width = ur;
     if (width > dr) width = dr;
