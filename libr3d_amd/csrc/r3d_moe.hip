@@ -1,9 +1,12 @@
 /* r3d_moe.hip -- moe_layer on gfx950 (r3d_moe.h has the formulas): kernels and entry.
  *
  * Few tokens choose among many experts, so the chosen experts' planes are the work: each is to be read once, and
- * HBM bounds it.  A wave takes 8 rows of a plane as i8_gemv_kernel does (r3d_i8_gemv.h): a 16-byte load a lane
- * brings a 128-byte line of each, and v_mfma_f32_16x16x32_bf16 is fed with (row i / 2, pieces of parity i % 2)
- * against (token j / 2, parity j % 2), of whose 16 x 16 results those with i % 2 = j % 2 are wanted.  Codes become
+ * HBM bounds it.  A 16-byte load a lane brings a wave 256 bytes of 4 rows of a plane, a piece of 16 a
+ * lane, four lanes to 64 bytes of a row: the order of K in a product is free as long as both sides share it, so
+ * v_mfma_f32_16x16x32_bf16 is fed with (row i / 4, pieces of class i % 4) against (token j / 4, class j % 4), and of the
+ * 16 x 16 results those with i % 4 = j % 4 are wanted.  Three quarters of the matrix core's work is thrown away and it
+ * still idles; the loads are what counts, and the cache looks up 64 bytes at a time only where lanes beside each other ask
+ * for them (with 128 bytes of 8 rows a load, two lanes beside each other: 28 look-ups for 16, 57 cycles a load, which bound it).  Codes become
  * bf16 in registers: int8 and e2m1 with its E8M0 scale are exact there (E8M0 0 is 2^-127, 255 NaN, and what leaves
  * bf16's range infinite), so the sums are f32 sums of exact products.
  *
@@ -14,7 +17,7 @@
  *   sum   y of each token's slots, in the order of its choice: nothing is added in an order that changes from run to run.
  *
  * up and down are one kernel: the units lie in a row, and each workgroup, one a compute unit, takes an equal run of
- * them; of a run's lines each of its 16 waves takes an equal run again, and what it leaves of a unit to the next wave
+ * them; of a run's spans each of its 8 waves takes an equal run again, and what it leaves of a unit to the next wave
  * meets through LDS.  The tokens' rows of a run's jobs are in LDS, where the waves read them beside their weights'
  * loads, and the line's loads are the only ones in the stream: with the tokens read from memory too, the
  * address unit was busy 9 cycles of 10 at 2.5 TB/s (64 tokens, 128 e2m1 experts).
@@ -55,8 +58,8 @@ struct MoeArgs {
     const uint8_t* ws;
     void* out;                          /* up: h, bf16 [parts][pairs][f]; down: sums, f32 [pairs][n] */
     int64_t w_expert, ws_expert, ws_pitch;
-    int w_pitch, job_rows, lines, cpr;  /* 128-byte lines a row of the plane, 1 KB loads a part of a token's row */
-    MoeDiv unit, line, grid, choice;    /* by units a job, lines, workgroups, top_k */
+    int w_pitch, job_rows, spans, cpr;  /* spans of 256 bytes a row of the plane, 1 KB loads a part of a token's row */
+    MoeDiv unit, line, grid, choice;    /* by units a job, spans, workgroups, top_k */
     /* up */
     int32_t* ids;
     float* weights;
@@ -88,7 +91,7 @@ __device__ __forceinline__ void moe_bf16(r3d_i32x4 w, uint32_t scale, r3d_i32x4 
             b[d >> 1][2 * (d & 1) + 1] = (int)r3d_pack_bf16x2((float)(int8_t)(v >> 16), (float)(v >> 24));
         }
     } else {
-        const float s = __uint_as_float(scale << 23);
+        const float s = __uint_as_float(scale);                      /* of which the conversion takes bits 23 to 30 alone */
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
             b[d][0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4((uint32_t)w[d], s, 0));
@@ -101,7 +104,12 @@ __device__ __forceinline__ void moe_bf16(r3d_i32x4 w, uint32_t scale, r3d_i32x4 
 
 /* ------------------------------------------------------------------------------ the choice */
 
-constexpr int kMoeWaves = 16, kMoeThreads = 64 * kMoeWaves;
+#ifndef MOE_W
+#define MOE_W 8
+#define MOE_D4 2
+#define MOE_D1 4
+#endif
+constexpr int kMoeWaves = MOE_W, kMoeThreads = 64 * kMoeWaves;
 constexpr int kMoeUnits = 128;          /* units whose scales lie in LDS at a time */
 
 struct MoeChoice {                      /* in LDS, the same in every workgroup */
@@ -200,7 +208,7 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t
 /* Choices of every token, then the experts' slots and jobs, `width` tokens each.  All lanes of the workgroup. */
 __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    if (tid < kMoeMaxE) S.mask[tid] = 0;
+    for (int i = tid; i < kMoeMaxE; i += kMoeThreads) S.mask[i] = 0;
     __syncthreads();
     for (int t = wave; t < P.M; t += kMoeWaves) {
         if (P.E <= 64) moe_choose<1>(P, S, t);
@@ -232,46 +240,58 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
         }
     }
     __syncthreads();
-    /* a lane a (token, choice) */
-    const int t = tid < P.pairs ? (int)P.choice.of(tid) : 0, e = tid < P.pairs ? S.id[tid] : -1;
-    int slot = -1;
-    if (e >= 0) {
-        slot = S.first[e] + __popcll(S.mask[e] & ((1ull << t) - 1));
-        S.tok[slot] = (uint8_t)t;
-        S.slot_w[slot] = S.w[tid];
+    for (int at = tid; at < P.pairs; at += kMoeThreads) {            /* a lane a (token, choice) */
+        const int t = P.choice.of(at), i = at - t * P.top_k, e = S.id[at];
+        int slot = -1;
+        if (e >= 0) {
+            slot = S.first[e] + __popcll(S.mask[e] & ((1ull << t) - 1));
+            S.tok[slot] = (uint8_t)t;
+            S.slot_w[slot] = S.w[at];
+        }
+        if (blockIdx.x == 0) {                                       /* and what the others and the caller need */
+            P.table->slot[at] = (int16_t)slot;
+            if (P.ids) P.ids[t * P.i_pitch + i] = e;
+            if (P.weights) P.weights[t * P.wt_pitch + i] = S.w[at];
+            if (at < S.jobs) P.table->job[at] = S.job[at];
+            if (at == 0) P.table->jobs = S.jobs;
+        }
     }
     __syncthreads();
-    if (blockIdx.x == 0) {
-        if (tid < S.jobs) P.table->job[tid] = S.job[tid];
-        if (tid < P.pairs) {
-            const int i = tid - t * P.top_k;
-            P.table->slot[tid] = (int16_t)slot;
-            if (P.ids) P.ids[t * P.i_pitch + i] = e;
-            if (P.weights) P.weights[t * P.wt_pitch + i] = S.w[tid];
-        }
-        if (tid == 0) P.table->jobs = S.jobs;
-    }
 }
 
 /* ------------------------------------------------------------------------------ products */
 
-/* Of a 16 x 16 result, whose lane (i / 4, j) holds rows i .. i + 3: the sum of both parities of row 2 (lane / 16) + lane % 2
- * and token lane / 2 % 8, one value a lane.  The even lane of a pair has wanted values in elements 0 and 2, the odd one
- * in 1 and 3; each sends the other's. */
-__device__ __forceinline__ float moe_value(r3d_f32x4 a) {
-    const bool odd = threadIdx.x & 1;
-    const float send = odd ? a[1] : a[2], keep = odd ? a[3] : a[0];
-    return keep + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(send), 0xB1, 15, 15, true));
+/* Four results v[T][t] of row tiles T and token tiles t, of which lane (i / 4, j) holds rows i .. i + 3 of column j and the
+ * class j % 4's is wanted: the sum over the classes of row lane / 16 and token lane / 4 % 4, of tile T = lane % 2 and
+ * t = lane / 2 % 2.  A sum over four lanes each, and a choice. */
+__device__ __forceinline__ float moe_value(r3d_f32x4 v00, r3d_f32x4 v10, r3d_f32x4 v01, r3d_f32x4 v11) {
+    const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+    auto mine = [&](r3d_f32x4 v) __attribute__((always_inline)) {
+        const float lo = b0 ? v[1] : v[0], hi = b0 ? v[3] : v[2];
+        return b1 ? hi : lo;
+    };
+    /* lanes 2 apart exchange what the other's token tile needs, then lanes beside each other the row tile's */
+    const float p00 = mine(v00), p10 = mine(v10), p01 = mine(v01), p11 = mine(v11);
+    auto from = [](float v, auto ctrl) __attribute__((always_inline)) {
+        return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), decltype(ctrl)::value, 15, 15, true));
+    };
+    using Two = std::integral_constant<int, 0x4E>;              /* lanes 2 3 0 1 of each four */
+    using One = std::integral_constant<int, 0xB1>;              /* 1 0 3 2 */
+    const float q0 = (b1 ? p01 : p00) + from(b1 ? p00 : p01, Two{});
+    const float q1 = (b1 ? p11 : p10) + from(b1 ? p10 : p11, Two{});
+    return (b0 ? q1 : q0) + from(b0 ? q0 : q1, One{});
 }
 
-/* LDS that a row of K columns in XH parts takes: whole 1 KB loads, and 16 bytes off a multiple of 128 so that
- * eight tokens' pieces meet no bank twice. */
-constexpr int moe_row(int64_t K, int parts) { return (int)(parts * ((2 * K + 1023) / 1024) * 1024 + 16); }
+/* LDS that a row of K columns in XH parts takes: whole 1 KB loads, and what keeps the pieces that eight lanes read, four of
+ * two tokens, apart. */
+constexpr int moe_row(int64_t K, int parts, int enc) {
+    return (int)(parts * ((2 * K + 1023) / 1024) * 1024 + (enc == MOE_BF16 ? 64 : 16));
+}
 
 template <int ENC, int CT, int XH, bool UP>
 __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
     constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X;
-    constexpr int L = ENC == MOE_FP4 ? 4 : 1, D = ENC == MOE_FP4 ? 2 : 4;   /* lines a step, steps in flight */
+    constexpr int L = ENC == MOE_FP4 ? 2 : 1, D = ENC == MOE_FP4 ? (CT == 1 ? MOE_D4 : 1) : MOE_D1;   /* spans a step, steps in flight */
     struct Jobs {
         uint32_t job[kMoeMaxPairs];
     };
@@ -287,16 +307,20 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         moe_plan(P, S);
         jobs = i8_uniform(S.jobs);
     } else {
-        const uint32_t job = P.table->job[tid];                      /* what lies past the jobs is not used */
+        constexpr int EACH = kMoeMaxPairs / kMoeThreads;
+        uint32_t job[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) job[i] = P.table->job[EACH * tid + i];    /* what lies past the jobs is not used */
         jobs = P.table->jobs;
         asm volatile("" ::"s"(P.x), "s"(P.w), "s"(P.ws), "s"(P.w_expert), "s"(P.w_pitch), "s"(P.line.m), "s"(P.grid.m));
-        S.job[tid] = job;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) S.job[EACH * tid + i] = job[i];
         __syncthreads();
     }
-    const int r8 = (lane >> 1) & 7, piece = (lane & 1) | (lane >> 4) << 1;   /* row, or column, and 16-byte piece of a line */
-    const int row1 = piece;                                          /* row of the lane's result (moe_value) */
-    const int nb = P.unit.d, lines = P.lines, pieces = P.K / N;      /* units a job */
-    const int part_lds = P.cpr * 1024, row_lds = XH * part_lds + 16;
+    const int r4 = (lane >> 2) & 3, cls = lane & 3, piece = (lane >> 4) * 4 + cls;   /* row, or column, and piece of a span */
+    const int row1 = (lane >> 4) + 4 * (lane & 1), col1 = r4 + 2 * (lane & 2);       /* of the lane's result (moe_value) */
+    const int nb = P.unit.d, spans = P.spans, pieces = P.K / N;      /* units a job */
+    const int part_lds = P.cpr * 1024, row_lds = moe_row(P.K, XH, ENC);
     /* a run an XCD, so that its L2 sees few jobs' tokens */
     const uint32_t G = P.grid.d, per = G >> 3, rem = G & 7, xcd = blockIdx.x & 7;
     const uint32_t g = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
@@ -327,28 +351,28 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 s_scale[i] = reinterpret_cast<const float*>(P.ws)[(int64_t)(S.job[j] & 511) * P.ws_expert + row];
             }
         }
-        /* this wave's lines, L a step and a unit's last ones fewer */
-        const int total = (end - u) * lines;                         /* times 16 under 2^31: moe_geom */
+        /* this wave's spans, L a step and a unit's last ones fewer */
+        const int total = (end - u) * spans;                         /* times 16 under 2^31: moe_geom */
         const int a = i8_uniform(total * wave / kMoeWaves), b = i8_uniform(total * (wave + 1) / kMoeWaves);
         int tokens = 0;                                              /* of the rows to be held, a lane each */
         if constexpr (UP) tokens = lane < held ? S.tok[slot_base + lane] : 0;
         struct Step {
-            r3d_i32x4 w[L][2];
-            uint32_t s[2];                                           /* e2m1: four scales of the row's 32, the piece's number's */
+            r3d_i32x4 w[L][4];
+            uint32_t s[2];                                           /* e2m1: four scales of row lane / 4, a span each */
         } ring[D];
         const int ua = i8_uniform((int)P.line.of(a));
-        int ll = a - ua * lines, lj = i8_uniform((int)P.unit.of(u + ua)), lb = u + ua - lj * nb, left = b - a;   /* where loads are */
+        int ll = a - ua * spans, lj = i8_uniform((int)P.unit.of(u + ua)), lb = u + ua - lj * nb, left = b - a;   /* where loads are */
         int cl = ll, cj = lj, cb = lb, cu = ua, todo = left;         /* where products are */
         __amdgpu_buffer_rsrc_t rW = r3d_rsrc(P.w, 0);
         const uint8_t* s_base = P.ws;
         uint32_t w_at[2] = {0, 0}, s_at[2] = {0, 0};
         bool both = true, entered = false;
-        /* A line's scales are 8 bytes of each row, a byte a lane.  Loads of a byte a lane from 8 rows a line fetch the
-         * rows' lines anew each time (the stream has long left the L1), so a step loads its 32 bytes at once, four a lane at
-         * any alignment, the plane's last four in place of some that lie past it; a lane's byte is then another lane's. */
-        const uint32_t s_row = (uint32_t)(r8 * P.ws_pitch), s_last = (uint32_t)s_plane - 4;
+        /* A span's scales are 16 bytes of each of the 16 rows, a byte a lane and row tile.  A step loads them four a lane, at
+         * any alignment (the plane's last four in place of some that lie past it), 16 bytes of a row by four lanes beside
+         * each other; a lane's byte is then another lane's. */
+        const uint32_t s_last = (uint32_t)s_plane - 4;
         auto load = [&](Step& st) __attribute__((always_inline)) {
-            const int n = left < lines - ll ? left : lines - ll;     /* 0: the wave's lines are done */
+            const int n = left < spans - ll ? left : spans - ll;     /* 0: the wave's spans are done */
             if (n > 0 && (ll == 0 || !entered)) {                    /* a unit's first line here */
                 entered = true;
                 const int64_t e = i8_uniform(S.job[lj]) & 511;
@@ -361,26 +385,27 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 s_at[0] = r0 * (uint32_t)P.ws_pitch;
                 s_at[1] = r1 * (uint32_t)P.ws_pitch;
             }
-            const uint32_t wo = (uint32_t)(r8 * P.w_pitch + 16 * piece);
+            const uint32_t wo = (uint32_t)(r4 * P.w_pitch + 16 * piece);
             if (ENC == MOE_FP4) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
+                for (int i = 0; i < 2; ++i) {
                     typedef uint32_t u32_u1 __attribute__((aligned(1)));
-                    const uint32_t o = s_at[r] + s_row + 8 * ll + 4 * piece;
-                    st.s[r] = *reinterpret_cast<const u32_u1*>(s_base + (o < s_last ? o : s_last));
+                    const uint32_t o = (lane < 32 ? s_at[0] : s_at[1]) + ((lane >> 2) & 7) * (uint32_t)P.ws_pitch + 16 * (ll + i) + 4 * cls;
+                    st.s[i] = *reinterpret_cast<const u32_u1*>(s_base + (o < s_last ? o : s_last));
                 }
             }
 #pragma unroll
             for (int i = 0; i < L; ++i) {
-                const bool in = i < n && 8 * (ll + i) + piece < pieces;
+                const bool in = i < n && 16 * (ll + i) + piece < pieces;
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    st.w[i][r] = i8_buf16<2>(rW, in && (r == 0 || both) ? wo : kI8Oob, w_at[r] + 128 * (ll + i));
+                for (int r = 0; r < 4; ++r)
+                    st.w[i][r] = i8_buf16<2>(rW, in && (r < 2 || both) ? wo : kI8Oob,
+                                             w_at[r >> 1] + (r & 1) * 4 * (uint32_t)P.w_pitch + 256 * (ll + i));
             }
             const int m = n < L ? n : L;
             left -= m;
             ll += m;
-            if (ll == lines) {
+            if (ll == spans) {
                 ll = 0;
                 if (++lb == nb) {
                     lb = 0;
@@ -418,29 +443,32 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         __syncthreads();
 
         int slot0 = 0, cnt = 0;
-        uint32_t xa[CT];
+        uint32_t xa[2 * CT];
         auto job_of = [&](int j) __attribute__((always_inline)) {
             const uint32_t job = i8_uniform(S.job[j]);
             slot0 = (job >> 9) & 2047;
             cnt = job >> 20;
 #pragma unroll
-            for (int t = 0; t < CT; ++t)                             /* a column without a token repeats the first one's */
-                xa[t] = (slot0 - slot_base + (8 * t + r8 < cnt ? 8 * t + r8 : 0)) * row_lds + 16 * X * piece;
+            for (int t = 0; t < 2 * CT; ++t)                         /* a column without a token repeats the first one's */
+                xa[t] = (slot0 - slot_base + (4 * t + r4 < cnt ? 4 * t + r4 : 0)) * row_lds + 16 * X * piece;
         };
         if (a < b) job_of(cj);
-        const int s_from = 4 * ((lane >> 5) | r8 << 1);              /* plus 16 lanes a line */
+        const int s_turn = (8 * cls + 9) & 31;
+        const int s_from = 4 * (4 * r4 + (lane >> 4));               /* plus 16 lanes a row tile */
         uint32_t c_at[2] = {(uint32_t)((UP ? 8 : 16) * cb) * (uint32_t)P.ws_pitch, 0};
         c_at[1] = c_at[0] + (uint32_t)(UP ? P.rows : 8) * (uint32_t)P.ws_pitch;
-        r3d_f32x4 acc[2][CT];
+        r3d_f32x4 acc[4][2 * CT];
         auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < CT; ++t) acc[0][t] = acc[1][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int t = 0; t < 2 * CT; ++t) acc[r][t] = r3d_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         };
         /* a whole unit's results */
         auto finish = [&](int un, int blk, const float (&val)[2][CT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int t = 0; t < CT; ++t) {
-                const int col = 8 * t + r8;
+                const int col = 8 * t + col1;
                 const int64_t slot = slot0 + (col < cnt ? col : 0);
                 float v[2] = {val[0][t], val[1][t]};
                 if constexpr (ENC == MOE_I8) {
@@ -452,10 +480,9 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                     float h = v[0] * v[1] * S.slot_w[slot];
                     uint16_t* const to = static_cast<uint16_t*>(P.out) + slot * P.rows + 8 * blk + row1;
                     for (int p = 0; p < P.parts; ++p) {
-                        const float other = __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(h), 0xB1, 15, 15, true));
-                        const uint32_t d = r3d_pack_bf16x2(h, other);
-                        if (!(lane & 1) && col < cnt) *reinterpret_cast<uint32_t*>(to + (int64_t)p * P.pairs * P.rows) = d;
-                        const float hi = __uint_as_float(d << 16);   /* what is left of h; nothing of inf and NaN */
+                        const uint16_t d = r3d_bf16_rne(h);
+                        if (col < cnt) to[(int64_t)p * P.pairs * P.rows] = d;
+                        const float hi = r3d_bf16_to_f32(d);         /* what is left of h; nothing of inf and NaN */
                         h = __builtin_fabsf(hi) < __builtin_inff() ? h - hi : 0.0f;
                     }
                 } else if (col < cnt) {
@@ -471,47 +498,70 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
 #pragma unroll
             for (int d = 0; d < D; ++d) {
                 if (todo > 0) {
-                    int n = todo < lines - cl ? todo : lines - cl;
+                    int n = todo < spans - cl ? todo : spans - cl;
                     n = n < L ? n : L;
+                    /* e2m1: a step with pieces past the row, or with scales that loads past the plane's end stand for */
+                    const bool edge = 16 * (cl + n) > pieces || c_at[1] + 7 * (uint32_t)P.ws_pitch + 16 * cl + 32 > s_last;
 #pragma unroll
                     for (int i = 0; i < L; ++i) {
                         if (i >= n) break;
-                        uint32_t scale[2] = {0, 0};
+                        uint32_t scale[4] = {0, 0, 0, 0};
                         if constexpr (ENC == MOE_FP4) {
+                            /* byte cls of the dword lane / 16 of the row's span, to bits 23-30 */
+                            uint32_t four[4];
 #pragma unroll
-                            for (int r = 0; r < 2; ++r) {
-                                /* byte 8 i + piece of the step's, in the dword of piece 2 i + piece / 4 */
-                                const uint32_t four = (uint32_t)__builtin_amdgcn_ds_bpermute(s_from + 64 * i, (int)ring[d].s[r]);
-                                const uint32_t o = c_at[r] + s_row + 8 * (cl + i) + (piece & 4);
-                                const uint32_t back = o < s_last ? 0 : o - s_last;
-                                scale[r] = __builtin_amdgcn_ubfe(four, 8 * (back + (piece & 3)), 8);
-                                /* past the row: 2^-127 of its zeros, not the next row's */
-                                scale[r] = 8 * (cl + i) + piece < pieces ? scale[r] : 0u;
+                            for (int r = 0; r < 4; ++r) four[r] = (uint32_t)__builtin_amdgcn_ds_bpermute(s_from + 64 * r, (int)ring[d].s[i]);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) scale[r] = __builtin_amdgcn_alignbit(four[r], four[r], s_turn);
+                            if (edge) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    const uint32_t o = c_at[r >> 1] + ((4 * r + r4) & 7) * (uint32_t)P.ws_pitch + 16 * (cl + i) + (piece & 12);
+                                    const uint32_t back = o < s_last ? 0 : o - s_last;
+                                    scale[r] = __builtin_amdgcn_ubfe(four[r], 8 * (back + cls), 8) << 23;
+                                    /* past the row: 2^-127 of its zeros, not the next row's */
+                                    scale[r] = 16 * (cl + i) + piece < pieces ? scale[r] : 0u;
+                                }
                             }
                         }
-                        r3d_i32x4 w0[X], w1[X];
-                        moe_bf16<ENC>(ring[d].w[i][0], scale[0], w0);
-                        moe_bf16<ENC>(ring[d].w[i][1], scale[1], w1);
 #pragma unroll
-                        for (int t = 0; t < CT; ++t)
+                        for (int h = 0; h < CT; ++h) {
+                            if (h > 0 && 8 * h >= cnt) break;        /* columns without a token */
+                            const bool two = 8 * h + 4 < cnt;
+                            r3d_i32x4 x[2][XH * X];
 #pragma unroll
-                            for (int k = 0; k < XH * X; ++k) {
-                                const r3d_i32x4 x = *reinterpret_cast<const r3d_i32x4*>(
-                                    s_x + xa[t] + k / X * part_lds + 128 * X * (cl + i) + 16 * (k % X));
-                                acc[0][t] = moe_mfma(w0[k % X], x, acc[0][t]);
-                                acc[1][t] = moe_mfma(w1[k % X], x, acc[1][t]);
+                            for (int k = 0; k < XH * X; ++k)
+                                x[0][k] = *reinterpret_cast<const r3d_i32x4*>(
+                                    s_x + xa[2 * h] + k / X * part_lds + 256 * X * (cl + i) + 16 * (k % X));
+                            if (two) {
+#pragma unroll
+                                for (int k = 0; k < XH * X; ++k)
+                                    x[1][k] = *reinterpret_cast<const r3d_i32x4*>(
+                                        s_x + xa[2 * h + 1] + k / X * part_lds + 256 * X * (cl + i) + 16 * (k % X));
                             }
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                r3d_i32x4 w[X];
+                                moe_bf16<ENC>(ring[d].w[i][r], scale[r], w);
+#pragma unroll
+                                for (int k = 0; k < XH * X; ++k) acc[r][2 * h] = moe_mfma(w[k % X], x[0][k], acc[r][2 * h]);
+                                if (two) {
+#pragma unroll
+                                    for (int k = 0; k < XH * X; ++k) acc[r][2 * h + 1] = moe_mfma(w[k % X], x[1][k], acc[r][2 * h + 1]);
+                                }
+                            }
+                        }
                     }
                     cl += n;
                     todo -= n;
-                    if (cl == lines || todo == 0) {                  /* the unit's end, or the run's */
+                    if (cl == spans || todo == 0) {                  /* the unit's end, or the run's */
                         float val[2][CT];
 #pragma unroll
                         for (int t = 0; t < CT; ++t) {
-                            val[0][t] = moe_value(acc[0][t]);
-                            val[1][t] = moe_value(acc[1][t]);
+                            val[0][t] = moe_value(acc[0][2 * t], acc[1][2 * t], acc[0][2 * t + 1], acc[1][2 * t + 1]);
+                            val[1][t] = moe_value(acc[2][2 * t], acc[3][2 * t], acc[2][2 * t + 1], acc[3][2 * t + 1]);
                         }
-                        if (whole && cl == lines) {
+                        if (whole && cl == spans) {
                             finish(cu, cb, val);
                         } else {
 #pragma unroll
@@ -519,7 +569,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
 #pragma unroll
                                 for (int r = 0; r < 2; ++r) s_part[wave][whole ? 0 : 1][r][t][lane] = val[r][t];
                         }
-                        if (cl == lines) {
+                        if (cl == spans) {
                             clear();
                             whole = true;
                             cl = 0;
@@ -541,7 +591,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         }
         __syncthreads();
         if (a < b && cl > 0 && whole) {                              /* begun here, ended by the waves after */
-            const int stop = (cu + 1) * lines;
+            const int stop = (cu + 1) * spans;
             float val[2][CT];
 #pragma unroll
             for (int t = 0; t < CT; ++t)
@@ -587,20 +637,20 @@ static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStre
     uint8_t* const h = reinterpret_cast<uint8_t*>(table + 1);
     float* const sums = reinterpret_cast<float*>(h + moe_h_bytes(P));
     const auto div = [](int64_t d) { return MoeDiv{(uint32_t)d, (uint32_t)(0xFFFFFFFFu / (uint32_t)d)}; };
-    const auto lines = [](int64_t K) { return (K / MoeCodes<ENC>::N + 7) / 8; };
+    const auto spans = [](int64_t K) { return (K / MoeCodes<ENC>::N + 15) / 16; };
     const auto loads = [](int64_t K) { return (int)((2 * K + 1023) / 1024); };
     const MoeArgs u{table, P.logits, P.l_pitch, (int)P.M, (int)P.E, (int)P.top_k, P.l_bf16, (int)P.n, (int)P.f, (int)pairs,
                     (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up_rows,
-                    (int)lines(P.n), loads(P.n), div(P.f / 8), div(lines(P.n)), div(g.blocks), div(P.top_k), P.ids, P.weights,
+                    (int)spans(P.n), loads(P.n), div(P.f / 8), div(spans(P.n)), div(g.blocks), div(P.top_k), P.ids, P.weights,
                     P.i_pitch, P.w_pitch, g.width, parts, P.act, P.sigmoid, P.renorm, P.weight_scale};
     hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 1, true>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
-                       (size_t)g.up_rows * moe_row(P.n, 1), stream, u);
+                       (size_t)g.up_rows * moe_row(P.n, 1, ENC), stream, u);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) {
         const MoeArgs d{table, nullptr, 0, (int)P.M, (int)P.E, (int)P.top_k, 0, (int)P.f, (int)P.n, (int)pairs, (int)(2 * P.f),
                         h, P.dn, P.dns, sums, P.dn_expert, P.dns_expert, P.dns_pitch, (int)P.dn_pitch, g.down_rows,
-                        (int)lines(P.f), loads(P.f), div((P.n + 15) / 16), div(lines(P.f)), div(g.blocks), div(P.top_k)};
-        const size_t lds = (size_t)g.down_rows * moe_row(P.f, parts);
+                        (int)spans(P.f), loads(P.f), div((P.n + 15) / 16), div(spans(P.f)), div(g.blocks), div(P.top_k)};
+        const size_t lds = (size_t)g.down_rows * moe_row(P.f, parts, ENC);
         const dim3 grid((unsigned)g.blocks), block(kMoeThreads);
         if (P.y_bf16) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 2, false>), grid, block, lds, stream, d);
         else hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 3, false>), grid, block, lds, stream, d);
