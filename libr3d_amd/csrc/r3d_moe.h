@@ -28,6 +28,8 @@ struct MoeTable {
     int32_t pad[3];
     uint32_t job[kMoeMaxPairs];         /* expert | first slot << 9 | tokens << 20 */
     int16_t slot[kMoeMaxPairs];         /* by (token, choice); -1: none */
+    int16_t id[kMoeMaxPairs];           /* choices of many tokens, and their weights */
+    float w[kMoeMaxPairs];
 };
 
 struct MoePlan {

@@ -106,8 +106,8 @@ __device__ __forceinline__ void moe_bf16(r3d_i32x4 w, uint32_t scale, r3d_i32x4 
 
 #ifndef MOE_W
 #define MOE_W 8
-#define MOE_D4 2
-#define MOE_D1 4
+#define MOE_D4 1
+#define MOE_D1 2
 #endif
 constexpr int kMoeWaves = MOE_W, kMoeThreads = 64 * kMoeWaves;
 constexpr int kMoeUnits = 128;          /* units whose scales lie in LDS at a time */
@@ -123,31 +123,39 @@ struct MoeChoice {                      /* in LDS, the same in every workgroup *
     int jobs;
 };
 
-/* Token t's choices and weights, a wave's work: lane l holds the logits of experts J l .. J l + J - 1 as whole
- * numbers in the same order, 0 for what is not there (NaN, -inf); each round takes the wave's largest, of equals the
- * first lane's first. */
+/* A lane's logits of token t as they lie in memory, experts J l .. J l + J - 1; -inf past the last one.  Every load before
+ * a use of one. */
 template <int J>
-__device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t) {
-    const int lane = threadIdx.x & 63;
-    float v[J];
-    uint32_t key[J];
+__device__ __forceinline__ void moe_logits(const MoeArgs& P, int t, uint32_t (&raw)[J]) {
+    const int e0 = J * (threadIdx.x & 63);
     if (P.l_bf16) {
         const uint16_t* const row = reinterpret_cast<const uint16_t*>(P.logits) + t * P.l_pitch;
-        uint32_t raw[J];                                         /* every load before a use of one */
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             raw[j] = 0xFF80u;
-            if (J * lane + j < P.E) raw[j] = row[J * lane + j];
+            if (e0 + j < P.E) raw[j] = row[e0 + j];
         }
-#pragma unroll
-        for (int j = 0; j < J; ++j) v[j] = __uint_as_float(raw[j] << 16);
     } else {
-        const float* const row = reinterpret_cast<const float*>(P.logits) + t * P.l_pitch;
+        const uint32_t* const row = reinterpret_cast<const uint32_t*>(P.logits) + t * P.l_pitch;
 #pragma unroll
-        for (int j = 0; j < J; ++j) v[j] = J * lane + j < P.E ? row[J * lane + j] : -__builtin_inff();
+        for (int j = 0; j < J; ++j) {
+            raw[j] = 0xFF800000u;
+            if (e0 + j < P.E) raw[j] = row[e0 + j];
+        }
     }
+}
+
+/* Token t's choices and weights, a wave's work: a lane's logits as whole numbers in the same order, 0 for what is not
+ * there (NaN, -inf); each round takes the wave's largest, of equals the first lane's first.  ids and weights are S's, or
+ * memory's. */
+template <int J, class Id>
+__device__ __forceinline__ void moe_choose(const MoeArgs& P, int t, const uint32_t (&raw)[J], Id* ids, float* weights, uint64_t* mask) {
+    const int lane = threadIdx.x & 63;
+    float v[J];
+    uint32_t key[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) {
+        v[j] = __uint_as_float(P.l_bf16 ? raw[j] << 16 : raw[j]);
         const uint32_t u = __float_as_uint(v[j] + 0.0f);                 /* -0 is 0 */
         key[j] = v[j] > -__builtin_inff() ? u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u) : 0u;
     }
@@ -199,22 +207,65 @@ __device__ __forceinline__ void moe_choose(const MoeArgs& P, MoeChoice& S, int t
         total = 1.0f;
     }
     if (lane < P.top_k) {
-        S.id[t * P.top_k + lane] = (int16_t)id;
-        S.w[t * P.top_k + lane] = there ? p / total * P.weight_scale : 0.0f;
-        if (there) atomicOr(reinterpret_cast<unsigned long long*>(&S.mask[id]), 1ull << t);
+        ids[t * P.top_k + lane] = (Id)id;
+        weights[t * P.top_k + lane] = there ? p / total * P.weight_scale : 0.0f;
+        if (mask && there) atomicOr(reinterpret_cast<unsigned long long*>(mask + id), 1ull << t);
     }
 }
 
-/* Choices of every token, then the experts' slots and jobs, `width` tokens each.  All lanes of the workgroup. */
+template <int J>
+__device__ __forceinline__ void moe_choose_own(const MoeArgs& P, MoeChoice& S) {
+    const int t = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t raw[J];
+    if (t < P.M) moe_logits<J>(P, t, raw);
+    __syncthreads();                                                 /* the masks are clear */
+    if (t < P.M) moe_choose<J>(P, t, raw, S.id, S.w, S.mask);
+}
+
+/* Choices of more tokens than a workgroup has waves: a wave a token, in a launch of its own (64 tokens made by every
+ * workgroup for itself took 17 us, 2.1 a token and wave). */
+__global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs P) {
+    const int t = blockIdx.x;
+    int16_t* const id = P.table->id;
+    float* const w = P.table->w;
+    if (P.E <= 128) {
+        uint32_t raw[2];
+        moe_logits<2>(P, t, raw);
+        moe_choose<2>(P, t, raw, id, w, nullptr);
+    } else {
+        uint32_t raw[8];
+        moe_logits<8>(P, t, raw);
+        moe_choose<8>(P, t, raw, id, w, nullptr);
+    }
+}
+
+/* Choices of every token (or what moe_route_kernel made of them), then the experts' slots and jobs, `width` tokens each.
+ * All lanes of the workgroup. */
 __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     for (int i = tid; i < kMoeMaxE; i += kMoeThreads) S.mask[i] = 0;
-    __syncthreads();
-    for (int t = wave; t < P.M; t += kMoeWaves) {
-        if (P.E <= 64) moe_choose<1>(P, S, t);
-        else if (P.E <= 128) moe_choose<2>(P, S, t);
-        else if (P.E <= 256) moe_choose<4>(P, S, t);
-        else moe_choose<8>(P, S, t);
+    if (P.M > kMoeWaves) {
+        constexpr int EACH = kMoeMaxPairs / kMoeThreads;
+        int id[EACH];
+        float w[EACH];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = tid + i * kMoeThreads;
+            id[i] = at < P.pairs ? P.table->id[at] : -1;
+            w[i] = at < P.pairs ? P.table->w[at] : 0.0f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int at = tid + i * kMoeThreads;
+            S.id[at] = (int16_t)id[i];
+            S.w[at] = w[i];
+            if (id[i] >= 0) atomicOr(reinterpret_cast<unsigned long long*>(&S.mask[id[i]]), 1ull << P.choice.of(at));
+        }
+    } else if (P.E <= 128) {
+        moe_choose_own<2>(P, S);
+    } else {
+        moe_choose_own<8>(P, S);
     }
     __syncthreads();
     if (wave == 0) {                                             /* a lane eight experts: slots and jobs before each */
@@ -358,7 +409,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
         if constexpr (UP) tokens = lane < held ? S.tok[slot_base + lane] : 0;
         struct Step {
             r3d_i32x4 w[L][4];
-            uint32_t s[2];                                           /* e2m1: four scales of row lane / 4, a span each */
+            uint32_t s[L];                                           /* e2m1: four scales of row lane / 4, a span each */
         } ring[D];
         const int ua = i8_uniform((int)P.line.of(a));
         int ll = a - ua * spans, lj = i8_uniform((int)P.unit.of(u + ua)), lb = u + ua - lj * nb, left = b - a;   /* where loads are */
@@ -388,7 +439,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
             const uint32_t wo = (uint32_t)(r4 * P.w_pitch + 16 * piece);
             if (ENC == MOE_FP4) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < L; ++i) {
                     typedef uint32_t u32_u1 __attribute__((aligned(1)));
                     const uint32_t o = (lane < 32 ? s_at[0] : s_at[1]) + ((lane >> 2) & 7) * (uint32_t)P.ws_pitch + 16 * (ll + i) + 4 * cls;
                     st.s[i] = *reinterpret_cast<const u32_u1*>(s_base + (o < s_last ? o : s_last));
@@ -643,6 +694,7 @@ static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStre
                     (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up_rows,
                     (int)spans(P.n), loads(P.n), div(P.f / 8), div(spans(P.n)), div(g.blocks), div(P.top_k), P.ids, P.weights,
                     P.i_pitch, P.w_pitch, g.width, parts, P.act, P.sigmoid, P.renorm, P.weight_scale};
+    if (P.M > kMoeWaves) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)P.M), dim3(64), 0, stream, u);
     hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 1, true>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
                        (size_t)g.up_rows * moe_row(P.n, 1, ENC), stream, u);
     hipError_t e = hipGetLastError();

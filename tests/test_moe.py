@@ -123,8 +123,8 @@ def test_refuses(dtype):
 
 
 def test_scratch_hook():
-    assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2)) == 6160 + 4 * 2 * (96 * 2 * 2 + 64 * 4)
-    assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2, y=torch.zeros(4, 64))) == 6160 + 4 * 2 * (96 * 2 * 3 + 64 * 4)
+    assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2)) == 12304 + 4 * 2 * (96 * 2 * 2 + 64 * 4)
+    assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2, y=torch.zeros(4, 64))) == 12304 + 4 * 2 * (96 * 2 * 3 + 64 * 4)
 
 
 def test_python_call_refuses_host_tensors():
