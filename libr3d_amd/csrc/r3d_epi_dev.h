@@ -117,15 +117,16 @@ __device__ __forceinline__ void epi_values(const EpiArgs& E, float* v, int64_t m
 /* A token's sums in LDS, 16 bytes off a multiple of 128: 16-byte stores of 8 tokens meet no bank twice. */
 constexpr int epi_row(int bn) { return 4 * bn + 16; }
 
-/* The epilogue of `rows` tokens from m0 on and BN columns from n0 on, their sums in LDS: eight columns a lane,
+/* The epilogue of ROWS tokens from m0 on and BN columns from n0 on, their sums in LDS: eight columns a lane,
  * the same ones for every token it takes, so that scales and bias are read once; y leaves and the residual
- * arrives in whole runs of a row. */
-template <class T, int BN, int THREADS>
-__device__ __forceinline__ void epi_tile(const typename T::TileArgs& P, const uint8_t* smem, int rows, int64_t m0,
-                                         int64_t n0) {
-    constexpr int CPR = BN / 8;
+ * arrives in whole runs of a row.  One token at a time: two and four at once, for their loads' sake, spill 24
+ * and 211 registers of the wide kernel, whose other half still holds its sums (2048 x 21504 x 5376 int8,
+ * gelu_tanh: one 247 us, four 283). */
+template <class T, int BN, int THREADS, int ROWS>
+__device__ __forceinline__ void epi_tile(const typename T::TileArgs& P, const uint8_t* smem, int64_t m0, int64_t n0) {
+    constexpr int CPR = BN / 8, STEP = THREADS / CPR;
     static_assert(THREADS % CPR == 0, "a lane keeps its columns");
-    const int cc = threadIdx.x % CPR;
+    const int cc = threadIdx.x % CPR, r0 = threadIdx.x / CPR;
     const int64_t n = n0 + 8 * cc;
     if (n >= P.N) return;                                       /* no barrier in here */
     float b[8], sb[8];
@@ -134,18 +135,26 @@ __device__ __forceinline__ void epi_tile(const typename T::TileArgs& P, const ui
 #pragma unroll
         for (int i = 0; i < 8; ++i) sb[i] = P.SB[(n + i < P.N ? n + i : P.N - 1) * P.sb_stride];
     }
-    for (int r = threadIdx.x / CPR; r < rows && m0 + r < P.M; r += THREADS / CPR) {
+    for (int r = r0; r < ROWS; r += STEP) {
+        const int64_t m = m0 + r;
+        if (m >= P.M) return;
+        float v[8], res[8];
+        const float sa = T::kScaled ? P.SA[m * P.sa_stride] : 1.0f;
+        if (P.e.res)
+            epi_load<8>(static_cast<const uint8_t*>(P.e.res) + m * P.e.r_pitch * (P.e.res_bf16 ? 2 : 4), P.e.res_bf16, n, P.N, res);
         const typename T::Acc4* s = reinterpret_cast<const typename T::Acc4*>(smem + r * epi_row(BN) + 32 * cc);
         const typename T::Acc4 lo = s[0], hi = s[1];
-        float v[8];
-        const float sa = T::kScaled ? P.SA[(m0 + r) * P.sa_stride] : 1.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float f = (float)(i < 4 ? lo[i & 3] : hi[i & 3]);
             v[i] = (T::kScaled ? f * sa * sb[i] : f) + b[i];
         }
-        epi_finish<8>(P.e, v, m0 + r, n, P.N);
-        epi_store<8>(P.e, P.Y, P.y_pitch, v, m0 + r, n, P.N);
+        act_values<8>(P.e.act, v);
+        if (P.e.res) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] += res[i];
+        }
+        epi_store<8>(P.e, P.Y, P.y_pitch, v, m, n, P.N);
     }
 }
 

@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(typename T::Til
                 *reinterpret_cast<typename T::Acc4*>(smem + (16 * (wm * WMF + b) + li) * epi_row(BN) +
                                                      4 * (16 * (wn * WNF + a) + 4 * q)) = acc[a][b];
         __syncthreads();
-        epi_tile<T, BN, 64 * WV>(P, smem, BM, m0, n0);
+        epi_tile<T, BN, 64 * WV, BM>(P, smem, m0, n0);
         return;
     }
     /* the bf16 tile through LDS, a token's row 32 bytes off a multiple of 128, then 16 bytes a lane */

@@ -202,8 +202,8 @@ __global__ __launch_bounds__(512) void i8_wide_kernel(typename T::TileArgs P) {
                             typename T::Acc4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
                     }
             __syncthreads();
-            epi_tile<T, BN, 512>(P, smem, 64, m0 + 64 * h, n0);
-            epi_tile<T, BN, 512>(P, smem + 64 * epi_row(BN), 64, m0 + 128 + 64 * h, n0);
+            epi_tile<T, BN, 512, 64>(P, smem, m0 + 64 * h, n0);
+            epi_tile<T, BN, 512, 64>(P, smem + 64 * epi_row(BN), m0 + 128 + 64 * h, n0);
         }
         return;
     }
