@@ -6,13 +6,13 @@
  * v_mfma_f32_16x16x32_bf16 is fed with (row i / 4, pieces of class i % 4) against (token j / 4, class j % 4), and of the
  * 16 x 16 results those with i % 4 = j % 4 are wanted.  Three quarters of the matrix core's work is thrown away and it
  * still idles; the loads are what counts, and the cache looks up 64 bytes at a time only where lanes beside each other ask
- * for them (with 128 bytes of 8 rows a load, two lanes beside each other: 28 look-ups for 16, 57 cycles a load, which bound it).  Codes become
- * bf16 in registers: int8 and e2m1 with its E8M0 scale are exact there (E8M0 0 is 2^-127, 255 NaN, and what leaves
- * bf16's range infinite), so the sums are f32 sums of exact products.
+ * for them (with 128 bytes of 8 rows a load, two lanes beside each other: 28 look-ups for 16, 57 cycles a load, which
+ * bound it).  Codes become bf16 in registers: int8 and e2m1 with its E8M0 scale are exact there (E8M0 0 is 2^-127, 255 NaN,
+ * and what leaves bf16's range infinite), so the sums are f32 sums of exact products.
  *
- *   up    every workgroup makes the same choice from the logits for itself (a few hundred cycles a token and wave,
- *         which costs less than a kernel of its own before this one), so that it knows the jobs: an expert and some
- *         of its tokens.  A unit is a job's 8 gate and 8 up rows of f; h leaves with its weight, to its token's slot.
+ *   up    every workgroup makes the same choice from the logits for itself, a wave a token (3.4 us with the first loads,
+ *         which costs less than a kernel of its own before this one; past 8 tokens, two rounds, a kernel of its own,
+ *         a workgroup a token, costs less), so that it knows the jobs: an expert and some of its tokens.  A unit is a job's 8 gate and 8 up rows of f; h leaves with its weight, to its token's slot.
  *   down  a unit is a job's 16 rows of n; its sums leave to its tokens' slots in f32.
  *   sum   y of each token's slots, in the order of its choice: nothing is added in an order that changes from run to run.
  *
@@ -104,12 +104,9 @@ __device__ __forceinline__ void moe_bf16(r3d_i32x4 w, uint32_t scale, r3d_i32x4 
 
 /* ------------------------------------------------------------------------------ the choice */
 
-#ifndef MOE_W
-#define MOE_W 8
-#define MOE_D4 1
-#define MOE_D1 2
-#endif
-constexpr int kMoeWaves = MOE_W, kMoeThreads = 64 * kMoeWaves;
+/* Two waves a SIMD.  Four were no faster at any of the sizes below, and neither were more spans in flight a wave: the
+ * CUs' share of HBM is reached with these. */
+constexpr int kMoeWaves = 8, kMoeThreads = 64 * kMoeWaves;
 constexpr int kMoeUnits = 128;          /* units whose scales lie in LDS at a time */
 
 struct MoeChoice {                      /* in LDS, the same in every workgroup */
@@ -342,7 +339,7 @@ constexpr int moe_row(int64_t K, int parts, int enc) {
 template <int ENC, int CT, int XH, bool UP>
 __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
     constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X;
-    constexpr int L = ENC == MOE_FP4 ? 2 : 1, D = ENC == MOE_FP4 ? (CT == 1 ? MOE_D4 : 1) : MOE_D1;   /* spans a step, steps in flight */
+    constexpr int L = ENC == MOE_FP4 ? 2 : 1, D = ENC == MOE_FP4 ? 1 : 2;   /* spans a step, steps in flight: 4 KB and 8 KB a wave */
     struct Jobs {
         uint32_t job[kMoeMaxPairs];
     };

@@ -145,7 +145,7 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
 
 /* LDS a workgroup: 160 KB, less its tables, the waves' shared units and int8's scales */
 static int64_t moe_lds(const MoePlan& P, int ct, bool up) {
-    return 160 * 1024 - (up ? 21 : 5) * 1024 - 16 * 1024 * ct - (P.enc == MOE_I8 ? 8 * 1024 : 0);
+    return 160 * 1024 - (up ? 21 : 5) * 1024 - 8 * 1024 * ct - (P.enc == MOE_I8 ? 8 * 1024 : 0);
 }
 
 bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {

@@ -16,8 +16,9 @@
  *   rmsnorm_block            prio 1000  n GE 1, dtype IN f32 bf16           norms, gate and residual between blocks
  *
  * R3D_NO_I8 hides the int8 rows, R3D_NO_I8_DEC the int8 decode row (and turns off its GEMV in the other
- * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler, R3D_NO_EPI gemm_nt_epi's rows, R3D_NO_BLOCK_NORM
- * rmsnorm_block, R3D_NO_MOE moe_layer (presence-tested, read once; hidden at registration as in r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * one, which takes those calls on its tiles), R3D_NO_SAMPLE the sampler, R3D_NO_EPI gemm_nt_epi's rows,
+ * R3D_NO_BLOCK_NORM rmsnorm_block, R3D_NO_MOE moe_layer (presence-tested, read once; hidden at registration as in
+ * r3d_rows.cpp).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 #include <stdint.h>
 #include <string.h>
 
@@ -292,7 +293,7 @@ const RadKernelInfo kRows[] = {
      RAD_DOMAIN_DEVICE, kPrioTile, cBand, 2, nullptr, 0, nullptr, nullptr, nullptr,
      r3d_rad_rmsnorm_block, nullptr, nullptr, nullptr, nullptr, nullptr},
     {"moe_layer", "moe_layer", "gemm",
-     "a mixture-of-experts layer for up to 64 tokens in two kernels: choice and gate/up products with their activation, then "
+     "a mixture-of-experts layer for up to 64 tokens: choice and gate/up products with their activation, then "
      "down products and the weighted sum; the chosen experts' planes are streamed once, codes become bf16 in registers",
      "E up to 512, top_k up to 16, n and f multiples of 8 (bf16), 16 (i8) or 32 (mxfp4); x and the code planes on 16 "
      "bytes; launch scratch of the size the hook asks for (16-byte aligned) required",
