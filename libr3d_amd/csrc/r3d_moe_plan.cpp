@@ -53,6 +53,8 @@ static int plan_experts(int enc, int64_t E, int64_t rows, int64_t cols, Experts*
         if (!pitch_ok(X->s_expert)) return RAD_E_STRIDE;
     } else if (enc == MOE_FP4) {
         if ((rc = planes_of(X->s, E, rows, cols / 32, &X->s_expert, &X->s_pitch))) return rc;
+        /* a load takes four scales, the plane's last four at most: rows that are apart, so that a plane has that many */
+        if (X->s_pitch < cols / 32) return RAD_E_STRIDE;
         if (X->s_pitch > (int64_t(1) << 31) / rows) return RAD_E_UNSUPPORTED;
     }
     return RAD_OK;
@@ -102,7 +104,7 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
     P->x_pitch *= 2;
     if ((uintptr_t)x->data & 15 || (M > 1 && (P->x_pitch & 15 || P->x_pitch > (1 << 24)))) return RAD_E_UNSUPPORTED;
     if (M == 1) P->x_pitch = 2 * n;                             /* a single row has no next one */
-    /* y is written when x and the logits are read, but by other workgroups than read them */
+    /* ids and weights are written while other workgroups still read x and the logits; y when nobody does */
     const Span outs[3] = {{y->data, M, n, P->y_pitch, elt_bytes(y->dtype)},
                           {id ? id->data : nullptr, M, k, P->i_pitch, 4}, {wt ? wt->data : nullptr, M, k, P->w_pitch, 4}};
     const Span ins[2] = {{x->data, M, n, P->x_pitch / 2, 2}, {lg->data, M, E, P->l_pitch, elt_bytes(lg->dtype)}};
@@ -110,7 +112,7 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
         if (!outs[i].data) continue;
         for (int j = 0; j < i; ++j)
             if (outs[j].data && spans_meet(outs[i], outs[j])) return RAD_E_INVAL;
-        if (i == 0) continue;                                   /* the second kernel reads neither x nor logits */
+        if (i == 0) continue;
         for (const Span& in : ins)
             if (spans_meet(outs[i], in)) return RAD_E_INVAL;
     }

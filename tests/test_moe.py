@@ -122,6 +122,19 @@ def test_refuses(dtype):
         assert got(gate_up_scale=call(dtype)._tensors[3][:7]) == R.RAD_E_SHAPE
 
 
+def test_scale_rows_lie_apart():
+    """A plane of one row's scales for all rows may be shorter than the four that a load takes."""
+    for name, rows, K in (("gate_up_scale", 192, 64), ("down_scale", 64, 96)):
+        one = torch.zeros(8, 1, K // 32, dtype=torch.uint8)
+        assert rc("mxfp4", **{name: one.expand(8, rows, K // 32)}) == R.RAD_E_STRIDE
+        near = torch.zeros(8 * rows * (K // 32), dtype=torch.uint8).as_strided((8, rows, K // 32), (rows, K // 32 - 1, 1))
+        assert rc("mxfp4", **{name: near}) == R.RAD_E_STRIDE
+        flat = torch.zeros(1, rows, K // 32, dtype=torch.uint8)
+        assert rc("mxfp4", **{name: flat.expand(8, rows, K // 32)}) == R.RAD_OK        # one plane for all experts
+    assert rc("i8", down_scale=torch.ones(1, 1).expand(8, 64)) == R.RAD_E_STRIDE
+    assert rc("i8", down_scale=torch.ones(1, 64).expand(8, 64)) == R.RAD_OK
+
+
 def test_scratch_hook():
     assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2)) == 12304 + 4 * 2 * (96 * 2 * 2 + 64 * 4)
     assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2, y=torch.zeros(4, 64))) == 12304 + 4 * 2 * (96 * 2 * 3 + 64 * 4)
