@@ -58,7 +58,8 @@ const DumpConfig& config() {
         const char* o = getenv("R3D_DUMP_OPS");
         std::string ops =
             o && *o ? o : "gemm_nt_q,quant_act_fp8,gated_quant_fp8,rmsnorm_quant_fp8,logits_gemm,"
-                         "quant_act_i8,gated_quant_i8,rmsnorm_quant_i8,sample_logits";
+                         "quant_act_i8,gated_quant_i8,rmsnorm_quant_i8,sample_logits,"
+                         "gemm_nt_epi,rmsnorm_block,moe_layer";
         size_t p = 0;
         while (p <= ops.size()) {
             const size_t e = ops.find(',', p);

@@ -18,6 +18,8 @@ PRE state, and those are compared with the POST state the GPU wrote:
   gemm_nt_q (i8a8), quant_act_i8, gated_quant_i8, rmsnorm_quant_i8, sample_logits
       in float64 on their own (tests/replay_rows.py): the product bit for bit, codes and
       scales within their roundings, tokens equal
+  gemm_nt_epi, rmsnorm_block, moe_layer                  in float64 within the bounds that
+      count their roundings (tests/replay_layers.py)
 --device re-launches each capture through libr3d_gfx950.so on a GPU instead (operands
 rebuilt from PRE at the same offsets, the same parameters, tunables and scratch size) and
 requires the outputs to equal POST byte for byte: the kernels are deterministic.
@@ -379,6 +381,9 @@ def replay_oracle(c):
     if c.row.endswith("_i8") or c.row.startswith("gemm_nt_q_i8a8") or c.row == "sample_logits":
         from tests import replay_rows
         return replay_rows.check(c)
+    if c.row.startswith("gemm_nt_epi") or c.row in ("rmsnorm_block", "moe_layer"):
+        from tests import replay_layers
+        return replay_layers.check(c)
     if c.row.startswith("gemm_nt_q_gated"):
         return check_gemm_gated(c, O, gu)
     if c.row.startswith("gemm_nt_q"):
