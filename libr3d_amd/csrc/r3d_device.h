@@ -87,14 +87,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t r3d_rsrc(const void* base, int
 }
 
 /* Buffer load of `bytes` (16, 4 or 2) per lane straight into LDS at lds + lane *
- * max(bytes, 4). */
-template <int BYTES>
+ * max(bytes, 4); AUX of 16 bytes: the load's cache policy (2: not to be kept). */
+template <int BYTES, int AUX = 0>
 __device__ __forceinline__ void r3d_buf_lds(__amdgpu_buffer_rsrc_t r, uint8_t* lds, uint32_t voff,
                                             uint32_t soff) {
     static_assert(BYTES == 16 || BYTES == 4 || BYTES == 2, "dwordx4, dword or ushort loads");
     if constexpr (BYTES == 16)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16,
-                                                 voff, soff, 0, 0);
+                                                 voff, soff, 0, AUX);
     else if constexpr (BYTES == 4)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 4,
                                                  voff, soff, 0, 0);

@@ -55,28 +55,41 @@ inline int i8_launch_tile(const I8Plan& P, const I8Geom& g, void* part, const Ep
                        P.sa_stride, P.sb_stride, P.y_pitch};
     if constexpr (T::kEpi) a.e = *epi;
     const dim3 grid((unsigned)g.blocks);
-#define R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, OFF_)                                           \
-    hipLaunchKernelGGL((i8_tile_kernel<T, WNF_, WMF_, WVN_, WVM_, NST_, OFF_>), grid,              \
+#define R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, OFF_, ONCE_)                                    \
+    hipLaunchKernelGGL((i8_tile_kernel<T, WNF_, WMF_, WVN_, WVM_, NST_, OFF_, ONCE_>), grid,       \
                        dim3(64 * WVN_ * WVM_),                                                 \
                        (size_t)i8_tile_lds(16 * WNF_ * WVN_, 16 * WMF_ * WVM_, NST_), stream, a)
 #define R3D_I8T2(WNF_, WMF_, WVN_, WVM_, NST_, ONST_)                                         \
-    if (P.off) { R3D_I8T(WNF_, WMF_, WVN_, WVM_, ONST_, true); }                                \
-    else { R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, false); }                                      \
+    if (P.off) { R3D_I8T(WNF_, WMF_, WVN_, WVM_, ONST_, true, false); }                         \
+    else { R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, false, false); }                               \
     break
+    /* gemm_nt_epi where one tile of tokens is all: nobody else asks for a tile's weights, and loads that the caches do not
+     * keep stream faster (ONCE; four layers' weights by turns, 21504 x 5376 bf16: M = 13 45.3 -> 40.3 us, 64 53.1 -> 49.4,
+     * 128 65.2 -> 61.7; i8a8 13 23.8 -> 21.3).  One layer's alone, again and again, stay in the 256 MB behind HBM without
+     * it (M = 13 34.8 us for 38.6), which no model's do.  Where tiles of tokens share the weights it loses: M = 333 105 ->
+     * 121 us. */
+#define R3D_I8T3(WNF_, WMF_, WVN_, WVM_, NST_, ONST_)                                         \
+    if (T::kEpi && a.grid_m == 1) {                                                             \
+        if (P.off) { R3D_I8T(WNF_, WMF_, WVN_, WVM_, ONST_, true, T::kEpi); }                   \
+        else { R3D_I8T(WNF_, WMF_, WVN_, WVM_, NST_, false, T::kEpi); }                         \
+        break;                                                                                  \
+    }                                                                                           \
+    R3D_I8T2(WNF_, WMF_, WVN_, WVM_, NST_, ONST_)
     switch (g.tile) {
         case I8_T_256x256:
             hipLaunchKernelGGL(i8_wide_kernel<T>, grid, dim3(512), (size_t)i8_tile_lds(256, 256, 2), stream, a);
             break;
-        case I8_T_128x256: R3D_I8T(4, 4, 2, 4, 3, false); break;
-        case I8_T_128x192: R3D_I8T(2, 6, 4, 2, 3, false); break;
-        case I8_T_128x128: R3D_I8T2(2, 4, 4, 2, 4, 5);
-        case I8_T_128x96: R3D_I8T2(2, 6, 4, 1, 4, 5);
-        case I8_T_128x64: R3D_I8T2(2, 4, 4, 1, 4, 5);
-        case I8_T_64x64: R3D_I8T2(1, 4, 4, 1, 4, 5);
-        case I8_T_64x32: R3D_I8T2(1, 2, 4, 1, 6, 6);
-        case I8_T_32x32: R3D_I8T2(1, 2, 2, 1, 10, 10);
-        default: R3D_I8T2(1, 1, 2, 1, 8, 8);
+        case I8_T_128x256: R3D_I8T(4, 4, 2, 4, 3, false, false); break;
+        case I8_T_128x192: R3D_I8T(2, 6, 4, 2, 3, false, false); break;
+        case I8_T_128x128: R3D_I8T3(2, 4, 4, 2, 4, 5);
+        case I8_T_128x96: R3D_I8T3(2, 6, 4, 1, 4, 5);
+        case I8_T_128x64: R3D_I8T3(2, 4, 4, 1, 4, 5);
+        case I8_T_64x64: R3D_I8T3(1, 4, 4, 1, 4, 5);
+        case I8_T_64x32: R3D_I8T3(1, 2, 4, 1, 6, 6);
+        case I8_T_32x32: R3D_I8T3(1, 2, 2, 1, 10, 10);
+        default: R3D_I8T3(1, 1, 2, 1, 8, 8);
     }
+#undef R3D_I8T3
 #undef R3D_I8T2
 #undef R3D_I8T
     const hipError_t e = hipGetLastError();

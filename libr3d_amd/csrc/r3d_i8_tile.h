@@ -22,6 +22,8 @@
  * NST - 1 steps ahead.  A wave reads the operands of one half step while the products of the other
  * run.
  *
+ * ONCE: weights that one workgroup alone asks for are loaded without being kept in the caches.
+ *
  * The sum is exact in i32, so K may be cut anywhere: with kc > 1 workgroup u takes K chunk
  * u / tiles of its tile and leaves an i32 plane, and i8_join_kernel adds the planes.
  *
@@ -51,7 +53,7 @@ struct I8TileArgs {
     int64_t sa_stride, sb_stride, y_pitch;
 };
 
-template <class T, int WNF, int WMF, int WVN, int WVM, int NST, bool OFF>
+template <class T, int WNF, int WMF, int WVN, int WVM, int NST, bool OFF, bool ONCE>
 __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(typename T::TileArgs P) {
     constexpr int WV = WVN * WVM, BN = 16 * WNF * WVN, BM = 16 * WMF * WVM;
     constexpr int WLD = BN / 8 / WV, ALD = BM / 8 / WV, LOADS = WLD + ALD;   /* 1 KB loads a wave */
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(64 * WVN * WVM) void i8_tile_kernel(typename T::Til
         const bool aok = (uint32_t)(128 * s + acol) < (uint32_t)(kend - k0);
 #pragma unroll
         for (int i = 0; i < WLD; ++i)
-            r3d_buf_lds<16>(rB, st + 1024 * (wave + WV * i), wok ? woff[i] : 0x80000000u, k);
+            r3d_buf_lds<16, ONCE ? 2 : 0>(rB, st + 1024 * (wave + WV * i), wok ? woff[i] : 0x80000000u, k);
 #pragma unroll
         for (int i = 0; i < ALD; ++i)
             r3d_buf_lds<16>(rA, st + AOFF + 1024 * (wave + WV * i), aok ? aoff[i] : 0x80000000u, k);
