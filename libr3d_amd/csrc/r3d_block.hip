@@ -40,7 +40,8 @@ __device__ __forceinline__ void block_e4m3(const float* v, uint8_t* qr, float* s
 #pragma unroll
     for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
     amax = r3d_max16(amax);
-    const float s = amax > 0.0f ? amax * (1.0f / 448.0f) : 1.0f;
+    /* a normal number, as quant_act_i8's: 1 / s of a smaller one is infinite, and 0 times that no code */
+    const float s = amax > 0.0f ? fmaxf(amax * (1.0f / 448.0f), 0x1p-126f) : 1.0f;
     const float inv = 1.0f / s;
     if (i >= n) return;
     if ((threadIdx.x & 15) == 0) sr[i >> 7] = s;

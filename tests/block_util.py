@@ -57,7 +57,7 @@ def check_e4m3(q, scale, v, ev):
     n = v.shape[1]
     pad = lambda t: torch.nn.functional.pad(t, (0, -n % 128)).unflatten(1, (-1, 128))  # noqa: E731
     amax = pad(v).abs().amax(2)
-    want = torch.where(amax > 0, amax / 448, torch.ones_like(amax))
+    want = torch.where(amax > 0, (amax / 448).clamp_min(2.0 ** -126), torch.ones_like(amax))
     assert ((scale.double() - want).abs() <= pad(ev).amax(2) / 448 + 3 * U * want).all()
     s = scale.double().repeat_interleave(128, 1)[:, :n]
     got = q.view(torch.float8_e4m3fn).double() * s

@@ -147,6 +147,17 @@ def test_rows_of_zeros_infinities_and_nans(gpu):
         assert not s8[i].isfinite() and not q8[i].any()
 
 
+@pytest.mark.parametrize("size", [1e-39, 1e-37, 3e-36, 1e-30])
+def test_weights_near_the_end_of_the_range(gpu, size):
+    """Scales of values that f32 has few numbers below, zeros among them."""
+    M, n = 3, 640
+    t = inputs(M, n, w="f32")
+    t["w_pre"] *= size
+    t["w_pre"][::7] = 0
+    for codes in ("i8", "e4m3"):
+        run(gpu, M, n, out="f32", codes=codes, data=dict(t))
+
+
 def test_streams_and_graph(gpu):
     M, n = 9, 5376
     t = inputs(M, n)
