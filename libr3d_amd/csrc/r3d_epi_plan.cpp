@@ -14,6 +14,7 @@ namespace r3d {
 
 /* Bases, pitches and K that the 16-byte kernels take, from their bytes. */
 static void epi_alignment(I8Plan* p) {
+    p->chain = 1;
     p->ua = (p->K & 15) || (((uintptr_t)p->A | (uintptr_t)p->B) & 15) || ((p->a_pitch | p->b_pitch) & 15) ||
             p->a_pitch > (1 << 22) || p->b_pitch > (1 << 22);
     p->off = (((uintptr_t)p->A | (uintptr_t)p->B) & 127) || ((p->a_pitch | p->b_pitch) & 127);

@@ -28,6 +28,7 @@ struct I8Plan {
     int64_t a_pitch, b_pitch, y_pitch, sa_stride, sb_stride;
     int ua;                  /* K, a base or a pitch off 16 bytes: the any-alignment kernel */
     int off;                 /* a base or a pitch off 128: rows begin inside lines */
+    int chain;               /* gemm_nt_epi: the GEMV's cost counts a wave's own lines too */
 };
 
 /* The operands and params of a gemm_nt_q call at i8a8; m_max: the row's bound on M (0: none). */

@@ -108,10 +108,14 @@ static double i8_tile_ns(const I8Cost& c, const I8Plan& P, int64_t per, int64_t 
 
 /* The GEMV's time in the same terms, work growing with the tokens: over 13494 shapes of 1..8 tokens the
  * cheaper of it and a tile is 1.0 % slower than the best launch, the GEMV wherever it fits 3.4 % (8 x 8192 x
- * 5376 12.1 -> 10.4 us on tiles of 32 rows; up to 3 tokens it is the faster one nearly everywhere). */
-static double i8_gemv_ns(const I8Plan& P, int ncu) {
+ * 5376 12.1 -> 10.4 us on tiles of 32 rows; up to 3 tokens it is the faster one nearly everywhere).
+ * gemm_nt_epi counts one thing more: with a workgroup a compute unit or less, a wave's chain of `per` lines may be longer than
+ * all that (bytes of a row; 1 x 128 x 43008 13.0 us, on tiles with 24 planes 7.8; 1 x 512 x 21504 8.5 and 7.5; 1 x 128 x 10752
+ * 5.3 and 5.6). */
+static double i8_gemv_ns(const I8Plan& P, int ncu, const I8Geom& g) {
     const double lines = (double)((P.N + 7) / 8) * ((P.K + 127) / 128) / ncu;
-    const double work = 11.8 * (1.0 + 0.0841 * P.M) * lines;
+    const double chain = P.chain && g.blocks <= ncu ? 165.0 * (1.0 + 0.06 * P.M) * g.per : 0.0;
+    const double work = fmax(11.8 * (1.0 + 0.0841 * P.M) * lines, chain);
     const double stream = (double)P.N * P.K * 1000 / 6120000 * (P.off ? 1.3 : 1.0);
     return 3610 + 32 * P.M + sqrt(work * work + stream * stream);
 }
@@ -138,7 +142,7 @@ void i8_geom(const I8Plan& P, int ncu, int64_t scratch, I8Geom* g) {
         g->per = (int)((steps + kc - 1) / kc);
         g->waves = kc > 4 ? kc : 4;
         g->blocks = (rows + g->waves / kc - 1) / (g->waves / kc);
-        best = i8_gemv_ns(P, ncu);
+        best = i8_gemv_ns(P, ncu, *g);
     }
     for (int t = 0; t < I8_TILES; ++t) {
         const I8Cost& c = kI8Cost[t];
