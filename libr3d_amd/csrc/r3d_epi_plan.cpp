@@ -70,6 +70,10 @@ int plan_epi(const RadArgs* a, bool bf16, EpiPlan* P) {
     const Span y{Y->data, M, N, p.y_pitch, elt_bytes(Y->dtype)};
     if (R && spans_clash(y, Span{R->data, M, N, P->r_pitch, elt_bytes(R->dtype)})) return RAD_E_INVAL;
     const int e = bf16 ? 2 : 1;
+    if (spans_meet(y, Span{A->data, M, K, p.a_pitch, e}) || spans_meet(y, Span{B->data, N, K, p.b_pitch, e}) ||
+        (C && spans_meet(y, Span{C->data, N, 1, P->bias_stride, elt_bytes(C->dtype)})) ||
+        (AS && spans_meet(y, Span{AS->data, M, 1, p.sa_stride, 4})) || (BS && spans_meet(y, Span{BS->data, N, 1, p.sb_stride, 4})))
+        return RAD_E_INVAL;
     p.a_pitch *= e;
     p.b_pitch *= e;
     /* every kernel's least: 16 rows under 32-bit offsets */

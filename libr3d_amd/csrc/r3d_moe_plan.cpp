@@ -25,7 +25,7 @@ static int planes_of(const RadTensor* t, int64_t E, int64_t rows, int64_t cols, 
 struct Experts {
     const RadTensor* w;
     const RadTensor* s;
-    int64_t expert, pitch, s_expert, s_pitch;
+    int64_t expert, pitch, s_expert, s_pitch, bytes;            /* bytes: of an expert's codes */
 };
 
 static int plan_experts(int enc, int64_t E, int64_t rows, int64_t cols, Experts* X) {
@@ -42,6 +42,7 @@ static int plan_experts(int enc, int64_t E, int64_t rows, int64_t cols, Experts*
     /* 16 bytes a lane: whole pieces on their own alignment, an expert's plane under 32-bit offsets */
     if ((row | X->expert | X->pitch) & 15 || (uintptr_t)X->w->data & 15) return RAD_E_UNSUPPORTED;
     if (X->pitch > (int64_t(1) << 31) / rows || (rows - 1) * X->pitch + row > 0x7FFFFFFF) return RAD_E_UNSUPPORTED;
+    X->bytes = (rows - 1) * X->pitch + row;
     if (enc == MOE_I8) {
         if (X->s->rank == 3) {                                       /* [E, rows, 1] */
             if (X->s->shape[0] != E || X->s->shape[1] != rows || X->s->shape[2] != 1) return RAD_E_SHAPE;
@@ -66,7 +67,7 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
     const RadTensor* y  = rad_arg_in(a, 6);
     const RadTensor* id = rad_arg_in(a, 7);
     const RadTensor* wt = rad_arg_in(a, 8);
-    Experts up{rad_arg_in(a, 2), rad_arg_in(a, 3), 0, 0, 0, 0}, down{rad_arg_in(a, 4), rad_arg_in(a, 5), 0, 0, 0, 0};
+    Experts up{rad_arg_in(a, 2), rad_arg_in(a, 3), 0, 0, 0, 0, 0}, down{rad_arg_in(a, 4), rad_arg_in(a, 5), 0, 0, 0, 0, 0};
     if (!x || !lg || !up.w || !down.w || !y) return RAD_E_INVAL;
     const char* dt = rad_args_gets(a, "dtype");
     P->enc = !dt ? -1 : !strcmp(dt, "bf16") ? MOE_BF16 : !strcmp(dt, "i8") ? MOE_I8 : !strcmp(dt, "mxfp4") ? MOE_FP4 : -1;
@@ -112,6 +113,9 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
         if (!outs[i].data) continue;
         for (int j = 0; j < i; ++j)
             if (outs[j].data && spans_meet(outs[i], outs[j])) return RAD_E_INVAL;
+        /* the planes, from an expert's first byte to the last one's last */
+        for (const Experts* X : {&up, &down})
+            if (spans_meet(outs[i], Span{X->w->data, 1, (E - 1) * X->expert + X->bytes, 0, 1})) return RAD_E_INVAL;
         if (i == 0) continue;
         for (const Span& in : ins)
             if (spans_meet(outs[i], in)) return RAD_E_INVAL;

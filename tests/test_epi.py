@@ -98,6 +98,23 @@ def test_refuses(dtype):
     assert got(y=shared.view(torch.bfloat16)[:, :48], residual=shared) == R.RAD_E_INVAL   # the same memory, other types
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "i8a8"])
+def test_refuses_a_result_over_its_operands(dtype):
+    """Workgroups read a and b while others write y."""
+    got = lambda **kw: rc(call(dtype, **kw), dtype)  # noqa: E731
+    mem = bf(4, 96)
+    of = (lambda t: t) if dtype == "bf16" else (lambda t: t.view(torch.int8)[:, :64])
+    assert got(y=mem[:, :48], a=of(mem[:, :64])) == R.RAD_E_INVAL
+    big = bf(48, 64)
+    assert got(y=big[:4, :48], b=of(big)) == R.RAD_E_INVAL
+    assert got(y=mem[:, 32:80], bias=mem[1, 40:88]) == R.RAD_E_INVAL
+    if dtype == "bf16":
+        assert got(y=mem[:, :48], a=bf(4, 64)) == R.RAD_OK
+    else:
+        f = torch.zeros(4, 96)
+        assert got(y=f[:, :48], a_scale=f[:, 5]) == got(y=f[:, :48], b_scale=f[1, :48]) == R.RAD_E_INVAL
+
+
 def test_python_calls_refuse_host_tensors():
     with pytest.raises(ValueError):
         R.gemm_nt_epi(bf(2, 8), bf(3, 8), bf(2, 3), dtype="bf16", N=3, K=8)

@@ -135,6 +135,15 @@ def test_scale_rows_lie_apart():
     assert rc("i8", down_scale=torch.ones(1, 64).expand(8, 64)) == R.RAD_OK
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "i8", "mxfp4"])
+def test_refuses_results_over_the_experts(dtype):
+    gu = call(dtype)._tensors[2]
+    assert rc(dtype, gate_up=gu, y=gu.view(-1).view(torch.bfloat16)[-256:].view(4, 64)) == R.RAD_E_INVAL
+    assert rc(dtype, gate_up=gu, ids=gu.view(-1).view(torch.int32)[:8].view(4, 2)) == R.RAD_E_INVAL
+    dn = call(dtype)._tensors[4]
+    assert rc(dtype, down=dn, weights=dn.view(-1).view(torch.float32)[64:72].view(4, 2)) == R.RAD_E_INVAL
+
+
 def test_scratch_hook():
     assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2)) == 12304 + 4 * 2 * (96 * 2 * 2 + 64 * 4)
     assert R.row_scratch_bytes(ROW, call(M=4, f=96, top_k=2, y=torch.zeros(4, 64))) == 12304 + 4 * 2 * (96 * 2 * 3 + 64 * 4)
