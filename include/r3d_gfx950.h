@@ -232,10 +232,12 @@ int r3d_gfx950_mfma_valu_probe(int nv, int lag3, int iters, void* work, int64_t*
 
 /* The second row table, with no counterpart in the reference: rows of ops and encodings past the
  * set that radiance's other plugins declare (int8: gemm_nt_q at i8a8 and its producers; a
- * sampler), in the same structures, resolved and launched the same way.  A loader compares the schemas of
+ * sampler; a product with an epilogue; the norms between blocks; an expert layer), in the same structures, resolved
+ * and launched the same way.  A loader compares the schemas of
  * rad_kernel_schema_at with other plugins', so these are listed apart; an engine that knows the ops
- * reads them here.  R3D_NO_I8, R3D_NO_I8_DEC and R3D_NO_SAMPLE hide rows at registration (R3D_NO_I8_DEC: the
- * decode row, and no int8 call takes its GEMV).  gemm_nt_q's schema is rad_kernel_schema_at's. */
+ * reads them here.  R3D_NO_I8, R3D_NO_I8_DEC, R3D_NO_SAMPLE, R3D_NO_EPI, R3D_NO_BLOCK_NORM and R3D_NO_MOE hide rows at
+ * registration (R3D_NO_I8_DEC: the decode row, and no int8 call takes its GEMV; gemm_nt_epi's do not take it
+ * either).  gemm_nt_q's schema is rad_kernel_schema_at's. */
 int r3d_gfx950_ext_schema_count(void);
 const RadOpSchema* r3d_gfx950_ext_schema_at(int i);
 int r3d_gfx950_ext_kernel_count(void);
@@ -287,6 +289,51 @@ int r3d_rad_rmsnorm_quant_i8(const RadArgs* a, RadStream s);
  * RAD_E_DEVICE for a failed launch.  Asynchronous on `s`; results do not depend on the run. */
 int r3d_rad_sample_logits(const RadArgs* a, RadStream s);
 int64_t r3d_rad_sample_logits_scratch(const RadArgs* a);
+
+/* gemm_nt_epi: Y[m, n] = act(S * sum_k A[m, k] B[n, k] + bias[n]) + residual[m, n], rounded once.  The _bf16 entry takes bf16
+ * a [M, K] and b [N, K] (S = 1, no scales), the _i8 entry int8 ones with a_scale f32 [M] or [M, 1] and b_scale f32 [N]
+ * or [N, 1] (S their product, the sum exact in i32).  Operands (a, a_scale?, b, b_scale?, bias? f32/bf16 [N],
+ * residual? f32/bf16 [M, N], y f32/bf16 [M, N]); params N, K, dtype "bf16" or "i8a8", act "none" (default), "relu", "silu",
+ * "sigmoid", "gelu" (erf) or "gelu_tanh"; M = numel(y) / N.  K <= 1048576 at bf16, 131071 at i8a8.  y may be the residual's own
+ * elements (same type and pitch) and meets no other operand; a residual or bias stride of 0 repeats one row or value.
+ * Any alignment and pitch of the elements' own size; K, bases or pitches off 16 bytes are slow.  Sums are f32 at bf16, in an
+ * order that the shape alone sets.  RAD_OK, RAD_E_INVAL / RAD_E_DTYPE / RAD_E_SHAPE / RAD_E_STRIDE /
+ * RAD_E_UNSUPPORTED for refused operands, RAD_E_DEVICE for a failed launch.  Asynchronous on `s`.
+ * The hooks: bytes of launch scratch (planes where K is split), optional as the int8 rows' is. */
+int r3d_rad_gemm_nt_epi_bf16(const RadArgs* a, RadStream s);
+int r3d_rad_gemm_nt_epi_i8(const RadArgs* a, RadStream s);
+int64_t r3d_rad_gemm_nt_epi_bf16_scratch(const RadArgs* a);
+int64_t r3d_rad_gemm_nt_epi_i8_scratch(const RadArgs* a);
+
+/* rmsnorm_block: what lies between two blocks of a model, a row of n values at a time:
+ *     t = x rs(x) (w_post + wadd), or x without w_post      rs(a) = 1 / sqrt(sum a^2 / n + eps)
+ *     h = res_scale residual + gate t                       to residual_out, rounded to bf16
+ *     v = h rs(h) (w_pre + wadd), of the f32 h              to out, and to q and scale as codes
+ * Operands (x bf16/f32 [M, n], residual? bf16 [M, n], w_post? [n], gate? [n], [M, 1] or [M, n], w_pre? [n], residual_out? bf16
+ * [M, n], out? bf16/f32 [M, n], q? [M, n], scale?); w_post, gate and w_pre of one type, bf16 or f32; w_pre with out or q, and
+ * q with scale: int8 with one f32 a row (quant_act_i8's quantiser, [M] or [M, 1]), or e4m3 (RAD_U8 too) with one a group of 128
+ * columns, [M, ceil(n / 128)], max(amax / 448, 2^-126), 1 for zeros.  Params n (<= 32768), eps, dtype (x's), wadd, res_scale
+ * (1), group.  An output may be the own elements of x, the residual or the gate (same type and pitch) and meets nothing else.
+ * Refusals and statuses as above; no scratch.  Asynchronous on `s`. */
+int r3d_rad_rmsnorm_block(const RadArgs* a, RadStream s);
+
+/* moe_layer: a mixture-of-experts layer for up to 64 tokens.  Of each token's router logits the top_k largest are chosen, by
+ * falling logit, ties to the lower index; NaN and -inf are not there, and a token of which nothing is has ids -1, weights 0
+ * and a y of zeros.  Weights: softmax over the logits or a sigmoid of each (score), divided by the chosen ones' sum (renorm,
+ * default 1), times weight_scale.  Then y = sum over the choices of W_down (weight * act(W_gate x) * (W_up x)).
+ * Operands (x bf16 [M, n], logits f32/bf16 [M, E], gate_up [E, 2f, n]: f gate rows, then f up rows; gate_up_scale?, down [E, n,
+ * f], down_scale?, y f32/bf16 [M, n], ids? i32 [M, top_k], weights? f32 [M, top_k]); params n, f, E (<= 512), top_k (<= 16),
+ * dtype, act (as above; silu), score "softmax" or "sigmoid", renorm, weight_scale.  dtype:
+ *     "bf16"   no scales; n, f multiples of 8
+ *     "i8"     int8 codes, f32 scales [E, rows] or [E, rows, 1]; multiples of 16
+ *     "mxfp4"  e2m1 codes, E8M0 scales [E, rows, columns / 32] (0: 2^-127, 255: NaN); multiples of 32
+ * x and the code planes on 16 bytes, their pitches too, an expert's plane under 2^31 bytes from its first to its last; any
+ * distance between experts.  h is kept to 2^-16 of itself where y is bf16 and 2^-24 where it is f32; results do not
+ * depend on the run.  y may be x's or the logits' memory; ids and weights may not.  Launch scratch of the size the hook gives,
+ * 16-byte aligned, is required (else RAD_E_UNSUPPORTED); calls that share it are ordered on one stream.  Refusals and statuses
+ * as above.  Asynchronous on `s`. */
+int r3d_rad_moe_layer(const RadArgs* a, RadStream s);
+int64_t r3d_rad_moe_layer_scratch(const RadArgs* a);
 
 /* Build identity with no counterpart in the reference: the SHA-256 (hex) of the compile
  * flags and of the sources this library was compiled from -- the flags as one line, then

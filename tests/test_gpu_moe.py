@@ -210,6 +210,21 @@ def test_tokens_do_not_meet(gpu):
         assert y[7].isnan().all() and not y[2].isfinite().any() and not y[4].isfinite().any()
 
 
+@pytest.mark.parametrize("M", [1, 5, 9, 64])
+def test_result_over_the_inputs(gpu, M):
+    """y in the memory of x, and (f32) of the logits."""
+    n, f, E, k = 64, 96, 64, 4
+    t = inputs("i8", M, n, f, E)
+    on = {m: None if v is None else v.to(gpu) for m, v in t.items()}
+    want = U.exact(**on, dtype="i8", f=f, top_k=k, parts=2), U.exact(**on, dtype="i8", f=f, top_k=k, parts=3)
+    for name, w in zip(("x", "logits"), want):
+        d = dict(on, x=on["x"].clone(), logits=on["logits"].clone())
+        ids, ws = torch.zeros(M, k, dtype=torch.int32, device=gpu), torch.zeros(M, k, device=gpu)
+        assert R.moe_layer(y=d[name], ids=ids, weights=ws, dtype="i8", n=n, f=f, E=E, top_k=k, **d) == R.RAD_OK
+        torch.cuda.synchronize()
+        U.check((d[name], ids, ws), w)
+
+
 def test_streams_and_graph(gpu):
     """Two streams at once with their scratch each, and a captured call replayed over new tokens, bit for bit as called."""
     for dtype, M in (("bf16", 3), ("i8", 40), ("mxfp4", 64)):
