@@ -4,7 +4,11 @@
  * that x, the residual and the gate are read once and every result is written once; that traffic is what bounds
  * it over many rows, and over few the chain of a load and two or three reductions over the workgroup.  All
  * arithmetic is in f32, the two sums of squares in f64; h goes on into the second norm as it stands in f32 and
- * is rounded to bf16 for residual_out alone, v is rounded (or quantised) once. */
+ * is rounded to bf16 for residual_out alone, v is rounded (or quantised) once.
+ *
+ * Measured on MI355X (a 1 GiB copy 5.05 TB/s): 2048 x 5376 with post norm, residual and both results 19.9 to 20.3 us, 4.4
+ * TB/s; 333 x 5376 with a gate and int8 codes 8.2 to 9.2; 1 x 5376 4.6 to 5.1.  Lanes and chunks by the rule of r3d_i8_plan.cpp's
+ * producers, whose shapes and chains are the same. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>

@@ -1,6 +1,11 @@
 /* r3d_epi.hip -- entries of gemm_nt_epi's rows (bf16 and i8a8), behind the same launch signature as every row.
  * The plan (r3d_epi_plan.cpp), the gfx950 chip gate, then kernels on the caller's stream.  No allocation, no
- * synchronisation, no host<->device traffic. */
+ * synchronisation, no host<->device traffic.
+ *
+ * Measured on MI355X (a 1 GiB copy 5.05 TB/s; the library's largest products 1.61 PFLOP/s bf16, 2.40 POP/s int8), bias in
+ * all but the second: 4 x 128 x 5376 bf16 5.8 us, a launch and one chain of loads; 1 x 5376 x 4096 int8 with residual 6.6; 13 x
+ * 21504 x 5376 bf16, gelu_tanh 40.3, 5.75 TB/s, bound by the weights; 333 x 8187 x 5360 bf16 45, the tile's own rate; 2048 x
+ * 21504 x 5376 int8, gelu_tanh 250 to 255, of which the epilogue's VALU some 30. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
