@@ -35,9 +35,9 @@ struct BlockPlan {
 
 int plan_block(const RadArgs* a, BlockPlan* P);
 
-/* Lanes of a row's workgroup and 8-element chunks a lane holds. */
+/* Lanes of a row's workgroup and 8-element chunks a lane holds; past: results are not kept in the caches. */
 struct BlockGeom {
-    int lanes, chunks;
+    int lanes, chunks, past;
 };
 BlockGeom block_geom(int64_t rows, int64_t n);
 

@@ -6,9 +6,8 @@
  * arithmetic is in f32, the two sums of squares in f64; h goes on into the second norm as it stands in f32 and
  * is rounded to bf16 for residual_out alone, v is rounded (or quantised) once.
  *
- * Measured on MI355X (a 1 GiB copy 5.05 TB/s): 2048 x 5376 with post norm, residual and both results 19.9 to 20.3 us, 4.4
- * TB/s; 333 x 5376 with a gate and int8 codes 8.2 to 9.2; 1 x 5376 4.6 to 5.1.  Lanes and chunks by the rule of r3d_i8_plan.cpp's
- * producers, whose shapes and chains are the same. */
+ * Measured on MI355X (a 1 GiB copy 5.05 TB/s): 2048 x 5376 with post norm, residual and both results 18.4 us, 4.8
+ * TB/s (20.7 with operands that come from HBM alone); 333 x 5376 with a gate and int8 codes 7.9; 1 x 5376 4.6 to 5.1. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -34,8 +33,41 @@ struct BlockArgs {
     int64_t n, x_pitch, r_pitch, g_pitch, ro_pitch, o_pitch, q_pitch, s_pitch;
     double eps;
     float wadd, res_scale;
-    int gate_kind, codes, out_bf16;
+    int gate_kind, codes, out_bf16, past;
 };
+
+/* Eight results to element i of a row of n on; past: not to be kept in the caches. */
+__device__ __forceinline__ void block_st8(uint8_t* row, int64_t i, int64_t n, const float* v, int bf16, int past) {
+    if (bf16) {
+        r3d_i32x4_u2 d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[j] = (int)r3d_pack_bf16x2(v[2 * j], v[2 * j + 1]);
+        r3d_i32x4_u2* const to = reinterpret_cast<r3d_i32x4_u2*>(row + 2 * i);
+        if (i + 8 <= n && past) {
+            __builtin_nontemporal_store(d, to);
+        } else if (i + 8 <= n) {
+            *to = d;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < n) reinterpret_cast<uint16_t*>(row)[i + j] = (uint16_t)((uint32_t)d[j >> 1] >> (16 * (j & 1)));
+        }
+    } else {
+        r3d_f32x4_u4* const to = reinterpret_cast<r3d_f32x4_u4*>(row + 4 * i);
+        const r3d_f32x4_u4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+        if (i + 8 <= n && past) {
+            __builtin_nontemporal_store(lo, to);
+            __builtin_nontemporal_store(hi, to + 1);
+        } else if (i + 8 <= n) {
+            to[0] = lo;
+            to[1] = hi;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (i + j < n) reinterpret_cast<float*>(row)[i + j] = v[j];
+        }
+    }
+}
 
 /* e4m3 codes of a chunk of 8: quant_act_fp8's arithmetic (r3d_band.h), a group of 128 in 16 lanes.  Every lane
  * takes part in the maximum; a lane past the row's end has zeros. */
@@ -148,7 +180,7 @@ __global__ __launch_bounds__(1024) void block_kernel(BlockArgs P) {
         uint8_t* const ro = P.res_out + row * P.ro_pitch * 2;
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (i0 + c * step < n) i8_st8(ro, i0 + c * step, n, h[c], 1);
+            if (i0 + c * step < n) block_st8(ro, i0 + c * step, n, h[c], 1, P.past);
     }
     if (!P.w_pre) return;
     double ss = 0.0;
@@ -171,7 +203,7 @@ __global__ __launch_bounds__(1024) void block_kernel(BlockArgs P) {
         uint8_t* const o = P.out + row * P.o_pitch * (P.out_bf16 ? 2 : 4);
 #pragma unroll
         for (int c = 0; c < C; ++c)
-            if (i0 + c * step < n) i8_st8(o, i0 + c * step, n, h[c], P.out_bf16);
+            if (i0 + c * step < n) block_st8(o, i0 + c * step, n, h[c], P.out_bf16, P.past);
     }
     if (P.codes == BLOCK_I8) {
         uint32_t m = 0;
@@ -202,7 +234,7 @@ static int block_entry(const RadArgs* a, RadStream s) {
     if (g.lanes < 64 || g.lanes > 1024 || 8 * (int64_t)g.lanes * g.chunks < P.n) return RAD_E_UNSUPPORTED;
     const BlockArgs k{P.x, P.res, P.w_post, P.gate, P.w_pre, P.res_out, P.out, P.q, P.scale, P.n, P.x_pitch,
                       P.r_pitch, P.g_pitch, P.ro_pitch, P.o_pitch, P.q_pitch, P.s_pitch, P.eps, P.wadd, P.res_scale,
-                      P.gate_kind, P.codes, P.out_bf16};
+                      P.gate_kind, P.codes, P.out_bf16, g.past};
     const dim3 grid((unsigned)P.rows), block((unsigned)g.lanes);
     hipStream_t stream = (hipStream_t)s;
 #define R3D_BLOCK_C(X_, W_)                                                                       \

@@ -131,14 +131,32 @@ int plan_block(const RadArgs* a, BlockPlan* P) {
 BlockGeom block_geom(int64_t rows, int64_t n) {
     const int64_t nc = (n + 7) / 8;
     auto lanes = [&](int c) { return (int)(((nc + c - 1) / c + 63) / 64 * 64); };
-    if (nc <= 256 || rows * nc < 400000) {
-        const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : lanes(3) <= 1024 ? 3 : 4;
-        return BlockGeom{lanes(c), c};
+    /* Few values: one row's chain, as few chunks a lane as some 768 lanes allow.  us at the chunks named, 64 rows of n:
+     *     2048     1: 3.5   2: 3.8   4: 4.4        5376     1: 5.3   2: 5.9   3: 5.7
+     *     8192     1: 6.0   2: 5.5   4: 5.6       16384     2: 7.9   3: 8.5   4: 7.5 */
+    if (rows * nc < 200000) {
+        const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : 4;
+        return BlockGeom{lanes(c), c, 0};
     }
-    int best = 0;
-    for (int c : {3, 2, 4})
-        if (lanes(c) <= 1024 && (!best || lanes(c) * c < lanes(best) * best)) best = c;
-    return BlockGeom{lanes(best), best};
+    /* Many: as many chunks in flight a compute unit as its registers hold (32, 28, 20 and 16 waves at 1 to 4 chunks a lane),
+     * fewer a lane where they tie.  2048 rows:
+     *     1024     1: 6.1   2: 5.6   3: 7.2   4: 8.7        5376     1: 28.9  2: 24.0  3: 20.4  4: 20.8
+     *     2560     1: 12.2  2: 10.7  3: 10.2  4: 11.9       8192     1: 29.0  2: 23.4  3: 31.2  4: 22.6
+     *     4096     1: 15.0  2: 13.1  3: 15.8  4: 12.1      16384     2: 59.3  3: 63.6  4: 44.8 */
+    static const int kWaves[] = {0, 32, 28, 20, 16};
+    int best = 4;
+    int64_t most = 0;
+    for (int c = 1; c <= 4; ++c) {
+        const int64_t held = lanes(c) <= 1024 ? kWaves[c] / (lanes(c) / 64) * nc : 0;
+        if (held > most) {
+            most = held;
+            best = c;
+        }
+    }
+    /* Two results of more than the 32 MB of the XCDs' L2 are written past the caches, which they would only fill: 2048 x 5376
+     * 24.3 -> 20.4 us, with a product of 2048 columns behind it 76.2 -> 74.4.  Smaller ones are still there when that product
+     * asks for them: 512 x 5376 and 2048 columns 32.5 us, past the caches 39.0. */
+    return BlockGeom{lanes(best), best, rows * nc >= (1 << 20)};
 }
 
 int describe_block(const char* row, const RadArgs* a, char* buf, int len) {
