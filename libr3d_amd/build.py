@@ -17,6 +17,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 PKG = os.path.join(ROOT, "libr3d_amd")
@@ -67,12 +69,17 @@ def source_id():
 
 
 def build_library():
-    tmp = LIB + ".tmp"
-    cmd = ([HIPCC] + FLAGS + ['-DR3D_BUILD_ID="%s"' % source_id()] +
-           [os.path.join(CSRC, s) for s in SOURCES] + ["-o", tmp])
-    out = _run(cmd)
-    if out.strip():
-        sys.stderr.write(out + "\n")
+    """Every source compiled, as many at once as there are CPUs to this process (MAX_JOBS at most), then one link."""
+    tmp, ident = LIB + ".tmp", '-DR3D_BUILD_ID="%s"' % source_id()
+    jobs = min(int(os.environ.get("MAX_JOBS") or 16), len(os.sched_getaffinity(0)))
+    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(max(jobs, 1)) as pool:
+        objects = [os.path.join(d, s + ".o") for s in SOURCES]
+        compiled = pool.map(lambda s, o: _run([HIPCC] + [f for f in FLAGS if f != "-shared"] +
+                                              [ident, "-c", os.path.join(CSRC, s), "-o", o]), SOURCES, objects)
+        outs = list(compiled) + [_run([HIPCC, "--offload-arch=gfx950", "-fPIC", "-shared"] + objects + ["-o", tmp])]
+    for out in outs:
+        if out.strip():
+            sys.stderr.write(out + "\n")
     os.replace(tmp, LIB)
     return LIB
 
