@@ -7,7 +7,7 @@
  * is rounded to bf16 for residual_out alone, v is rounded (or quantised) once.
  *
  * Measured on MI355X (a 1 GiB copy 5.05 TB/s): 2048 x 5376 with post norm, residual and both results 18.4 us, 4.8
- * TB/s (20.7 with operands that come from HBM alone); 333 x 5376 with a gate and int8 codes 7.9; 1 x 5376 4.6 to 5.1. */
+ * TB/s (20.7 with operands that come from HBM alone); 333 x 5376 with a gate and int8 codes 7.4 to 8.6; 1 x 5376 4.6 to 5.1. */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
