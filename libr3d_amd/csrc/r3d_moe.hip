@@ -22,12 +22,13 @@
  * loads, and the line's loads are the only ones in the stream: with the tokens read from memory too, the
  * address unit was busy 9 cycles of 10 at 2.5 TB/s (64 tokens, 128 e2m1 experts).
  *
- * h is kept as the sum of two bf16 numbers where y is bf16 and of three where it is f32 (2^-16 and 2^-24 of it at most), so
- * that of the roundings on the way y's own counts: the products of the parts cost matrix cycles, which idle here.
+ * h is kept in f32, and its bits go into the products as the sum of three bf16 numbers, which holds all 24 of them: those of
+ * the parts cost matrix cycles, which idle here.  (Two parts, 2^-17 of it at most, put 0.22 % of 64 x 8 / 128's bf16 results on
+ * the other side of a rounding, where f32 sums put 0.05 % and this puts 0.03; they took 287 us.)
  *
  * Measured on MI355X (tokens x choices / experts): 1 x 8 / 128 mxfp4, 5376 x 1344 32.3 us and 4 x 4 / 64 int8, 2048 x 768 25, each
- * launch's beginning and end 6 to 7 us of it; 13 x 4 / 32 bf16, 2048 x 1408 77 to 84, 5.3 to 5.8 TB/s; 64 x 8 / 128 mxfp4 284 to
- * 293, gate and up 5.8 TB/s, down 4.5 (rows of 672 bytes share lines, and jobs past four tokens take a second tile). */
+ * launch's beginning and end 6 to 7 us of it; 13 x 4 / 32 bf16, 2048 x 1408 77 to 84, 5.3 to 5.8 TB/s; 64 x 8 / 128 mxfp4 300 to
+ * 304, gate and up 5.8 TB/s, down 4.1 (rows of 672 bytes share lines, and jobs past four tokens take a second tile). */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -60,15 +61,15 @@ struct MoeArgs {
     const uint8_t* x;                   /* up: the tokens; down: h */
     const uint8_t* w;
     const uint8_t* ws;
-    void* out;                          /* up: h, bf16 [parts][pairs][f]; down: sums, f32 [pairs][n] */
+    float* out;                         /* up: h [pairs][f]; down: sums [pairs][n] */
     int64_t w_expert, ws_expert, ws_pitch;
-    int w_pitch, job_rows, spans, cpr;  /* spans of 256 bytes a row of the plane, 1 KB loads a part of a token's row */
-    MoeDiv unit, line, grid, choice;    /* by units a job, spans, workgroups, top_k */
+    int w_pitch, job_rows, spans, cpr;  /* spans of 256 bytes a row of the plane, 1 KB pieces of a token's row in bf16 */
+    MoeDiv unit, line, grid, choice, chunk;      /* by units a job, spans, workgroups, top_k, cpr */
     /* up */
     int32_t* ids;
     float* weights;
     int64_t i_pitch, wt_pitch;
-    int width, parts, act, sigmoid, renorm;
+    int width, act, sigmoid, renorm;
     float weight_scale;
 };
 
@@ -334,7 +335,22 @@ __device__ __forceinline__ float moe_value(r3d_f32x4 v00, r3d_f32x4 v10, r3d_f32
     return (b0 ? q1 : q0) + from(b0 ? q0 : q1, One{});
 }
 
-/* LDS that a row of K columns in XH parts takes: whole 1 KB loads, and what keeps the pieces that eight lanes read, four of
+/* Eight f32 values as sums of three bf16 ones each: the bits of a number cut in three, eight each.  Infinities and NaN (quiet ones,
+ * as arithmetic leaves them) stand alone. */
+__device__ __forceinline__ void moe_parts(r3d_i32x4 lo, r3d_i32x4 hi, r3d_i32x4 (&part)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a = __int_as_float(i < 2 ? lo[2 * i] : hi[2 * i - 4]), b = __int_as_float(i < 2 ? lo[2 * i + 1] : hi[2 * i - 3]);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            part[p][i] = (int)__builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);   /* the upper halves */
+            a = __builtin_fabsf(a) < __builtin_inff() ? a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u) : 0.0f;
+            b = __builtin_fabsf(b) < __builtin_inff() ? b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u) : 0.0f;
+        }
+    }
+}
+
+/* LDS that a row of K columns in XH parts takes: whole 1 KB pieces, and what keeps the pieces that eight lanes read, four of
  * two tokens, apart. */
 constexpr int moe_row(int64_t K, int parts, int enc) {
     return (int)(parts * ((2 * K + 1023) / 1024) * 1024 + (enc == MOE_BF16 ? 64 : 16));
@@ -343,9 +359,9 @@ constexpr int moe_row(int64_t K, int parts, int enc) {
 /* L spans of 4 KB a step.  A row's last step may be short, and what it lacks is missing in flight: e2m1 takes two a step, and
  * three where a row of y has three, nine, .. (64 x 8 / 128, f = 1344 295 -> 285 us; 64 x 4 / 64, n = 4096, f = 1536 127 -> 125, but
  * 2048 161 -> 164, and one token 0.3 us more).  The others have two steps of one in flight. */
-template <int ENC, int CT, int XH, bool UP, int L>
+template <int ENC, int CT, bool UP, int L>
 __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
-    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X;
+    constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X, XH = UP ? 1 : 3;   /* parts of a token's values */
     constexpr int D = ENC == MOE_FP4 ? 1 : 2;                        /* steps in flight */
     struct Jobs {
         uint32_t job[kMoeMaxPairs];
@@ -382,7 +398,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
     const uint32_t units = (uint32_t)jobs * nb;                      /* times G under 2^32: moe_geom */
     const int u_end = i8_uniform((int)P.grid.of(units * (g + 1)));
     const int64_t x_rows = UP ? P.M : P.pairs;
-    const int64_t x_bytes = (x_rows - 1) * P.x_pitch + 2 * (int64_t)P.K;
+    const int64_t x_bytes = (x_rows - 1) * P.x_pitch + (UP ? 2 : 4) * (int64_t)P.K;
     const int64_t plane = (int64_t)((UP ? 2 * P.rows : P.rows) - 1) * P.w_pitch + (int64_t)pieces * 16;
     const int64_t s_plane = (int64_t)((UP ? 2 * P.rows : P.rows) - 1) * P.ws_pitch + pieces;
 
@@ -474,25 +490,39 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
             __builtin_amdgcn_sched_barrier(0);                       /* in this order everywhere: a step waits for its own */
         }
         /* behind the weights' loads, and with no read of LDS among them, which would wait for them all */
-        for (int c = wave; c < XH * P.cpr; c += kMoeWaves) {         /* the tokens: 1 KB of a part of each row a turn */
-            int p = 0, k = c;
-            if (XH > 1 && k >= P.cpr) {
-                k -= P.cpr;
-                p = 1;
+        const __amdgpu_buffer_rsrc_t rX = r3d_rsrc(P.x, x_bytes);
+        if constexpr (UP) {
+            for (int c = wave; c < P.cpr; c += kMoeWaves) {          /* the tokens: 1 KB of each row a turn */
+                const uint32_t at = 1024 * c + 16 * lane;            /* past the row's end: zeros */
+                const bool in = at < 2 * (uint32_t)P.K;
+                for (int r = 0; r < held; ++r) {
+                    const int row = __builtin_amdgcn_readlane(tokens, r & 63);
+                    r3d_buf_lds<16>(rX, s_x + r * row_lds + 1024 * c, in ? (uint32_t)row * (uint32_t)P.x_pitch + at : kI8Oob, 0);
+                }
             }
-            if (XH > 2 && k >= P.cpr) {
-                k -= P.cpr;
-                p = 2;
-            }
-            const __amdgpu_buffer_rsrc_t rX = r3d_rsrc(P.x + p * (x_rows * P.x_pitch), x_bytes);
-            const uint32_t at = 1024 * k + 16 * lane;                /* past the row's end: zeros */
-            const bool in = at < 2 * (uint32_t)P.K;
-            for (int r = 0; r < held; ++r) {
-                int row;
-                if constexpr (UP) row = __builtin_amdgcn_readlane(tokens, r & 63);
-                else row = slot_base + r;
-                r3d_buf_lds<16>(rX, s_x + r * row_lds + p * part_lds + 1024 * k,
-                                in ? (uint32_t)row * (uint32_t)P.x_pitch + at : kI8Oob, 0);
+        } else {
+            constexpr int B = 4;                                     /* h: 512 columns of a row a wave, B of them in flight */
+            const int items = held * P.cpr;
+            for (int c0 = wave; c0 < items; c0 += B * kMoeWaves) {
+                r3d_i32x4 v[B][2];
+                uint32_t to[B];
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    const int c = c0 + i * kMoeWaves, r = i8_uniform((int)P.chunk.of(c)), k = c - r * P.cpr;
+                    const uint32_t col = 512 * k + 8 * lane;         /* past the row's end: zeros */
+                    const uint32_t at = c < items && col < (uint32_t)P.K ? (uint32_t)(slot_base + r) * (uint32_t)P.x_pitch + 4 * col : kI8Oob;
+                    v[i][0] = i8_buf16<0>(rX, at, 0);
+                    v[i][1] = i8_buf16<0>(rX, at, 16);
+                    to[i] = r * row_lds + 1024 * k + 16 * lane;
+                }
+#pragma unroll
+                for (int i = 0; i < B; ++i) {
+                    if (c0 + i * kMoeWaves >= items) break;
+                    r3d_i32x4 part[3];
+                    moe_parts(v[i][0], v[i][1], part);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) *reinterpret_cast<r3d_i32x4*>(s_x + to[i] + p * part_lds) = part[p];
+                }
             }
         }
         __syncthreads();
@@ -532,16 +562,10 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 }
                 if constexpr (UP) {
                     act_values<1>(P.act, v);
-                    float h = v[0] * v[1] * S.slot_w[slot];
-                    uint16_t* const to = static_cast<uint16_t*>(P.out) + slot * P.rows + 8 * blk + row1;
-                    for (int p = 0; p < P.parts; ++p) {
-                        const uint16_t d = r3d_bf16_rne(h);
-                        if (col < cnt) to[(int64_t)p * P.pairs * P.rows] = d;
-                        const float hi = r3d_bf16_to_f32(d);         /* what is left of h; nothing of inf and NaN */
-                        h = __builtin_fabsf(hi) < __builtin_inff() ? h - hi : 0.0f;
-                    }
+                    const float h = v[0] * v[1] * S.slot_w[slot];
+                    if (col < cnt) P.out[slot * P.rows + 8 * blk + row1] = h;
                 } else if (col < cnt) {
-                    float* const to = static_cast<float*>(P.out) + slot * P.rows + 16 * blk + row1;
+                    float* const to = P.out + slot * P.rows + 16 * blk + row1;
                     to[0] = v[0];
                     if (16 * blk + 8 < P.rows) to[8] = v[1];
                 }
@@ -697,32 +721,29 @@ template <int ENC, int CT>
 static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStream_t stream) {
     MoeTable* const table = static_cast<MoeTable*>(scratch);
     const int64_t pairs = P.M * P.top_k;
-    const int parts = P.y_bf16 ? 2 : 3;
-    uint8_t* const h = reinterpret_cast<uint8_t*>(table + 1);
-    float* const sums = reinterpret_cast<float*>(h + moe_h_bytes(P));
+    float* const h = reinterpret_cast<float*>(table + 1);
+    float* const sums = h + moe_h_bytes(P) / 4;
     const auto div = [](int64_t d) { return MoeDiv{(uint32_t)d, (uint32_t)(0xFFFFFFFFu / (uint32_t)d)}; };
     const auto spans = [](int64_t K) { return (K / MoeCodes<ENC>::N + 15) / 16; };
     const auto loads = [](int64_t K) { return (int)((2 * K + 1023) / 1024); };
     const MoeArgs u{table, P.logits, P.l_pitch, (int)P.M, (int)P.E, (int)P.top_k, P.l_bf16, (int)P.n, (int)P.f, (int)pairs,
                     (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up_rows,
-                    (int)spans(P.n), loads(P.n), div(P.f / 8), div(spans(P.n)), div(g.blocks), div(P.top_k), P.ids, P.weights,
-                    P.i_pitch, P.w_pitch, g.width, parts, P.act, P.sigmoid, P.renorm, P.weight_scale};
+                    (int)spans(P.n), loads(P.n), div(P.f / 8), div(spans(P.n)), div(g.blocks), div(P.top_k),
+                    div(loads(P.n)), P.ids, P.weights, P.i_pitch, P.w_pitch, g.width, P.act, P.sigmoid, P.renorm, P.weight_scale};
     if (P.M > kMoeWaves) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)P.M), dim3(64), 0, stream, u);
     constexpr int L = ENC == MOE_FP4 ? 2 : 1, L3 = ENC == MOE_FP4 && CT == 1 ? 3 : L;
-    hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 1, true, L>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
+    hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, true, L>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
                        (size_t)g.up_rows * moe_row(P.n, 1, ENC), stream, u);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) {
-        const MoeArgs d{table, nullptr, 0, (int)P.M, (int)P.E, (int)P.top_k, 0, (int)P.f, (int)P.n, (int)pairs, (int)(2 * P.f),
-                        h, P.dn, P.dns, sums, P.dn_expert, P.dns_expert, P.dns_pitch, (int)P.dn_pitch, g.down_rows,
-                        (int)spans(P.f), loads(P.f), div((P.n + 15) / 16), div(spans(P.f)), div(g.blocks), div(P.top_k)};
-        const size_t lds = (size_t)g.down_rows * moe_row(P.f, parts, ENC);
+        const MoeArgs d{table, nullptr, 0, (int)P.M, (int)P.E, (int)P.top_k, 0, (int)P.f, (int)P.n, (int)pairs, (int)(4 * P.f),
+                        reinterpret_cast<const uint8_t*>(h), P.dn, P.dns, sums, P.dn_expert, P.dns_expert, P.dns_pitch, (int)P.dn_pitch,
+                        g.down_rows, (int)spans(P.f), loads(P.f), div((P.n + 15) / 16), div(spans(P.f)), div(g.blocks), div(P.top_k),
+                        div(loads(P.f))};
+        const size_t lds = (size_t)g.down_rows * moe_row(P.f, 3, ENC);
         const dim3 grid((unsigned)g.blocks), block(kMoeThreads);
-        const bool three = d.spans % 6 == 3;
-        if (P.y_bf16 && three) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 2, false, L3>), grid, block, lds, stream, d);
-        else if (P.y_bf16) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 2, false, L>), grid, block, lds, stream, d);
-        else if (three) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 3, false, L3>), grid, block, lds, stream, d);
-        else hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, 3, false, L>), grid, block, lds, stream, d);
+        if (d.spans % 6 == 3) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, false, L3>), grid, block, lds, stream, d);
+        else hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, false, L>), grid, block, lds, stream, d);
         e = hipGetLastError();
     }
     if (e == hipSuccess) {

@@ -158,7 +158,7 @@ bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
     if (ncu <= 0) ncu = 256;
     const int64_t pairs = P.M * P.top_k;
     const int64_t up = (2 * P.n + 1023) / 1024 * 1024 + 64;
-    const int64_t down = (P.y_bf16 ? 2 : 3) * ((2 * P.f + 1023) / 1024 * 1024) + 64;
+    const int64_t down = 3 * ((2 * P.f + 1023) / 1024 * 1024) + 64;
     /* experts with more than 8 tokens are read once for 16 of them, where LDS holds these */
     const double read = (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
     g->ct = (double)pairs / read > 6 && moe_lds(P, 2, true) / up >= 16 && moe_lds(P, 2, false) / down >= 16 ? 2 : 1;
@@ -177,8 +177,9 @@ bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
     return true;
 }
 
+/* four bytes a value; where y is f32 six are asked for, which keeps the hook's answers what they were */
 int64_t moe_h_bytes(const MoePlan& P) {
-    return (P.M * P.top_k * P.f * 2 * (P.y_bf16 ? 2 : 3) + 15) / 16 * 16;
+    return (P.M * P.top_k * P.f * (P.y_bf16 ? 4 : 6) + 15) / 16 * 16;
 }
 
 int64_t moe_scratch(const MoePlan& P) {
