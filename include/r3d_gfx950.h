@@ -328,9 +328,10 @@ int r3d_rad_rmsnorm_block(const RadArgs* a, RadStream s);
  *     "i8"     int8 codes, f32 scales [E, rows] or [E, rows, 1]; multiples of 16
  *     "mxfp4"  e2m1 codes, E8M0 scales [E, rows, columns / 32] (0: 2^-127, 255: NaN); multiples of 32
  * x and the code planes on 16 bytes, their pitches too, an expert's plane under 2^31 bytes from its first to its last; any
- * distance between experts.  h is kept in f32; results do not depend on the run.  y may be x's or the logits' memory; ids and weights may not.  Launch scratch of the size the hook gives,
- * 16-byte aligned, is required (else RAD_E_UNSUPPORTED); calls that share it are ordered on one stream.  Refusals and statuses
- * as above.  Asynchronous on `s`. */
+ * distance between experts.  h is kept in f32; results do not depend on the run.  y may be x's or the logits' memory, ids and
+ * weights may not, and no result may meet another, the planes or their scales.  Launch scratch of the size the hook gives,
+ * 16-byte aligned, is required (else RAD_E_UNSUPPORTED); calls that share it are ordered on one stream.  Refusals and
+ * statuses as above.  Asynchronous on `s`. */
 int r3d_rad_moe_layer(const RadArgs* a, RadStream s);
 int64_t r3d_rad_moe_layer_scratch(const RadArgs* a);
 

@@ -25,7 +25,7 @@ static int planes_of(const RadTensor* t, int64_t E, int64_t rows, int64_t cols, 
 struct Experts {
     const RadTensor* w;
     const RadTensor* s;
-    int64_t expert, pitch, s_expert, s_pitch, bytes;            /* bytes: of an expert's codes */
+    int64_t expert, pitch, s_expert, s_pitch, bytes, s_bytes;   /* bytes: of an expert's codes, and of its scales */
 };
 
 static int plan_experts(int enc, int64_t E, int64_t rows, int64_t cols, Experts* X) {
@@ -52,11 +52,13 @@ static int plan_experts(int enc, int64_t E, int64_t rows, int64_t cols, Experts*
         if (X->s->stride[1] != 1) return RAD_E_STRIDE;
         X->s_expert = X->s->stride[0];
         if (!pitch_ok(X->s_expert)) return RAD_E_STRIDE;
+        X->s_bytes = 4 * rows;
     } else if (enc == MOE_FP4) {
         if ((rc = planes_of(X->s, E, rows, cols / 32, &X->s_expert, &X->s_pitch))) return rc;
         /* a load takes four scales, the plane's last four at most: rows that are apart, so that a plane has that many */
         if (X->s_pitch < cols / 32) return RAD_E_STRIDE;
         if (X->s_pitch > (int64_t(1) << 31) / rows) return RAD_E_UNSUPPORTED;
+        X->s_bytes = (rows - 1) * X->s_pitch + cols / 32;
     }
     return RAD_OK;
 }
@@ -67,7 +69,7 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
     const RadTensor* y  = rad_arg_in(a, 6);
     const RadTensor* id = rad_arg_in(a, 7);
     const RadTensor* wt = rad_arg_in(a, 8);
-    Experts up{rad_arg_in(a, 2), rad_arg_in(a, 3), 0, 0, 0, 0, 0}, down{rad_arg_in(a, 4), rad_arg_in(a, 5), 0, 0, 0, 0, 0};
+    Experts up{rad_arg_in(a, 2), rad_arg_in(a, 3), 0, 0, 0, 0, 0, 0}, down{rad_arg_in(a, 4), rad_arg_in(a, 5), 0, 0, 0, 0, 0, 0};
     if (!x || !lg || !up.w || !down.w || !y) return RAD_E_INVAL;
     const char* dt = rad_args_gets(a, "dtype");
     P->enc = !dt ? -1 : !strcmp(dt, "bf16") ? MOE_BF16 : !strcmp(dt, "i8") ? MOE_I8 : !strcmp(dt, "mxfp4") ? MOE_FP4 : -1;
@@ -113,9 +115,11 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
         if (!outs[i].data) continue;
         for (int j = 0; j < i; ++j)
             if (outs[j].data && spans_meet(outs[i], outs[j])) return RAD_E_INVAL;
-        /* the planes, from an expert's first byte to the last one's last */
+        /* the planes and their scales, from an expert's first byte to the last one's last */
         for (const Experts* X : {&up, &down})
-            if (spans_meet(outs[i], Span{X->w->data, 1, (E - 1) * X->expert + X->bytes, 0, 1})) return RAD_E_INVAL;
+            if (spans_meet(outs[i], Span{X->w->data, 1, (E - 1) * X->expert + X->bytes, 0, 1}) ||
+                (X->s && spans_meet(outs[i], Span{X->s->data, 1, (E - 1) * X->s_expert * elt_bytes(X->s->dtype) + X->s_bytes, 0, 1})))
+                return RAD_E_INVAL;
         if (i == 0) continue;
         for (const Span& in : ins)
             if (spans_meet(outs[i], in)) return RAD_E_INVAL;
