@@ -23,11 +23,21 @@ __device__ __forceinline__ float i8_sigmoid(float g) {
     return g != g ? g : r;
 }
 
-/* sigmoid(x) of 1 / (1 + 2^(-x log2 e)) as the hardware's exp2 and reciprocal give it (an ulp each): a relative error
- * of |x| 2^-24 in the lower tail, where the value is small; x sigmoid(x) is off by less than 6 2^-24 |x| everywhere.  Six
- * instructions for i8_sigmoid's eighteen: an epilogue over a large product's values is bound by them (2048 x 21504 x 5376,
- * int8, gelu_tanh: 267 -> 252 us). */
+/* sigmoid(x) = 1 / (1 + 2^(-x log2 e)) within 3 ulp where that is a normal number, under which it may be 0, in ten instructions for
+ * i8_sigmoid's eighteen: r of the rounded product by the hardware's exp2 and reciprocal (an ulp each), then what its rounding and
+ * the constant's left out, lo, by the slope: r - r (1 - r) ln 2 lo.  A NaN counts as a number: the caller's. */
 __device__ __forceinline__ float act_sigmoid(float x) {
+    const float c = __builtin_amdgcn_fmed3f(x, -1000.0f, 1000.0f);      /* inf - inf */
+    const float t = c * -1.44269504f;
+    const float lo = __builtin_fmaf(c, -1.92596299e-8f, __builtin_fmaf(c, -1.44269504f, -t));
+    const float r = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t));
+    return __builtin_fmaf(__builtin_fmaf(r, r, -r) * 0.693147181f, lo, r);
+}
+
+/* The same without lo: a relative error of 1.25 |x| 2^-24 more in the lower tail.  For an x whose own roundings count for more than
+ * that there (gelu_tanh's: 6 |x| 2^-24).  Six instructions fewer, and an epilogue over a large product's values is bound by
+ * them (2048 x 21504 x 5376, int8, us: silu 238 by this one, 242 by act_sigmoid; none 233, gelu_tanh 242). */
+__device__ __forceinline__ float act_sigmoid_of_rounded(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.44269504f));
 }
 
@@ -48,7 +58,7 @@ __device__ __forceinline__ void act_values(int act, float* v) {
             break;
         case ACT_SIGMOID:
 #pragma unroll
-            for (int i = 0; i < W; ++i) v[i] = act_sigmoid(v[i]);
+            for (int i = 0; i < W; ++i) v[i] = v[i] != v[i] ? v[i] : act_sigmoid(v[i]);
             break;
         case ACT_GELU:
 #pragma unroll
@@ -57,7 +67,7 @@ __device__ __forceinline__ void act_values(int act, float* v) {
         case ACT_GELU_TANH:
 #pragma unroll
             for (int i = 0; i < W; ++i)
-                v[i] *= act_sigmoid(v[i] * __builtin_fmaf(v[i] * v[i], 1.59576912f * 0.044715f, 1.59576912f));
+                v[i] *= act_sigmoid_of_rounded(v[i] * __builtin_fmaf(v[i] * v[i], 1.59576912f * 0.044715f, 1.59576912f));
             break;
         default: break;
     }
