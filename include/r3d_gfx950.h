@@ -322,7 +322,8 @@ int r3d_rad_rmsnorm_block(const RadArgs* a, RadStream s);
  * and a y of zeros.  Weights: softmax over the logits or a sigmoid of each (score), divided by the chosen ones' sum (renorm,
  * default 1), times weight_scale.  Then y = sum over the choices of W_down (weight * act(W_gate x) * (W_up x)).
  * Operands (x bf16 [M, n], logits f32/bf16 [M, E], gate_up [E, 2f, n]: f gate rows, then f up rows; gate_up_scale?, down [E, n,
- * f], down_scale?, y f32/bf16 [M, n], ids? i32 [M, top_k], weights? f32 [M, top_k]); params n, f, E (<= 512), top_k (<= 16),
+ * f], down_scale?, y f32/bf16 [M, n], ids? i32 [M, top_k], weights? f32 [M, top_k]); params n (<= 66560; i8: 62464), f (<= 65536),
+ * E (<= 512), top_k (<= 16),
  * dtype, act (as above; silu), score "softmax" or "sigmoid", renorm, weight_scale.  dtype:
  *     "bf16"   no scales; n, f multiples of 8
  *     "i8"     int8 codes, f32 scales [E, rows] or [E, rows, 1]; multiples of 16

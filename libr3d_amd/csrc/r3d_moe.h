@@ -18,13 +18,22 @@ enum { MOE_BF16 = 0, MOE_I8, MOE_FP4 };
 constexpr int kMoeMaxM = 64;            /* an expert's tokens are a 64-bit mask */
 constexpr int kMoeMaxE = 512;           /* a lane of a workgroup an expert */
 constexpr int kMoeMaxK = 16;            /* choices a token */
-constexpr int64_t kMoeMaxN = 1 << 19;   /* n and f: h of all pairs stays under 2^30 bytes */
+constexpr int64_t kMoeMaxN = 66560;     /* of one token's columns in LDS (int8, which keeps scales there too: 62464) */
+constexpr int64_t kMoeMaxF = 1 << 16;
 constexpr int kMoeMaxPairs = kMoeMaxM * kMoeMaxK;
+constexpr int kMoeMaxBlocks = 256, kMoeMinBlocks = 32;      /* compute units of a device, and of its smallest partition */
+/* h of all pairs lies under 32-bit offsets, units times workgroups under 2^32 (a unit is 8 rows of f or 16 of n), and
+ * a run's spans (128 columns at least) times a workgroup's 8 waves under 2^31 */
+static_assert(kMoeMaxPairs * kMoeMaxF * 4 <= int64_t(1) << 28, "h");
+static_assert(kMoeMaxPairs * (kMoeMaxF / 8) * (kMoeMaxBlocks + 1) < int64_t(1) << 32, "units of gate and up");
+static_assert(kMoeMaxPairs * ((kMoeMaxN + 15) / 16) * (kMoeMaxBlocks + 1) < int64_t(1) << 32, "units of down");
+static_assert((kMoeMaxPairs * (kMoeMaxF / 8) / kMoeMinBlocks + 1) * (kMoeMaxN / 128) * 8 < int64_t(1) << 31, "spans of gate and up");
+static_assert((kMoeMaxPairs * ((kMoeMaxN + 15) / 16) / kMoeMinBlocks + 1) * (kMoeMaxF / 128) * 8 < int64_t(1) << 31, "spans of down");
 
 /* What the first kernel leaves for the others at the head of the scratch; h and the slots' sums follow.  A slot is a
  * chosen (token, expert), in the experts' order. */
 struct MoeTable {
-    int32_t jobs;                       /* groups of an expert's tokens, in the experts' order */
+    int32_t jobs;                       /* the down kernel's groups of an expert's tokens, in the experts' order */
     int32_t pad[3];
     uint32_t job[kMoeMaxPairs];         /* expert | first slot << 9 | tokens << 20 */
     int16_t slot[kMoeMaxPairs];         /* by (token, choice); -1: none */
@@ -52,11 +61,18 @@ struct MoePlan {
 
 int plan_moe(const RadArgs* a, MoePlan* P);
 
-/* The launch on ncu compute units: tokens a job (in 8 ct columns), rows of them that LDS holds in each kernel. */
-struct MoeGeom {
-    int ct, width, up_rows, down_rows;
-    int64_t blocks;
+/* A product's launch: tokens a job (in 8 ct columns), and rows of them that LDS holds. */
+struct MoeTiles {
+    int ct, width, rows;
 };
+/* The launch on ncu compute units. */
+struct MoeGeom {
+    MoeTiles up, down;
+    int parts;                          /* down: launches, of `spans` spans of a row of h each (the last may have fewer) */
+    int64_t spans, blocks;
+};
+/* Columns of a span, 256 bytes of a row of an expert's plane. */
+constexpr int64_t moe_span(int enc) { return enc == MOE_BF16 ? 128 : enc == MOE_I8 ? 256 : 512; }
 /* false: LDS does not hold a single row */
 bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g);
 

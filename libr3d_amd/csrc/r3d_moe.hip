@@ -1,7 +1,7 @@
 /* r3d_moe.hip -- moe_layer on gfx950 (r3d_moe.h has the formulas): kernels and entry.
  *
- * Few tokens choose among many experts, so the chosen experts' planes are the work: each is to be read once, and
- * HBM bounds it.  A 16-byte load a lane brings a wave 256 bytes of 4 rows of a plane, a piece of 16 a
+ * Few tokens choose among many experts, so the chosen experts' planes are the work: each is read once for every 8 of its
+ * tokens (16 where many share it), for fewer where LDS does not hold as many of them, and HBM bounds it.  A 16-byte load a lane brings a wave 256 bytes of 4 rows of a plane, a piece of 16 a
  * lane, four lanes to 64 bytes of a row: the order of K in a product is free as long as both sides share it, so
  * v_mfma_f32_16x16x32_bf16 is fed with (row i / 4, pieces of class i % 4) against (token j / 4, class j % 4), and of the
  * 16 x 16 results those with i % 4 = j % 4 are wanted.  Three quarters of the matrix core's work is thrown away and it
@@ -13,7 +13,7 @@
  *   up    every workgroup makes the same choice from the logits for itself, a wave a token (3.4 us with the first loads,
  *         which costs less than a kernel of its own before this one; past 8 tokens, two rounds, a kernel of its own,
  *         a workgroup a token, costs less), so that it knows the jobs: an expert and some of its tokens.  A unit is a job's 8 gate and 8 up rows of f; h leaves with its weight, to its token's slot.
- *   down  a unit is a job's 16 rows of n; its sums leave to its tokens' slots in f32.
+ *   down  a unit is a job's 16 rows of n; its sums leave to its tokens' slots in f32.  Long rows of h may take several launches.
  *   sum   y of each token's slots, in the order of its choice: nothing is added in an order that changes from run to run.
  *
  * up and down are one kernel: the units lie in a row, and each workgroup, one a compute unit, takes an equal run of
@@ -69,8 +69,10 @@ struct MoeArgs {
     int32_t* ids;
     float* weights;
     int64_t i_pitch, wt_pitch;
-    int width, act, sigmoid, renorm;
+    MoeDiv width, down_width;           /* tokens a job */
+    int act, sigmoid, renorm;
     float weight_scale;
+    int add;                            /* down: to the sums of the columns before */
 };
 
 /* 16 bytes of codes: how many weights, and 16-byte pieces of bf16 that these become */
@@ -241,8 +243,8 @@ __global__ __launch_bounds__(64) void moe_route_kernel(MoeArgs P) {
     }
 }
 
-/* Choices of every token (or what moe_route_kernel made of them), then the experts' slots and jobs, `width` tokens each.
- * All lanes of the workgroup. */
+/* Choices of every token (or what moe_route_kernel made of them), then the experts' slots and jobs, up to `width` tokens each;
+ * workgroup 0 writes the down kernel's too, whose rows in LDS are longer or shorter.  All lanes of the workgroup. */
 __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     for (int i = tid; i < kMoeMaxE; i += kMoeThreads) S.mask[i] = 0;
@@ -271,24 +273,34 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
     }
     __syncthreads();
     if (wave == 0) {                                             /* a lane eight experts: slots and jobs before each */
-        uint32_t cnt[8], nj[8];
-        uint64_t own = 0;
+        uint32_t cnt[8];
+        uint64_t own = 0;                                        /* slots, jobs and the down kernel's jobs, 21 bits each */
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             cnt[i] = __popcll(S.mask[8 * lane + i]);
-            nj[i] = cnt[i] <= (uint32_t)P.width ? (cnt[i] > 0) : (cnt[i] + P.width - 1) / P.width;
-            own += (uint64_t)nj[i] << 32 | cnt[i];
+            own += (uint64_t)P.down_width.of(cnt[i] + P.down_width.d - 1) << 42 |
+                   (uint64_t)P.width.of(cnt[i] + P.width.d - 1) << 21 | cnt[i];
         }
         const uint64_t upto = r3d_wave_scan(own);
-        uint32_t slot = (uint32_t)(upto - own), j = (uint32_t)((upto - own) >> 32);
-        if (lane == 63) S.jobs = (int)(upto >> 32);
+        uint32_t slot = (uint32_t)(upto - own) & 0x1FFFFF;
+        auto write = [&](uint32_t* job, uint32_t j, const MoeDiv& width) __attribute__((always_inline)) {
+            uint32_t s = slot;
+            for (int i = 0; i < 8; ++i)
+                for (uint32_t left = cnt[i]; left > 0; ++j) {
+                    const uint32_t n = left < width.d ? left : width.d;
+                    job[j] = (uint32_t)(8 * lane + i) | s << 9 | n << 20;
+                    s += n;
+                    left -= n;
+                }
+        };
+        write(S.job, (uint32_t)((upto - own) >> 21) & 0x1FFFFF, P.width);
+        if (blockIdx.x == 0) write(P.table->job, (uint32_t)((upto - own) >> 42), P.down_width);
+        if (lane == 63) {
+            S.jobs = (int)(upto >> 21) & 0x1FFFFF;
+            if (blockIdx.x == 0) P.table->jobs = (int32_t)(upto >> 42);
+        }
         for (int i = 0; i < 8; ++i) {
             S.first[8 * lane + i] = (uint16_t)slot;
-            for (uint32_t left = cnt[i]; left > 0; ++j) {
-                const uint32_t n = left < (uint32_t)P.width ? left : P.width;
-                S.job[j] = (uint32_t)(8 * lane + i) | (slot + cnt[i] - left) << 9 | n << 20;
-                left -= n;
-            }
             slot += cnt[i];
         }
     }
@@ -305,8 +317,6 @@ __device__ __forceinline__ void moe_plan(const MoeArgs& P, MoeChoice& S) {
             P.table->slot[at] = (int16_t)slot;
             if (P.ids) P.ids[t * P.i_pitch + i] = e;
             if (P.weights) P.weights[t * P.wt_pitch + i] = S.w[at];
-            if (at < S.jobs) P.table->job[at] = S.job[at];
-            if (at == 0) P.table->jobs = S.jobs;
         }
     }
     __syncthreads();
@@ -395,7 +405,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
     /* a run an XCD, so that its L2 sees few jobs' tokens */
     const uint32_t G = P.grid.d, per = G >> 3, rem = G & 7, xcd = blockIdx.x & 7;
     const uint32_t g = xcd * per + (xcd < rem ? xcd : rem) + (blockIdx.x >> 3);
-    const uint32_t units = (uint32_t)jobs * nb;                      /* times G under 2^32: moe_geom */
+    const uint32_t units = (uint32_t)jobs * nb;                      /* times G under 2^32 (r3d_moe.h) */
     const int u_end = i8_uniform((int)P.grid.of(units * (g + 1)));
     const int64_t x_rows = UP ? P.M : P.pairs;
     const int64_t x_bytes = (x_rows - 1) * P.x_pitch + (UP ? 2 : 4) * (int64_t)P.K;
@@ -423,7 +433,7 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
             }
         }
         /* this wave's spans, L a step and a unit's last ones fewer */
-        const int total = (end - u) * spans;                         /* times 16 under 2^31: moe_geom */
+        const int total = (end - u) * spans;                         /* times 8 under 2^31 (r3d_moe.h) */
         const int a = i8_uniform(total * wave / kMoeWaves), b = i8_uniform(total * (wave + 1) / kMoeWaves);
         int tokens = 0;                                              /* of the rows to be held, a lane each */
         if constexpr (UP) tokens = lane < held ? S.tok[slot_base + lane] : 0;
@@ -566,8 +576,8 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                     if (col < cnt) P.out[slot * P.rows + 8 * blk + row1] = h;
                 } else if (col < cnt) {
                     float* const to = P.out + slot * P.rows + 16 * blk + row1;
-                    to[0] = v[0];
-                    if (16 * blk + 8 < P.rows) to[8] = v[1];
+                    to[0] = P.add ? to[0] + v[0] : v[0];
+                    if (16 * blk + 8 < P.rows) to[8] = P.add ? to[8] + v[1] : v[1];
                 }
             }
         };
@@ -717,7 +727,7 @@ __global__ __launch_bounds__(256) void moe_sum_kernel(const float* __restrict__ 
         *reinterpret_cast<r3d_f32x4_u4*>(static_cast<float*>(y) + m * y_pitch + c) = v;
 }
 
-template <int ENC, int CT>
+template <int ENC>
 static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStream_t stream) {
     MoeTable* const table = static_cast<MoeTable*>(scratch);
     const int64_t pairs = P.M * P.top_k;
@@ -727,23 +737,30 @@ static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStre
     const auto spans = [](int64_t K) { return (K / MoeCodes<ENC>::N + 15) / 16; };
     const auto loads = [](int64_t K) { return (int)((2 * K + 1023) / 1024); };
     const MoeArgs u{table, P.logits, P.l_pitch, (int)P.M, (int)P.E, (int)P.top_k, P.l_bf16, (int)P.n, (int)P.f, (int)pairs,
-                    (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up_rows,
+                    (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up.rows,
                     (int)spans(P.n), loads(P.n), div(P.f / 8), div(spans(P.n)), div(g.blocks), div(P.top_k),
-                    div(loads(P.n)), P.ids, P.weights, P.i_pitch, P.w_pitch, g.width, P.act, P.sigmoid, P.renorm, P.weight_scale};
+                    div(loads(P.n)), P.ids, P.weights, P.i_pitch, P.w_pitch, div(g.up.width), div(g.down.width), P.act, P.sigmoid, P.renorm, P.weight_scale};
     if (P.M > kMoeWaves) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)P.M), dim3(64), 0, stream, u);
-    constexpr int L = ENC == MOE_FP4 ? 2 : 1, L3 = ENC == MOE_FP4 && CT == 1 ? 3 : L;
-    hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, true, L>), dim3((unsigned)g.blocks), dim3(kMoeThreads),
-                       (size_t)g.up_rows * moe_row(P.n, 1, ENC), stream, u);
+    constexpr int L = ENC == MOE_FP4 ? 2 : 1, L3 = ENC == MOE_FP4 ? 3 : 1;
+    const dim3 grid((unsigned)g.blocks), block(kMoeThreads);
+    const size_t up_lds = (size_t)g.up.rows * moe_row(P.n, 1, ENC);
+    if (g.up.ct == 1) hipLaunchKernelGGL((moe_stream_kernel<ENC, 1, true, L>), grid, block, up_lds, stream, u);
+    else hipLaunchKernelGGL((moe_stream_kernel<ENC, 2, true, L>), grid, block, up_lds, stream, u);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess) {
-        const MoeArgs d{table, nullptr, 0, (int)P.M, (int)P.E, (int)P.top_k, 0, (int)P.f, (int)P.n, (int)pairs, (int)(4 * P.f),
-                        reinterpret_cast<const uint8_t*>(h), P.dn, P.dns, sums, P.dn_expert, P.dns_expert, P.dns_pitch, (int)P.dn_pitch,
-                        g.down_rows, (int)spans(P.f), loads(P.f), div((P.n + 15) / 16), div(spans(P.f)), div(g.blocks), div(P.top_k),
-                        div(loads(P.f))};
-        const size_t lds = (size_t)g.down_rows * moe_row(P.f, 3, ENC);
-        const dim3 grid((unsigned)g.blocks), block(kMoeThreads);
-        if (d.spans % 6 == 3) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, false, L3>), grid, block, lds, stream, d);
-        else hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, false, L>), grid, block, lds, stream, d);
+    for (int part = 0; part < g.parts && e == hipSuccess; ++part) {
+        const int64_t k0 = part * g.spans * moe_span(ENC), left = P.f - k0;
+        const int64_t K = part + 1 < g.parts ? g.spans * moe_span(ENC) : left;
+        MoeArgs d{table, nullptr, 0, (int)P.M, (int)P.E, (int)P.top_k, 0, (int)K, (int)P.n, (int)pairs, (int)(4 * P.f),
+                  reinterpret_cast<const uint8_t*>(h + k0), P.dn + part * g.spans * 256, P.dns, sums, P.dn_expert, P.dns_expert,
+                  P.dns_pitch, (int)P.dn_pitch, g.down.rows, (int)spans(K), loads(K), div((P.n + 15) / 16), div(spans(K)),
+                  div(g.blocks), div(P.top_k), div(loads(K))};
+        if (ENC == MOE_FP4) d.ws += part * g.spans * 16;
+        d.add = part > 0;
+        const size_t lds = (size_t)g.down.rows * moe_row(K, 3, ENC);
+        constexpr int CT = ENC == MOE_BF16 ? 2 : 1;
+        if (g.down.ct == 2) hipLaunchKernelGGL((moe_stream_kernel<ENC, CT, false, L>), grid, block, lds, stream, d);
+        else if (d.spans % 6 == 3) hipLaunchKernelGGL((moe_stream_kernel<ENC, 1, false, L3>), grid, block, lds, stream, d);
+        else hipLaunchKernelGGL((moe_stream_kernel<ENC, 1, false, L>), grid, block, lds, stream, d);
         e = hipGetLastError();
     }
     if (e == hipSuccess) {
@@ -764,13 +781,9 @@ static int moe_entry(const RadArgs* a, RadStream s) {
     MoeGeom g;
     if (!moe_geom(P, cu_count(), &g)) return RAD_E_UNSUPPORTED;
     hipStream_t t = (hipStream_t)s;
-#define R3D_MOE(ENC_)                                          \
-    return g.ct == 1 ? moe_launch<ENC_, 1>(P, g, a->scratch, t) \
-                     : moe_launch<ENC_, 2>(P, g, a->scratch, t)
-    if (P.enc == MOE_BF16) R3D_MOE(MOE_BF16);
-    if (P.enc == MOE_I8) R3D_MOE(MOE_I8);
-    R3D_MOE(MOE_FP4);
-#undef R3D_MOE
+    return P.enc == MOE_BF16 ? moe_launch<MOE_BF16>(P, g, a->scratch, t)
+           : P.enc == MOE_I8 ? moe_launch<MOE_I8>(P, g, a->scratch, t)
+                             : moe_launch<MOE_FP4>(P, g, a->scratch, t);
 }
 
 }  // namespace r3d

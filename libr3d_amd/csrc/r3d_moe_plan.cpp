@@ -86,7 +86,7 @@ int plan_moe(const RadArgs* a, MoePlan* P) {
     if (!rad_args_geti(a, "n", &n) || !rad_args_geti(a, "f", &f) || !rad_args_geti(a, "E", &E) ||
         !rad_args_geti(a, "top_k", &k) || n <= 0 || f <= 0 || E <= 0 || k <= 0 || n > kDimMax || f > kDimMax || k > E)
         return RAD_E_SHAPE;
-    if (E > kMoeMaxE || k > kMoeMaxK || n > kMoeMaxN || f > kMoeMaxN) return RAD_E_UNSUPPORTED;
+    if (E > kMoeMaxE || k > kMoeMaxK || n > kMoeMaxN || f > kMoeMaxF) return RAD_E_UNSUPPORTED;
     /* whole 16-byte pieces of codes (plan_experts), and 8 rows of an expert a wave */
     if ((n | f) & (P->enc == MOE_FP4 ? 31 : P->enc == MOE_I8 ? 15 : 7)) return RAD_E_UNSUPPORTED;
     const long long yn = rad_tensor_numel(y);
@@ -158,27 +158,51 @@ static int64_t moe_lds(const MoePlan& P, int ct, bool up) {
     return 160 * 1024 - (up ? 21 : 5) * 1024 - 8 * 1024 * ct - (P.enc == MOE_I8 ? 8 * 1024 : 0);
 }
 
+/* The tokens of a job, `row` bytes of LDS each: a job's part of the planes is read once for all of them, 8 at most, 16 where
+ * experts have more than 6 tokens (crowded) and LDS holds 16.  us of a call of 2048 x 1024, 16 and 8 in the gate and up product: 64
+ * experts top 8, M = 24 to 48 (3 to 6 tokens) mxfp4 59 to 66, 59 to 64, i8 79 to 90, 78 to 88, bf16 135 to 153, 134 to 148; M = 56, 64 mxfp4 67,
+ * 70 and 68, 74, i8 92, 100 and 95, 104, bf16 154, 161 and 158, 180.  In the down product, whose tokens are in three parts each, the
+ * second eight cost mxfp4 and int8 more matrix cycles (and registers) than a second read takes: M = 64 of 16 top 4, 8 and 16,
+ * mxfp4 42.4, 54.1, i8 48.9, 53.7, bf16 62.4, 62.6; of 64 top 8 60.7, 78.4; 73.2, 74.8; 121, 112; 4096 x 1024, 8 top 8 87, 96; 124, 118; 243, 210. */
+static bool moe_tiles(const MoePlan& P, bool up, int64_t row, bool crowded, MoeTiles* t) {
+    t->ct = crowded && (up || P.enc == MOE_BF16) && moe_lds(P, 2, up) / row >= 16 ? 2 : 1;
+    int64_t rows = moe_lds(P, t->ct, up) / row;
+    const int64_t pairs = P.M * P.top_k, most = pairs < 64 ? pairs : 64;      /* rows whose tokens lie in a wave's lanes */
+    if (rows > most) rows = most;
+    t->rows = (int)rows;
+    t->width = rows < 8 * t->ct ? (int)rows : 8 * t->ct;
+    return rows >= 1;
+}
+
 bool moe_geom(const MoePlan& P, int ncu, MoeGeom* g) {
-    if (ncu <= 0) ncu = 256;
-    const int64_t pairs = P.M * P.top_k;
-    const int64_t up = (2 * P.n + 1023) / 1024 * 1024 + 64;
-    const int64_t down = 3 * ((2 * P.f + 1023) / 1024 * 1024) + 64;
-    /* experts with more than 8 tokens are read once for 16 of them, where LDS holds these */
-    const double read = (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
-    g->ct = (double)pairs / read > 6 && moe_lds(P, 2, true) / up >= 16 && moe_lds(P, 2, false) / down >= 16 ? 2 : 1;
-    int64_t ur = moe_lds(P, g->ct, true) / up, dr = moe_lds(P, g->ct, false) / down;
-    const int64_t most = pairs < 64 ? pairs : 64;               /* rows whose tokens lie in a wave's lanes */
-    if (ur > most) ur = most;
-    if (dr > most) dr = most;
-    int64_t width = 8 * g->ct;
-    if (width > ur) width = ur;
-    if (width > dr) width = dr;
-    if (width < 1) return false;
-    g->width = (int)width;
-    g->up_rows = (int)ur;
-    g->down_rows = (int)dr;
+    if (ncu <= 0 || ncu > kMoeMaxBlocks) ncu = kMoeMaxBlocks;
     g->blocks = ncu;
-    return true;
+    /* experts that someone chose, and their tokens, of choices spread evenly */
+    const double read = (double)P.E * (1.0 - pow(1.0 - (double)P.top_k / (double)P.E, (double)P.M));
+    const double tokens = (double)(P.M * P.top_k) / read;
+    if (!moe_tiles(P, true, (2 * P.n + 1023) / 1024 * 1024 + 64, tokens > 6, &g->up)) return false;
+    /* LDS holds few tokens of a long row of h, and the planes would be read again for every few: the row may be cut into parts, a
+     * launch each, that add to the slots' sums.  A launch costs some 6 us, a read goes at 4.5 TB/s.  4096 x 14336, 8 experts top 2, us in
+     * 1, 2, 3, 4 and 6 parts: M = 64 mxfp4 760, 426, 397, 412, 418, i8 1167, 698, 632, 602, 592; M = 16 mxfp4 238, 177, 172, 179, 187;
+     * M = 1 46, 53, 60, 65, 79.  Of 28 such calls the parts taken were 6 % from the best at most.  More than 8 tokens are not worth
+     * another launch: bf16 4096 x 2048, M = 64, 150 in one, 157 in two with 16; x 3584 261 and 267. */
+    const int64_t span = moe_span(P.enc), spans = (P.f + span - 1) / span;
+    const double plane = (double)P.n * (double)P.f * (P.enc == MOE_BF16 ? 2.0 : P.enc == MOE_I8 ? 1.0 : 0.53);
+    double best = 0.0;
+    g->parts = 0;
+    for (int64_t parts = 1; parts <= 16 && parts <= spans && (g->parts == 0 || g->down.width < 8); ++parts) {
+        const int64_t each = (spans + parts - 1) / parts, K = parts == 1 ? P.f : each * span;
+        MoeTiles t;
+        if (!moe_tiles(P, false, 3 * ((2 * K + 1023) / 1024 * 1024) + 64, tokens > 6, &t)) continue;
+        const double reads = tokens > t.width ? (tokens + 0.5 * (t.width - 1)) / t.width : 1.0;
+        const double us = 6.0 * (double)parts + reads * read * plane / 4.5e6;
+        if (g->parts > 0 && us >= best) continue;
+        best = us;
+        g->down = t;
+        g->parts = (int)((spans + each - 1) / each);
+        g->spans = each;
+    }
+    return g->parts > 0;
 }
 
 /* four bytes a value; where y is f32 six are asked for, which keeps the hook's answers what they were */
@@ -195,7 +219,7 @@ int64_t moe_scratch_bytes(const RadArgs* a) {
     if (plan_moe(a, &P) == RAD_OK) return moe_scratch(P);
     long long n = 0, f = 0, k = 0, M = 0;                       /* not a whole call yet: y in f32 */
     if (!rad_args_geti(a, "n", &n) || !rad_args_geti(a, "f", &f) || !rad_args_geti(a, "top_k", &k) || n <= 0 || f <= 0 ||
-        k <= 0 || n > kMoeMaxN || f > kMoeMaxN || k > kMoeMaxK)
+        k <= 0 || n > kMoeMaxN || f > kMoeMaxF || k > kMoeMaxK)
         return 0;
     const RadTensor* y = rad_arg_in(a, 6);
     if (y) M = rad_tensor_numel(y) / n;
@@ -224,10 +248,10 @@ int describe_moe(const char* row, const RadArgs* a, char* buf, int len) {
         snprintf(buf, (size_t)len, "refused rc=%d (LDS)", RAD_E_UNSUPPORTED);
         return RAD_E_UNSUPPORTED;
     }
-    snprintf(buf, (size_t)len, "arm=moe enc=%s M=%lld n=%lld f=%lld E=%lld top_k=%lld score=%s renorm=%d act=%d y=%s ct=%d "
-             "width=%d up_rows=%d down_rows=%d blocks=%lld", kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
+    snprintf(buf, (size_t)len, "arm=moe enc=%s M=%lld n=%lld f=%lld E=%lld top_k=%lld score=%s renorm=%d act=%d y=%s up_ct=%d "
+             "up_width=%d up_rows=%d down_ct=%d down_width=%d down_rows=%d parts=%d blocks=%lld", kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
              (long long)P.E, (long long)P.top_k, P.sigmoid ? "sigmoid" : "softmax", P.renorm, P.act,
-             P.y_bf16 ? "bf16" : "f32", g.ct, g.width, g.up_rows, g.down_rows, (long long)g.blocks);
+             P.y_bf16 ? "bf16" : "f32", g.up.ct, g.up.width, g.up.rows, g.down.ct, g.down.width, g.down.rows, g.parts, (long long)g.blocks);
     return RAD_OK;
 }
 

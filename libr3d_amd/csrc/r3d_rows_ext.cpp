@@ -294,9 +294,10 @@ const RadKernelInfo kRows[] = {
      r3d_rad_rmsnorm_block, nullptr, nullptr, nullptr, nullptr, nullptr},
     {"moe_layer", "moe_layer", "gemm",
      "a mixture-of-experts layer for up to 64 tokens: choice and gate/up products with their activation, then "
-     "down products and the weighted sum; the chosen experts' planes are streamed once, codes become bf16 in registers",
-     "E up to 512, top_k up to 16, n and f multiples of 8 (bf16), 16 (i8) or 32 (mxfp4); x and the code planes on 16 "
-     "bytes; launch scratch of the size the hook asks for (16-byte aligned) required",
+     "down products and the weighted sum; the chosen experts' planes are streamed, once for every 8 or 16 of an expert's "
+     "tokens (fewer where n is over 8192 or so), codes become bf16 in registers",
+     "E up to 512, top_k up to 16, n and f multiples of 8 (bf16), 16 (i8) or 32 (mxfp4), n up to 66560 (i8: 62464), f up to "
+     "65536; x and the code planes on 16 bytes; launch scratch of the size the hook asks for (16-byte aligned) required",
      "bf16 x, f32/bf16 logits [M, E], gate_up [E, 2f, n] (gate rows, then up) and down [E, n, f] in bf16, in int8 with f32 "
      "scales [E, rows], or in e2m1 with E8M0 scales [E, rows, K / 32]; f32/bf16 y, i32 ids and f32 weights [M, top_k]",
      RAD_DOMAIN_DEVICE, kPrioTile, cMoe, 2, nullptr, 0, nullptr, nullptr, nullptr,
