@@ -118,14 +118,16 @@ __global__ __launch_bounds__(1024) void block_kernel(BlockArgs P) {
 #pragma unroll
         for (int c = 0; c < C; ++c) r[c] = i8_ld8<true>(rr, i0 + c * step, n);
     }
-    if (P.gate_kind == BLOCK_GATE_ROWS) {
+    /* f32 weights are twice the registers: past two chunks their gate waits for the first sum (with every load before it four
+     * chunks spilled 17 to 25 registers: 2048 x 8192 41.7 us for 24.6, with a gate an element 51.3 for 38.4) */
+    constexpr bool EARLY_GATE = WBF16 || C <= 2, EARLY = C <= (WBF16 ? 2 : 1);
+    if (EARLY_GATE && P.gate_kind == BLOCK_GATE_ROWS) {
 #pragma unroll
         for (int c = 0; c < C; ++c) g[c] = i8_ld8<WBF16>(gr, i0 + c * step, n);
     }
     float gt = 1.0f;
     if (P.gate_kind == BLOCK_GATE_TOKEN)
         gt = WBF16 ? r3d_bf16_to_f32(*reinterpret_cast<const uint16_t*>(gr)) : *reinterpret_cast<const float*>(gr);
-    constexpr bool EARLY = C <= 2;
     if (EARLY && P.w_pre) {
 #pragma unroll
         for (int c = 0; c < C; ++c) wn[c] = i8_ld8<WBF16>(P.w_pre, i0 + c * step, n);
@@ -146,6 +148,10 @@ __global__ __launch_bounds__(1024) void block_kernel(BlockArgs P) {
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[c][j] = __fmul_rn(__fmul_rn(h[c][j], rs), __fadd_rn(wp[c].at(j), P.wadd));
+    }
+    if (!EARLY_GATE && P.gate_kind == BLOCK_GATE_ROWS) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) g[c] = i8_ld8<WBF16>(gr, i0 + c * step, n);
     }
     if (P.gate_kind == BLOCK_GATE_ROWS) {
 #pragma unroll

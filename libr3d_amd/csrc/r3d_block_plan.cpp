@@ -132,17 +132,22 @@ BlockGeom block_geom(int64_t rows, int64_t n) {
     const int64_t nc = (n + 7) / 8;
     auto lanes = [&](int c) { return (int)(((nc + c - 1) / c + 63) / 64 * 64); };
     /* Few values: one row's chain, as few chunks a lane as some 768 lanes allow.  us at the chunks named, 64 rows of n:
-     *     2048     1: 3.5   2: 3.8   4: 4.4        5376     1: 5.3   2: 5.9   3: 5.7
-     *     8192     1: 6.0   2: 5.5   4: 5.6       16384     2: 7.9   3: 8.5   4: 7.5 */
+     *     2048     1: 3.5   2: 3.8   4: 4.4        5376     1: 5.5   2: 6.0   3: 5.9
+     *     8192     1: 5.9   2: 5.5   4: 5.7       16384     2: 7.9   3: 8.5   4: 7.5
+     * and on both sides of the limit, f32 weights within 4 % of these:
+     *     256 x 5376 (172032)  1: 6.9  2: 7.4  3: 7.2      333 x 5376 (223776)   1: 8.7  2: 9.1  3: 8.1
+     *     512 x 2048 (131072)  1: 5.2  2: 5.5  4: 5.7      1024 x 2048 (262144)  1: 7.1  2: 6.7  4: 6.6
+     *     333 x 4096 (170496)  1: 6.5  2: 6.1  4: 7.2      512 x 4096 (262144)   1: 7.3  2: 6.9  4: 7.9 (taken, the worst case) */
     if (rows * nc < 200000) {
         const int c = nc <= 768 ? 1 : nc <= 1536 ? 2 : 4;
         return BlockGeom{lanes(c), c, 0};
     }
-    /* Many: as many chunks in flight a compute unit as its registers hold (32, 28, 20 and 16 waves at 1 to 4 chunks a lane),
-     * fewer a lane where they tie.  2048 rows:
-     *     1024     1: 6.1   2: 5.6   3: 7.2   4: 8.7        5376     1: 28.9  2: 24.0  3: 20.4  4: 20.8
-     *     2560     1: 12.2  2: 10.7  3: 10.2  4: 11.9       8192     1: 29.0  2: 23.4  3: 31.2  4: 22.6
-     *     4096     1: 15.0  2: 13.1  3: 15.8  4: 12.1      16384     2: 59.3  3: 63.6  4: 44.8 */
+    /* Many: as many chunks in flight a compute unit as registers hold, fewer a lane where they tie.  The waves are the kernel's with
+     * bf16 weights (32, 28, 20 and 16 at 1 to 4 chunks a lane); f32 weights hold 32, 20, 16 to 20 and 16 and are as fast by the same
+     * choice (2048 rows of 5376 22.6, 2560 13.9, 8192 24.6 us).  2048 rows, results as below:
+     *     1024     1: 6.9   2: 6.3   3: 7.9   4: 9.4        5376     1: 28.1  2: 24.5  3: 20.8  4: 21.1
+     *     2560     1: 14.8  2: 14.8  3: 14.1  4: 15.9       8192     1: 29.8  2: 24.2  3: 31.3  4: 23.4
+     *     4096     1: 14.8  2: 12.9  3: 16.0  4: 12.0       16384 (1024 rows)   2: 33.4  3: 34.8  4: 25.4 */
     static const int kWaves[] = {0, 32, 28, 20, 16};
     int best = 4;
     int64_t most = 0;
@@ -153,9 +158,10 @@ BlockGeom block_geom(int64_t rows, int64_t n) {
             best = c;
         }
     }
-    /* Two results of more than the 32 MB of the XCDs' L2 are written past the caches, which they would only fill: 2048 x 5376
-     * 24.3 -> 20.4 us, with a product of 2048 columns behind it 76.2 -> 74.4.  Smaller ones are still there when that product
-     * asks for them: 512 x 5376 and 2048 columns 32.5 us, past the caches 39.0. */
+    /* From 2^20 chunks on, where two bf16 results fill the 32 MB of the XCDs' L2, results of every kind are written past the caches: alone
+     * 2048 x 5376 24.2 -> 20.8 us; with a product of 2048 columns behind, whose weights come from HBM, 76.2 -> 73.3, int8 codes 55.3 ->
+     * 52.4, one bf16 result 71.6 -> 70.4, f32 45.5 -> 44.3 (a pass over them behind).  It costs where that product's weights are still in the
+     * 256 MB before HBM: 60.6 -> 71.5, and at 512 x 5376, which stays under the limit, 31.7 -> 38.4 (from HBM 41.9 -> 40.0). */
     return BlockGeom{lanes(best), best, rows * nc >= (1 << 20)};
 }
 
