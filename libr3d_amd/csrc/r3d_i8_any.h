@@ -39,7 +39,7 @@ __device__ __forceinline__ r3d_i32x4 i8_keep(r3d_i32x4 v, int left) {
 
 /* What a product's kernels are made for: the matrix instructions over 16-byte operand pieces (64 int8
  * codes or 32 bf16 of K in the four lanes of a row: the same bytes in the same lanes), their sums, and what
- * happens to these.  I8Ops is gemm_nt_q at i8a8; gemm_nt_epi's are in r3d_epi_dev.h. */
+ * happens to these.  I8Ops is gemm_nt_q at i8a8; gemm_nt_epi's are in r3d_epi_ops.h. */
 struct I8GemvArgs;
 struct I8TileArgs;
 typedef int r3d_i32x16 __attribute__((ext_vector_type(16)));

@@ -110,8 +110,9 @@ static double i8_tile_ns(const I8Cost& c, const I8Plan& P, int64_t per, int64_t 
  * cheaper of it and a tile is 1.0 % slower than the best launch, the GEMV wherever it fits 3.4 % (8 x 8192 x
  * 5376 12.1 -> 10.4 us on tiles of 32 rows; up to 3 tokens it is the faster one nearly everywhere).
  * gemm_nt_epi counts one thing more: with a workgroup a compute unit or less, a wave's chain of `per` lines may be longer than
- * all that (bytes of a row; 1 x 128 x 43008 13.0 us, on tiles with 24 planes 7.8; 1 x 512 x 21504 8.5 and 7.5; 1 x 128 x 10752
- * 5.3 and 5.6). */
+ * all that.  us by the GEMV and on tiles, 128 rows of 10752, 21504 and 43008 bytes: 1 token 5.7, 6.9; 8.4, 7.8; 13.4, 8.6; 2 tokens 6.0,
+ * 7.1; 9.0, 7.6; 4 tokens 6.6, 7.2 (past that its LDS holds no more tokens); 1024 rows 1 token 6.2, 7.6; 8.7, 9.4; 13.7, 12.3.  Of 24 such
+ * shapes, 128 to 1024 rows, bf16 and int8, at 1, 2, 4 and 8 tokens each takes its faster one, ties within 2 % aside. */
 static double i8_gemv_ns(const I8Plan& P, int ncu, const I8Geom& g) {
     const double lines = (double)((P.N + 7) / 8) * ((P.K + 127) / 128) / ncu;
     const double chain = P.chain && g.blocks <= ncu ? 165.0 * (1.0 + 0.06 * P.M) * g.per : 0.0;
