@@ -1,4 +1,5 @@
-/* r3d_moe.h -- host-side plan of moe_layer: a mixture-of-experts layer for a few tokens, in three kernels (past 8 tokens four).
+/* r3d_moe.h -- host-side plan of moe_layer: a mixture-of-experts layer for a few tokens, in three launches (past 8 tokens four, and
+ * more where an expert is wide).
  *     choice   the top_k largest router logits of a token, by falling logit, ties to the lower index
  *     weights  softmax over the logits, or a sigmoid of each; of the chosen ones' sum where renorm; times weight_scale
  *     h        weight * act(W_gate x) * (W_up x)          the chosen expert's f rows each

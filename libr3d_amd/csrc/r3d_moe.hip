@@ -28,7 +28,7 @@
  *
  * Measured on MI355X (tokens x choices / experts): 1 x 8 / 128 mxfp4, 5376 x 1344 32.3 us and 4 x 4 / 64 int8, 2048 x 768 25, each
  * launch's beginning and end 6 to 7 us of it; 13 x 4 / 32 bf16, 2048 x 1408 77 to 84, 5.3 to 5.8 TB/s; 64 x 8 / 128 mxfp4 300 to
- * 304, gate and up 5.8 TB/s, down 4.1 (rows of 672 bytes share lines, and jobs past four tokens take a second tile). */
+ * 307, gate and up 5.8 TB/s, down 3.6 (three parts, and jobs past four tokens take a second tile). */
 #include <hip/hip_runtime.h>
 
 #include <stdio.h>
@@ -367,8 +367,8 @@ constexpr int moe_row(int64_t K, int parts, int enc) {
 }
 
 /* L spans of 4 KB a step.  A row's last step may be short, and what it lacks is missing in flight: e2m1 takes two a step, and
- * three where a row of y has three, nine, .. (64 x 8 / 128, f = 1344 295 -> 285 us; 64 x 4 / 64, n = 4096, f = 1536 127 -> 125, but
- * 2048 161 -> 164, and one token 0.3 us more).  The others have two steps of one in flight. */
+ * three where a row of h has three, nine, .. (f = 1344, top 8 of 128: 64 tokens 315 -> 301 us, 8 105 -> 102, one 32.6 -> 32.7; 64 x 4 /
+ * 64, n = 4096, f = 1536 137.6 -> 137.2; elsewhere three are up to 2 % slower).  The others have two steps of one in flight. */
 template <int ENC, int CT, bool UP, int L>
 __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
     constexpr int N = MoeCodes<ENC>::N, X = MoeCodes<ENC>::X, XH = UP ? 1 : 3;   /* parts of a token's values */

@@ -101,3 +101,40 @@ def test_steps_of_three_spans(gpu, f):
     for M, n in ((1, 64), (6, 96), (30, 48 * 32)):
         for y in ("bf16", "f32"):
             run(gpu, "mxfp4", M, n, f, 5, 2, y=y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_parts_of_padded_planes(gpu, dtype):
+    """Rows and planes of the experts further apart than their columns, and h in parts."""
+    M, n, f, E, k = 60, 2048, 9 * 512 + 32, 2, 1
+    logits = crowd(M, E, k, 100)
+    assert case(dtype, M, n, f, E, k, logits)[0]["parts"] > 1
+    run(gpu, dtype, M, n, f, E, k, y="f32", logits=logits, extra=32, pad=3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_parts_captured(gpu, dtype):
+    """A call of several down launches, captured once and replayed over new tokens with other work between, bit for bit as called."""
+    M, n, f, E, k = 64, 512, 14336, 2, 2
+    assert case(dtype, M, n, f, E, k, crowd(M, E, k, 100))[0]["parts"] > 1
+    t = inputs(dtype, M, n, f, E)
+    on = {m: None if v is None else v.to(gpu) for m, v in t.items()}
+    y = torch.zeros(M, n, device=gpu)
+    ops = R.MoeLayerOperands(y=y, dtype=dtype, n=n, f=f, E=E, top_k=k, **on)
+    ops.set_scratch(torch.full((R.row_scratch_bytes("moe_layer", ops),), 0xA5, dtype=torch.uint8, device=gpu))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        assert R.launch_row("moe_layer", ops, torch.cuda.current_stream().cuda_stream) == R.RAD_OK
+    for i in range(3):
+        g = torch.Generator().manual_seed(i)
+        on["x"].copy_(torch.randn(M, n, generator=g).bfloat16())
+        on["logits"].copy_(torch.randn(M, E, generator=g))
+        y.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        _, _, _, want, err = U.exact(**on, dtype=dtype, f=f, top_k=k, parts=3)
+        U.E.check(y, want, err)
+        again = torch.zeros_like(y)
+        assert R.moe_layer(y=again, dtype=dtype, n=n, f=f, E=E, top_k=k, **on) == R.RAD_OK
+        torch.cuda.synchronize()
+        assert torch.equal(y, again)
