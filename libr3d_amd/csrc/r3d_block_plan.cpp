@@ -160,8 +160,8 @@ BlockGeom block_geom(int64_t rows, int64_t n) {
     }
     /* From 2^20 chunks on, where two bf16 results fill the 32 MB of the XCDs' L2, results of every kind are written past the caches: alone
      * 2048 x 5376 24.2 -> 20.8 us; with a product of 2048 columns behind, whose weights come from HBM, 76.2 -> 73.3, int8 codes 55.3 ->
-     * 52.4, one bf16 result 71.6 -> 70.4, f32 45.5 -> 44.3 (a pass over them behind).  It costs where that product's weights are still in the
-     * 256 MB before HBM: 60.6 -> 71.5, and at 512 x 5376, which stays under the limit, 31.7 -> 38.4 (from HBM 41.9 -> 40.0). */
+     * 52.4, one bf16 result 71.6 -> 70.4, f32 45.5 -> 44.3 (a pass over them behind).  It costs where that product's weights are
+     * still in the 256 MB before HBM: 60.6 -> 71.5, and at 512 x 5376, which stays under the limit, 31.7 -> 38.4 (from HBM 41.9 -> 40.0). */
     return BlockGeom{lanes(best), best, rows * nc >= (1 << 20)};
 }
 

@@ -1,14 +1,15 @@
 /* r3d_moe.hip -- moe_layer on gfx950 (r3d_moe.h has the formulas): kernels and entry.
  *
- * Few tokens choose among many experts, so the chosen experts' planes are the work: each is read once for every 8 of its
- * tokens (16 where many share it), for fewer where LDS does not hold as many of them, and HBM bounds it.  A 16-byte load a lane brings a wave 256 bytes of 4 rows of a plane, a piece of 16 a
- * lane, four lanes to 64 bytes of a row: the order of K in a product is free as long as both sides share it, so
- * v_mfma_f32_16x16x32_bf16 is fed with (row i / 4, pieces of class i % 4) against (token j / 4, class j % 4), and of the
- * 16 x 16 results those with i % 4 = j % 4 are wanted.  Three quarters of the matrix core's work is thrown away and it
- * still idles; the loads are what counts, and the cache looks up 64 bytes at a time only where lanes beside each other ask
- * for them (with 128 bytes of 8 rows a load, two lanes beside each other: 28 look-ups for 16, 57 cycles a load, which
- * bound it).  Codes become bf16 in registers: int8 and e2m1 with its E8M0 scale are exact there (E8M0 0 is 2^-127, 255 NaN,
- * and what leaves bf16's range infinite), so the sums are f32 sums of exact products.
+ * Few tokens choose among many experts, so the chosen experts' planes are the work: each is read once for every 8 of
+ * its tokens (16 where many share it), for fewer where LDS does not hold as many of them, and HBM bounds it.  A 16-byte
+ * load a lane brings a wave 256 bytes of 4 rows of a plane, a piece of 16 a lane, four lanes to 64 bytes of a row: the
+ * order of K in a product is free as long as both sides share it, so v_mfma_f32_16x16x32_bf16 is fed with (row i / 4,
+ * pieces of class i % 4) against (token j / 4, class j % 4), and of the 16 x 16 results those with i % 4 = j % 4 are
+ * wanted.  Three quarters of the matrix core's work is thrown away and it still idles; the loads are what counts, and
+ * the cache looks up 64 bytes at a time only where lanes beside each other ask for them (with 128 bytes of 8 rows a
+ * load, two lanes beside each other: 28 look-ups for 16, 57 cycles a load, which bound it).  Codes become bf16 in
+ * registers: int8 and e2m1 with its E8M0 scale are exact there (E8M0 0 is 2^-127, 255 NaN, and what leaves bf16's range
+ * infinite), so the sums are f32 sums of exact products.
  *
  *   up    every workgroup makes the same choice from the logits for itself, a wave a token (3.4 us with the first loads,
  *         which costs less than a kernel of its own before this one; past 8 tokens, two rounds, a kernel of its own,
@@ -520,7 +521,8 @@ __global__ __launch_bounds__(kMoeThreads) void moe_stream_kernel(MoeArgs P) {
                 for (int i = 0; i < B; ++i) {
                     const int c = c0 + i * kMoeWaves, r = i8_uniform((int)P.chunk.of(c)), k = c - r * P.cpr;
                     const uint32_t col = 512 * k + 8 * lane;         /* past the row's end: zeros */
-                    const uint32_t at = c < items && col < (uint32_t)P.K ? (uint32_t)(slot_base + r) * (uint32_t)P.x_pitch + 4 * col : kI8Oob;
+                    const bool in = c < items && col < (uint32_t)P.K;
+                    const uint32_t at = in ? (uint32_t)(slot_base + r) * (uint32_t)P.x_pitch + 4 * col : kI8Oob;
                     v[i][0] = i8_buf16<0>(rX, at, 0);
                     v[i][1] = i8_buf16<0>(rX, at, 16);
                     to[i] = r * row_lds + 1024 * k + 16 * lane;
@@ -739,7 +741,8 @@ static int moe_launch(const MoePlan& P, const MoeGeom& g, void* scratch, hipStre
     const MoeArgs u{table, P.logits, P.l_pitch, (int)P.M, (int)P.E, (int)P.top_k, P.l_bf16, (int)P.n, (int)P.f, (int)pairs,
                     (int)P.x_pitch, P.x, P.gu, P.gus, h, P.gu_expert, P.gus_expert, P.gus_pitch, (int)P.gu_pitch, g.up.rows,
                     (int)spans(P.n), loads(P.n), div(P.f / 8), div(spans(P.n)), div(g.blocks), div(P.top_k),
-                    div(loads(P.n)), P.ids, P.weights, P.i_pitch, P.w_pitch, div(g.up.width), div(g.down.width), P.act, P.sigmoid, P.renorm, P.weight_scale};
+                    div(loads(P.n)), P.ids, P.weights, P.i_pitch, P.w_pitch, div(g.up.width), div(g.down.width), P.act, P.sigmoid,
+                    P.renorm, P.weight_scale};
     if (P.M > kMoeWaves) hipLaunchKernelGGL(moe_route_kernel, dim3((unsigned)P.M), dim3(64), 0, stream, u);
     constexpr int L = ENC == MOE_FP4 ? 2 : 1, L3 = ENC == MOE_FP4 ? 3 : 1;
     const dim3 grid((unsigned)g.blocks), block(kMoeThreads);

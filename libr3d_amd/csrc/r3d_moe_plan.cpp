@@ -159,11 +159,15 @@ static int64_t moe_lds(const MoePlan& P, int ct, bool up) {
 }
 
 /* The tokens of a job, `row` bytes of LDS each: a job's part of the planes is read once for all of them, 8 at most, 16 where
- * experts have more than 6 tokens (crowded) and LDS holds 16.  us of a call of 2048 x 1024, 16 and 8 in the gate and up product: 64
- * experts top 8, M = 24 to 48 (3 to 6 tokens) mxfp4 59 to 66, 59 to 64, i8 79 to 90, 78 to 88, bf16 135 to 153, 134 to 148; M = 56, 64 mxfp4 67,
- * 70 and 68, 74, i8 92, 100 and 95, 104, bf16 154, 161 and 158, 180.  In the down product, whose tokens are in three parts each, the
- * second eight cost mxfp4 and int8 more matrix cycles (and registers) than a second read takes: M = 64 of 16 top 4, 8 and 16,
- * mxfp4 42.4, 54.1, i8 48.9, 53.7, bf16 62.4, 62.6; of 64 top 8 60.7, 78.4; 73.2, 74.8; 121, 112; 4096 x 1024, 8 top 8 87, 96; 124, 118; 243, 210. */
+ * experts have more than 6 tokens (crowded) and LDS holds 16.  us of a call of 2048 x 1024, 64 experts top 8, with 16 and 8 in the
+ * gate and up product:
+ *     M = 24 to 48 (3 to 6 tokens)   mxfp4 59 to 66, 59 to 64      i8 79 to 90, 78 to 88      bf16 135 to 153, 134 to 148
+ *     M = 56 and 64                  mxfp4 67 and 70, 68 and 74    i8 92 and 100, 95 and 104  bf16 154 and 161, 158 and 180
+ * In the down product, whose tokens are in three parts each, the second eight cost mxfp4 and int8 more matrix cycles (and
+ * registers) than a second read takes.  M = 64, with 8 and 16:
+ *     2048 x 1024, 16 experts top 4  mxfp4 42.4, 54.1              i8 48.9, 53.7              bf16 62.4, 62.6
+ *     2048 x 768, 64 experts top 8   mxfp4 60.7, 78.4              i8 73.2, 74.8              bf16 121, 112
+ *     4096 x 1024, 8 experts top 8   mxfp4 87, 96                  i8 124, 118                bf16 243, 210 */
 static bool moe_tiles(const MoePlan& P, bool up, int64_t row, bool crowded, MoeTiles* t) {
     t->ct = crowded && (up || P.enc == MOE_BF16) && moe_lds(P, 2, up) / row >= 16 ? 2 : 1;
     int64_t rows = moe_lds(P, t->ct, up) / row;
@@ -249,7 +253,8 @@ int describe_moe(const char* row, const RadArgs* a, char* buf, int len) {
         return RAD_E_UNSUPPORTED;
     }
     snprintf(buf, (size_t)len, "arm=moe enc=%s M=%lld n=%lld f=%lld E=%lld top_k=%lld score=%s renorm=%d act=%d y=%s up_ct=%d "
-             "up_width=%d up_rows=%d down_ct=%d down_width=%d down_rows=%d parts=%d blocks=%lld", kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
+             "up_width=%d up_rows=%d down_ct=%d down_width=%d down_rows=%d parts=%d blocks=%lld",
+             kEnc[P.enc], (long long)P.M, (long long)P.n, (long long)P.f,
              (long long)P.E, (long long)P.top_k, P.sigmoid ? "sigmoid" : "softmax", P.renorm, P.act,
              P.y_bf16 ? "bf16" : "f32", g.up.ct, g.up.width, g.up.rows, g.down.ct, g.down.width, g.down.rows, g.parts, (long long)g.blocks);
     return RAD_OK;
